@@ -754,6 +754,152 @@ int cyfa_norm_train(const CyfaNormTrainArgs* a, int dtype, int grad, void* hip_s
     return check_launch(what);
 }
 
+int cyfa_logprobs(const CyfaLogprobArgs* a, int dtype, int grad, void* hip_stream) {
+    const char* what = "cyfa_logprobs";
+    if (!a) return fail(CYFA_ERR_VALUE, "%s: null args", what);
+    if (dtype < CYFA_DTYPE_BF16 || dtype > CYFA_DTYPE_F16) return fail(CYFA_ERR_VALUE, "%s: dtype %d", what, dtype);
+    if (a->rows < 0 || a->inner <= 0 || a->V <= 0 || a->k < 0 || a->k > a->V)
+        return fail(CYFA_ERR_VALUE, "%s: rows=%lld inner=%lld V=%d k=%d", what, a->rows, a->inner, a->V, a->k);
+    if (a->k > CYFA_LOGPROBS_MAX_TOP)
+        return fail(CYFA_ERR_UNSUPPORTED, "%s: k=%d of at most %d alternatives", what, a->k, CYFA_LOGPROBS_MAX_TOP);
+    if (a->V > cyfa::LOGPROBS_MAX_V) return fail(CYFA_ERR_UNSUPPORTED, "%s: V=%d", what, a->V);
+    const int size = dtype == CYFA_DTYPE_F32 ? 4 : 2;
+    const void* words4[] = {a->logprob, a->entropy, a->stats, a->top_logprobs, a->loss, a->count, a->d_logprob, a->d_entropy, a->d_top,
+                            a->d_loss};
+    for (const void* ptr : words4)
+        if (!aligned(ptr, 4)) return fail(CYFA_ERR_ALIGN, "%s: f32 tensors need 4-byte alignment", what);
+    if (!aligned(a->x, size) || !aligned(a->dx, size) || !aligned(a->tokens, 8) || !aligned(a->top_ids, 8))
+        return fail(CYFA_ERR_ALIGN, "%s: tensors need their element's alignment", what);
+    if (a->rows > 0) {
+        if (!a->x || !a->tokens) return fail(CYFA_ERR_VALUE, "%s: null required pointer", what);
+        if (!grad && (!a->logprob || (a->k > 0 && (!a->top_logprobs || !a->top_ids))))
+            return fail(CYFA_ERR_VALUE, "%s: null output", what);
+        if (grad && (!a->dx || !a->stats || (a->d_entropy && !a->entropy) || (a->d_top && (!a->top_ids || a->k == 0)) ||
+                     (a->d_loss && (!a->count || a->d_logprob))))
+            return fail(CYFA_ERR_VALUE, "%s: a gradient without what the forward left for it", what);
+    }
+    if (!grad && (a->loss == nullptr) != (a->count == nullptr)) return fail(CYFA_ERR_VALUE, "%s: loss and count, both or none", what);
+    if (a->rows == 0 && (grad || !a->loss)) return CYFA_OK;
+    cyfa::LogprobParams p{};
+    p.rows = a->rows;
+    p.inner = a->inner;
+    p.outer_stride = a->outer_stride;
+    p.row_stride = a->row_stride;
+    p.V = a->V;
+    p.x = a->x;
+    p.tokens = a->tokens;
+    p.ignore = a->ignore;
+    p.logprob = a->logprob;
+    p.entropy = a->entropy;
+    p.stats = a->stats;
+    p.k = a->k;
+    p.top_logprobs = a->top_logprobs;
+    p.top_ids = a->top_ids;
+    p.loss = a->loss;
+    p.count = a->count;
+    p.d_logprob = a->d_logprob;
+    p.d_entropy = a->d_entropy;
+    p.d_top = a->d_top;
+    p.d_loss = a->d_loss;
+    p.dx = a->dx;
+    cyfa::launch_logprobs(p, dtype, grad != 0, (hipStream_t)hip_stream);
+    return check_launch(what);
+}
+
+size_t cyfa_embed_grad_workspace_bytes(long long n, long long V, int D) {
+    if (n < 0 || V <= 0 || D <= 0 || n > 0x7fffffffll || V > cyfa::EMBED_MAX_V) return 0;
+    return cyfa::embed_workspace(nullptr, n, V, D, nullptr);
+}
+
+int cyfa_embed(const CyfaEmbedArgs* a, int dtype, int grad, void* hip_stream) {
+    const char* what = "cyfa_embed";
+    if (!a) return fail(CYFA_ERR_VALUE, "%s: null args", what);
+    if (dtype < CYFA_DTYPE_BF16 || dtype > CYFA_DTYPE_F16) return fail(CYFA_ERR_VALUE, "%s: dtype %d", what, dtype);
+    if (a->n < 0 || a->V <= 0 || a->D <= 0) return fail(CYFA_ERR_VALUE, "%s: n=%lld V=%lld D=%d", what, a->n, a->V, a->D);
+    if (a->n > 0x7fffffffll || a->V > cyfa::EMBED_MAX_V)
+        return fail(CYFA_ERR_UNSUPPORTED, "%s: n=%lld V=%lld are too many", what, a->n, a->V);
+    const int size = dtype == CYFA_DTYPE_F32 ? 4 : 2;
+    if (!aligned(a->ids, 8) || !aligned(a->weight, size) || !aligned(a->out, size) || !aligned(a->dy, size) ||
+        !aligned(a->dweight, size))
+        return fail(CYFA_ERR_ALIGN, "%s: tensors need their element's alignment", what);
+    if (a->n > 0 && (!a->ids || (grad ? !a->dy : !a->weight || !a->out)))
+        return fail(CYFA_ERR_VALUE, "%s: null required pointer", what);
+    if (!grad && a->n == 0) return CYFA_OK;
+    cyfa::EmbedParams p{};
+    p.n = a->n;
+    p.V = a->V;
+    p.D = a->D;
+    p.ids = a->ids;
+    p.weight = a->weight;
+    p.scale = a->scale;
+    p.out = a->out;
+    p.padding = a->padding;
+    p.dy = a->dy;
+    p.dweight = a->dweight;
+    if (grad) {
+        if (!a->dweight) return fail(CYFA_ERR_VALUE, "%s: null dweight", what);
+        if (!a->workspace || a->workspace_bytes < cyfa::embed_workspace(&p, a->n, a->V, a->D, a->workspace))
+            return fail(CYFA_ERR_WORKSPACE, "%s: workspace of %zu bytes", what, a->workspace ? a->workspace_bytes : (size_t)0);
+        if (!aligned(a->workspace, 256)) return fail(CYFA_ERR_ALIGN, "%s: workspace needs 256-byte alignment", what);
+    }
+    cyfa::launch_embed(p, dtype, grad != 0, (hipStream_t)hip_stream);
+    return check_launch(what);
+}
+
+size_t cyfa_residual_grad_workspace_bytes(long long rows, int D) {
+    return rows < 0 || D <= 0 ? 0 : cyfa::residual_workspace_bytes(rows, D);
+}
+
+int cyfa_residual_norm(const CyfaResidualArgs* a, int dtype, int grad, void* hip_stream) {
+    const char* what = "cyfa_residual_norm";
+    if (!a) return fail(CYFA_ERR_VALUE, "%s: null args", what);
+    if (dtype < CYFA_DTYPE_BF16 || dtype > CYFA_DTYPE_F16) return fail(CYFA_ERR_VALUE, "%s: dtype %d", what, dtype);
+    if (a->rows < 0 || a->D <= 0) return fail(CYFA_ERR_VALUE, "%s: rows=%lld D=%d", what, a->rows, a->D);
+    if (a->D > cyfa::RESIDUAL_MAX_D)
+        return fail(CYFA_ERR_UNSUPPORTED, "%s: D=%d of at most %d columns", what, a->D, cyfa::RESIDUAL_MAX_D);
+    const int size = dtype == CYFA_DTYPE_F32 ? 4 : 2;
+    const void* rows[] = {a->x, a->y, a->gate, a->s, a->h, a->d_s, a->d_h, a->dx, a->dy, a->dgate};
+    for (const void* ptr : rows)
+        if (!aligned(ptr, size)) return fail(CYFA_ERR_ALIGN, "%s: tensors need their element's alignment", what);
+    const void* words4[] = {a->weight, a->post, a->stats, a->dweight, a->dpost};
+    for (const void* ptr : words4)
+        if (!aligned(ptr, 4)) return fail(CYFA_ERR_ALIGN, "%s: f32 tensors need 4-byte alignment", what);
+    if (!a->weight) return fail(CYFA_ERR_VALUE, "%s: null weight", what);
+    if (a->rows > 0 && (!a->x || !a->y || (grad ? !a->stats : !a->s || !a->h)))
+        return fail(CYFA_ERR_VALUE, "%s: null required pointer", what);
+    if (grad && ((a->dgate && !a->gate) || (a->dpost && !a->post)))
+        return fail(CYFA_ERR_VALUE, "%s: a gradient of an input that is not there", what);
+    if (a->rows == 0 && !grad) return CYFA_OK;
+    if (grad) {
+        if (!a->workspace || a->workspace_bytes < cyfa::residual_workspace_bytes(a->rows, a->D))
+            return fail(CYFA_ERR_WORKSPACE, "%s: workspace of %zu bytes", what, a->workspace ? a->workspace_bytes : (size_t)0);
+        if (!aligned(a->workspace, 16)) return fail(CYFA_ERR_ALIGN, "%s: workspace needs 16-byte alignment", what);
+    }
+    cyfa::ResidualParams p{};
+    p.rows = a->rows;
+    p.D = a->D;
+    p.x = a->x;
+    p.y = a->y;
+    p.gate = a->gate;
+    p.weight = a->weight;
+    p.post = a->post;
+    p.scale = a->scale;
+    p.eps = a->eps;
+    p.s = a->s;
+    p.h = a->h;
+    p.stats = a->stats;
+    p.d_s = a->d_s;
+    p.d_h = a->d_h;
+    p.dx = a->dx;
+    p.dy = a->dy;
+    p.dgate = a->dgate;
+    p.dweight = a->dweight;
+    p.dpost = a->dpost;
+    p.part = (float*)a->workspace;
+    cyfa::launch_residual_norm(p, dtype, grad != 0, (hipStream_t)hip_stream);
+    return check_launch(what);
+}
+
 int cyfa_mask_rows(const long long* mask, int B, int T, float* values, void* valid, int* lengths, void* hip_stream) {
     const char* what = "cyfa_mask_rows";
     if (B < 0 || T < 0) return fail(CYFA_ERR_VALUE, "%s: B=%d T=%d", what, B, T);

@@ -537,4 +537,68 @@ int launch_gate_path(const GatePathParams& p, hipStream_t stream);
 int launch_gates(const __bf16* abd, long long abd_row, const float* dt_bias, const float* A_log, float* g, float* beta,
                  float* delta, int rows, int H, hipStream_t stream);
 
+// Log probabilities, entropy and alternatives of rows of logits, their mean as
+// a loss, and the gradients (cyfa_logprobs.hip); dtype as CYFA_DTYPE_*.
+struct LogprobParams {
+    long long rows, inner;       // row r at x[(r / inner) outer_stride + (r % inner) row_stride]
+    long long outer_stride, row_stride;
+    int V;
+    const void* x;
+    const long long* tokens;     // [rows]; ignore: not counted, outside [0, V): NaN
+    long long ignore;
+    float *logprob, *entropy;    // [rows], entropy nullable
+    float* stats;                // nullable [rows, 2]: the maximum, log2 of the sum
+    int k;
+    float* top_logprobs;         // [rows, k]
+    long long* top_ids;          // [rows, k]
+    float *loss, *count;         // nullable [1]: the mean of -logprob, the number of rows in it
+    // gradients
+    const float *d_logprob, *d_entropy, *d_top;  // nullable [rows], [rows], [rows, k]
+    const float* d_loss;         // nullable [1], in place of d_logprob
+    void* dx;                    // [rows, V]
+};
+constexpr int LOGPROBS_MAX_V = 1 << 28;  // column indexes and their vectors stay in 32 bits
+constexpr int LOGPROBS_MAX_GRID = 1 << 20;  // rows of a launch taken by workgroups of their own
+void launch_logprobs(const LogprobParams& p, int dtype, bool grad, hipStream_t stream);
+
+// The scaled embedding lookup and its gradient (cyfa_embed.hip).
+struct EmbedParams {
+    long long n, V;
+    int D;
+    const long long* ids;        // [n]
+    const void* weight;          // [V, D]
+    float scale;
+    void* out;                   // [n, D]
+    // gradient
+    long long padding;           // id without a gradient; -1: none
+    const void* dy;              // [n, D]
+    void* dweight;               // [V, D]
+    int *offsets, *order;        // embed_workspace
+    float* part;
+    int chunk;                   // set by the launcher
+};
+constexpr long long EMBED_MAX_V = 1ll << 26;  // 512 ids to a workgroup of 1024 threads, below 2^32 threads
+size_t embed_workspace(EmbedParams* p, long long n, long long V, int D, void* base);
+void launch_embed(const EmbedParams& p, int dtype, bool grad, hipStream_t stream);
+
+// A block's output norm and gate, the residual add and the next norm, and the
+// gradients (cyfa_residual.hip).
+struct ResidualParams {
+    long long rows;
+    int D;
+    const void *x, *y, *gate;    // [rows, D], gate nullable
+    const float *weight, *post;  // [D], post nullable
+    float scale, eps;
+    void *s, *h;                 // [rows, D]
+    float* stats;                // nullable [rows, 2]: r1, r2
+    const void *d_s, *d_h;       // nullable [rows, D]
+    void *dx, *dy, *dgate;       // nullable [rows, D]
+    float *dweight, *dpost;      // nullable [D]
+    float* part;                 // residual_workspace_bytes
+    long long rows_wg;           // set by the launcher
+};
+constexpr int RESIDUAL_MAX_D = 8192;
+size_t residual_workspace_bytes(long long rows, int D);
+void launch_residual_norm(const ResidualParams& p, int dtype, bool grad, hipStream_t stream);
+
 }  // namespace cyfa

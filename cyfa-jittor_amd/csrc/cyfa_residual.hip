@@ -1,0 +1,324 @@
+// cyfa_residual.hip -- the join between two blocks: a block's output norm and
+// gate, the scaled residual add and the next block's norm, and the gradients.
+// For a row x, y [, gate] of D columns:
+//   n = y r1, r1 = (mean y^2 + eps)^-1/2          (with post; else u = y)
+//   u = n post,  b = u [sigmoid(gate)]
+//   s = x + scale b
+//   h = s r2 weight, r2 = (mean s^2 + eps)^-1/2   (of s before its rounding)
+// and from the cotangents ds, dh of s and h, with m = s r2 and e = dh weight:
+//   dx      = ds + r2 (e - m mean(e m))
+//   db      = scale dx,  du = db [sigmoid(gate)],  dgate = db u sigmoid(gate) (1 - sigmoid(gate))
+//   dy      = r1 (du post - n mean(du post n))    (du without post)
+//   dweight = sum over rows of dh m,  dpost = sum over rows of du n
+// mean(du post n) follows from sums over ds, e and m, so that one reduction
+// over the row serves both means.
+#include "cyfa_internal.h"
+#include "cyfa_rows.h"
+
+namespace cyfa {
+
+namespace {
+
+// Lane t of the T threads of a row holds the vectors t + j T (j < J) of VN
+// elements. The last vector of a row of no whole number of vectors is read
+// ending at the row's end, and its elements that the vector before it holds
+// count as zero and are not stored; so are all elements of vectors past it.
+template <class E, int VN, int T, int J>
+struct Row {
+    typedef E vec __attribute__((ext_vector_type(VN)));
+
+    int at[J], skip[J];  // column of the vector's first element; elements that do not count
+
+    __device__ __forceinline__ Row(int D, int t) {
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const int c = (t + j * T) * VN;
+            at[j] = min(c, D - VN);
+            skip[j] = min(c - at[j], VN);
+        }
+    }
+
+    template <class X>
+    __device__ __forceinline__ void load(const X* row, float (&v)[J][VN]) const {
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            typedef X xvec __attribute__((ext_vector_type(VN)));
+            xvec e;
+            __builtin_memcpy(&e, row + at[j], sizeof(e));
+#pragma unroll
+            for (int c = 0; c < VN; c++) v[j][c] = c < skip[j] ? 0.f : (float)e[c];
+        }
+    }
+
+    template <class X>
+    __device__ __forceinline__ void store(X* row, const float (&v)[J][VN]) const {
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            typedef X xvec __attribute__((ext_vector_type(VN)));
+            if (skip[j] == 0) {
+                xvec e;
+#pragma unroll
+                for (int c = 0; c < VN; c++) e[c] = (X)v[j][c];
+                __builtin_memcpy(row + at[j], &e, sizeof(e));
+            } else if (skip[j] < VN) {
+#pragma unroll
+                for (int c = 1; c < VN; c++)
+                    if (c >= skip[j]) row[at[j] + c] = (X)v[j][c];
+            }
+        }
+    }
+};
+
+// Sums over the T threads of a row, in a fixed order, in every thread of it.
+template <int T, int K>
+__device__ __forceinline__ void row_sums(float (&v)[K], float (*red)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; k++) v[k] = wave_sum(v[k]);
+    if (T == 64) return;
+    const int wv = threadIdx.x >> 6;
+    __syncthreads();  // red is free
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int k = 0; k < K; k++) red[wv][k] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; k++) v[k] = (red[0][k] + red[1][k]) + (red[2][k] + red[3][k]);
+}
+
+template <class E, int VN, int T, int J>
+__global__ __launch_bounds__(256) void residual_norm_kernel(ResidualParams p) {
+    __shared__ float red[4][1];
+    constexpr int RW = 256 / T;
+    const Row<E, VN, T, J> cols(p.D, threadIdx.x % T);
+    for (long long r = (long long)blockIdx.x * RW + threadIdx.x / T; r < p.rows; r += (long long)gridDim.x * RW) {
+        const long long o = r * p.D;
+        float s[J][VN], b[J][VN];
+        cols.load(static_cast<const E*>(p.x) + o, s);
+        cols.load(static_cast<const E*>(p.y) + o, b);
+        float ss[1] = {0.f};
+        if (p.post) {
+            float w[J][VN];
+            cols.load(p.post, w);
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int c = 0; c < VN; c++) ss[0] = fmaf(b[j][c], b[j][c], ss[0]);
+            row_sums<T>(ss, red);
+            const float r1 = rsqrtf(ss[0] / (float)p.D + p.eps);
+            if (p.stats && threadIdx.x % T == 0) p.stats[2 * r] = r1;
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int c = 0; c < VN; c++) b[j][c] *= r1 * w[j][c];
+        }
+        if (p.gate) {
+            float g[J][VN];
+            cols.load(static_cast<const E*>(p.gate) + o, g);
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int c = 0; c < VN; c++) b[j][c] *= sigmoidf(g[j][c]);
+        }
+        ss[0] = 0.f;
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int c = 0; c < VN; c++) {
+                s[j][c] = fmaf(p.scale, b[j][c], s[j][c]);
+                ss[0] = fmaf(s[j][c], s[j][c], ss[0]);
+            }
+        cols.store(static_cast<E*>(p.s) + o, s);
+        row_sums<T>(ss, red);
+        const float r2 = rsqrtf(ss[0] / (float)p.D + p.eps);
+        if (p.stats && threadIdx.x % T == 0) p.stats[2 * r + 1] = r2;
+        cols.load(p.weight, b);
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int c = 0; c < VN; c++) s[j][c] *= r2 * b[j][c];
+        cols.store(static_cast<E*>(p.h) + o, s);
+    }
+}
+
+// Workgroups of p.rows_wg rows; each leaves its sums for dweight and dpost in
+// part [workgroup][2][D], which residual_sum_kernel adds.
+template <class E, int VN, int T, int J>
+__global__ __launch_bounds__(256) void residual_grad_kernel(ResidualParams p) {
+    constexpr int RW = 256 / T, C = J * T * VN;
+    __shared__ float red[4][3];
+    __shared__ float sums[RW > 1 ? RW : 1][RW > 1 ? C : 1];
+    const int t = threadIdx.x % T;
+    const Row<E, VN, T, J> cols(p.D, t);
+    float dw[J][VN], dp[J][VN], w[J][VN], pw[J][VN];
+#pragma unroll
+    for (int j = 0; j < J; j++)
+#pragma unroll
+        for (int c = 0; c < VN; c++) dw[j][c] = dp[j][c] = 0.f;
+    cols.load(p.weight, w);
+    if (p.post) cols.load(p.post, pw);
+    const long long end = min((long long)(blockIdx.x + 1) * p.rows_wg, p.rows);
+    for (long long r = (long long)blockIdx.x * p.rows_wg + threadIdx.x / T; r < end; r += RW) {
+        const long long o = r * p.D;
+        float s[J][VN], y[J][VN], g[J][VN], e[J][VN], d[J][VN];
+        cols.load(static_cast<const E*>(p.x) + o, s);
+        cols.load(static_cast<const E*>(p.y) + o, y);
+        if (p.gate) cols.load(static_cast<const E*>(p.gate) + o, g);
+        if (p.d_h) cols.load(static_cast<const E*>(p.d_h) + o, e);
+        if (p.d_s) cols.load(static_cast<const E*>(p.d_s) + o, d);
+        const float r1 = p.post ? p.stats[2 * r] : 1.f, r2 = p.stats[2 * r + 1];
+        float sum[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int c = 0; c < VN; c++) {
+                float q = p.scale;
+                if (p.gate) {
+                    g[j][c] = sigmoidf(g[j][c]);
+                    q *= g[j][c];
+                }
+                float u = y[j][c];
+                if (p.post) {
+                    y[j][c] *= r1;
+                    u = y[j][c] * pw[j][c];
+                }
+                const float m = fmaf(q, u, s[j][c]) * r2;
+                s[j][c] = m;
+                if (!p.d_h) e[j][c] = 0.f;
+                if (!p.d_s) d[j][c] = 0.f;
+                dw[j][c] = fmaf(e[j][c], m, dw[j][c]);
+                e[j][c] *= w[j][c];
+                sum[0] = fmaf(e[j][c], m, sum[0]);
+                if (p.post) {  // q u: scale sigmoid(gate) post n
+                    sum[1] = fmaf(q * u, fmaf(r2, e[j][c], d[j][c]), sum[1]);
+                    sum[2] = fmaf(q * u, m, sum[2]);
+                }
+            }
+        if (p.post) {
+            row_sums<T>(sum, red);
+        } else {
+            float one[1] = {sum[0]};
+            row_sums<T>(one, reinterpret_cast<float(*)[1]>(red));
+            sum[0] = one[0];
+        }
+        const float a = sum[0] / (float)p.D * r2;
+        const float mean = (sum[1] - a * sum[2]) / (float)p.D;
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int c = 0; c < VN; c++) d[j][c] += fmaf(r2, e[j][c], -a * s[j][c]);
+        if (p.dx) cols.store(static_cast<E*>(p.dx) + o, d);
+        if (p.gate) {
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int c = 0; c < VN; c++) {
+                    const float u = p.post ? y[j][c] * pw[j][c] : y[j][c];
+                    e[j][c] = p.scale * d[j][c] * u * g[j][c] * (1.f - g[j][c]);
+                }
+            if (p.dgate) cols.store(static_cast<E*>(p.dgate) + o, e);
+        }
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int c = 0; c < VN; c++) {
+                float du = p.scale * d[j][c];
+                if (p.gate) du *= g[j][c];
+                if (p.post) {
+                    dp[j][c] = fmaf(du, y[j][c], dp[j][c]);
+                    du = r1 * (du * pw[j][c] - y[j][c] * mean);
+                }
+                d[j][c] = du;
+            }
+        if (p.dy) cols.store(static_cast<E*>(p.dy) + o, d);
+    }
+    const auto leave = [&](float (&v)[J][VN], int which) {
+        float* out = p.part + ((long long)blockIdx.x * 2 + which) * p.D;
+        if (RW == 1) {
+            cols.store(out, v);
+            return;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int c = 0; c < VN; c++) sums[threadIdx.x / T][(t + j * T) * VN + c] = v[j][c];
+        __syncthreads();
+        for (int c = threadIdx.x; c < p.D; c += 256) {
+            // column c of the vector that counts it: the last vector ends at D
+            const int whole = p.D / VN * VN, at = c < whole ? c : c + VN - (p.D - whole);
+            float v = 0.f;
+#pragma unroll
+            for (int i = 0; i < RW; i++) v += sums[i][at];
+            out[c] = v;
+        }
+    };
+    if (p.dweight) leave(dw, 0);
+    if (p.dpost) leave(dp, 1);
+}
+
+// dweight and dpost: the sums of part's rows, eight threads per column each
+// every eighth row in order, then the eight in order.
+__global__ __launch_bounds__(256) void residual_sum_kernel(ResidualParams p, int rows) {
+    __shared__ float red[8][32];
+    float* out = blockIdx.y ? p.dpost : p.dweight;
+    if (!out) return;
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+    float s = 0.f;
+    if (c < p.D)
+        for (int i = k; i < rows; i += 8) s += p.part[((long long)i * 2 + blockIdx.y) * p.D + c];
+    red[k][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (threadIdx.x < 32 && c < p.D) {
+        for (int i = 1; i < 8; i++) s += red[i][threadIdx.x];
+        out[c] = s;
+    }
+}
+
+// Rows of a workgroup of the gradient: a multiple of 4, at least 4.
+long long grad_rows(long long rows) {
+    const long long n = (rows + 511) / 512;
+    return n < 4 ? 4 : (n + 3) / 4 * 4;
+}
+
+template <class E, int VN, int T, int J>
+void launch(ResidualParams p, bool grad, hipStream_t stream) {
+    if (!grad) {
+        const long long groups = (p.rows + 256 / T - 1) / (256 / T);
+        hipLaunchKernelGGL((residual_norm_kernel<E, VN, T, J>), dim3((unsigned)min(groups, 1ll << 20)), dim3(256), 0, stream, p);
+        return;
+    }
+    p.rows_wg = grad_rows(p.rows);
+    const int n = (int)((p.rows + p.rows_wg - 1) / p.rows_wg);
+    if (n) hipLaunchKernelGGL((residual_grad_kernel<E, VN, T, J>), dim3(n), dim3(256), 0, stream, p);
+    if (p.dweight || p.dpost) hipLaunchKernelGGL(residual_sum_kernel, dim3((p.D + 31) / 32, 2), dim3(256), 0, stream, p, n);
+}
+
+template <class E>
+void launch_type(const ResidualParams& p, bool grad, hipStream_t stream) {
+    constexpr int N = 16 / sizeof(E);
+    if (p.D < N) return launch<E, 1, 64, 1>(p, grad, stream);
+    if (p.D <= 64 * N) return launch<E, N, 64, 1>(p, grad, stream);
+    if (p.D <= 128 * N) return launch<E, N, 64, 2>(p, grad, stream);
+    if (p.D <= 256 * N) return launch<E, N, 256, 1>(p, grad, stream);
+    if (p.D <= 512 * N) return launch<E, N, 256, 2>(p, grad, stream);
+    if (p.D <= 1024 * N) return launch<E, N, 256, 4>(p, grad, stream);
+    if constexpr (N == 4) launch<E, N, 256, 8>(p, grad, stream);
+}
+
+}  // namespace
+
+size_t residual_workspace_bytes(long long rows, int D) {
+    const long long w = grad_rows(rows);
+    return rows > 0 ? (size_t)((rows + w - 1) / w) * 2 * D * 4 : 16;
+}
+
+void launch_residual_norm(const ResidualParams& p, int dtype, bool grad, hipStream_t stream) {
+    if (dtype == 0)
+        launch_type<bf16_t>(p, grad, stream);
+    else if (dtype == 1)
+        launch_type<float>(p, grad, stream);
+    else
+        launch_type<f16_t>(p, grad, stream);
+}
+
+}  // namespace cyfa

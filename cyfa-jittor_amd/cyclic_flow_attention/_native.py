@@ -14,7 +14,7 @@ import torch
 import torch.nn.functional as F
 
 LIB_PATH = Path(os.environ.get("CYFA_LIB", Path(__file__).with_name("libcyfa_hip.so")))
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 CYFA_OK = 0
 CYFA_ERR_VALUE = -1
@@ -177,6 +177,35 @@ class CyfaGatePathArgs(ctypes.Structure):
     ]
 
 
+class CyfaLogprobArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_longlong), ("inner", ctypes.c_longlong), ("outer_stride", ctypes.c_longlong),
+        ("row_stride", ctypes.c_longlong), ("V", _c_int), ("x", _c_void_p), ("tokens", _c_void_p),
+        ("ignore", ctypes.c_longlong), ("logprob", _c_void_p), ("entropy", _c_void_p), ("stats", _c_void_p),
+        ("k", _c_int), ("top_logprobs", _c_void_p), ("top_ids", _c_void_p), ("loss", _c_void_p), ("count", _c_void_p),
+        ("d_logprob", _c_void_p), ("d_entropy", _c_void_p), ("d_top", _c_void_p), ("d_loss", _c_void_p),
+        ("dx", _c_void_p),
+    ]
+
+
+class CyfaEmbedArgs(ctypes.Structure):
+    _fields_ = [
+        ("n", ctypes.c_longlong), ("V", ctypes.c_longlong), ("D", _c_int), ("ids", _c_void_p), ("weight", _c_void_p),
+        ("scale", _c_float), ("out", _c_void_p), ("padding", ctypes.c_longlong), ("dy", _c_void_p),
+        ("dweight", _c_void_p), ("workspace", _c_void_p), ("workspace_bytes", _c_size_t),
+    ]
+
+
+class CyfaResidualArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_longlong), ("D", _c_int), ("x", _c_void_p), ("y", _c_void_p), ("gate", _c_void_p),
+        ("weight", _c_void_p), ("post", _c_void_p), ("scale", _c_float), ("eps", _c_float), ("s", _c_void_p),
+        ("h", _c_void_p), ("stats", _c_void_p), ("d_s", _c_void_p), ("d_h", _c_void_p), ("dx", _c_void_p),
+        ("dy", _c_void_p), ("dgate", _c_void_p), ("dweight", _c_void_p), ("dpost", _c_void_p),
+        ("workspace", _c_void_p), ("workspace_bytes", _c_size_t),
+    ]
+
+
 # Every symbol include/cyfa_abi.h declares, with its ctypes signature.
 SIGNATURES = {
     "cyfa_chunk_fwd": (_c_int, [ctypes.POINTER(CyfaChunkArgs), _c_void_p]),
@@ -212,6 +241,11 @@ SIGNATURES = {
     "cyfa_decode_step_general": (_c_int, [ctypes.POINTER(CyfaDecodeArgs), _c_int, _c_void_p]),
     "cyfa_chunk_bwd_workspace_bytes": (_c_size_t, [_c_int] * 6),
     "cyfa_chunk_bwd": (_c_int, [ctypes.POINTER(CyfaChunkArgs), _c_int, ctypes.POINTER(CyfaChunkBwdArgs), _c_void_p]),
+    "cyfa_logprobs": (_c_int, [ctypes.POINTER(CyfaLogprobArgs), _c_int, _c_int, _c_void_p]),
+    "cyfa_embed_grad_workspace_bytes": (_c_size_t, [ctypes.c_longlong, ctypes.c_longlong, _c_int]),
+    "cyfa_embed": (_c_int, [ctypes.POINTER(CyfaEmbedArgs), _c_int, _c_int, _c_void_p]),
+    "cyfa_residual_grad_workspace_bytes": (_c_size_t, [ctypes.c_longlong, _c_int]),
+    "cyfa_residual_norm": (_c_int, [ctypes.POINTER(CyfaResidualArgs), _c_int, _c_int, _c_void_p]),
     "cyfa_last_error": (ctypes.c_char_p, []),
     "cyfa_abi_version": (_c_int, []),
 }
@@ -904,3 +938,158 @@ def gates(abd, dt_bias, A_log):
     _check(load_library().cyfa_gates(ptr(flat), flat.stride(0), ptr(db), ptr(al), ptr(g), ptr(beta), ptr(delta),
                                       rows, H, stream_handle(dev)), "cyfa_gates")
     return g, beta, delta
+
+
+# The element types of the operators around a model's blocks (CYFA_DTYPE_*).
+LM_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+LOGPROBS_MAX_TOP = 32
+RESIDUAL_MAX_D = 8192
+
+
+def _lm_call(what, args, dtype, grad, dev):
+    """lib.<what>(args, dtype, grad, stream) on ``dev``'s current stream, with
+    that device current (a launch takes its code from the current device)."""
+    fn = getattr(load_library(), what)
+    if dev.index == torch.cuda.current_device():
+        rc = fn(ctypes.byref(args), LM_DTYPES[dtype], grad, stream_handle(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(ctypes.byref(args), LM_DTYPES[dtype], grad, stream_handle(dev))
+    if rc != CYFA_OK:
+        _raise(rc, what + " failed")
+
+
+def logit_rows(logits):
+    """(rows, arguments of CyfaLogprobArgs, the tensor they describe) of logits
+    [..., V]: the tensor itself where its rows are contiguous and one or two
+    strides apart, else a copy."""
+    V = logits.shape[-1]
+    if logits.stride(-1) != 1 and V > 1:
+        logits = logits.contiguous()
+    if logits.dim() == 1 or logits.numel() == 0:
+        inner, outer_stride, row_stride = 1, 0, 0
+    elif logits.dim() == 2:
+        inner, outer_stride, row_stride = logits.shape[0], 0, logits.stride(0)
+    else:
+        logits = logits.reshape(-1, *logits.shape[-2:])
+        inner, outer_stride, row_stride = logits.shape[1], logits.stride(0), logits.stride(1)
+    rows = logits.numel() // V
+    return rows, dict(rows=rows, inner=max(inner, 1), outer_stride=outer_stride, row_stride=row_stride, V=V,
+                      x=logits.data_ptr()), logits
+
+
+def logprobs(logits, tokens, k, ignore, stats=False):
+    """(logprob, entropy, top_logprobs or None, top_ids or None, stats or None)
+    of logits [..., V] for int64 contiguous tokens [...]."""
+    dev = require_device(logits, tokens)
+    rows, fields, logits = logit_rows(logits)
+    shape = tokens.shape
+    logprob, entropy = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(2))
+    top = ids = None
+    if k:
+        top = torch.empty(shape + (k,), dtype=torch.float32, device=dev)
+        ids = torch.empty(shape + (k,), dtype=torch.int64, device=dev)
+    st = torch.empty(rows, 2, dtype=torch.float32, device=dev) if stats else None
+    args = CyfaLogprobArgs(**fields, tokens=tokens.data_ptr(), ignore=ignore, logprob=logprob.data_ptr(),
+                           entropy=entropy.data_ptr(), stats=ptr(st), k=k, top_logprobs=ptr(top), top_ids=ptr(ids))
+    _lm_call("cyfa_logprobs", args, logits.dtype, 0, dev)
+    return logprob, entropy, top, ids, st
+
+
+def logprobs_grad(logits, tokens, k, ignore, stats, entropy, ids, d_logprob, d_entropy, d_top):
+    """The gradient of logits from the cotangents (fp32 contiguous or None) of
+    logprobs' first three results."""
+    dev = require_device(logits, tokens, d_logprob, d_entropy, d_top)
+    dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    _, fields, logits = logit_rows(logits)
+    args = CyfaLogprobArgs(**fields, tokens=tokens.data_ptr(), ignore=ignore, stats=stats.data_ptr(),
+                           entropy=entropy.data_ptr(), k=k, top_ids=ptr(ids), d_logprob=ptr(d_logprob),
+                           d_entropy=ptr(d_entropy), d_top=ptr(d_top), dx=dx.data_ptr())
+    _lm_call("cyfa_logprobs", args, dx.dtype, 1, dev)
+    return dx
+
+
+def token_loss(logits, labels, ignore):
+    """(loss, what token_loss_grad needs): the mean of -logprob over the labels
+    (int64, contiguous) that are not ``ignore``."""
+    dev = require_device(logits, labels)
+    rows, fields, logits = logit_rows(logits)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    kept = torch.empty(3 * rows + 1, dtype=torch.float32, device=dev)  # stats, logprob, count
+    at = kept.data_ptr()
+    args = CyfaLogprobArgs(**fields, tokens=labels.data_ptr(), ignore=ignore, stats=at, logprob=at + 8 * rows,
+                           loss=loss.data_ptr(), count=at + 12 * rows)
+    _lm_call("cyfa_logprobs", args, logits.dtype, 0, dev)
+    return loss, kept
+
+
+def token_loss_grad(logits, labels, ignore, kept, d_loss):
+    """The gradient of logits from the loss's cotangent (fp32, on the device)."""
+    dev = require_device(logits, labels, d_loss)
+    dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    rows, fields, logits = logit_rows(logits)
+    at = kept.data_ptr()
+    args = CyfaLogprobArgs(**fields, tokens=labels.data_ptr(), ignore=ignore, stats=at, count=at + 12 * rows,
+                           d_loss=d_loss.data_ptr(), dx=dx.data_ptr())
+    _lm_call("cyfa_logprobs", args, dx.dtype, 1, dev)
+    return dx
+
+
+def embed(ids, weight, scale):
+    """scale weight[ids] for int64 contiguous ids [...] and contiguous weight [V, D]."""
+    dev = require_device(ids, weight)
+    V, D = weight.shape
+    out = torch.empty(ids.shape + (D,), dtype=weight.dtype, device=dev)
+    args = CyfaEmbedArgs(n=ids.numel(), V=V, D=D, ids=ids.data_ptr(), weight=weight.data_ptr(), scale=scale,
+                         out=out.data_ptr())
+    _lm_call("cyfa_embed", args, weight.dtype, 0, dev)
+    return out
+
+
+def embed_grad(ids, V, dy, scale, padding):
+    """The gradient [V, D] of embed's weight from dy [..., D], contiguous."""
+    dev = require_device(ids, dy)
+    D = dy.shape[-1]
+    n = ids.numel()
+    dw = torch.empty(V, D, dtype=dy.dtype, device=dev)
+    size = int(load_library().cyfa_embed_grad_workspace_bytes(n, V, D))
+    workspace = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)  # alive until the launch
+    args = CyfaEmbedArgs(n=n, V=V, D=D, ids=ids.data_ptr(), scale=scale, padding=padding, dy=dy.data_ptr(),
+                         dweight=dw.data_ptr(), workspace=workspace.data_ptr(), workspace_bytes=size)
+    _lm_call("cyfa_embed", args, dy.dtype, 1, dev)
+    return dw
+
+
+def residual_norm(x, y, weight, post, gate, scale, eps, stats=False):
+    """(s, h, stats or None) of cyfa_residual_norm; x, y and gate contiguous of
+    one shape and dtype, weight and post fp32 [D]."""
+    dev = require_device(x, y, weight, post, gate)
+    D = x.shape[-1]
+    rows = x.numel() // D
+    s, h = torch.empty_like(x), torch.empty_like(x)
+    st = torch.empty(rows, 2, dtype=torch.float32, device=dev) if stats else None
+    args = CyfaResidualArgs(rows=rows, D=D, x=x.data_ptr(), y=y.data_ptr(), gate=ptr(gate), weight=weight.data_ptr(),
+                            post=ptr(post), scale=scale, eps=eps, s=s.data_ptr(), h=h.data_ptr(), stats=ptr(st))
+    _lm_call("cyfa_residual_norm", args, x.dtype, 0, dev)
+    return s, h, st
+
+
+def residual_norm_grad(x, y, weight, post, gate, scale, eps, stats, d_s, d_h, needed):
+    """Gradients (dx, dy, dweight, dpost, dgate) of residual_norm's results from
+    their cotangents (contiguous, or None), None where ``needed`` is false."""
+    dev = require_device(x, y, weight, post, gate, d_s, d_h)
+    D = x.shape[-1]
+    rows = x.numel() // D
+    plain = post is None and gate is None and scale == 1.0  # dy is dx
+    dx = torch.empty_like(x) if needed[0] or (plain and needed[1]) else None
+    dy = torch.empty_like(x) if needed[1] and not plain else None
+    dw, dp = (torch.empty(D, dtype=torch.float32, device=dev) if n else None for n in needed[2:4])
+    dg = torch.empty_like(x) if needed[4] else None
+    size = int(load_library().cyfa_residual_grad_workspace_bytes(rows, D))
+    workspace = torch.empty(size, dtype=torch.uint8, device=dev)  # alive until the launch
+    args = CyfaResidualArgs(rows=rows, D=D, x=x.data_ptr(), y=y.data_ptr(), gate=ptr(gate), weight=weight.data_ptr(),
+                            post=ptr(post), scale=scale, eps=eps, stats=stats.data_ptr(), d_s=ptr(d_s), d_h=ptr(d_h),
+                            dx=ptr(dx), dy=ptr(dy), dgate=ptr(dg), dweight=ptr(dw), dpost=ptr(dp),
+                            workspace=workspace.data_ptr(), workspace_bytes=size)
+    _lm_call("cyfa_residual_norm", args, x.dtype, 1, dev)
+    return dx if needed[0] else None, dx if plain and needed[1] else dy, dw, dp, dg

@@ -1,0 +1,206 @@
+"""The vocabulary's two ends of a causal language model on the gfx950 HIP path:
+the scaled embedding lookup, and log probabilities of tokens with their mean as
+the training loss (the reference's nn.Embedding and cross_entropy_loss,
+models/cyfa/modeling_cyfa.py:59-66, 101-106 of Chyxx/CyFA-Jittor v0.1.2).
+
+Each computes in fp32 whatever the dtype (bf16, fp16 or fp32) and rounds its
+results once. Where an input requires a gradient the call is recorded for
+autograd and its backward runs as HIP kernels too; a backward pass that is
+itself recorded (``create_graph=True``) runs in torch operations.
+"""
+
+from typing import NamedTuple
+
+import torch
+import torch.nn.functional as F
+
+from .. import _native
+
+
+class TokenLogprobs(NamedTuple):
+    """token_logprobs' results; the last two are None without alternatives."""
+
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor | None
+    top_ids: torch.Tensor | None
+
+
+def _check_logits(what, logits, tokens, name):
+    if logits.dtype not in _native.LM_DTYPES:
+        raise NotImplementedError(f"{what}: logits must be bf16, fp16 or fp32, got {logits.dtype}")
+    if logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError(f"{what}: logits must be [..., vocabulary], got {tuple(logits.shape)}")
+    if tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"{what}: {name} must have shape {tuple(logits.shape[:-1])}, got {tuple(tokens.shape)}")
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{what}: {name} must be int64 or int32, got {tokens.dtype}")
+    return tokens.to(torch.int64).contiguous()
+
+
+def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
+    """Log probabilities of ``tokens`` [...] under softmax(``logits`` [..., V]),
+    the entropy of each row, and its ``top_k`` (at most 32) most probable tokens.
+
+    Returns TokenLogprobs(logprob [...], entropy [...], top_logprobs
+    [..., top_k], top_ids [..., top_k]), fp32 and int64; the alternatives in
+    falling order, the lower id first among equal logits. The logits may be
+    strided (a slice of the time axis is read in place). A token equal to
+    ``ignore_index`` has logprob 0 and gives no gradient through it; one outside
+    [0, V) otherwise has logprob NaN. Logits of -inf have probability 0 and add
+    nothing to the entropy; a row of nothing else has no probabilities, and its
+    results are NaN, as those of a row that holds a NaN or +inf.
+
+    Differentiable in the logits through logprob, entropy and top_logprobs; a
+    row whose cotangents are all zero gets a gradient of zeros, whatever it holds.
+    """
+    tokens = _check_logits("token_logprobs", logits, tokens, "tokens")
+    top_k = int(top_k)
+    if not 0 <= top_k <= logits.shape[-1]:
+        raise ValueError(f"token_logprobs: top_k must be in [0, {logits.shape[-1]}], got {top_k}")
+    if top_k > _native.LOGPROBS_MAX_TOP:
+        raise NotImplementedError(f"token_logprobs: at most {_native.LOGPROBS_MAX_TOP} alternatives, got {top_k}")
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top_k, int(ignore_index)))
+    return TokenLogprobs(*_native.logprobs(logits, tokens, top_k, int(ignore_index))[:4])
+
+
+def _recorded(*cotangents):
+    """Whether this backward pass is itself recorded, or batched (vmap)."""
+    return (torch.is_grad_enabled() or torch._C._functorch.peek_interpreter_stack() is not None
+            or any(t is not None and torch._C._functorch.is_legacy_batchedtensor(t) for t in cotangents))
+
+
+def _torch_backward(fn, inputs, needed, cotangents):
+    """Gradients of fn(*inputs) in torch operations, recorded when this
+    backward pass is."""
+    recorded = torch.is_grad_enabled()
+    with torch.enable_grad():
+        pairs = [(o, c) for o, c in zip(fn(*inputs), cotangents) if c is not None]
+        wanted = [t for t, n in zip(inputs, needed) if n]
+        if not pairs or not wanted:
+            return tuple(torch.zeros_like(t) if n else None for t, n in zip(inputs, needed))
+        outs, cots = zip(*pairs)
+        grads = iter(torch.autograd.grad(outs, wanted, cots, create_graph=recorded, allow_unused=True))
+    return tuple(next(grads) if n else None for n in needed)
+
+
+def _plain_logprobs(logits, tokens, ids, ignore_index):
+    """(logprob, entropy, top_logprobs) in torch operations."""
+    lp = F.log_softmax(logits.float(), -1)
+    ignored = tokens == ignore_index
+    logprob = lp.gather(-1, tokens.masked_fill(ignored, 0)[..., None])[..., 0].masked_fill(ignored, 0.0)
+    p = lp.exp()
+    entropy = -(p * lp.masked_fill(p == 0, 0.0)).sum(-1)
+    return (logprob, entropy) if ids is None else (logprob, entropy, lp.gather(-1, ids))
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    """token_logprobs with its gradient: keeps the logits and, of each row, the
+    maximum, the log of the sum and the entropy."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, top_k, ignore_index):
+        logprob, entropy, top, ids, stats = _native.logprobs(logits, tokens, top_k, ignore_index, stats=True)
+        ctx.save_for_backward(logits, tokens, stats, entropy, ids)
+        ctx.args = (top_k, ignore_index)
+        ctx.set_materialize_grads(False)
+        if ids is not None:
+            ctx.mark_non_differentiable(ids)
+        return logprob, entropy, top, ids
+
+    @staticmethod
+    def backward(ctx, d_logprob, d_entropy, d_top, _):
+        logits, tokens, stats, entropy, ids = ctx.saved_tensors
+        top_k, ignore_index = ctx.args
+        cots = (d_logprob, d_entropy, d_top)
+        if _recorded(*cots):
+            return _torch_backward(lambda x: _plain_logprobs(x, tokens, ids, ignore_index), (logits,), (True,),
+                                   cots) + (None,) * 3
+        cots = [None if c is None else c.contiguous() for c in cots]
+        return _native.logprobs_grad(logits, tokens, top_k, ignore_index, stats, entropy, ids, *cots), None, None, None
+
+
+def token_loss(logits, labels, ignore_index=-100):
+    """The mean of -log softmax(``logits`` [..., V])[label] over the ``labels``
+    [...] that are not ``ignore_index``, an fp32 scalar: F.cross_entropy of the
+    logits in fp32, without forming them, and with NaN for a label outside
+    [0, V). No label that counts: NaN, as F.cross_entropy. Differentiable in the
+    logits; rows of ignored labels get zeros. The labels are those of the rows
+    as they are (a causal model shifts them: label t is the token after t)."""
+    labels = _check_logits("token_loss", logits, labels, "labels")
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _TokenLoss.apply(logits, labels, int(ignore_index))
+    return _native.token_loss(logits, labels, int(ignore_index))[0]
+
+
+def _plain_loss(logits, labels, ignore_index):
+    return (F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), labels.reshape(-1), ignore_index=ignore_index),)
+
+
+class _TokenLoss(torch.autograd.Function):
+    """token_loss with its gradient."""
+
+    @staticmethod
+    def forward(ctx, logits, labels, ignore_index):
+        loss, kept = _native.token_loss(logits, labels, ignore_index)
+        ctx.save_for_backward(logits, labels, kept)
+        ctx.ignore_index = ignore_index
+        return loss
+
+    @staticmethod
+    def backward(ctx, d_loss):
+        logits, labels, kept = ctx.saved_tensors
+        if _recorded(d_loss):
+            return _torch_backward(lambda x: _plain_loss(x, labels, ctx.ignore_index), (logits,), (True,),
+                                   (d_loss,)) + (None, None)
+        return _native.token_loss_grad(logits, labels, ctx.ignore_index, kept, d_loss.contiguous()), None, None
+
+
+def embed_tokens(ids, weight, scale=1.0, padding_idx=None):
+    """scale weight[ids]: rows of ``weight`` [V, D] for integer ``ids`` [...],
+    [..., D] in the weight's dtype. An id outside [0, V) gives a row of NaN.
+
+    The gradient of the weight is dense and adds each id's cotangents in the
+    order of the positions, in fp32 and rounded once, so that two backward
+    passes give the same bits; the row of ``padding_idx`` (negative: from the
+    end) and ids outside [0, V) get none."""
+    if weight.dtype not in _native.LM_DTYPES:
+        raise NotImplementedError(f"embed_tokens: the weight must be bf16, fp16 or fp32, got {weight.dtype}")
+    if weight.dim() != 2 or 0 in weight.shape:
+        raise ValueError(f"embed_tokens: the weight must be [vocabulary, width], got {tuple(weight.shape)}")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"embed_tokens: ids must be int64 or int32, got {ids.dtype}")
+    V = weight.shape[0]
+    if padding_idx is None:
+        padding_idx = -1
+    elif not -V <= padding_idx < V:
+        raise ValueError(f"embed_tokens: padding_idx must be in [-{V}, {V}), got {padding_idx}")
+    else:
+        padding_idx = int(padding_idx) % V
+    ids = ids.to(torch.int64).contiguous()
+    weight = weight.contiguous()
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return _EmbedTokens.apply(ids, weight, float(scale), padding_idx)
+    return _native.embed(ids, weight, float(scale))
+
+
+class _EmbedTokens(torch.autograd.Function):
+    """embed_tokens with its gradient."""
+
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.args = (weight.shape[0], scale, padding_idx)
+        return _native.embed(ids, weight, scale)
+
+    @staticmethod
+    def backward(ctx, dy):
+        (ids,) = ctx.saved_tensors
+        V, scale, padding_idx = ctx.args
+        if _recorded(dy):  # (linear in dy)
+            kept = ((ids >= 0) & (ids < V) & (ids != padding_idx)).reshape(-1, 1)
+            rows = torch.where(kept, dy.float().reshape(-1, dy.shape[-1]) * scale, 0.0)
+            dw = rows.new_zeros(V, dy.shape[-1]).index_add(0, ids.reshape(-1).clamp(0, V - 1), rows)
+            return None, dw.to(dy.dtype), None, None
+        return None, _native.embed_grad(ids, V, dy.contiguous(), scale, padding_idx), None, None

@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define CYFA_ABI_VERSION 16
+#define CYFA_ABI_VERSION 17
 
 enum {
     CYFA_OK = 0,
@@ -244,7 +244,7 @@ int cyfa_decode_layer_step(const CyfaDecodeArgs *args, const CyfaDecodeLayerArgs
 int cyfa_readout_table(const float *readout, float *table, int H, int M, void *hip_stream);
 
 /* Element type of q, k, v and o in the general-shape entry points. */
-enum { CYFA_DTYPE_BF16 = 0, CYFA_DTYPE_F32 = 1 };
+enum { CYFA_DTYPE_BF16 = 0, CYFA_DTYPE_F32 = 1, CYFA_DTYPE_F16 = 2 }; /* F16: where an entry point names it */
 
 /* Workspace bytes of cyfa_chunk_fwd_general (0 for a non-positive argument):
  * per (b, h, token padded to a multiple of 64) row the normalised rows, the
@@ -579,6 +579,89 @@ int cyfa_silu_mul(const void *gu, void *out, int rows, int F, void *hip_stream);
  * Replaces layers/cyfa.py:323-326. */
 int cyfa_gates(const void *abd, long long abd_row, const float *dt_bias, const float *A_log, float *g, float *beta,
                float *delta, int rows, int H, void *hip_stream);
+
+/* Log probabilities of given tokens (grad 0) and their gradients (grad 1), for
+ * rows of logits x (CYFA_DTYPE_BF16, _F32 or _F16) of V columns, row r at
+ * x[(r / inner) outer_stride + (r % inner) row_stride], any alignment; with
+ * p = softmax(x[r]), t = tokens[r]:
+ *   logprob[r] = log p_t (0 where t is ignore; NaN where t is outside [0, V))
+ *   entropy[r] = -sum p log p
+ *   top_ids[r], top_logprobs[r]: the k most probable, the lower index first
+ *     among equals, a NaN logit before all others
+ *   loss = the mean of -logprob over the rows whose token is not ignore, count = their number
+ * sums in f32 (the loss's in f64). A row of nothing but -inf has no probabilities:
+ * NaN. grad 1 reads stats, entropy (with d_entropy), top_ids (with d_top) and
+ * count (with d_loss) as grad 0 left them and writes dx [rows, V], contiguous;
+ * rows whose cotangents are all zero become zero without reading x. No
+ * counterpart in the reference but the loss (models/cyfa/modeling_cyfa.py:101-106). */
+typedef struct CyfaLogprobArgs {
+    long long rows, inner;        /* inner > 0 */
+    long long outer_stride, row_stride;
+    int V;
+    const void *x;
+    const long long *tokens;      /* [rows] */
+    long long ignore;
+    float *logprob;               /* [rows] */
+    float *entropy;               /* nullable [rows] */
+    float *stats;                 /* [rows, 2], nullable in grad 0: maximum, log2 of the sum of e^(x - maximum) */
+    int k;                        /* 0 .. CYFA_LOGPROBS_MAX_TOP, at most V */
+    float *top_logprobs;          /* [rows, k] */
+    long long *top_ids;           /* [rows, k] */
+    float *loss, *count;          /* nullable [1], both or none */
+    const float *d_logprob, *d_entropy, *d_top, *d_loss; /* grad 1: nullable; d_loss [1] in place of d_logprob */
+    void *dx;                     /* grad 1 */
+} CyfaLogprobArgs;
+
+#define CYFA_LOGPROBS_MAX_TOP 32
+int cyfa_logprobs(const CyfaLogprobArgs *args, int dtype, int grad, void *hip_stream);
+
+/* The embedding lookup out[i] = scale weight[ids[i]] (grad 0) and its gradient
+ * dweight[v] = scale sum of dy[i] over ids[i] = v, i in order (grad 1), in f32
+ * and rounded once; weight, out, dy, dweight CYFA_DTYPE_BF16, _F32 or _F16,
+ * contiguous, any alignment. An id outside [0, V) gives a row of NaN and has no
+ * gradient, nor has the id padding (-1: none). n < 2^31, V <= 2^26. Replaces
+ * nn.Embedding (models/cyfa/modeling_cyfa.py:59-66) and its adjoint. */
+typedef struct CyfaEmbedArgs {
+    long long n, V;
+    int D;
+    const long long *ids;         /* [n] */
+    const void *weight;           /* grad 0: [V, D] */
+    float scale;
+    void *out;                    /* grad 0: [n, D] */
+    long long padding;
+    const void *dy;               /* grad 1: [n, D] */
+    void *dweight;                /* grad 1: [V, D], every row written */
+    void *workspace;              /* grad 1: cyfa_embed_grad_workspace_bytes(n, V, D) bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} CyfaEmbedArgs;
+
+size_t cyfa_embed_grad_workspace_bytes(long long n, long long V, int D);
+int cyfa_embed(const CyfaEmbedArgs *args, int dtype, int grad, void *hip_stream);
+
+/* The join between two blocks (CyFABlock.execute, models/cyfa/modeling_cyfa.py:
+ * 48-51, with a block's output norm, gate and residual scale) on contiguous rows
+ * [rows, D], D up to 8192, of CYFA_DTYPE_BF16, _F32 or _F16, any alignment:
+ *   b = y [rsqrt(mean y^2 + eps) post] [sigmoid(gate)],  s = x + scale b
+ *   h = s rsqrt(mean s^2 + eps) weight, of s before its rounding      (grad 0)
+ * and from the cotangents d_s and d_h the gradients (grad 1), sums in f32 and
+ * in a fixed order. */
+typedef struct CyfaResidualArgs {
+    long long rows;
+    int D;
+    const void *x, *y, *gate;     /* gate nullable */
+    const float *weight, *post;   /* f32 [D], post nullable */
+    float scale, eps;
+    void *s, *h;                  /* grad 0 */
+    float *stats;                 /* [rows, 2], nullable in grad 0: the two reciprocal roots */
+    const void *d_s, *d_h;        /* grad 1, nullable */
+    void *dx, *dy, *dgate;        /* grad 1, nullable */
+    float *dweight, *dpost;       /* grad 1, nullable f32 [D] */
+    void *workspace;              /* grad 1: cyfa_residual_grad_workspace_bytes(rows, D) bytes, 16-byte aligned */
+    size_t workspace_bytes;
+} CyfaResidualArgs;
+
+size_t cyfa_residual_grad_workspace_bytes(long long rows, int D);
+int cyfa_residual_norm(const CyfaResidualArgs *args, int dtype, int grad, void *hip_stream);
 
 /* Thread-local message of the last failing call (never NULL). No reference
  * counterpart: Jittor reports kernel errors as C++ exceptions. */
