@@ -206,18 +206,18 @@ def _own_score(case, st):
     if not case["train"]:
         with torch.no_grad():
             r = _ops().token_logprobs(st["logits"], st["tokens"], top_k=case["top"])
-        return _score_outputs(case, r.logprob, r.entropy, r.top_logprobs, r.top_ids)
+        return _score_outputs(case, r)
     r = _ops().token_logprobs(st["logits"], st["tokens"], top_k=case["top"])
     outs, cots = [r.logprob, r.entropy], [st["d_logprob"], st["d_entropy"]]
     if case["top"]:
         outs.append(r.top_logprobs)
         cots.append(st["d_top"])
     (dx,) = torch.autograd.grad(outs, [st["logits"]], cots)
-    return _score_outputs(case, r.logprob.detach(), r.entropy.detach(), r.top_logprobs.detach(), r.top_ids) + [dx]
+    return [t.detach() for t in _score_outputs(case, r)] + [dx]
 
 
-def _score_outputs(case, logprob, entropy, top_logprobs, top_ids):
-    return [logprob, entropy, top_logprobs, top_ids] if case["top"] else [logprob, entropy]
+def _score_outputs(case, r):
+    return [r.logprob, r.entropy, r.top_logprobs, r.top_ids] if case["top"] else [r.logprob, r.entropy]
 
 
 def _own_loss(case, st):
