@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedParams p) {
 // positions behind those of the waves before it. Ids outside [0, V) and the
 // padding id count nowhere.
 //   offsets[v] .. offsets[v + 1]: where v's positions lie in order
-constexpr int ES_NT = 1024, ES_WAVES = ES_NT / 64;
+constexpr int ES_NT = 1024, ES_WAVES = ES_NT / 64, ES_U = 16;
 constexpr int ES_RANGE = 512;  // most ids of a workgroup: 35 KB of LDS
 
 __global__ __launch_bounds__(ES_NT) void embed_sort_kernel(EmbedParams p, int range) {
@@ -48,25 +48,39 @@ __global__ __launch_bounds__(ES_NT) void embed_sort_kernel(EmbedParams p, int ra
     int* start = lds + ES_WAVES * range;    // [range]
     int* misc = start + range;              // [2 * ES_WAVES]
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const long long v0 = (long long)blockIdx.x * range;
-    const int mine = (int)min((long long)range, p.V - v0);
+    const int v0 = blockIdx.x * range, mine = min(range, (int)p.V - v0);
     const long long stretch = ((p.n + ES_NT - 1) / ES_NT) * 64;
     const long long first = wv * stretch, last = min(first + stretch, p.n);
+    // ES_U times 64 positions from i0: each lane's ids relative to v0, or -1 below
+    // the range, range or more above it; nowhere: INT_MAX. All loads in flight at
+    // once, those past the end of the last position.
+    const auto load = [&](long long i0, int (&local)[ES_U]) {
+        long long id[ES_U];
+#pragma unroll
+        for (int u = 0; u < ES_U; u++) id[u] = p.ids[min(i0 + 64 * u + lane, p.n - 1)];
+#pragma unroll
+        for (int u = 0; u < ES_U; u++) {
+            const bool counts = i0 + 64 * u + lane < last && id[u] >= 0 && id[u] < p.V && id[u] != p.padding;
+            local[u] = counts ? max((int)id[u] - v0, -1) : 0x7fffffff;
+        }
+    };
     for (int i = tid; i < ES_WAVES * range; i += ES_NT) cursor[i] = 0;
     __syncthreads();
-    int below = 0;
-    for (long long i = first + lane; i < last; i += 64) {
-        const long long id = p.ids[i];
-        if (id < 0 || id >= p.V || id == p.padding) continue;
-        if (id < v0) below++;
-        else if (id < v0 + mine) atomicAdd(&cursor[wv * range + (int)(id - v0)], 1);
+    int below = 0, local[ES_U];
+    for (long long i0 = first; i0 < last; i0 += 64 * ES_U) {
+        load(i0, local);
+#pragma unroll
+        for (int u = 0; u < ES_U; u++) {
+            below += local[u] < 0;
+            if ((unsigned)local[u] < (unsigned)mine) atomicAdd(&cursor[wv * range + local[u]], 1);
+        }
     }
     for (int d = 32; d > 0; d >>= 1) below += __shfl_xor(below, d);
     if (lane == 0) misc[wv] = below;
     __syncthreads();
     below = 0;
     for (int w = 0; w < ES_WAVES; w++) below += misc[w];
-    // this id's positions of the waves before, and of the ids before (range <= ES_RANGE)
+    // this id's positions of the waves before, and of the ids before (range <= ES_NT)
     int total = 0;
     if (tid < mine)
         for (int w = 0; w < ES_WAVES; w++) {
@@ -88,63 +102,71 @@ __global__ __launch_bounds__(ES_NT) void embed_sort_kernel(EmbedParams p, int ra
         if (v0 + tid == p.V - 1) p.offsets[p.V] = below + scan;
     }
     __syncthreads();
-    for (long long i0 = first; i0 < last; i0 += 64) {
-        const long long i = i0 + lane;
-        int local = -1;
-        if (i < last) {
-            const long long id = p.ids[i];
-            if (id >= v0 && id < v0 + mine && id != p.padding) local = (int)(id - v0);
-        }
-        uint64_t todo = __ballot(local >= 0);
-        while (todo) {  // one id of these 64 positions after another
-            const int id = __builtin_amdgcn_readlane(local, __builtin_ctzll(todo));
-            const uint64_t same = __ballot(local == id);
-            int* at = &cursor[wv * range + id];
-            const int c = *at;
-            if (local == id) p.order[start[id] + c + __popcll(same & ((1ull << lane) - 1))] = (int)i;
-            *at = c + __popcll(same);  // (every lane, the same value)
-            todo &= ~same;
+    const bool once = stretch <= 64 * ES_U;  // the ids are still in registers
+    for (long long i0 = first; i0 < last; i0 += 64 * ES_U) {
+        if (!once) load(i0, local);
+#pragma unroll
+        for (int u = 0; u < ES_U; u++) {
+            uint64_t todo = __ballot((unsigned)local[u] < (unsigned)mine);
+            while (todo) {  // one id of these 64 positions after another
+                const int id = __builtin_amdgcn_readlane(local[u], __builtin_ctzll(todo));
+                const uint64_t same = __ballot(local[u] == id);
+                int* at = &cursor[wv * range + id];
+                const int c = *at;
+                if (local[u] == id) p.order[start[id] + c + __popcll(same & ((1ull << lane) - 1))] = (int)(i0 + 64 * u + lane);
+                *at = c + __popcll(same);  // (every lane, the same value)
+                todo &= ~same;
+            }
         }
     }
 }
 
-// The sum of dy's rows of sorted positions [s, e), columns of one vector of this lane.
-template <class E, int U>
+// Adds dy's rows of the sorted positions [s, e) (the same in every lane) in
+// order, the columns of one vector of this lane, EG_U rows' loads in flight.
+constexpr int EG_U = 8;
+
+template <class E>
 __device__ __forceinline__ void add_rows(const EmbedParams& p, const E* dy, int s, int e, float (&acc)[RowVec<E>::N]) {
     constexpr int N = RowVec<E>::N;
-    for (int i = s; i < e; i += U) {
-        typename RowVec<E>::type v[U];
+    for (int i = s; i < e; i += EG_U) {
+        typename RowVec<E>::type v[EG_U];
 #pragma unroll
-        for (int u = 0; u < U; u++) v[u] = load_row(dy + (long long)p.order[i + u < e ? i + u : e - 1] * p.D);
+        for (int u = 0; u < EG_U; u++) v[u] = load_row(dy + (long long)p.order[min(i + u, e - 1)] * p.D);
 #pragma unroll
-        for (int u = 0; u < U; u++)
+        for (int u = 0; u < EG_U; u++)
             if (i + u < e)
 #pragma unroll
                 for (int c = 0; c < N; c++) acc[c] += (float)v[u][c];
     }
 }
 
+// An id with many positions is shared out: every EMBED_CHUNK sorted positions
+// that all hold one id are added by a wave of embed_part_kernel, and
+// embed_grad_kernel adds the id's chunks and what is left at both ends.
+//
 // Columns of a wave: 64 vectors; the last, ragged vector of a row is read and
 // written ending at the row's end, so that it overlaps the one before it
 // (the same values are stored twice), and rows below one vector go column by column.
+constexpr int EMBED_CHUNK = 32;
+
 template <class E>
 __global__ __launch_bounds__(256) void embed_part_kernel(EmbedParams p) {
     constexpr int N = RowVec<E>::N;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int cols = (p.D + 64 * N - 1) / (64 * N), n = p.offsets[p.V];
-    const long long units = (long long)(n / p.chunk) * cols, waves = (long long)gridDim.x * 4;
-    for (long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += waves) {
-        const long long c = unit / cols;
-        const int s = (int)(c * p.chunk), e = s + p.chunk;
+    const long long units = (long long)(n / EMBED_CHUNK) * cols, waves = (long long)gridDim.x * 4;
+    for (long long unit = (long long)blockIdx.x * 4 + wv; unit < units; unit += waves) {
+        const int c = (int)(unit / cols);
+        const int s = c * EMBED_CHUNK, e = s + EMBED_CHUNK;
         const int d = (int)(unit % cols) * 64 * N + lane * N;
         if (p.ids[p.order[s]] != p.ids[p.order[e - 1]] || d >= p.D) continue;  // not one id's whole chunk
-        float* out = p.part + c * p.D;
+        float* out = p.part + (long long)c * p.D;
         if (p.D >= N) {
             const int at = min(d, p.D - N);
             float acc[N];
 #pragma unroll
             for (int i = 0; i < N; i++) acc[i] = 0.f;
-            add_rows<E, 8>(p, static_cast<const E*>(p.dy) + at, s, e, acc);
+            add_rows<E>(p, static_cast<const E*>(p.dy) + at, s, e, acc);
 #pragma unroll
             for (int i = 0; i < N; i++) out[at + i] = acc[i];
         } else {
@@ -160,17 +182,16 @@ __global__ __launch_bounds__(256) void embed_part_kernel(EmbedParams p) {
 template <class E>
 __global__ __launch_bounds__(256) void embed_grad_kernel(EmbedParams p) {
     constexpr int N = RowVec<E>::N;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int cols = (p.D + 64 * N - 1) / (64 * N);
     const long long units = p.V * cols, waves = (long long)gridDim.x * 4;
-    for (long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += waves) {
+    for (long long unit = (long long)blockIdx.x * 4 + wv; unit < units; unit += waves) {
         const long long v = unit / cols;
         const int d = (int)(unit % cols) * 64 * N + lane * N;
         const int s = p.offsets[v], e = p.offsets[v + 1];
         if (d >= p.D) continue;
-        // whole chunks [c0, c1) of this id were added by embed_part_kernel
-        const int c0 = (s + p.chunk - 1) / p.chunk, c1 = e / p.chunk;
-        const bool parts = c0 < c1;
+        const int c0 = (s + EMBED_CHUNK - 1) / EMBED_CHUNK, c1 = e / EMBED_CHUNK;
+        const bool parts = c0 < c1;  // whole chunks [c0, c1) of this id
         E* out = static_cast<E*>(p.dweight) + v * p.D;
         if (p.D >= N) {
             const int at = min(d, p.D - N);
@@ -178,12 +199,20 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(EmbedParams p) {
             float acc[N];
 #pragma unroll
             for (int i = 0; i < N; i++) acc[i] = 0.f;
-            add_rows<E, 8>(p, dy, s, parts ? c0 * p.chunk : e, acc);
+            add_rows<E>(p, dy, s, parts ? c0 * EMBED_CHUNK : e, acc);
             if (parts) {
-                for (int c = c0; c < c1; c++)
+                for (int c = c0; c < c1; c += EG_U) {
+                    float part[EG_U][N];
 #pragma unroll
-                    for (int i = 0; i < N; i++) acc[i] += p.part[(long long)c * p.D + at + i];
-                add_rows<E, 8>(p, dy, c1 * p.chunk, e, acc);
+                    for (int u = 0; u < EG_U; u++)
+                        __builtin_memcpy(part[u], p.part + (long long)min(c + u, c1 - 1) * p.D + at, sizeof(part[u]));
+#pragma unroll
+                    for (int u = 0; u < EG_U; u++)
+                        if (c + u < c1)
+#pragma unroll
+                            for (int i = 0; i < N; i++) acc[i] += part[u][i];
+                }
+                add_rows<E>(p, dy, c1 * EMBED_CHUNK, e, acc);
             }
             typename RowVec<E>::type o;
 #pragma unroll
@@ -193,10 +222,10 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(EmbedParams p) {
             for (int i = 0; i < p.D; i++) {
                 float a = 0.f;
                 const E* dy = static_cast<const E*>(p.dy) + i;
-                for (int j = s; j < (parts ? c0 * p.chunk : e); j++) a += (float)dy[(long long)p.order[j] * p.D];
+                for (int j = s; j < (parts ? c0 * EMBED_CHUNK : e); j++) a += (float)dy[(long long)p.order[j] * p.D];
                 if (parts) {
                     for (int c = c0; c < c1; c++) a += p.part[(long long)c * p.D + i];
-                    for (int j = c1 * p.chunk; j < e; j++) a += (float)dy[(long long)p.order[j] * p.D];
+                    for (int j = c1 * EMBED_CHUNK; j < e; j++) a += (float)dy[(long long)p.order[j] * p.D];
                 }
                 out[i] = (E)(a * p.scale);
             }
@@ -204,20 +233,17 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(EmbedParams p) {
     }
 }
 
-constexpr int EMBED_CHUNK = 64;
-
 template <class E>
-void launch(EmbedParams p, bool grad, hipStream_t stream) {
+void launch(const EmbedParams& p, bool grad, hipStream_t stream) {
     if (!grad) {
         hipLaunchKernelGGL(embed_kernel<E>, dim3((unsigned)min((p.n + 3) / 4, 1ll << 20)), dim3(256), 0, stream, p);
         return;
     }
-    p.chunk = EMBED_CHUNK;
     const int range = (int)min((p.V + 255) / 256, (long long)ES_RANGE);
     hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)((p.V + range - 1) / range)), dim3(ES_NT),
                        ((ES_WAVES + 1) * range + 2 * ES_WAVES) * sizeof(int), stream, p, range);
     const int cols = (p.D + 64 * RowVec<E>::N - 1) / (64 * RowVec<E>::N);
-    const long long chunks = p.n / p.chunk;
+    const long long chunks = p.n / EMBED_CHUNK;
     if (chunks)
         hipLaunchKernelGGL(embed_part_kernel<E>, dim3((unsigned)min((chunks * cols + 3) / 4, 1ll << 20)), dim3(256), 0, stream, p);
     hipLaunchKernelGGL(embed_grad_kernel<E>, dim3((unsigned)min((p.V * cols + 3) / 4, 1ll << 20)), dim3(256), 0, stream, p);

@@ -575,7 +575,6 @@ struct EmbedParams {
     void* dweight;               // [V, D]
     int *offsets, *order;        // embed_workspace
     float* part;
-    int chunk;                   // set by the launcher
 };
 constexpr long long EMBED_MAX_V = 1ll << 26;  // 512 ids to a workgroup of 1024 threads, below 2^32 threads
 size_t embed_workspace(EmbedParams* p, long long n, long long V, int D, void* base);

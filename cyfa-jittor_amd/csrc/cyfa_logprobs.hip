@@ -17,8 +17,8 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;
-constexpr int LP_NT = 256, LP_NV = 4;   // threads and vectors per thread of a tile of a row
 constexpr int LP_CAP = 1024;            // candidates for the alternatives held in LDS
+constexpr int LP_NV = 4;                // vectors of a thread in a tile of a row
 
 // The order of the alternatives as an unsigned key: larger values first (a NaN
 // largest, as torch.topk has it; -0 equals +0), then the lower index.
@@ -50,136 +50,162 @@ __device__ __forceinline__ void rescale(RowSums& a, float m) {
     a.m = m;
 }
 
-// Adds elements x[0 .. n): -inf counts nothing (its product with t would be a NaN).
-template <int n>
-__device__ __forceinline__ void add_elements(RowSums& a, const float (&x)[n]) {
-    float m = a.m;
-#pragma unroll
-    for (int i = 0; i < n; i++) m = fmaxf(m, x[i]);
-    rescale(a, m);
-#pragma unroll
-    for (int i = 0; i < n; i++) {
-        const float t = (x[i] - m) * kLog2e, e = fast_exp2(t);
-        a.s += e;
-        a.s1 = fmaf(fmaxf(t, -200.f), e, a.s1);
-    }
-}
+// The exponent of an element that counts nothing: 0 times minus infinity would be a NaN.
+constexpr float kNothing = -200.f;
 
 template <class E>
 __device__ __forceinline__ const E* row_of(const LogprobParams& p, long long r) {
     return static_cast<const E*>(p.x) + (r / p.inner) * p.outer_stride + (r % p.inner) * p.row_stride;
 }
 
-template <class E>
-__global__ __launch_bounds__(LP_NT) void logprobs_kernel(LogprobParams p) {
-    constexpr int N = RowVec<E>::N, W = LP_NT / 64;
+// The k-th largest of the 64 lanes' values x (no NaN), but for an order of the
+// last 6 bits: ranked as integers in the values' order with the lane in place
+// of those bits, so that all differ; the smallest of the first k. In every lane.
+__device__ __forceinline__ float kth_largest(float x, int k) {
+    const uint32_t mine = (value_key(x) & ~63u) | (uint32_t)(threadIdx.x & 63);
+    int rank = 0;
+#pragma unroll 16
+    for (int i = 0; i < 64; i++) rank += (uint32_t)__builtin_amdgcn_readlane((int)mine, i) > mine;
+    return -wave_max(rank < k ? -x : -INFINITY);
+}
+
+// One workgroup of NT threads to a row (rows beyond the grid in turn), tiles of
+// NT * LP_NV vectors of it in registers: a row of one tile is read from memory
+// once, also for its alternatives.
+template <class E, int NT, bool TOP>
+__global__ __launch_bounds__(NT) void logprobs_kernel(LogprobParams p) {
+    constexpr int N = RowVec<E>::N, W = NT / 64;
     __shared__ RowSums red[W];
-    __shared__ uint64_t keys[W][64];
-    __shared__ uint64_t cand[LP_CAP];
-    __shared__ uint64_t thr_s;
+    __shared__ float best_s[TOP ? W : 1][64];
+    __shared__ uint64_t cand[TOP ? LP_CAP : 1];
+    __shared__ uint64_t next_s[TOP ? W : 1];
+    __shared__ float thr_s;
     __shared__ int count_s;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const int nvec = p.V / N, tail = p.V - nvec * N;
     for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const E* x = row_of<E>(p, r);
-        // Every element of this thread with its index, tile by tile.
-        const auto each_vector = [&](auto&& f) {
-            for (int v0 = 0; v0 < nvec; v0 += LP_NT * LP_NV) {
-                typename RowVec<E>::type v[LP_NV];
+        const long long t = p.tokens[r];
+        const bool ignored = t == p.ignore;
+        if (ignored && !TOP && !p.entropy) {  // (the loss: nothing of this row counts)
+            if (tid == 0) p.logprob[r] = 0.f;
+            continue;
+        }
+        const bool inside = t >= 0 && t < p.V;
+        const float xt = inside ? (float)x[t] : __builtin_nanf("");
+        const float last = tid < tail ? (float)x[nvec * N + tid] : -INFINITY;
+        typename RowVec<E>::type v[LP_NV];
+        // Vectors past the end are read as the last one and dropped: no branch
+        // among the loads, at which the compiler would wait for those in flight.
+        const auto load_tile = [&](int v0) {
 #pragma unroll
-                for (int j = 0; j < LP_NV; j++) {
-                    const int i = v0 + j * LP_NT + tid;
-                    if (i < nvec) v[j] = load_row(x + (size_t)i * N);
-                }
+            for (int j = 0; j < LP_NV; j++) v[j] = load_row(x + (size_t)min(v0 + j * NT + tid, nvec - 1) * N);
+        };
+        // f(element, index) of this thread's elements in tile v0
+        const auto each = [&](int v0, auto&& f) {
 #pragma unroll
-                for (int j = 0; j < LP_NV; j++) {
-                    const int i = v0 + j * LP_NT + tid;
-                    if (i < nvec) {
-                        float e[N];
+            for (int j = 0; j < LP_NV; j++) {
+                const int i = v0 + j * NT + tid;
+                if (i < nvec) {
 #pragma unroll
-                        for (int c = 0; c < N; c++) e[c] = (float)v[j][c];
-                        f(e, i * N);
-                    }
+                    for (int c = 0; c < N; c++) f((float)v[j][c], i * N + c);
                 }
             }
         };
-        const float last = tid < tail ? (float)x[nvec * N + tid] : -INFINITY;
         RowSums a = {kLowest, 0.f, 0.f};
-        each_vector([&](const float (&e)[N], int) { add_elements(a, e); });
-        add_elements(a, {last});
-        float m = wave_max(a.m);
+        float best = last;
+        const auto add = [&](float e) {
+            const float u = (e - a.m) * kLog2e, q = fast_exp2(u);
+            a.s += q;
+            a.s1 = fmaf(fmaxf(u, kNothing), q, a.s1);
+        };
+        for (int v0 = 0; v0 < nvec; v0 += NT * LP_NV) {
+            load_tile(v0);
+            each(v0, [&](float e, int) { best = fmaxf(best, e); });
+            rescale(a, fmaxf(a.m, best));
+            each(v0, [&](float e, int) { add(e); });
+        }
+        rescale(a, fmaxf(a.m, best));
+        if (tid < tail) add(last);
+        const float m = wave_max(a.m);
         rescale(a, m);
         a.s = wave_sum(a.s);
         a.s1 = wave_sum(a.s1);
-        if (lane == 0) red[wv] = a;
-        __syncthreads();
-        a = red[0];
-        for (int w = 1; w < W; w++) {
-            RowSums b = red[w];
-            const float mm = fmaxf(a.m, b.m);
-            rescale(a, mm);
-            rescale(b, mm);
-            a.s += b.s;
-            a.s1 += b.s1;
+        if (W > 1) {
+            if (lane == 0) red[wv] = a;
+            if (TOP) best_s[wv][lane] = best;
+            __syncthreads();
+            a = red[0];
+#pragma unroll
+            for (int w = 1; w < W; w++) {
+                RowSums b = red[w];
+                const float mm = fmaxf(a.m, b.m);
+                rescale(a, mm);
+                rescale(b, mm);
+                a.s += b.s;
+                a.s1 += b.s1;
+            }
         }
-        const float ls = logf(a.s), entropy = ls - kLn2 * (a.s1 / a.s);
+        const float ls = logf(a.s);
         if (tid == 0) {
-            const long long t = p.tokens[r];
-            const bool ignored = t == p.ignore;
-            const float lp = t >= 0 && t < p.V ? ((float)x[t] - a.m) - ls : __builtin_nanf("");
-            p.logprob[r] = ignored ? 0.f : lp;
-            if (p.entropy) p.entropy[r] = entropy;
+            p.logprob[r] = ignored ? 0.f : (xt - a.m) - ls;
+            if (p.entropy) p.entropy[r] = ls - kLn2 * (a.s1 / a.s);
             if (p.stats) {
                 p.stats[2 * r] = a.m;
                 p.stats[2 * r + 1] = ls * kLog2e;
             }
         }
-        if (p.k > 0) {
-            // The k-th largest of the best elements of 64 sets of threads: at
-            // least k elements reach it, and seldom many more.
-            uint64_t best = 0;
-            const auto take = [&](float e, int i) {
-                const uint64_t key = order_key(e, i);
-                best = key > best ? key : best;
-            };
-            each_vector([&](const float (&e)[N], int i) {
-#pragma unroll
-                for (int c = 0; c < N; c++) take(e[c], i + c);
-            });
-            if (tid < tail) take(last, nvec * N + tid);
-            keys[wv][lane] = best;
-            if (tid == 0) count_s = 0;
-            __syncthreads();
-            if (wv == 0) {
-                for (int w = 1; w < W; w++) best = keys[w][lane] > best ? keys[w][lane] : best;
-                int rank = 0;
-                for (int i = 0; i < 64; i++) rank += __shfl(best, i) > best;
-                const uint64_t at = __ballot(rank == p.k - 1 && best != 0);
-                const uint64_t kth = __shfl(best, at ? __builtin_ctzll(at) : 0);
-                if (lane == 0) thr_s = at ? kth : 1;  // (fewer than k sets hold an element: every element)
-            }
-            __syncthreads();
-            const uint64_t thr = thr_s;
-            const auto keep = [&](float e, int i) {
-                const uint64_t key = order_key(e, i);
-                if (key >= thr) {
-                    const int n = atomicAdd(&count_s, 1);
-                    if (n < LP_CAP) cand[n] = key;
-                }
-            };
-            each_vector([&](const float (&e)[N], int i) {
-#pragma unroll
-                for (int c = 0; c < N; c++) keep(e[c], i + c);
-            });
-            if (tid < tail) keep(last, nvec * N + tid);
-            __syncthreads();
-            const int n = count_s;
+        if (TOP) {
             const auto put = [&](int rank, uint64_t key) {
                 p.top_ids[r * p.k + rank] = 0xffffffffu - (uint32_t)key;
                 p.top_logprobs[r * p.k + rank] = (key_value(key) - a.m) - ls;
             };
-            if (n <= LP_CAP) {
-                for (int c = tid; c < n; c += LP_NT) {
+            const bool one_tile = nvec <= NT * LP_NV;
+            const auto each_of_row = [&](auto&& f) {
+                for (int v0 = 0; v0 < nvec; v0 += NT * LP_NV) {
+                    if (!one_tile) load_tile(v0);
+                    each(v0, f);
+                }
+                if (tid < tail) f(last, nvec * N + tid);
+            };
+            // A threshold that k elements reach and seldom many more: the k-th
+            // largest of the largest elements of 64 sets of threads. The
+            // candidates' ranks among themselves are those in the row.
+            int n = -1;
+            if (a.s == a.s) {  // no NaN, no +inf
+                if (wv == 0) {
+                    for (int w = 1; w < W; w++) best = fmaxf(best, best_s[w][lane]);
+                    const float thr = kth_largest(best, p.k);
+                    if (lane == 0) {
+                        thr_s = thr;
+                        count_s = 0;
+                    }
+                }
+                __syncthreads();
+                const float thr = thr_s;
+                const auto hold = [&](float e, int i) {
+                    const int at = atomicAdd(&count_s, 1);
+                    if (at < LP_CAP) cand[at] = order_key(e, i);
+                };
+                each_of_row([&](float e, int i) {
+                    if (e >= thr) hold(e, i);
+                });
+                __syncthreads();
+                n = count_s;
+                if (n > LP_CAP) {  // many equal elements: all above them, and those of the lowest columns
+                    __syncthreads();
+                    if (tid == 0) count_s = 0;
+                    __syncthreads();
+                    each_of_row([&](float e, int i) {
+                        if (e > thr || (e == thr && i < LP_CAP / 2)) hold(e, i);
+                    });
+                    __syncthreads();
+                    n = count_s;
+                    if (n < p.k || n > LP_CAP) n = -1;
+                }
+            }
+            if (n >= 0) {
+                for (int c = tid; c < n; c += NT) {
                     const uint64_t key = cand[c];
                     int rank = 0;
                     for (int i = 0; i < n; i++) rank += cand[i] > key;
@@ -188,30 +214,25 @@ __global__ __launch_bounds__(LP_NT) void logprobs_kernel(LogprobParams p) {
             } else {  // k rounds, each the largest key below the one before
                 uint64_t below = ~0ull;
                 for (int rank = 0; rank < p.k; rank++) {
-                    best = 0;
-                    const auto next = [&](float e, int i) {
+                    uint64_t next = 0;
+                    each_of_row([&](float e, int i) {
                         const uint64_t key = order_key(e, i);
-                        if (key < below && key > best) best = key;
-                    };
-                    each_vector([&](const float (&e)[N], int i) {
-#pragma unroll
-                        for (int c = 0; c < N; c++) next(e[c], i + c);
+                        if (key < below && key > next) next = key;
                     });
-                    if (tid < tail) next(last, nvec * N + tid);
                     for (int d = 32; d > 0; d >>= 1) {
-                        const uint64_t o = __shfl_xor(best, d);
-                        best = o > best ? o : best;
+                        const uint64_t o = __shfl_xor(next, d);
+                        next = o > next ? o : next;
                     }
                     __syncthreads();
-                    if (lane == 0) keys[wv][0] = best;
+                    if (lane == 0) next_s[wv] = next;
                     __syncthreads();
-                    for (int w = 0; w < W; w++) best = keys[w][0] > best ? keys[w][0] : best;
-                    if (tid == 0) put(rank, best);
-                    below = best;
+                    for (int w = 0; w < W; w++) next = next_s[w] > next ? next_s[w] : next;
+                    if (tid == 0) put(rank, next);
+                    below = next;
                 }
             }
         }
-        __syncthreads();  // red, keys, cand and count_s are free for the next row
+        if (W > 1 || TOP) __syncthreads();  // the shared arrays are free for the next row
     }
 }
 
@@ -220,12 +241,24 @@ __global__ __launch_bounds__(LP_NT) void logprobs_kernel(LogprobParams p) {
 __global__ __launch_bounds__(1024) void loss_mean_kernel(LogprobParams p) {
     __shared__ double sums[16];
     __shared__ double counts[16];
+    constexpr int U = 8;  // rows of a thread whose loads are in flight together
     double s = 0., n = 0.;
-    for (long long r = threadIdx.x; r < p.rows; r += 1024)
-        if (p.tokens[r] != p.ignore) {
-            s += (double)p.logprob[r];
-            n += 1.;
+    for (long long r0 = threadIdx.x; r0 < p.rows; r0 += 1024 * U) {
+        long long t[U];
+        float lp[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long long r = min(r0 + 1024 * u, p.rows - 1);
+            t[u] = p.tokens[r];
+            lp[u] = p.logprob[r];
         }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (r0 + 1024 * u < p.rows && t[u] != p.ignore) {
+                s += (double)lp[u];
+                n += 1.;
+            }
+    }
     s = wave_sum(s);
     n = wave_sum(n);
     if ((threadIdx.x & 63) == 0) {
@@ -244,75 +277,108 @@ __global__ __launch_bounds__(1024) void loss_mean_kernel(LogprobParams p) {
     }
 }
 
-template <class E>
-__global__ __launch_bounds__(LP_NT) void logprobs_grad_kernel(LogprobParams p) {
+// The gradient of the columns [c0, c1) of a row by a workgroup: blockIdx.y's
+// share of the row, whole vectors.
+constexpr int LG_NT = 256, LG_NV = 4;
+
+template <class E, bool ENTROPY>
+__global__ __launch_bounds__(LG_NT) void logprobs_grad_kernel(LogprobParams p, int share) {
     constexpr int N = RowVec<E>::N;
     const int tid = threadIdx.x;
-    const int nvec = p.V / N, tail = p.V - nvec * N;
+    const int c0 = blockIdx.y * share, c1 = min(c0 + share, p.V);
+    const int nvec = (c1 - c0) / N, tail = c1 - c0 - nvec * N;
     for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        const E* x = row_of<E>(p, r);
-        E* dx = static_cast<E*>(p.dx) + r * p.V;
+        const E* x = row_of<E>(p, r) + c0;
+        E* dx = static_cast<E*>(p.dx) + r * p.V + c0;
         const long long t = p.tokens[r];
+        const float m = p.stats[2 * r], ls = p.stats[2 * r + 1];
         float dlp = 0.f;
         if (t != p.ignore) dlp = p.d_loss ? -*p.d_loss / *p.count : p.d_logprob ? p.d_logprob[r] : 0.f;
         if (dlp != 0.f && (t < 0 || t >= p.V)) dlp = __builtin_nanf("");
-        const float dh = p.d_entropy ? p.d_entropy[r] : 0.f;
+        const float dh = ENTROPY ? p.d_entropy[r] : 0.f;
         float total = dlp;
         bool any = dlp != 0.f || dh != 0.f;
-        if (p.d_top)
-            for (int j = 0; j < p.k; j++) {
-                const float d = p.d_top[r * p.k + j];
-                total += d;
-                any |= d != 0.f;
-            }
+        const int k = p.d_top ? p.k : 0;
+        for (int j = 0; j < k; j++) {
+            const float d = p.d_top[r * p.k + j];
+            total += d;
+            any |= d != 0.f;
+        }
         typename RowVec<E>::type o;
         if (!any) {
 #pragma unroll
             for (int c = 0; c < N; c++) o[c] = (E)0.f;
-            for (int i = tid; i < nvec; i += LP_NT) store_row(dx + (size_t)i * N, o);
+            for (int i = tid; i < nvec; i += LG_NT) store_row(dx + (size_t)i * N, o);
             if (tid < tail) dx[nvec * N + tid] = (E)0.f;
             continue;
         }
-        const float m = p.stats[2 * r], ls = p.stats[2 * r + 1];
         // dx = p (a + b log2 p) for the elements that no output reads by itself
-        const float a = -total - (dh != 0.f ? dh * p.entropy[r] : 0.f), b = -dh * kLn2;
+        const float a = -total - (ENTROPY && dh != 0.f ? dh * p.entropy[r] : 0.f), b = -dh * kLn2;
         const auto grad = [&](float e) {
             const float l = (e - m) * kLog2e - ls;
             const float q = fast_exp2(l);
-            return q * fmaf(fmaxf(l, -200.f), b, a);
+            return ENTROPY ? q * fmaf(fmaxf(l, kNothing), b, a) : q * a;
         };
-        for (int i = tid; i < nvec; i += LP_NT) {
-            const typename RowVec<E>::type v = load_row(x + (size_t)i * N);
+        for (int i0 = 0; i0 < nvec; i0 += LG_NT * LG_NV) {
+            typename RowVec<E>::type v[LG_NV];
 #pragma unroll
-            for (int c = 0; c < N; c++) o[c] = (E)grad((float)v[c]);
-            store_row(dx + (size_t)i * N, o);
+            for (int j = 0; j < LG_NV; j++) v[j] = load_row(x + (size_t)min(i0 + j * LG_NT + tid, nvec - 1) * N);
+#pragma unroll
+            for (int j = 0; j < LG_NV; j++) {
+                const int i = i0 + j * LG_NT + tid;
+                if (i < nvec) {
+#pragma unroll
+                    for (int c = 0; c < N; c++) o[c] = (E)grad((float)v[j][c]);
+                    store_row(dx + (size_t)i * N, o);
+                }
+            }
         }
         if (tid < tail) dx[nvec * N + tid] = (E)grad((float)x[nvec * N + tid]);
-        __syncthreads();  // the elements that outputs read are written again
-        const int k = p.d_top ? p.k : 0;
+        __syncthreads();  // the elements that outputs read themselves are written again
         if (tid <= k) {
             const auto index = [&](int j) { return j == 0 ? t : p.top_ids[r * p.k + j - 1]; };
             const auto cot = [&](int j) { return j == 0 ? dlp : p.d_top[r * p.k + j - 1]; };
             const long long i = index(tid);
             float sum = 0.f;
-            bool first = i >= 0 && i < p.V;
-            for (int j = 0; j <= k; j++)
-                if (index(j) == i) {
-                    if (j < tid) first = false;
-                    sum += cot(j);
-                }
-            if (first) dx[i] = (E)(grad((float)x[i]) + sum);
+            bool first = i >= c0 && i < c1;
+            if (first)
+                for (int j = 0; j <= k; j++)
+                    if (index(j) == i) {
+                        if (j < tid) first = false;
+                        sum += cot(j);
+                    }
+            if (first) dx[i - c0] = (E)(grad((float)x[i - c0]) + sum);
         }
     }
 }
 
+template <class E, int NT>
+void launch_rows(const LogprobParams& p, hipStream_t stream) {
+    const dim3 grid((unsigned)min(p.rows, (long long)LOGPROBS_MAX_GRID));
+    if (p.k > 0)
+        hipLaunchKernelGGL((logprobs_kernel<E, NT, true>), grid, dim3(NT), 0, stream, p);
+    else
+        hipLaunchKernelGGL((logprobs_kernel<E, NT, false>), grid, dim3(NT), 0, stream, p);
+}
+
 template <class E>
 void launch(const LogprobParams& p, bool grad, hipStream_t stream) {
-    const dim3 grid((unsigned)min(p.rows, (long long)LOGPROBS_MAX_GRID));
-    if (grad)
-        hipLaunchKernelGGL(logprobs_grad_kernel<E>, grid, dim3(LP_NT), 0, stream, p);
-    else
-        hipLaunchKernelGGL(logprobs_kernel<E>, grid, dim3(LP_NT), 0, stream, p);
+    constexpr int N = RowVec<E>::N;
+    if (grad) {
+        const long long shares = min((1024 + p.rows - 1) / p.rows, (long long)(p.V + LG_NT * N - 1) / (LG_NT * N));
+        const int share = (int)(((p.V + shares - 1) / shares + N - 1) / N * N);
+        const dim3 grid((unsigned)min(p.rows, (long long)LOGPROBS_MAX_GRID), (unsigned)((p.V + share - 1) / share));
+        if (p.d_entropy)
+            hipLaunchKernelGGL((logprobs_grad_kernel<E, true>), grid, dim3(LG_NT), 0, stream, p, share);
+        else
+            hipLaunchKernelGGL((logprobs_grad_kernel<E, false>), grid, dim3(LG_NT), 0, stream, p, share);
+    } else if (p.V <= 64 * LP_NV * N) {
+        launch_rows<E, 64>(p, stream);
+    } else if (p.V <= 256 * LP_NV * N || p.rows >= 512) {
+        launch_rows<E, 256>(p, stream);
+    } else {
+        launch_rows<E, 1024>(p, stream);
+    }
 }
 
 }  // namespace

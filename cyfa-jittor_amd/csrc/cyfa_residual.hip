@@ -256,20 +256,28 @@ __global__ __launch_bounds__(256) void residual_grad_kernel(ResidualParams p) {
     if (p.dpost) leave(dp, 1);
 }
 
-// dweight and dpost: the sums of part's rows, eight threads per column each
-// every eighth row in order, then the eight in order.
-__global__ __launch_bounds__(256) void residual_sum_kernel(ResidualParams p, int rows) {
-    __shared__ float red[8][32];
+// dweight and dpost: the sums of part's rows, 32 threads per column each every
+// 32nd row in order (RS_U loads in flight), then the 32 in order.
+constexpr int RS_U = 8;
+
+__global__ __launch_bounds__(1024) void residual_sum_kernel(ResidualParams p, int rows) {
+    __shared__ float red[32][33];
     float* out = blockIdx.y ? p.dpost : p.dweight;
     if (!out) return;
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+    const int col = threadIdx.x & 31, c = min((int)blockIdx.x * 32 + col, p.D - 1), k = threadIdx.x >> 5;
     float s = 0.f;
-    if (c < p.D)
-        for (int i = k; i < rows; i += 8) s += p.part[((long long)i * 2 + blockIdx.y) * p.D + c];
-    red[k][threadIdx.x & 31] = s;
+    for (int i = k; i < rows; i += 32 * RS_U) {
+        float v[RS_U];
+#pragma unroll
+        for (int u = 0; u < RS_U; u++) v[u] = p.part[((long long)min(i + 32 * u, rows - 1) * 2 + blockIdx.y) * p.D + c];
+#pragma unroll
+        for (int u = 0; u < RS_U; u++)
+            if (i + 32 * u < rows) s += v[u];
+    }
+    red[k][col] = s;
     __syncthreads();
-    if (threadIdx.x < 32 && c < p.D) {
-        for (int i = 1; i < 8; i++) s += red[i][threadIdx.x];
+    if (k == 0 && (int)blockIdx.x * 32 + col < p.D) {
+        for (int i = 1; i < 32; i++) s += red[i][col];
         out[c] = s;
     }
 }
@@ -290,7 +298,7 @@ void launch(ResidualParams p, bool grad, hipStream_t stream) {
     p.rows_wg = grad_rows(p.rows);
     const int n = (int)((p.rows + p.rows_wg - 1) / p.rows_wg);
     if (n) hipLaunchKernelGGL((residual_grad_kernel<E, VN, T, J>), dim3(n), dim3(256), 0, stream, p);
-    if (p.dweight || p.dpost) hipLaunchKernelGGL(residual_sum_kernel, dim3((p.D + 31) / 32, 2), dim3(256), 0, stream, p, n);
+    if (p.dweight || p.dpost) hipLaunchKernelGGL(residual_sum_kernel, dim3((p.D + 31) / 32, 2), dim3(1024), 0, stream, p, n);
 }
 
 template <class E>
