@@ -807,7 +807,7 @@ int cyfa_logprobs(const CyfaLogprobArgs* a, int dtype, int grad, void* hip_strea
 }
 
 size_t cyfa_embed_grad_workspace_bytes(long long n, long long V, int D) {
-    if (n < 0 || V <= 0 || D <= 0 || n > 0x7fffffffll || V > cyfa::EMBED_MAX_V) return 0;
+    if (n < 0 || V <= 0 || D <= 0 || n > cyfa::EMBED_MAX_N || V > cyfa::EMBED_MAX_V || D > cyfa::EMBED_MAX_D) return 0;
     return cyfa::embed_workspace(nullptr, n, V, D, nullptr);
 }
 
@@ -816,8 +816,9 @@ int cyfa_embed(const CyfaEmbedArgs* a, int dtype, int grad, void* hip_stream) {
     if (!a) return fail(CYFA_ERR_VALUE, "%s: null args", what);
     if (dtype < CYFA_DTYPE_BF16 || dtype > CYFA_DTYPE_F16) return fail(CYFA_ERR_VALUE, "%s: dtype %d", what, dtype);
     if (a->n < 0 || a->V <= 0 || a->D <= 0) return fail(CYFA_ERR_VALUE, "%s: n=%lld V=%lld D=%d", what, a->n, a->V, a->D);
-    if (a->n > 0x7fffffffll || a->V > cyfa::EMBED_MAX_V)
+    if (a->n > cyfa::EMBED_MAX_N || a->V > cyfa::EMBED_MAX_V)
         return fail(CYFA_ERR_UNSUPPORTED, "%s: n=%lld V=%lld are too many", what, a->n, a->V);
+    if (a->D > cyfa::EMBED_MAX_D) return fail(CYFA_ERR_UNSUPPORTED, "%s: D=%d", what, a->D);
     const int size = dtype == CYFA_DTYPE_F32 ? 4 : 2;
     if (!aligned(a->ids, 8) || !aligned(a->weight, size) || !aligned(a->out, size) || !aligned(a->dy, size) ||
         !aligned(a->dweight, size))

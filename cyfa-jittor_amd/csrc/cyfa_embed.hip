@@ -33,46 +33,53 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedParams p) {
     }
 }
 
-// Positions sorted by id. A workgroup owns the ids [v0, v0 + range) and reads
-// every id twice: it counts, wave by wave, how often each of its ids comes up
-// and how many ids lie below v0, then each wave places its stretch of the
-// positions behind those of the waves before it. Ids outside [0, V) and the
-// padding id count nowhere.
-//   offsets[v] .. offsets[v + 1]: where v's positions lie in order
+// Positions sorted by id, in the order of id mod G, then of id / G (G a power
+// of two, a workgroup for each remainder: the most frequent ids, which most
+// vocabularies number together, come to different workgroups). A workgroup reads
+// every id: it counts, wave by wave, how often each of its ids comes up and how
+// many ids belong to the workgroups before it, then each wave places its stretch
+// of the positions behind those of the waves before it. Ids outside [0, V) and
+// the padding id count nowhere.
+//   slot(v) = (v mod G) range + v / G;  offsets[slot] .. offsets[slot + 1]: where v's positions lie in order
 constexpr int ES_NT = 1024, ES_WAVES = ES_NT / 64, ES_U = 16;
 constexpr int ES_RANGE = 512;  // most ids of a workgroup: 35 KB of LDS
 
-__global__ __launch_bounds__(ES_NT) void embed_sort_kernel(EmbedParams p, int range) {
+__global__ __launch_bounds__(ES_NT) void embed_sort_kernel(EmbedParams p) {
     extern __shared__ int lds[];
+    const int range = p.range, shift = p.shift;
     int* cursor = lds;                      // [ES_WAVES][range]
     int* start = lds + ES_WAVES * range;    // [range]
     int* misc = start + range;              // [2 * ES_WAVES]
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const int v0 = blockIdx.x * range, mine = min(range, (int)p.V - v0);
+    const unsigned mine = blockIdx.x, groups = gridDim.x;
+    const unsigned padding = (unsigned)p.padding;  // -1: above every id
     const long long stretch = ((p.n + ES_NT - 1) / ES_NT) * 64;
     const long long first = wv * stretch, last = min(first + stretch, p.n);
-    // ES_U times 64 positions from i0: each lane's ids relative to v0, or -1 below
-    // the range, range or more above it; nowhere: INT_MAX. All loads in flight at
-    // once, those past the end of the last position.
-    const auto load = [&](long long i0, int (&local)[ES_U]) {
+    // The ids of ES_U times 64 positions from i0, all loads in flight at once; ~0: counts nowhere.
+    const auto load = [&](long long i0, unsigned (&ids)[ES_U]) {
         long long id[ES_U];
+        const long long* from = p.ids + i0;
+        const int left = (int)min(last - i0, (long long)64 * ES_U);  // at least 1
 #pragma unroll
-        for (int u = 0; u < ES_U; u++) id[u] = p.ids[min(i0 + 64 * u + lane, p.n - 1)];
+        for (int u = 0; u < ES_U; u++) id[u] = from[min(64 * u + lane, left - 1)];
 #pragma unroll
         for (int u = 0; u < ES_U; u++) {
-            const bool counts = i0 + 64 * u + lane < last && id[u] >= 0 && id[u] < p.V && id[u] != p.padding;
-            local[u] = counts ? max((int)id[u] - v0, -1) : 0x7fffffff;
+            const unsigned low = (unsigned)id[u];
+            const bool counts = (id[u] >> 32) == 0 && low < (unsigned)p.V && low != padding && 64 * u + lane < left;
+            ids[u] = counts ? low : ~0u;
         }
     };
     for (int i = tid; i < ES_WAVES * range; i += ES_NT) cursor[i] = 0;
     __syncthreads();
-    int below = 0, local[ES_U];
+    int below = 0;
+    unsigned ids[ES_U];
     for (long long i0 = first; i0 < last; i0 += 64 * ES_U) {
-        load(i0, local);
+        load(i0, ids);
 #pragma unroll
         for (int u = 0; u < ES_U; u++) {
-            below += local[u] < 0;
-            if ((unsigned)local[u] < (unsigned)mine) atomicAdd(&cursor[wv * range + local[u]], 1);
+            const unsigned group = ids[u] & (groups - 1);
+            below += group < mine && ids[u] != ~0u;
+            if (group == mine && ids[u] != ~0u) atomicAdd(&cursor[wv * range + (int)(ids[u] >> shift)], 1);
         }
     }
     for (int d = 32; d > 0; d >>= 1) below += __shfl_xor(below, d);
@@ -82,7 +89,7 @@ __global__ __launch_bounds__(ES_NT) void embed_sort_kernel(EmbedParams p, int ra
     for (int w = 0; w < ES_WAVES; w++) below += misc[w];
     // this id's positions of the waves before, and of the ids before (range <= ES_NT)
     int total = 0;
-    if (tid < mine)
+    if (tid < range)
         for (int w = 0; w < ES_WAVES; w++) {
             const int c = cursor[w * range + tid];
             cursor[w * range + tid] = total;
@@ -96,27 +103,34 @@ __global__ __launch_bounds__(ES_NT) void embed_sort_kernel(EmbedParams p, int ra
     if (lane == 63) misc[ES_WAVES + wv] = scan;
     __syncthreads();
     for (int w = 0; w < wv; w++) scan += misc[ES_WAVES + w];
-    if (tid < mine) {
+    if (tid < range) {
         start[tid] = below + scan - total;
-        p.offsets[v0 + tid] = below + scan - total;
-        if (v0 + tid == p.V - 1) p.offsets[p.V] = below + scan;
+        p.offsets[(long long)mine * range + tid] = below + scan - total;
+        if (mine == groups - 1 && tid == range - 1) p.offsets[(long long)groups * range] = below + scan;
     }
     __syncthreads();
     const bool once = stretch <= 64 * ES_U;  // the ids are still in registers
     for (long long i0 = first; i0 < last; i0 += 64 * ES_U) {
-        if (!once) load(i0, local);
+        if (!once) load(i0, ids);
 #pragma unroll
         for (int u = 0; u < ES_U; u++) {
-            uint64_t todo = __ballot((unsigned)local[u] < (unsigned)mine);
-            while (todo) {  // one id of these 64 positions after another
-                const int id = __builtin_amdgcn_readlane(local[u], __builtin_ctzll(todo));
-                const uint64_t same = __ballot(local[u] == id);
-                int* at = &cursor[wv * range + id];
-                const int c = *at;
-                if (local[u] == id) p.order[start[id] + c + __popcll(same & ((1ull << lane) - 1))] = (int)(i0 + 64 * u + lane);
-                *at = c + __popcll(same);  // (every lane, the same value)
-                todo &= ~same;
+            const bool here = (ids[u] & (groups - 1)) == mine && ids[u] != ~0u;
+            const int id = (int)(ids[u] >> shift);
+            uint64_t same = __ballot(here);
+            if (!same) continue;
+            for (int b = 1; b < range; b <<= 1) {  // the lanes with this lane's id, bit by bit
+                const uint64_t bit = __ballot((id & b) != 0);
+                same &= (id & b) ? bit : ~bit;
             }
+            // (LDS serves a wave's accesses in order: the next step reads what this one wrote)
+            if (here) {
+                int* at = &cursor[wv * range + id];
+                const int c = *at, rank = __popcll(same & ((1ull << lane) - 1)), count = __popcll(same);
+                p.order[start[id] + c + rank] = (int)(i0 + 64 * u + lane);
+                if (rank == count - 1) *at = c + count;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         }
     }
 }
@@ -148,17 +162,16 @@ __device__ __forceinline__ void add_rows(const EmbedParams& p, const E* dy, int 
 // written ending at the row's end, so that it overlaps the one before it
 // (the same values are stored twice), and rows below one vector go column by column.
 constexpr int EMBED_CHUNK = 32;
+constexpr int EMBED_GRID = 4096;  // workgroups, 8 of a compute unit at a time
 
 template <class E>
 __global__ __launch_bounds__(256) void embed_part_kernel(EmbedParams p) {
     constexpr int N = RowVec<E>::N;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int cols = (p.D + 64 * N - 1) / (64 * N), n = p.offsets[p.V];
-    const long long units = (long long)(n / EMBED_CHUNK) * cols, waves = (long long)gridDim.x * 4;
-    for (long long unit = (long long)blockIdx.x * 4 + wv; unit < units; unit += waves) {
-        const int c = (int)(unit / cols);
+    const int chunks = p.offsets[(long long)p.range << p.shift] / EMBED_CHUNK;
+    const int d = blockIdx.y * 64 * N + lane * N;
+    for (int c = blockIdx.x * 4 + wv; c < chunks; c += gridDim.x * 4) {
         const int s = c * EMBED_CHUNK, e = s + EMBED_CHUNK;
-        const int d = (int)(unit % cols) * 64 * N + lane * N;
         if (p.ids[p.order[s]] != p.ids[p.order[e - 1]] || d >= p.D) continue;  // not one id's whole chunk
         float* out = p.part + (long long)c * p.D;
         if (p.D >= N) {
@@ -167,8 +180,7 @@ __global__ __launch_bounds__(256) void embed_part_kernel(EmbedParams p) {
 #pragma unroll
             for (int i = 0; i < N; i++) acc[i] = 0.f;
             add_rows<E>(p, static_cast<const E*>(p.dy) + at, s, e, acc);
-#pragma unroll
-            for (int i = 0; i < N; i++) out[at + i] = acc[i];
+            __builtin_memcpy(out + at, acc, sizeof(acc));
         } else {
             for (int i = 0; i < p.D; i++) {
                 float a = 0.f;
@@ -183,16 +195,21 @@ template <class E>
 __global__ __launch_bounds__(256) void embed_grad_kernel(EmbedParams p) {
     constexpr int N = RowVec<E>::N;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int cols = (p.D + 64 * N - 1) / (64 * N);
-    const long long units = p.V * cols, waves = (long long)gridDim.x * 4;
-    for (long long unit = (long long)blockIdx.x * 4 + wv; unit < units; unit += waves) {
-        const long long v = unit / cols;
-        const int d = (int)(unit % cols) * 64 * N + lane * N;
-        const int s = p.offsets[v], e = p.offsets[v + 1];
+    const int d = blockIdx.y * 64 * N + lane * N, V = (int)p.V, waves = gridDim.x * 4;
+    const auto slot = [&](int v) {
+        v = min(v, V - 1);
+        return p.offsets + ((long long)(v & ((1 << p.shift) - 1)) * p.range + (v >> p.shift));
+    };
+    int v = blockIdx.x * 4 + wv;
+    int next_s = slot(v)[0], next_e = slot(v)[1];  // (the next row's positions are on their way while this one is added)
+    for (; v < V; v += waves) {
+        const int s = next_s, e = next_e;
+        next_s = slot(v + waves)[0];
+        next_e = slot(v + waves)[1];
         if (d >= p.D) continue;
         const int c0 = (s + EMBED_CHUNK - 1) / EMBED_CHUNK, c1 = e / EMBED_CHUNK;
         const bool parts = c0 < c1;  // whole chunks [c0, c1) of this id
-        E* out = static_cast<E*>(p.dweight) + v * p.D;
+        E* out = static_cast<E*>(p.dweight) + (long long)v * p.D;
         if (p.D >= N) {
             const int at = min(d, p.D - N);
             const E* dy = static_cast<const E*>(p.dy) + at;
@@ -239,23 +256,30 @@ void launch(const EmbedParams& p, bool grad, hipStream_t stream) {
         hipLaunchKernelGGL(embed_kernel<E>, dim3((unsigned)min((p.n + 3) / 4, 1ll << 20)), dim3(256), 0, stream, p);
         return;
     }
-    const int range = (int)min((p.V + 255) / 256, (long long)ES_RANGE);
-    hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)((p.V + range - 1) / range)), dim3(ES_NT),
-                       ((ES_WAVES + 1) * range + 2 * ES_WAVES) * sizeof(int), stream, p, range);
+    hipLaunchKernelGGL(embed_sort_kernel, dim3(1u << p.shift), dim3(ES_NT), ((ES_WAVES + 1) * p.range + 2 * ES_WAVES) * sizeof(int),
+                       stream, p);
+    // workgroups of four waves, a wave for 64 vectors of a row, the rows in turn
     const int cols = (p.D + 64 * RowVec<E>::N - 1) / (64 * RowVec<E>::N);
+    const auto grid = [&](long long rows) {
+        return dim3((unsigned)max(1ll, min((rows + 3) / 4, (long long)EMBED_GRID / cols)), cols);
+    };
     const long long chunks = p.n / EMBED_CHUNK;
-    if (chunks)
-        hipLaunchKernelGGL(embed_part_kernel<E>, dim3((unsigned)min((chunks * cols + 3) / 4, 1ll << 20)), dim3(256), 0, stream, p);
-    hipLaunchKernelGGL(embed_grad_kernel<E>, dim3((unsigned)min((p.V * cols + 3) / 4, 1ll << 20)), dim3(256), 0, stream, p);
+    if (chunks) hipLaunchKernelGGL(embed_part_kernel<E>, grid(chunks), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL(embed_grad_kernel<E>, grid(p.V), dim3(256), 0, stream, p);
 }
 
 }  // namespace
 
-// offsets int [V + 1], order int [n], part fp32 [n / chunk, D], each 256-byte aligned
+// offsets int [slots + 1], order int [n], part fp32 [n / chunk, D], each 256-byte aligned
 size_t embed_workspace(EmbedParams* p, long long n, long long V, int D, void* base) {
     const auto up = [](size_t b) { return (b + 255) / 256 * 256; };
-    const size_t offsets = up((size_t)(V + 1) * 4), order = up((size_t)n * 4);
+    int shift = 8;  // a workgroup of the sort for each of 256 compute units, more for many ids
+    while ((V + (1ll << shift) - 1) >> shift > ES_RANGE) shift++;
+    const int range = (int)((V + (1ll << shift) - 1) >> shift);
+    const size_t offsets = up((((size_t)range << shift) + 1) * 4), order = up((size_t)n * 4);
     if (p) {
+        p->shift = shift;
+        p->range = range;
         p->offsets = (int*)base;
         p->order = (int*)((char*)base + offsets);
         p->part = (float*)((char*)base + offsets + order);

@@ -573,10 +573,13 @@ struct EmbedParams {
     long long padding;           // id without a gradient; -1: none
     const void* dy;              // [n, D]
     void* dweight;               // [V, D]
+    int shift, range;            // the sort's workgroups 2^shift, ids of each; set with the workspace
     int *offsets, *order;        // embed_workspace
     float* part;
 };
-constexpr long long EMBED_MAX_V = 1ll << 26;  // 512 ids to a workgroup of 1024 threads, below 2^32 threads
+constexpr long long EMBED_MAX_N = 1ll << 30;
+constexpr int EMBED_MAX_D = 1 << 20;
+constexpr long long EMBED_MAX_V = 1ll << 26;  // 512 ids to a workgroup of the sort, 2^17 workgroups
 size_t embed_workspace(EmbedParams* p, long long n, long long V, int D, void* base);
 void launch_embed(const EmbedParams& p, int dtype, bool grad, hipStream_t stream);
 

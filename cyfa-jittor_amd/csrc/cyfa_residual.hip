@@ -50,6 +50,19 @@ struct Row {
         }
     }
 
+    // The same in two steps: the vectors, in flight while other work runs, then their elements.
+    __device__ __forceinline__ void fetch(const void* rows, long long offset, vec (&v)[J]) const {
+#pragma unroll
+        for (int j = 0; j < J; j++) __builtin_memcpy(&v[j], static_cast<const E*>(rows) + offset + at[j], sizeof(vec));
+    }
+
+    __device__ __forceinline__ void widen(const vec (&v)[J], float (&f)[J][VN]) const {
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int c = 0; c < VN; c++) f[j][c] = c < skip[j] ? 0.f : (float)v[j][c];
+    }
+
     template <class X>
     __device__ __forceinline__ void store(X* row, const float (&v)[J][VN]) const {
 #pragma unroll
@@ -157,15 +170,31 @@ __global__ __launch_bounds__(256) void residual_grad_kernel(ResidualParams p) {
     cols.load(p.weight, w);
     if (p.post) cols.load(p.post, pw);
     const long long end = min((long long)(blockIdx.x + 1) * p.rows_wg, p.rows);
-    for (long long r = (long long)blockIdx.x * p.rows_wg + threadIdx.x / T; r < end; r += RW) {
+    const long long first = (long long)blockIdx.x * p.rows_wg + threadIdx.x / T;
+    // the next row's operands are in flight while this one's are worked on
+    typename Row<E, VN, T, J>::vec xv[J], yv[J], gv[J], ev[J], dv[J];
+    float r1n, r2n;
+    const auto fetch = [&](long long r) {
+        const long long o = min(r, p.rows - 1) * p.D;
+        cols.fetch(p.x, o, xv);
+        cols.fetch(p.y, o, yv);
+        if (p.gate) cols.fetch(p.gate, o, gv);
+        if (p.d_h) cols.fetch(p.d_h, o, ev);
+        if (p.d_s) cols.fetch(p.d_s, o, dv);
+        r1n = p.stats[2 * min(r, p.rows - 1)];
+        r2n = p.stats[2 * min(r, p.rows - 1) + 1];
+    };
+    fetch(first);
+    for (long long r = first; r < end; r += RW) {
         const long long o = r * p.D;
         float s[J][VN], y[J][VN], g[J][VN], e[J][VN], d[J][VN];
-        cols.load(static_cast<const E*>(p.x) + o, s);
-        cols.load(static_cast<const E*>(p.y) + o, y);
-        if (p.gate) cols.load(static_cast<const E*>(p.gate) + o, g);
-        if (p.d_h) cols.load(static_cast<const E*>(p.d_h) + o, e);
-        if (p.d_s) cols.load(static_cast<const E*>(p.d_s) + o, d);
-        const float r1 = p.post ? p.stats[2 * r] : 1.f, r2 = p.stats[2 * r + 1];
+        cols.widen(xv, s);
+        cols.widen(yv, y);
+        if (p.gate) cols.widen(gv, g);
+        if (p.d_h) cols.widen(ev, e);
+        if (p.d_s) cols.widen(dv, d);
+        const float r1 = p.post ? r1n : 1.f, r2 = r2n;
+        if (r + RW < end) fetch(r + RW);
         float sum[3] = {0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < J; j++)

@@ -949,9 +949,10 @@ RESIDUAL_MAX_D = 8192
 def _lm_call(what, args, dtype, grad, dev):
     """lib.<what>(args, dtype, grad, stream) on ``dev``'s current stream, with
     that device current (a launch takes its code from the current device)."""
-    fn = getattr(load_library(), what)
-    if dev.index == torch.cuda.current_device():
-        rc = fn(ctypes.byref(args), LM_DTYPES[dtype], grad, stream_handle(dev))
+    fn = getattr(_lib or load_library(), what)
+    index = dev.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(ctypes.byref(args), LM_DTYPES[dtype], grad, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
             rc = fn(ctypes.byref(args), LM_DTYPES[dtype], grad, stream_handle(dev))
@@ -960,37 +961,34 @@ def _lm_call(what, args, dtype, grad, dev):
 
 
 def logit_rows(logits):
-    """(rows, arguments of CyfaLogprobArgs, the tensor they describe) of logits
-    [..., V]: the tensor itself where its rows are contiguous and one or two
-    strides apart, else a copy."""
+    """(rows, inner, outer_stride, row_stride, V, data pointer) of logits
+    [..., V] as CyfaLogprobArgs begins, and the tensor they describe: the tensor
+    itself where its rows are contiguous and one or two strides apart, else a copy."""
     V = logits.shape[-1]
+    rows = logits.numel() // V
+    if rows == 0 or logits.is_contiguous():
+        return (rows, max(rows, 1), 0, V, V, logits.data_ptr()), logits
     if logits.stride(-1) != 1 and V > 1:
         logits = logits.contiguous()
-    if logits.dim() == 1 or logits.numel() == 0:
-        inner, outer_stride, row_stride = 1, 0, 0
-    elif logits.dim() == 2:
-        inner, outer_stride, row_stride = logits.shape[0], 0, logits.stride(0)
-    else:
-        logits = logits.reshape(-1, *logits.shape[-2:])
-        inner, outer_stride, row_stride = logits.shape[1], logits.stride(0), logits.stride(1)
-    rows = logits.numel() // V
-    return rows, dict(rows=rows, inner=max(inner, 1), outer_stride=outer_stride, row_stride=row_stride, V=V,
-                      x=logits.data_ptr()), logits
+    if logits.dim() <= 2:
+        return (rows, rows, 0, logits.stride(0), V, logits.data_ptr()), logits
+    logits = logits.reshape(-1, *logits.shape[-2:])
+    return (rows, logits.shape[1], logits.stride(0), logits.stride(1), V, logits.data_ptr()), logits
 
 
 def logprobs(logits, tokens, k, ignore, stats=False):
     """(logprob, entropy, top_logprobs or None, top_ids or None, stats or None)
     of logits [..., V] for int64 contiguous tokens [...]."""
     dev = require_device(logits, tokens)
-    rows, fields, logits = logit_rows(logits)
+    fields, logits = logit_rows(logits)
     shape = tokens.shape
     logprob, entropy = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(2))
     top = ids = None
     if k:
         top = torch.empty(shape + (k,), dtype=torch.float32, device=dev)
         ids = torch.empty(shape + (k,), dtype=torch.int64, device=dev)
-    st = torch.empty(rows, 2, dtype=torch.float32, device=dev) if stats else None
-    args = CyfaLogprobArgs(**fields, tokens=tokens.data_ptr(), ignore=ignore, logprob=logprob.data_ptr(),
+    st = torch.empty(fields[0], 2, dtype=torch.float32, device=dev) if stats else None
+    args = CyfaLogprobArgs(*fields, tokens=tokens.data_ptr(), ignore=ignore, logprob=logprob.data_ptr(),
                            entropy=entropy.data_ptr(), stats=ptr(st), k=k, top_logprobs=ptr(top), top_ids=ptr(ids))
     _lm_call("cyfa_logprobs", args, logits.dtype, 0, dev)
     return logprob, entropy, top, ids, st
@@ -999,10 +997,10 @@ def logprobs(logits, tokens, k, ignore, stats=False):
 def logprobs_grad(logits, tokens, k, ignore, stats, entropy, ids, d_logprob, d_entropy, d_top):
     """The gradient of logits from the cotangents (fp32 contiguous or None) of
     logprobs' first three results."""
-    dev = require_device(logits, tokens, d_logprob, d_entropy, d_top)
+    dev = logits.device
     dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-    _, fields, logits = logit_rows(logits)
-    args = CyfaLogprobArgs(**fields, tokens=tokens.data_ptr(), ignore=ignore, stats=stats.data_ptr(),
+    fields, logits = logit_rows(logits)
+    args = CyfaLogprobArgs(*fields, tokens=tokens.data_ptr(), ignore=ignore, stats=stats.data_ptr(),
                            entropy=entropy.data_ptr(), k=k, top_ids=ptr(ids), d_logprob=ptr(d_logprob),
                            d_entropy=ptr(d_entropy), d_top=ptr(d_top), dx=dx.data_ptr())
     _lm_call("cyfa_logprobs", args, dx.dtype, 1, dev)
@@ -1013,11 +1011,12 @@ def token_loss(logits, labels, ignore):
     """(loss, what token_loss_grad needs): the mean of -logprob over the labels
     (int64, contiguous) that are not ``ignore``."""
     dev = require_device(logits, labels)
-    rows, fields, logits = logit_rows(logits)
+    fields, logits = logit_rows(logits)
+    rows = fields[0]
     loss = torch.empty((), dtype=torch.float32, device=dev)
     kept = torch.empty(3 * rows + 1, dtype=torch.float32, device=dev)  # stats, logprob, count
     at = kept.data_ptr()
-    args = CyfaLogprobArgs(**fields, tokens=labels.data_ptr(), ignore=ignore, stats=at, logprob=at + 8 * rows,
+    args = CyfaLogprobArgs(*fields, tokens=labels.data_ptr(), ignore=ignore, stats=at, logprob=at + 8 * rows,
                            loss=loss.data_ptr(), count=at + 12 * rows)
     _lm_call("cyfa_logprobs", args, logits.dtype, 0, dev)
     return loss, kept
@@ -1025,11 +1024,11 @@ def token_loss(logits, labels, ignore):
 
 def token_loss_grad(logits, labels, ignore, kept, d_loss):
     """The gradient of logits from the loss's cotangent (fp32, on the device)."""
-    dev = require_device(logits, labels, d_loss)
+    dev = logits.device
     dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-    rows, fields, logits = logit_rows(logits)
-    at = kept.data_ptr()
-    args = CyfaLogprobArgs(**fields, tokens=labels.data_ptr(), ignore=ignore, stats=at, count=at + 12 * rows,
+    fields, logits = logit_rows(logits)
+    rows, at = fields[0], kept.data_ptr()
+    args = CyfaLogprobArgs(*fields, tokens=labels.data_ptr(), ignore=ignore, stats=at, count=at + 12 * rows,
                            d_loss=d_loss.data_ptr(), dx=dx.data_ptr())
     _lm_call("cyfa_logprobs", args, dx.dtype, 1, dev)
     return dx
@@ -1048,7 +1047,7 @@ def embed(ids, weight, scale):
 
 def embed_grad(ids, V, dy, scale, padding):
     """The gradient [V, D] of embed's weight from dy [..., D], contiguous."""
-    dev = require_device(ids, dy)
+    dev = dy.device
     D = dy.shape[-1]
     n = ids.numel()
     dw = torch.empty(V, D, dtype=dy.dtype, device=dev)
@@ -1077,7 +1076,7 @@ def residual_norm(x, y, weight, post, gate, scale, eps, stats=False):
 def residual_norm_grad(x, y, weight, post, gate, scale, eps, stats, d_s, d_h, needed):
     """Gradients (dx, dy, dweight, dpost, dgate) of residual_norm's results from
     their cotangents (contiguous, or None), None where ``needed`` is false."""
-    dev = require_device(x, y, weight, post, gate, d_s, d_h)
+    dev = x.device
     D = x.shape[-1]
     rows = x.numel() // D
     plain = post is None and gate is None and scale == 1.0  # dy is dx

@@ -67,8 +67,12 @@ def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
 
 def _recorded(*cotangents):
     """Whether this backward pass is itself recorded, or batched (vmap)."""
-    return (torch.is_grad_enabled() or torch._C._functorch.peek_interpreter_stack() is not None
-            or any(t is not None and torch._C._functorch.is_legacy_batchedtensor(t) for t in cotangents))
+    if torch.is_grad_enabled() or torch._C._functorch.peek_interpreter_stack() is not None:
+        return True
+    for t in cotangents:
+        if t is not None and torch._C._functorch.is_legacy_batchedtensor(t):
+            return True
+    return False
 
 
 def _torch_backward(fn, inputs, needed, cotangents):

@@ -619,7 +619,7 @@ int cyfa_logprobs(const CyfaLogprobArgs *args, int dtype, int grad, void *hip_st
  * dweight[v] = scale sum of dy[i] over ids[i] = v, i in order (grad 1), in f32
  * and rounded once; weight, out, dy, dweight CYFA_DTYPE_BF16, _F32 or _F16,
  * contiguous, any alignment. An id outside [0, V) gives a row of NaN and has no
- * gradient, nor has the id padding (-1: none). n < 2^31, V <= 2^26. Replaces
+ * gradient, nor has the id padding (-1: none). n <= 2^30, V <= 2^26, D <= 2^20. Replaces
  * nn.Embedding (models/cyfa/modeling_cyfa.py:59-66) and its adjoint. */
 typedef struct CyfaEmbedArgs {
     long long n, V;
