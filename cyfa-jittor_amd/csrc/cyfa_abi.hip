@@ -754,6 +754,11 @@ int cyfa_norm_train(const CyfaNormTrainArgs* a, int dtype, int grad, void* hip_s
     return check_launch(what);
 }
 
+size_t cyfa_logprobs_workspace_bytes(long long rows, int V, int k, int dtype) {
+    if (rows < 0 || V <= 0 || V > cyfa::LOGPROBS_MAX_V || k < 0 || k > CYFA_LOGPROBS_MAX_TOP) return 0;
+    return cyfa::logprobs_workspace_bytes(rows, V, k, dtype == CYFA_DTYPE_F32 ? 4 : 2);
+}
+
 int cyfa_logprobs(const CyfaLogprobArgs* a, int dtype, int grad, void* hip_stream) {
     const char* what = "cyfa_logprobs";
     if (!a) return fail(CYFA_ERR_VALUE, "%s: null args", what);
@@ -780,6 +785,10 @@ int cyfa_logprobs(const CyfaLogprobArgs* a, int dtype, int grad, void* hip_strea
     }
     if (!grad && (a->loss == nullptr) != (a->count == nullptr)) return fail(CYFA_ERR_VALUE, "%s: loss and count, both or none", what);
     if (a->rows == 0 && (grad || !a->loss)) return CYFA_OK;
+    const size_t need = grad ? 0 : cyfa::logprobs_workspace_bytes(a->rows, a->V, a->k, size);
+    if (need && (!a->workspace || a->workspace_bytes < need))
+        return fail(CYFA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
+    if (need && !aligned(a->workspace, 8)) return fail(CYFA_ERR_ALIGN, "%s: workspace needs 8-byte alignment", what);
     cyfa::LogprobParams p{};
     p.rows = a->rows;
     p.inner = a->inner;
@@ -802,6 +811,7 @@ int cyfa_logprobs(const CyfaLogprobArgs* a, int dtype, int grad, void* hip_strea
     p.d_top = a->d_top;
     p.d_loss = a->d_loss;
     p.dx = a->dx;
+    p.parts = (float*)a->workspace;
     cyfa::launch_logprobs(p, dtype, grad != 0, (hipStream_t)hip_stream);
     return check_launch(what);
 }

@@ -556,7 +556,13 @@ struct LogprobParams {
     const float *d_logprob, *d_entropy, *d_top;  // nullable [rows], [rows], [rows, k]
     const float* d_loss;         // nullable [1], in place of d_logprob
     void* dx;                    // [rows, V]
+    // rows shared out to several workgroups (logprobs_workspace_bytes)
+    float* parts;                // [rows, parts, 3]
+    unsigned long long* part_keys;  // [rows, parts, k], set by the launcher
+    int part;                    // columns of a part, set by the launcher
 };
+size_t logprobs_workspace_bytes(long long rows, int V, int k, int size);
+constexpr int LOGPROBS_MAX_TOP = 32;
 constexpr int LOGPROBS_MAX_V = 1 << 28;  // column indexes and their vectors stay in 32 bits
 constexpr int LOGPROBS_MAX_GRID = 1 << 20;  // rows of a launch taken by workgroups of their own
 void launch_logprobs(const LogprobParams& p, int dtype, bool grad, hipStream_t stream);
@@ -598,6 +604,7 @@ struct ResidualParams {
     float *dweight, *dpost;      // nullable [D]
     float* part;                 // residual_workspace_bytes
     long long rows_wg;           // set by the launcher
+    float inverse_d;
 };
 constexpr int RESIDUAL_MAX_D = 8192;
 size_t residual_workspace_bytes(long long rows, int D);

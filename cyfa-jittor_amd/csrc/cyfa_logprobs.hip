@@ -18,6 +18,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;
 constexpr int LP_CAP = 1024;            // candidates for the alternatives held in LDS
+constexpr int LP_PARTS = 16;             // most parts of a row
 constexpr int LP_NV = 4;                // vectors of a thread in a tile of a row
 
 // The order of the alternatives as an unsigned key: larger values first (a NaN
@@ -64,15 +65,40 @@ __device__ __forceinline__ const E* row_of(const LogprobParams& p, long long r) 
 __device__ __forceinline__ float kth_largest(float x, int k) {
     const uint32_t mine = (value_key(x) & ~63u) | (uint32_t)(threadIdx.x & 63);
     int rank = 0;
-#pragma unroll 16
+#pragma unroll 8
     for (int i = 0; i < 64; i++) rank += (uint32_t)__builtin_amdgcn_readlane((int)mine, i) > mine;
     return -wave_max(rank < k ? -x : -INFINITY);
 }
 
+// a += b of another set of elements.
+__device__ __forceinline__ void join(RowSums& a, RowSums b) {
+    const float m = fmaxf(a.m, b.m);
+    rescale(a, m);
+    rescale(b, m);
+    a.s += b.s;
+    a.s1 += b.s1;
+}
+
+// Row r's results but its alternatives.
+__device__ __forceinline__ void put_row(const LogprobParams& p, long long r, const RowSums& a, float ls, float xt, bool ignored) {
+    p.logprob[r] = ignored ? 0.f : (xt - a.m) - ls;
+    if (p.entropy) p.entropy[r] = ls - kLn2 * (a.s1 / a.s);
+    if (p.stats) {
+        p.stats[2 * r] = a.m;
+        p.stats[2 * r + 1] = ls * kLog2e;
+    }
+}
+
+__device__ __forceinline__ void put_top(const LogprobParams& p, long long r, int rank, uint64_t key, const RowSums& a, float ls) {
+    p.top_ids[r * p.k + rank] = 0xffffffffu - (uint32_t)key;
+    p.top_logprobs[r * p.k + rank] = (key_value(key) - a.m) - ls;
+}
+
 // One workgroup of NT threads to a row (rows beyond the grid in turn), tiles of
 // NT * LP_NV vectors of it in registers: a row of one tile is read from memory
-// once, also for its alternatives.
-template <class E, int NT, bool TOP>
+// once, also for its alternatives. With PARTS, to part blockIdx.y of a row, whose
+// sums and alternatives go to the workspace for logprobs_join_kernel.
+template <class E, int NT, bool TOP, bool PARTS>
 __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobParams p) {
     constexpr int N = RowVec<E>::N, W = NT / 64;
     __shared__ RowSums red[W];
@@ -82,34 +108,33 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobParams p) {
     __shared__ float thr_s;
     __shared__ int count_s;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const int nvec = p.V / N, tail = p.V - nvec * N;
+    const int c0 = PARTS ? blockIdx.y * p.part : 0, cols = PARTS ? min(p.part, p.V - c0) : p.V;
+    const int nvec = cols / N, tail = cols - nvec * N;
     for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        const E* x = row_of<E>(p, r);
+        const E* x = row_of<E>(p, r) + c0;
         const long long t = p.tokens[r];
         const bool ignored = t == p.ignore;
         if (ignored && !TOP && !p.entropy) {  // (the loss: nothing of this row counts)
-            if (tid == 0) p.logprob[r] = 0.f;
+            if (!PARTS && tid == 0) p.logprob[r] = 0.f;
             continue;
         }
-        const bool inside = t >= 0 && t < p.V;
-        const float xt = inside ? (float)x[t] : __builtin_nanf("");
+        const float xt = !PARTS && t >= 0 && t < p.V ? (float)x[t] : __builtin_nanf("");
         const float last = tid < tail ? (float)x[nvec * N + tid] : -INFINITY;
         typename RowVec<E>::type v[LP_NV];
+        float top[LP_NV];  // the largest element of each
         // Vectors past the end are read as the last one and dropped: no branch
         // among the loads, at which the compiler would wait for those in flight.
         const auto load_tile = [&](int v0) {
 #pragma unroll
             for (int j = 0; j < LP_NV; j++) v[j] = load_row(x + (size_t)min(v0 + j * NT + tid, nvec - 1) * N);
         };
-        // f(element, index) of this thread's elements in tile v0
-        const auto each = [&](int v0, auto&& f) {
+        const auto largest = [&](int v0) {
 #pragma unroll
             for (int j = 0; j < LP_NV; j++) {
-                const int i = v0 + j * NT + tid;
-                if (i < nvec) {
+                top[j] = -INFINITY;
+                if (v0 + j * NT + tid < nvec)
 #pragma unroll
-                    for (int c = 0; c < N; c++) f((float)v[j][c], i * N + c);
-                }
+                    for (int c = 0; c < N; c++) top[j] = fmaxf(top[j], (float)v[j][c]);
             }
         };
         RowSums a = {kLowest, 0.f, 0.f};
@@ -121,9 +146,15 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobParams p) {
         };
         for (int v0 = 0; v0 < nvec; v0 += NT * LP_NV) {
             load_tile(v0);
-            each(v0, [&](float e, int) { best = fmaxf(best, e); });
+            largest(v0);
+#pragma unroll
+            for (int j = 0; j < LP_NV; j++) best = fmaxf(best, top[j]);
             rescale(a, fmaxf(a.m, best));
-            each(v0, [&](float e, int) { add(e); });
+#pragma unroll
+            for (int j = 0; j < LP_NV; j++)
+                if (v0 + j * NT + tid < nvec)
+#pragma unroll
+                    for (int c = 0; c < N; c++) add((float)v[j][c]);
         }
         rescale(a, fmaxf(a.m, best));
         if (tid < tail) add(last);
@@ -136,37 +167,42 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobParams p) {
             if (TOP) best_s[wv][lane] = best;
             __syncthreads();
             a = red[0];
-#pragma unroll
-            for (int w = 1; w < W; w++) {
-                RowSums b = red[w];
-                const float mm = fmaxf(a.m, b.m);
-                rescale(a, mm);
-                rescale(b, mm);
-                a.s += b.s;
-                a.s1 += b.s1;
-            }
+#pragma unroll 3
+            for (int w = 1; w < W; w++) join(a, red[w]);
         }
         const float ls = logf(a.s);
+        const long long at = r * gridDim.y + blockIdx.y;
         if (tid == 0) {
-            p.logprob[r] = ignored ? 0.f : (xt - a.m) - ls;
-            if (p.entropy) p.entropy[r] = ls - kLn2 * (a.s1 / a.s);
-            if (p.stats) {
-                p.stats[2 * r] = a.m;
-                p.stats[2 * r + 1] = ls * kLog2e;
-            }
+            if (PARTS)
+                reinterpret_cast<RowSums*>(p.parts)[at] = a;
+            else
+                put_row(p, r, a, ls, xt, ignored);
         }
         if (TOP) {
             const auto put = [&](int rank, uint64_t key) {
-                p.top_ids[r * p.k + rank] = 0xffffffffu - (uint32_t)key;
-                p.top_logprobs[r * p.k + rank] = (key_value(key) - a.m) - ls;
+                if (PARTS)
+                    p.part_keys[at * p.k + rank] = key;
+                else
+                    put_top(p, r, rank, key, a, ls);
             };
+            // f(element, column) of this thread's elements that reach ``from`` (and NaN, with from -inf)
             const bool one_tile = nvec <= NT * LP_NV;
-            const auto each_of_row = [&](auto&& f) {
+            const auto each = [&](float from, auto&& f) {
                 for (int v0 = 0; v0 < nvec; v0 += NT * LP_NV) {
-                    if (!one_tile) load_tile(v0);
-                    each(v0, f);
+                    if (!one_tile) {
+                        load_tile(v0);
+                        largest(v0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < LP_NV; j++) {
+                        const int i = v0 + j * NT + tid;
+                        if (i < nvec && top[j] >= from) {
+#pragma unroll
+                            for (int c = 0; c < N; c++) f((float)v[j][c], c0 + i * N + c);
+                        }
+                    }
                 }
-                if (tid < tail) f(last, nvec * N + tid);
+                if (tid < tail) f(last, c0 + nvec * N + tid);
             };
             // A threshold that k elements reach and seldom many more: the k-th
             // largest of the largest elements of 64 sets of threads. The
@@ -187,7 +223,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobParams p) {
                     const int at = atomicAdd(&count_s, 1);
                     if (at < LP_CAP) cand[at] = order_key(e, i);
                 };
-                each_of_row([&](float e, int i) {
+                each(thr, [&](float e, int i) {
                     if (e >= thr) hold(e, i);
                 });
                 __syncthreads();
@@ -196,8 +232,8 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobParams p) {
                     __syncthreads();
                     if (tid == 0) count_s = 0;
                     __syncthreads();
-                    each_of_row([&](float e, int i) {
-                        if (e > thr || (e == thr && i < LP_CAP / 2)) hold(e, i);
+                    each(thr, [&](float e, int i) {
+                        if (e > thr || (e == thr && i < c0 + LP_CAP / 2)) hold(e, i);
                     });
                     __syncthreads();
                     n = count_s;
@@ -208,6 +244,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobParams p) {
                 for (int c = tid; c < n; c += NT) {
                     const uint64_t key = cand[c];
                     int rank = 0;
+#pragma unroll 8
                     for (int i = 0; i < n; i++) rank += cand[i] > key;
                     if (rank < p.k) put(rank, key);
                 }
@@ -215,7 +252,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobParams p) {
                 uint64_t below = ~0ull;
                 for (int rank = 0; rank < p.k; rank++) {
                     uint64_t next = 0;
-                    each_of_row([&](float e, int i) {
+                    each(-INFINITY, [&](float e, int i) {
                         const uint64_t key = order_key(e, i);
                         if (key < below && key > next) next = key;
                     });
@@ -233,6 +270,37 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobParams p) {
             }
         }
         if (W > 1 || TOP) __syncthreads();  // the shared arrays are free for the next row
+    }
+}
+
+// A row's results from those of its ``parts`` parts, a workgroup to a row.
+template <class E>
+__global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobParams p, int parts) {
+    __shared__ uint64_t keys[LP_PARTS * LOGPROBS_MAX_TOP];
+    for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const long long t = p.tokens[r];
+        const bool ignored = t == p.ignore;
+        if (ignored && p.k == 0 && !p.entropy) {
+            if (threadIdx.x == 0) p.logprob[r] = 0.f;
+            continue;
+        }
+        const RowSums* part = reinterpret_cast<const RowSums*>(p.parts) + r * parts;
+        RowSums a = part[0];
+        for (int i = 1; i < parts; i++) join(a, part[i]);
+        const float ls = logf(a.s);
+        if (threadIdx.x == 0) put_row(p, r, a, ls, t >= 0 && t < p.V ? (float)row_of<E>(p, r)[t] : __builtin_nanf(""), ignored);
+        if (p.k == 0) continue;
+        const int n = parts * p.k;
+        for (int i = threadIdx.x; i < n; i += 256) keys[i] = p.part_keys[r * n + i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < n; c += 256) {
+            const uint64_t key = keys[c];
+            int rank = 0;
+#pragma unroll 8
+            for (int i = 0; i < n; i++) rank += keys[i] > key;
+            if (rank < p.k) put_top(p, r, rank, key, a, ls);
+        }
+        __syncthreads();
     }
 }
 
@@ -352,13 +420,34 @@ __global__ __launch_bounds__(LG_NT) void logprobs_grad_kernel(LogprobParams p, i
     }
 }
 
+// Parts of a row, a workgroup each: those of its tiles, where the rows leave
+// compute units idle and have more than one.
+int row_parts(long long rows, int V, int size) {
+    const long long tile = 1024 * LP_NV * (16 / size), tiles = (V + tile - 1) / tile;
+    return (int)max(1ll, min(min(tiles, 256 / rows), (long long)LP_PARTS));
+}
+
 template <class E, int NT>
 void launch_rows(const LogprobParams& p, hipStream_t stream) {
     const dim3 grid((unsigned)min(p.rows, (long long)LOGPROBS_MAX_GRID));
     if (p.k > 0)
-        hipLaunchKernelGGL((logprobs_kernel<E, NT, true>), grid, dim3(NT), 0, stream, p);
+        hipLaunchKernelGGL((logprobs_kernel<E, NT, true, false>), grid, dim3(NT), 0, stream, p);
     else
-        hipLaunchKernelGGL((logprobs_kernel<E, NT, false>), grid, dim3(NT), 0, stream, p);
+        hipLaunchKernelGGL((logprobs_kernel<E, NT, false, false>), grid, dim3(NT), 0, stream, p);
+}
+
+template <class E>
+void launch_parts(LogprobParams p, int parts, hipStream_t stream) {
+    constexpr int N = RowVec<E>::N;
+    p.part = ((p.V + parts - 1) / parts + N - 1) / N * N;
+    parts = (p.V + p.part - 1) / p.part;
+    p.part_keys = (unsigned long long*)(p.parts + ((p.rows * parts * 3 + 1) / 2 * 2));
+    const dim3 grid((unsigned)p.rows, parts);
+    if (p.k > 0)
+        hipLaunchKernelGGL((logprobs_kernel<E, 1024, true, true>), grid, dim3(1024), 0, stream, p);
+    else
+        hipLaunchKernelGGL((logprobs_kernel<E, 1024, false, true>), grid, dim3(1024), 0, stream, p);
+    hipLaunchKernelGGL(logprobs_join_kernel<E>, dim3((unsigned)p.rows), dim3(256), 0, stream, p, parts);
 }
 
 template <class E>
@@ -376,12 +465,21 @@ void launch(const LogprobParams& p, bool grad, hipStream_t stream) {
         launch_rows<E, 64>(p, stream);
     } else if (p.V <= 256 * LP_NV * N || p.rows >= 512) {
         launch_rows<E, 256>(p, stream);
+    } else if (const int parts = row_parts(p.rows, p.V, sizeof(E)); parts > 1) {
+        launch_parts<E>(p, parts, stream);
     } else {
         launch_rows<E, 1024>(p, stream);
     }
 }
 
 }  // namespace
+
+// Bytes of the parts' sums and keys, 0 where rows are not shared out.
+size_t logprobs_workspace_bytes(long long rows, int V, int k, int size) {
+    if (rows <= 0 || rows >= 512) return 0;
+    const int parts = row_parts(rows, V, size);
+    return parts > 1 ? (size_t)((rows * parts * 3 + 1) / 2 * 2) * 4 + (size_t)rows * parts * k * 8 : 0;
+}
 
 void launch_logprobs(const LogprobParams& p, int dtype, bool grad, hipStream_t stream) {
     if (p.rows == 0)

@@ -28,8 +28,9 @@ struct Row {
     typedef E vec __attribute__((ext_vector_type(VN)));
 
     int at[J], skip[J];  // column of the vector's first element; elements that do not count
+    bool full;           // all count, in every thread
 
-    __device__ __forceinline__ Row(int D, int t) {
+    __device__ __forceinline__ Row(int D, int t) : full(D == J * T * VN) {
 #pragma unroll
         for (int j = 0; j < J; j++) {
             const int c = (t + j * T) * VN;
@@ -46,8 +47,17 @@ struct Row {
             xvec e;
             __builtin_memcpy(&e, row + at[j], sizeof(e));
 #pragma unroll
-            for (int c = 0; c < VN; c++) v[j][c] = c < skip[j] ? 0.f : (float)e[c];
+            for (int c = 0; c < VN; c++) v[j][c] = (float)e[c];
         }
+        mask(v);
+    }
+
+    __device__ __forceinline__ void mask(float (&v)[J][VN]) const {
+        if (full) return;
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int c = 0; c < VN; c++) v[j][c] = c < skip[j] ? 0.f : v[j][c];
     }
 
     // The same in two steps: the vectors, in flight while other work runs, then their elements.
@@ -60,7 +70,8 @@ struct Row {
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
-            for (int c = 0; c < VN; c++) f[j][c] = c < skip[j] ? 0.f : (float)v[j][c];
+            for (int c = 0; c < VN; c++) f[j][c] = (float)v[j][c];
+        mask(f);
     }
 
     template <class X>
@@ -95,13 +106,20 @@ __device__ __forceinline__ void row_sums(float (&v)[K], float (*red)[K]) {
         for (int k = 0; k < K; k++) red[wv][k] = v[k];
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; k++) v[k] = (red[0][k] + red[1][k]) + (red[2][k] + red[3][k]);
+    for (int k = 0; k < K; k++) {
+        v[k] = 0.f;
+#pragma unroll
+        for (int w = 0; w < T / 64; w += 4) v[k] += (red[w][k] + red[w + 1][k]) + (red[w + 2][k] + red[w + 3][k]);
+    }
 }
 
+// Threads of a workgroup whose rows take T each.
+constexpr int block_of(int T) { return T > 256 ? T : 256; }
+
 template <class E, int VN, int T, int J>
-__global__ __launch_bounds__(256) void residual_norm_kernel(ResidualParams p) {
-    __shared__ float red[4][1];
-    constexpr int RW = 256 / T;
+__global__ __launch_bounds__(block_of(T)) void residual_norm_kernel(ResidualParams p) {
+    constexpr int RW = block_of(T) / T;
+    __shared__ float red[block_of(T) / 64][1];
     const Row<E, VN, T, J> cols(p.D, threadIdx.x % T);
     for (long long r = (long long)blockIdx.x * RW + threadIdx.x / T; r < p.rows; r += (long long)gridDim.x * RW) {
         const long long o = r * p.D;
@@ -117,7 +135,7 @@ __global__ __launch_bounds__(256) void residual_norm_kernel(ResidualParams p) {
 #pragma unroll
                 for (int c = 0; c < VN; c++) ss[0] = fmaf(b[j][c], b[j][c], ss[0]);
             row_sums<T>(ss, red);
-            const float r1 = rsqrtf(ss[0] / (float)p.D + p.eps);
+            const float r1 = rsqrtf(ss[0] * p.inverse_d + p.eps);
             if (p.stats && threadIdx.x % T == 0) p.stats[2 * r] = r1;
 #pragma unroll
             for (int j = 0; j < J; j++)
@@ -142,7 +160,7 @@ __global__ __launch_bounds__(256) void residual_norm_kernel(ResidualParams p) {
             }
         cols.store(static_cast<E*>(p.s) + o, s);
         row_sums<T>(ss, red);
-        const float r2 = rsqrtf(ss[0] / (float)p.D + p.eps);
+        const float r2 = rsqrtf(ss[0] * p.inverse_d + p.eps);
         if (p.stats && threadIdx.x % T == 0) p.stats[2 * r + 1] = r2;
         cols.load(p.weight, b);
 #pragma unroll
@@ -154,59 +172,80 @@ __global__ __launch_bounds__(256) void residual_norm_kernel(ResidualParams p) {
 }
 
 // Workgroups of p.rows_wg rows; each leaves its sums for dweight and dpost in
-// part [workgroup][2][D], which residual_sum_kernel adds.
-template <class E, int VN, int T, int J>
-__global__ __launch_bounds__(256) void residual_grad_kernel(ResidualParams p) {
-    constexpr int RW = 256 / T, C = J * T * VN;
-    __shared__ float red[4][3];
-    __shared__ float sums[RW > 1 ? RW : 1][RW > 1 ? C : 1];
+// part [workgroup][2][D], which residual_sum_kernel adds. The weights stay in
+// LDS (rows of a wave) or in registers; two waves per SIMD have to fit, so that
+// one's loads cover the other's arithmetic.
+template <class E, int VN, int T, int J, bool POST, bool GATE>
+__global__ __launch_bounds__(block_of(T), 2) void residual_grad_kernel(ResidualParams p) {
+    constexpr int RW = block_of(T) / T, C = J * T * VN;
+    __shared__ float red[block_of(T) / 64][3];
+    __shared__ __align__(16) float sums[RW > 1 ? RW : 1][RW > 1 ? C : 1];
+    __shared__ __align__(16) float weights[2][RW > 1 ? C : 1];
     const int t = threadIdx.x % T;
     const Row<E, VN, T, J> cols(p.D, t);
-    float dw[J][VN], dp[J][VN], w[J][VN], pw[J][VN];
+    float dw[J][VN], dp[J][VN], kept[2][J][VN];
 #pragma unroll
     for (int j = 0; j < J; j++)
 #pragma unroll
         for (int c = 0; c < VN; c++) dw[j][c] = dp[j][c] = 0.f;
-    cols.load(p.weight, w);
-    if (p.post) cols.load(p.post, pw);
+    cols.load(p.weight, kept[0]);
+    if (POST) cols.load(p.post, kept[1]);
+    if (RW > 1) {
+        if (threadIdx.x < T)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < J; j++)
+#pragma unroll
+                    for (int c = 0; c < VN; c++) weights[i][(t + j * T) * VN + c] = kept[i][j][c];
+        __syncthreads();
+    }
+    const auto weight = [&](int which, float (&w)[J][VN]) {
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int c = 0; c < VN; c++) w[j][c] = RW > 1 ? weights[which][(t + j * T) * VN + c] : kept[which][j][c];
+    };
     const long long end = min((long long)(blockIdx.x + 1) * p.rows_wg, p.rows);
     const long long first = (long long)blockIdx.x * p.rows_wg + threadIdx.x / T;
     // the next row's operands are in flight while this one's are worked on
     typename Row<E, VN, T, J>::vec xv[J], yv[J], gv[J], ev[J], dv[J];
     float r1n, r2n;
     const auto fetch = [&](long long r) {
-        const long long o = min(r, p.rows - 1) * p.D;
+        const long long o = r * p.D;
         cols.fetch(p.x, o, xv);
         cols.fetch(p.y, o, yv);
-        if (p.gate) cols.fetch(p.gate, o, gv);
+        if (GATE) cols.fetch(p.gate, o, gv);
         if (p.d_h) cols.fetch(p.d_h, o, ev);
         if (p.d_s) cols.fetch(p.d_s, o, dv);
-        r1n = p.stats[2 * min(r, p.rows - 1)];
-        r2n = p.stats[2 * min(r, p.rows - 1) + 1];
+        r1n = p.stats[2 * r];
+        r2n = p.stats[2 * r + 1];
     };
-    fetch(first);
+    fetch(min(first, end - 1));
     for (long long r = first; r < end; r += RW) {
         const long long o = r * p.D;
         float s[J][VN], y[J][VN], g[J][VN], e[J][VN], d[J][VN];
         cols.widen(xv, s);
         cols.widen(yv, y);
-        if (p.gate) cols.widen(gv, g);
+        if (GATE) cols.widen(gv, g);
         if (p.d_h) cols.widen(ev, e);
         if (p.d_s) cols.widen(dv, d);
-        const float r1 = p.post ? r1n : 1.f, r2 = r2n;
-        if (r + RW < end) fetch(r + RW);
-        float sum[3] = {0.f, 0.f, 0.f};
+        const float r1 = POST ? r1n : 1.f, r2 = r2n;
+        fetch(min(r + RW, end - 1));  // (the last time a row that the caches hold)
+        float sum[3] = {0.f, 0.f, 0.f}, w[J][VN], pw[J][VN];
+        weight(0, w);
+        if (POST) weight(1, pw);
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
             for (int c = 0; c < VN; c++) {
                 float q = p.scale;
-                if (p.gate) {
+                if (GATE) {
                     g[j][c] = sigmoidf(g[j][c]);
                     q *= g[j][c];
                 }
                 float u = y[j][c];
-                if (p.post) {
+                if (POST) {
                     y[j][c] *= r1;
                     u = y[j][c] * pw[j][c];
                 }
@@ -217,42 +256,44 @@ __global__ __launch_bounds__(256) void residual_grad_kernel(ResidualParams p) {
                 dw[j][c] = fmaf(e[j][c], m, dw[j][c]);
                 e[j][c] *= w[j][c];
                 sum[0] = fmaf(e[j][c], m, sum[0]);
-                if (p.post) {  // q u: scale sigmoid(gate) post n
-                    sum[1] = fmaf(q * u, fmaf(r2, e[j][c], d[j][c]), sum[1]);
+                d[j][c] = fmaf(r2, e[j][c], d[j][c]);  // ds + r2 e, dx without its mean
+                if (POST) {  // q u: scale sigmoid(gate) post n
+                    sum[1] = fmaf(q * u, d[j][c], sum[1]);
                     sum[2] = fmaf(q * u, m, sum[2]);
                 }
             }
-        if (p.post) {
+        if (POST) {
             row_sums<T>(sum, red);
         } else {
             float one[1] = {sum[0]};
             row_sums<T>(one, reinterpret_cast<float(*)[1]>(red));
             sum[0] = one[0];
         }
-        const float a = sum[0] / (float)p.D * r2;
-        const float mean = (sum[1] - a * sum[2]) / (float)p.D;
+        const float a = sum[0] * p.inverse_d * r2;
+        const float mean = (sum[1] - a * sum[2]) * p.inverse_d;
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
-            for (int c = 0; c < VN; c++) d[j][c] += fmaf(r2, e[j][c], -a * s[j][c]);
+            for (int c = 0; c < VN; c++) d[j][c] = fmaf(-a, s[j][c], d[j][c]);
         if (p.dx) cols.store(static_cast<E*>(p.dx) + o, d);
-        if (p.gate) {
+        if (POST) weight(1, pw);
+        if (GATE && p.dgate) {
 #pragma unroll
             for (int j = 0; j < J; j++)
 #pragma unroll
                 for (int c = 0; c < VN; c++) {
-                    const float u = p.post ? y[j][c] * pw[j][c] : y[j][c];
+                    const float u = POST ? y[j][c] * pw[j][c] : y[j][c];
                     e[j][c] = p.scale * d[j][c] * u * g[j][c] * (1.f - g[j][c]);
                 }
-            if (p.dgate) cols.store(static_cast<E*>(p.dgate) + o, e);
+            cols.store(static_cast<E*>(p.dgate) + o, e);
         }
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
             for (int c = 0; c < VN; c++) {
                 float du = p.scale * d[j][c];
-                if (p.gate) du *= g[j][c];
-                if (p.post) {
+                if (GATE) du *= g[j][c];
+                if (POST) {
                     dp[j][c] = fmaf(du, y[j][c], dp[j][c]);
                     du = r1 * (du * pw[j][c] - y[j][c] * mean);
                 }
@@ -272,7 +313,7 @@ __global__ __launch_bounds__(256) void residual_grad_kernel(ResidualParams p) {
 #pragma unroll
             for (int c = 0; c < VN; c++) sums[threadIdx.x / T][(t + j * T) * VN + c] = v[j][c];
         __syncthreads();
-        for (int c = threadIdx.x; c < p.D; c += 256) {
+        for (int c = threadIdx.x; c < p.D; c += block_of(T)) {
             // column c of the vector that counts it: the last vector ends at D
             const int whole = p.D / VN * VN, at = c < whole ? c : c + VN - (p.D - whole);
             float v = 0.f;
@@ -282,7 +323,7 @@ __global__ __launch_bounds__(256) void residual_grad_kernel(ResidualParams p) {
         }
     };
     if (p.dweight) leave(dw, 0);
-    if (p.dpost) leave(dp, 1);
+    if (POST && p.dpost) leave(dp, 1);
 }
 
 // dweight and dpost: the sums of part's rows, 32 threads per column each every
@@ -319,14 +360,24 @@ long long grad_rows(long long rows) {
 
 template <class E, int VN, int T, int J>
 void launch(ResidualParams p, bool grad, hipStream_t stream) {
+    p.inverse_d = 1.f / (float)p.D;
+    const dim3 block(block_of(T));
     if (!grad) {
-        const long long groups = (p.rows + 256 / T - 1) / (256 / T);
-        hipLaunchKernelGGL((residual_norm_kernel<E, VN, T, J>), dim3((unsigned)min(groups, 1ll << 20)), dim3(256), 0, stream, p);
+        constexpr int RW = block_of(T) / T;
+        const long long groups = (p.rows + RW - 1) / RW;
+        hipLaunchKernelGGL((residual_norm_kernel<E, VN, T, J>), dim3((unsigned)min(groups, 1ll << 20)), block, 0, stream, p);
         return;
     }
     p.rows_wg = grad_rows(p.rows);
     const int n = (int)((p.rows + p.rows_wg - 1) / p.rows_wg);
-    if (n) hipLaunchKernelGGL((residual_grad_kernel<E, VN, T, J>), dim3(n), dim3(256), 0, stream, p);
+    if (n && p.post && p.gate)
+        hipLaunchKernelGGL((residual_grad_kernel<E, VN, T, J, true, true>), dim3(n), block, 0, stream, p);
+    else if (n && p.post)
+        hipLaunchKernelGGL((residual_grad_kernel<E, VN, T, J, true, false>), dim3(n), block, 0, stream, p);
+    else if (n && p.gate)
+        hipLaunchKernelGGL((residual_grad_kernel<E, VN, T, J, false, true>), dim3(n), block, 0, stream, p);
+    else if (n)
+        hipLaunchKernelGGL((residual_grad_kernel<E, VN, T, J, false, false>), dim3(n), block, 0, stream, p);
     if (p.dweight || p.dpost) hipLaunchKernelGGL(residual_sum_kernel, dim3((p.D + 31) / 32, 2), dim3(1024), 0, stream, p, n);
 }
 
@@ -338,8 +389,8 @@ void launch_type(const ResidualParams& p, bool grad, hipStream_t stream) {
     if (p.D <= 128 * N) return launch<E, N, 64, 2>(p, grad, stream);
     if (p.D <= 256 * N) return launch<E, N, 256, 1>(p, grad, stream);
     if (p.D <= 512 * N) return launch<E, N, 256, 2>(p, grad, stream);
-    if (p.D <= 1024 * N) return launch<E, N, 256, 4>(p, grad, stream);
-    if constexpr (N == 4) launch<E, N, 256, 8>(p, grad, stream);
+    if (p.D <= 1024 * N) return launch<E, N, 512, 2>(p, grad, stream);
+    if constexpr (N == 4) launch<E, N, 512, 4>(p, grad, stream);
 }
 
 }  // namespace

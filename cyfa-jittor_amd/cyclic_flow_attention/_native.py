@@ -184,7 +184,7 @@ class CyfaLogprobArgs(ctypes.Structure):
         ("ignore", ctypes.c_longlong), ("logprob", _c_void_p), ("entropy", _c_void_p), ("stats", _c_void_p),
         ("k", _c_int), ("top_logprobs", _c_void_p), ("top_ids", _c_void_p), ("loss", _c_void_p), ("count", _c_void_p),
         ("d_logprob", _c_void_p), ("d_entropy", _c_void_p), ("d_top", _c_void_p), ("d_loss", _c_void_p),
-        ("dx", _c_void_p),
+        ("dx", _c_void_p), ("workspace", _c_void_p), ("workspace_bytes", _c_size_t),
     ]
 
 
@@ -241,6 +241,7 @@ SIGNATURES = {
     "cyfa_decode_step_general": (_c_int, [ctypes.POINTER(CyfaDecodeArgs), _c_int, _c_void_p]),
     "cyfa_chunk_bwd_workspace_bytes": (_c_size_t, [_c_int] * 6),
     "cyfa_chunk_bwd": (_c_int, [ctypes.POINTER(CyfaChunkArgs), _c_int, ctypes.POINTER(CyfaChunkBwdArgs), _c_void_p]),
+    "cyfa_logprobs_workspace_bytes": (_c_size_t, [ctypes.c_longlong, _c_int, _c_int, _c_int]),
     "cyfa_logprobs": (_c_int, [ctypes.POINTER(CyfaLogprobArgs), _c_int, _c_int, _c_void_p]),
     "cyfa_embed_grad_workspace_bytes": (_c_size_t, [ctypes.c_longlong, ctypes.c_longlong, _c_int]),
     "cyfa_embed": (_c_int, [ctypes.POINTER(CyfaEmbedArgs), _c_int, _c_int, _c_void_p]),
@@ -976,6 +977,18 @@ def logit_rows(logits):
     return (rows, logits.shape[1], logits.stride(0), logits.stride(1), V, logits.data_ptr()), logits
 
 
+def _logprobs_workspace(args, dtype, dev):
+    """The call's workspace, set in args; the caller keeps it until the launch."""
+    if args.rows >= 512:  # (rows enough for the compute units: none)
+        return None
+    n = int(load_library().cyfa_logprobs_workspace_bytes(args.rows, args.V, args.k, LM_DTYPES[dtype]))
+    if n == 0:
+        return None
+    workspace = torch.empty(n, dtype=torch.uint8, device=dev)
+    args.workspace, args.workspace_bytes = workspace.data_ptr(), n
+    return workspace
+
+
 def logprobs(logits, tokens, k, ignore, stats=False):
     """(logprob, entropy, top_logprobs or None, top_ids or None, stats or None)
     of logits [..., V] for int64 contiguous tokens [...]."""
@@ -990,6 +1003,7 @@ def logprobs(logits, tokens, k, ignore, stats=False):
     st = torch.empty(fields[0], 2, dtype=torch.float32, device=dev) if stats else None
     args = CyfaLogprobArgs(*fields, tokens=tokens.data_ptr(), ignore=ignore, logprob=logprob.data_ptr(),
                            entropy=entropy.data_ptr(), stats=ptr(st), k=k, top_logprobs=ptr(top), top_ids=ptr(ids))
+    workspace = _logprobs_workspace(args, logits.dtype, dev)  # noqa: F841 (alive until the launch)
     _lm_call("cyfa_logprobs", args, logits.dtype, 0, dev)
     return logprob, entropy, top, ids, st
 
@@ -1018,6 +1032,7 @@ def token_loss(logits, labels, ignore):
     at = kept.data_ptr()
     args = CyfaLogprobArgs(*fields, tokens=labels.data_ptr(), ignore=ignore, stats=at, logprob=at + 8 * rows,
                            loss=loss.data_ptr(), count=at + 12 * rows)
+    workspace = _logprobs_workspace(args, logits.dtype, dev)  # noqa: F841 (alive until the launch)
     _lm_call("cyfa_logprobs", args, logits.dtype, 0, dev)
     return loss, kept
 

@@ -610,9 +610,12 @@ typedef struct CyfaLogprobArgs {
     float *loss, *count;          /* nullable [1], both or none */
     const float *d_logprob, *d_entropy, *d_top, *d_loss; /* grad 1: nullable; d_loss [1] in place of d_logprob */
     void *dx;                     /* grad 1 */
+    void *workspace;              /* grad 0: cyfa_logprobs_workspace_bytes(rows, V, k, dtype) bytes, 8-byte aligned; */
+    size_t workspace_bytes;       /* few rows of many columns alone need one */
 } CyfaLogprobArgs;
 
 #define CYFA_LOGPROBS_MAX_TOP 32
+size_t cyfa_logprobs_workspace_bytes(long long rows, int V, int k, int dtype);
 int cyfa_logprobs(const CyfaLogprobArgs *args, int dtype, int grad, void *hip_stream);
 
 /* The embedding lookup out[i] = scale weight[ids[i]] (grad 0) and its gradient

@@ -46,7 +46,8 @@ def _check_logprobs(got, x, tokens, k, what=""):
 @pytest.mark.parametrize("rows,V,dtype,k", [
     (1, 1, F32, 1), (3, 7, BF, 7), (2, 8, F16, 3), (5, 255, BF, 32), (4, 257, F32, 20), (7, 1000, F16, 5), (66, 2051, BF, 1),
     (2, 8192, F32, 0), (3, 32000, BF, 20), (2, 32768, BF, 32), (3, 50001, BF, 5), (2, 70003, F32, 9), (300, 513, BF, 0),
-    (1, 131072, F16, 31)])
+    (1, 131072, F16, 31), (1, 300000, BF, 32), (40, 40000, F32, 7), (100, 33001, BF, 2), (250, 16385, F32, 0), (6, 98305, F16, 0),
+    (520, 40001, BF, 3)])
 def test_logprobs(rows, V, dtype, k):
     x = (_randn(rows + V, rows, V) * 3).to(dtype)  # 16-bit logits of a large vocabulary hold many equal ones
     tokens = _randint(V, V, rows)
@@ -76,6 +77,32 @@ def test_logprobs_of_masked_rows(dtype):
     _check_logprobs(got, x, tokens, 12)
     assert got.logprob[1].item() == 0.0 and got.entropy[1].item() == 0.0
     assert abs(got.logprob[2].item() + math.log(V)) < 1e-5
+
+
+def test_logprobs_of_masked_rows_in_parts():
+    """Rows shared out to several workgroups: parts of nothing but -inf, of the
+    lowest value, with a NaN, with all of the alternatives."""
+    V = 100003
+    x = (_randn(1, 6, V) * 2).to(BF)
+    x[0, 40000:] = -INF
+    x[1] = -INF
+    x[1, V - 1] = 2.0
+    x[2, 70000] = NAN
+    x[3] = torch.finfo(BF).min
+    x[4, 33000:33020] = 30.0
+    x[5] = -INF
+    tokens = torch.tensor([5, V - 1, 3, 99999, 33001, 0])
+    got = _ops().token_logprobs(x.cuda(), tokens.cuda(), top_k=20)
+    keep = torch.tensor([0, 1, 3, 4])
+    _check_logprobs(type(got)(*(t.cpu()[keep] for t in got)), x[keep], tokens[keep], 20)
+    assert torch.equal(got.top_ids.cpu(), lm.order(x.double(), 20))
+    for row in (2, 5):
+        assert got.logprob[row].isnan() and got.entropy[row].isnan()
+    labels = tokens.cuda()
+    labels[2] = labels[5] = -100
+    loss = _ops().token_loss(x.cuda(), labels)
+    ref, err = lm.logprobs(x[keep].double(), tokens[keep])["logprob"]
+    lm.assert_within(loss, -ref.mean(), lm.rounded(ref.mean(), err.mean(), F32), "loss")
 
 
 def test_logprobs_of_rows_without_probabilities():

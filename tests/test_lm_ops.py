@@ -44,6 +44,13 @@ def test_logprobs_validates_before_launch():
     assert call(1, d_loss=0x60000) == call(1, d_loss=0x60000, count=0x70000, d_logprob=0x70000) == VALUE
     assert call(0, rows=0) == call(1, rows=0) == _native.CYFA_OK
     lib = _native.load_library()
+    size = lib.cyfa_logprobs_workspace_bytes
+    assert size(4, 100, 0, 0) == size(512, 1 << 20, 5, 0) == size(-1, 8, 0, 0) == size(4, 0, 0, 0) == 0
+    n = size(4, 1 << 20, 5, 0)
+    assert n >= 4 * 16 * (12 + 5 * 8)
+    assert call(0, V=1 << 20) == WORKSPACE
+    assert call(0, V=1 << 20, workspace=0x90000, workspace_bytes=size(4, 1 << 20, 0, 0) - 1) == WORKSPACE
+    assert call(0, V=1 << 20, workspace=0x90004, workspace_bytes=n) == ALIGN
     assert lib.cyfa_logprobs(None, 0, 0, None) == lib.cyfa_embed(None, 0, 0, None) == VALUE
     assert lib.cyfa_residual_norm(None, 0, 0, None) == VALUE
 
