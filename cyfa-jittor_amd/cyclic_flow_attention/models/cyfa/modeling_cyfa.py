@@ -12,7 +12,10 @@ import torch.nn.functional as F
 from torch import nn
 
 from ... import _native
-from ...layers.cyfa import CyclicFlowAttention, FusedWeight, RMSNorm, inference_fast_path
+from ...layers.autograd import hip_autograd_ok
+from ...layers.cyfa import CyclicFlowAttention, FusedWeight, RMSNorm, inference_fast_path, plain_module
+from ...ops.residual import residual_norm
+from ...ops.vocab import embed_tokens, token_logprobs, token_loss
 
 
 def mlp_width(config):
@@ -96,6 +99,18 @@ class GatedMLP(nn.Module):
         return x + self(norm(x))
 
 
+def join_norm(x, y, norm):
+    """(x + y, norm(x + y)): the residual add between two halves of a block and
+    the norm after it. A training step on the GPU runs both, and their adjoint,
+    as one residual_norm launch each."""
+    if (x.dtype in _native.LM_DTYPES and x.shape == y.shape and x.dtype == y.dtype and 0 < x.shape[-1] <= _native.RESIDUAL_MAX_D
+            and plain_module(norm, RMSNorm) and tuple(norm.weight.shape) == x.shape[-1:]
+            and hip_autograd_ok(x, y, norm.weight)):
+        return residual_norm(x, y, norm.weight, eps=norm.eps)
+    s = x + y
+    return s, norm(s)
+
+
 class CyFABlock(nn.Module):
     def __init__(self, config):
         super().__init__()
@@ -118,8 +133,8 @@ class CyFABlock(nn.Module):
 
     def forward(self, x, cache=None, use_cache=False, attention_mask=None):
         y, cache = self.attn(self.attn_norm(x), cache, use_cache, attention_mask)
-        residual = x + y
-        return residual + self.mlp(self.mlp_norm(residual)), cache
+        residual, h = join_norm(x, y, self.mlp_norm)
+        return residual + self.mlp(h), cache
 
 
 class CyclicFlowAttentionModel(nn.Module):
@@ -129,10 +144,31 @@ class CyclicFlowAttentionModel(nn.Module):
         self.layers = nn.ModuleList([CyFABlock(config) for _ in range(config.num_hidden_layers)])
         self.norm = RMSNorm(config.hidden_size, config.norm_eps)
 
+    def embed(self, input_ids):
+        """The embeddings of input_ids. A training step on the GPU looks them up
+        with the gradient by sorted tokens (the same bits every time)."""
+        e = self.embeddings
+        if (plain_module(e, nn.Embedding) and e.weight.requires_grad and e.weight.dtype in _native.LM_DTYPES
+                and e.max_norm is None and not e.sparse and not e.scale_grad_by_freq
+                and input_ids.dtype in (torch.int64, torch.int32) and input_ids.device == e.weight.device
+                and type(input_ids) is torch.Tensor and hip_autograd_ok(e.weight)):
+            return embed_tokens(input_ids, e.weight, padding_idx=e.padding_idx)
+        return e(input_ids)
+
     def forward(self, input_ids, cache=None, use_cache=False, attention_mask=None):
-        x = self.embeddings(input_ids)
+        x = self.embed(input_ids)
         new = []
         if not inference_fast_path(x):
+            if self.layers and all(plain_module(layer, CyFABlock) for layer in self.layers):
+                # each block's second residual add runs with the norm after it
+                h = self.layers[0].attn_norm(x)
+                norms = [layer.attn_norm for layer in self.layers[1:]] + [self.norm]
+                for i, (layer, norm) in enumerate(zip(self.layers, norms)):
+                    y, s = layer.attn(h, None if cache is None else cache[i], use_cache, attention_mask)
+                    x, m = join_norm(x, y, layer.mlp_norm)
+                    x, h = join_norm(x, layer.mlp(m), norm)
+                    new.append(s)
+                return h, (new if use_cache else None)
             for i, layer in enumerate(self.layers):
                 x, s = layer(x, None if cache is None else cache[i], use_cache, attention_mask)
                 new.append(s)
@@ -215,12 +251,34 @@ class CyclicFlowAttentionForCausalLM(nn.Module):
             logits = self.lm_head(hidden)
         loss = None
         if labels is not None:
-            loss = F.cross_entropy(
-                logits[:, :-1].float().reshape(-1, self.config.vocab_size),
-                labels[:, 1:].reshape(-1),
-                ignore_index=-100,
-            )
+            if (logits.dtype in _native.LM_DTYPES and logits.dim() == 3 and labels.dtype == torch.int64
+                    and type(labels) is torch.Tensor and labels.shape == logits.shape[:2] and labels.device == logits.device
+                    and (hip_autograd_ok(logits) or inference_fast_path(logits))):
+                # labels shifted instead of logits: the gradient is written once, in place
+                loss = token_loss(logits, F.pad(labels[:, 1:], (0, 1), value=-100))
+            else:
+                loss = F.cross_entropy(
+                    logits[:, :-1].float().reshape(-1, self.config.vocab_size),
+                    labels[:, 1:].reshape(-1),
+                    ignore_index=-100,
+                )
         return {"logits": logits, "loss": loss, "cache": cache}
+
+    @torch.no_grad()
+    def score(self, input_ids, top_k=0, attention_mask=None):
+        """Log probabilities of the tokens input_ids [B, T] after the first, each
+        given those before it, with the entropy of every prediction and its
+        top_k most probable tokens: ops.TokenLogprobs of [B, T - 1] (a GPU model).
+        With a right-padding attention_mask [B, T], padded tokens have logprob 0."""
+        hidden, _ = self.model(input_ids, attention_mask=attention_mask)
+        if inference_fast_path(hidden):
+            logits = _native.linear(hidden, self.lm_head.weight)
+        else:
+            logits = self.lm_head(hidden)
+        tokens = input_ids[:, 1:]
+        if attention_mask is not None:
+            tokens = tokens.masked_fill(attention_mask[:, 1:] == 0, -100)
+        return token_logprobs(logits[:, :-1], tokens, top_k=top_k)
 
     def to_bfloat16(self):
         for name, p in self.named_parameters():

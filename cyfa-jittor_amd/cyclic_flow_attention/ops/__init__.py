@@ -5,6 +5,6 @@ causal language model's blocks."""
 from .chunk import chunk_cyfa
 from .fused_recurrent import fused_recurrent_cyfa
 from .residual import residual_norm
-from .vocab import embed_tokens, token_logprobs, token_loss
+from .vocab import TokenLogprobs, embed_tokens, token_logprobs, token_loss
 
-__all__ = ["chunk_cyfa", "embed_tokens", "fused_recurrent_cyfa", "residual_norm", "token_logprobs", "token_loss"]
+__all__ = ["TokenLogprobs", "chunk_cyfa", "embed_tokens", "fused_recurrent_cyfa", "residual_norm", "token_logprobs", "token_loss"]
