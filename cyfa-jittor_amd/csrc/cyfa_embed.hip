@@ -38,100 +38,103 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedParams p) {
 // vocabularies number together, come to different workgroups). A workgroup reads
 // every id: it counts, wave by wave, how often each of its ids comes up and how
 // many ids belong to the workgroups before it, then each wave places its stretch
-// of the positions behind those of the waves before it. Ids outside [0, V) and
-// the padding id count nowhere.
+// of the positions behind those of the waves before it. Ids outside [0, V) count
+// nowhere.
 //   slot(v) = (v mod G) range + v / G;  offsets[slot] .. offsets[slot + 1]: where v's positions lie in order
 constexpr int ES_NT = 1024, ES_WAVES = ES_NT / 64, ES_U = 16;
-constexpr int ES_RANGE = 512;  // most ids of a workgroup: 35 KB of LDS
+constexpr int ES_RANGE = 512;  // most ids of a workgroup: 33 KB of LDS
 
 __global__ __launch_bounds__(ES_NT) void embed_sort_kernel(EmbedParams p) {
     extern __shared__ int lds[];
     const int range = p.range, shift = p.shift;
-    int* cursor = lds;                      // [ES_WAVES][range]
-    int* start = lds + ES_WAVES * range;    // [range]
-    int* misc = start + range;              // [2 * ES_WAVES]
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    int* cursor = lds;                   // [ES_WAVES][range]: how many, then where the next goes
+    int* misc = lds + ES_WAVES * range;  // [2 * ES_WAVES]
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned mine = blockIdx.x, groups = gridDim.x;
-    const unsigned padding = (unsigned)p.padding;  // -1: above every id
     const long long stretch = ((p.n + ES_NT - 1) / ES_NT) * 64;
     const long long first = wv * stretch, last = min(first + stretch, p.n);
-    // The ids of ES_U times 64 positions from i0, all loads in flight at once; ~0: counts nowhere.
-    const auto load = [&](long long i0, unsigned (&ids)[ES_U]) {
-        long long id[ES_U];
-        const long long* from = p.ids + i0;
-        const int left = (int)min(last - i0, (long long)64 * ES_U);  // at least 1
-#pragma unroll
-        for (int u = 0; u < ES_U; u++) id[u] = from[min(64 * u + lane, left - 1)];
-#pragma unroll
-        for (int u = 0; u < ES_U; u++) {
-            const unsigned low = (unsigned)id[u];
-            const bool counts = (id[u] >> 32) == 0 && low < (unsigned)p.V && low != padding && 64 * u + lane < left;
-            ids[u] = counts ? low : ~0u;
-        }
-    };
+    int* own = cursor + wv * range;
     for (int i = tid; i < ES_WAVES * range; i += ES_NT) cursor[i] = 0;
     __syncthreads();
     int below = 0;
-    unsigned ids[ES_U];
-    for (long long i0 = first; i0 < last; i0 += 64 * ES_U) {
-        load(i0, ids);
+    unsigned ids[ES_U];  // of 64 ES_U positions, ~0 where one counts nowhere
+#pragma unroll 1
+    for (int pass = 0; pass < 2; pass++) {
+#pragma unroll 1
+        for (long long i0 = first; i0 < last; i0 += 64 * ES_U) {
+            const int left = (int)min(last - i0, (long long)64 * ES_U);  // at least 1
+            if (pass == 0 || stretch > 64 * ES_U) {  // (else the ids are still here)
+                const unsigned long long* from = reinterpret_cast<const unsigned long long*>(p.ids) + i0;
+                unsigned long long id[ES_U];  // all loads in flight at once, those past the end of the last position
 #pragma unroll
-        for (int u = 0; u < ES_U; u++) {
-            const unsigned group = ids[u] & (groups - 1);
-            below += group < mine && ids[u] != ~0u;
-            if (group == mine && ids[u] != ~0u) atomicAdd(&cursor[wv * range + (int)(ids[u] >> shift)], 1);
-        }
-    }
-    for (int d = 32; d > 0; d >>= 1) below += __shfl_xor(below, d);
-    if (lane == 0) misc[wv] = below;
-    __syncthreads();
-    below = 0;
-    for (int w = 0; w < ES_WAVES; w++) below += misc[w];
-    // this id's positions of the waves before, and of the ids before (range <= ES_NT)
-    int total = 0;
-    if (tid < range)
-        for (int w = 0; w < ES_WAVES; w++) {
-            const int c = cursor[w * range + tid];
-            cursor[w * range + tid] = total;
-            total += c;
-        }
-    int scan = total;
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(scan, d);
-        if (lane >= d) scan += o;
-    }
-    if (lane == 63) misc[ES_WAVES + wv] = scan;
-    __syncthreads();
-    for (int w = 0; w < wv; w++) scan += misc[ES_WAVES + w];
-    if (tid < range) {
-        start[tid] = below + scan - total;
-        p.offsets[(long long)mine * range + tid] = below + scan - total;
-        if (mine == groups - 1 && tid == range - 1) p.offsets[(long long)groups * range] = below + scan;
-    }
-    __syncthreads();
-    const bool once = stretch <= 64 * ES_U;  // the ids are still in registers
-    for (long long i0 = first; i0 < last; i0 += 64 * ES_U) {
-        if (!once) load(i0, ids);
+                for (int u = 0; u < ES_U; u++) id[u] = from[min(64 * u + lane, left - 1)];
 #pragma unroll
-        for (int u = 0; u < ES_U; u++) {
-            const bool here = (ids[u] & (groups - 1)) == mine && ids[u] != ~0u;
-            const int id = (int)(ids[u] >> shift);
-            uint64_t same = __ballot(here);
-            if (!same) continue;
-            for (int b = 1; b < range; b <<= 1) {  // the lanes with this lane's id, bit by bit
-                const uint64_t bit = __ballot((id & b) != 0);
-                same &= (id & b) ? bit : ~bit;
+                for (int u = 0; u < ES_U; u++) ids[u] = id[u] < (unsigned long long)p.V ? (unsigned)id[u] : ~0u;
+                if (left < 64 * ES_U)
+#pragma unroll
+                    for (int u = 0; u < ES_U; u++) ids[u] = 64 * u + lane < left ? ids[u] : ~0u;
             }
-            // (LDS serves a wave's accesses in order: the next step reads what this one wrote)
-            if (here) {
-                int* at = &cursor[wv * range + id];
-                const int c = *at, rank = __popcll(same & ((1ull << lane) - 1)), count = __popcll(same);
-                p.order[start[id] + c + rank] = (int)(i0 + 64 * u + lane);
-                if (rank == count - 1) *at = c + count;
+#pragma unroll
+            for (int u = 0; u < ES_U; u++) {
+                if (64 * u >= left) break;
+                const unsigned group = ids[u] & (groups - 1);
+                const int id = (int)(ids[u] >> shift);  // (~0: past every range, in the last group)
+                const bool here = group == mine && id < range;
+                if (pass == 0) {
+                    below += __popcll(__ballot(group < mine));
+                    if (here) atomicAdd(&own[id], 1);
+                    continue;
+                }
+                uint64_t same = __ballot(here);
+                if (!same) continue;
+                for (int b = 1; b < range; b <<= 1) {  // the lanes with this lane's id, bit by bit
+                    const uint64_t bit = __ballot((id & b) != 0);
+                    same &= (id & b) ? bit : ~bit;
+                }
+                // (LDS serves a wave's accesses in order: the next step reads what this one wrote)
+                if (here) {
+                    const int c = own[id], rank = __popcll(same & ((1ull << lane) - 1)), count = __popcll(same);
+                    p.order[c + rank] = (int)(i0 + 64 * u + lane);
+                    if (rank == count - 1) own[id] = c + count;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
         }
+        if (pass == 1) break;
+        if (lane == 0) misc[wv] = below;
+        __syncthreads();
+        below = 0;
+#pragma unroll
+        for (int w = 0; w < ES_WAVES; w++) below += misc[w];
+        // how many of this thread's id, and of the ids before it (range <= ES_NT)
+        int c[ES_WAVES], total = 0;
+        if (tid < range)
+#pragma unroll
+            for (int w = 0; w < ES_WAVES; w++) {
+                c[w] = cursor[w * range + tid];
+                total += c[w];
+            }
+        int scan = total;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(scan, d);
+            if (lane >= d) scan += o;
+        }
+        if (lane == 63) misc[ES_WAVES + wv] = scan;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < ES_WAVES; w++) scan += w < wv ? misc[ES_WAVES + w] : 0;
+        if (tid < range) {
+            int at = below + scan - total;
+            p.offsets[(long long)mine * range + tid] = at;
+            if (mine == groups - 1 && tid == range - 1) p.offsets[(long long)groups * range] = below + scan;
+#pragma unroll
+            for (int w = 0; w < ES_WAVES; w++) {
+                cursor[w * range + tid] = at;
+                at += c[w];
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -162,6 +165,7 @@ __device__ __forceinline__ void add_rows(const EmbedParams& p, const E* dy, int 
 // written ending at the row's end, so that it overlaps the one before it
 // (the same values are stored twice), and rows below one vector go column by column.
 constexpr int EMBED_CHUNK = 32;
+constexpr size_t EMBED_STREAM = 128 << 20;
 constexpr int EMBED_GRID = 4096;  // workgroups, 8 of a compute unit at a time
 
 template <class E>
@@ -172,7 +176,8 @@ __global__ __launch_bounds__(256) void embed_part_kernel(EmbedParams p) {
     const int d = blockIdx.y * 64 * N + lane * N;
     for (int c = blockIdx.x * 4 + wv; c < chunks; c += gridDim.x * 4) {
         const int s = c * EMBED_CHUNK, e = s + EMBED_CHUNK;
-        if (p.ids[p.order[s]] != p.ids[p.order[e - 1]] || d >= p.D) continue;  // not one id's whole chunk
+        const long long id = p.ids[p.order[s]];
+        if (id != p.ids[p.order[e - 1]] || id == p.padding || d >= p.D) continue;  // not one id's whole chunk
         float* out = p.part + (long long)c * p.D;
         if (p.D >= N) {
             const int at = min(d, p.D - N);
@@ -191,7 +196,8 @@ __global__ __launch_bounds__(256) void embed_part_kernel(EmbedParams p) {
     }
 }
 
-template <class E>
+// STREAM: the gradient's lines, each written whole by one wave, go past the caches.
+template <class E, bool STREAM>
 __global__ __launch_bounds__(256) void embed_grad_kernel(EmbedParams p) {
     constexpr int N = RowVec<E>::N;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -203,7 +209,7 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(EmbedParams p) {
     int v = blockIdx.x * 4 + wv;
     int next_s = slot(v)[0], next_e = slot(v)[1];  // (the next row's positions are on their way while this one is added)
     for (; v < V; v += waves) {
-        const int s = next_s, e = next_e;
+        const int s = next_s, e = v == p.padding ? s : next_e;
         next_s = slot(v + waves)[0];
         next_e = slot(v + waves)[1];
         if (d >= p.D) continue;
@@ -234,7 +240,10 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(EmbedParams p) {
             typename RowVec<E>::type o;
 #pragma unroll
             for (int i = 0; i < N; i++) o[i] = (E)(acc[i] * p.scale);
-            store_row(out + at, o);
+            if (STREAM)
+                __builtin_nontemporal_store(o, reinterpret_cast<typename RowVec<E>::type*>(out + at));
+            else
+                store_row(out + at, o);
         } else {
             for (int i = 0; i < p.D; i++) {
                 float a = 0.f;
@@ -256,7 +265,7 @@ void launch(const EmbedParams& p, bool grad, hipStream_t stream) {
         hipLaunchKernelGGL(embed_kernel<E>, dim3((unsigned)min((p.n + 3) / 4, 1ll << 20)), dim3(256), 0, stream, p);
         return;
     }
-    hipLaunchKernelGGL(embed_sort_kernel, dim3(1u << p.shift), dim3(ES_NT), ((ES_WAVES + 1) * p.range + 2 * ES_WAVES) * sizeof(int),
+    hipLaunchKernelGGL(embed_sort_kernel, dim3(1u << p.shift), dim3(ES_NT), (ES_WAVES * p.range + 2 * ES_WAVES) * sizeof(int),
                        stream, p);
     // workgroups of four waves, a wave for 64 vectors of a row, the rows in turn
     const int cols = (p.D + 64 * RowVec<E>::N - 1) / (64 * RowVec<E>::N);
@@ -265,7 +274,15 @@ void launch(const EmbedParams& p, bool grad, hipStream_t stream) {
     };
     const long long chunks = p.n / EMBED_CHUNK;
     if (chunks) hipLaunchKernelGGL(embed_part_kernel<E>, grid(chunks), dim3(256), 0, stream, p);
-    hipLaunchKernelGGL(embed_grad_kernel<E>, grid(p.V), dim3(256), 0, stream, p);
+    // A gradient that the last-level cache cannot keep beside its inputs is
+    // streamed: 32000 x 2048 fp32 (262 MB) 54 us a launch, 74 through the caches;
+    // 131072 x 1024 bf16 55, 65. Rows off the 128-byte lines, which two waves write
+    // in part, lose by it (131072 x 1000 bf16 78, 68), and a gradient of 66 MB
+    // gains 1.5 us that its reader may pay.
+    if ((size_t)p.V * p.D * sizeof(E) >= EMBED_STREAM && p.D * sizeof(E) % 128 == 0 && (uintptr_t)p.dweight % 128 == 0)
+        hipLaunchKernelGGL((embed_grad_kernel<E, true>), grid(p.V), dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL((embed_grad_kernel<E, false>), grid(p.V), dim3(256), 0, stream, p);
 }
 
 }  // namespace

@@ -34,6 +34,8 @@ def residual_norm(x, y, weight, post_weight=None, gate=None, scale=1.0, eps=1e-6
     for name, t in (("weight", weight), ("post_weight", post_weight)):
         if t is not None and (tuple(t.shape) != (D,) or not t.dtype.is_floating_point):
             raise ValueError(f"residual_norm: {name} must be a float tensor of shape ({D},), got {tuple(t.shape)} {t.dtype}")
+    if isinstance(scale, torch.Tensor):
+        raise ValueError("residual_norm: the scale must be a number (a tensor's gradient would be lost)")
     given = (x.contiguous(), y.contiguous(), weight.float().contiguous(),
              None if post_weight is None else post_weight.float().contiguous(),
              None if gate is None else gate.contiguous())

@@ -92,8 +92,11 @@ def _torch_backward(fn, inputs, needed, cotangents):
 def _plain_logprobs(logits, tokens, ids, ignore_index):
     """(logprob, entropy, top_logprobs) in torch operations."""
     lp = F.log_softmax(logits.float(), -1)
+    V = logits.shape[-1]
+    logprob = lp.gather(-1, tokens.clamp(0, V - 1)[..., None])[..., 0]
     ignored = tokens == ignore_index
-    logprob = lp.gather(-1, tokens.masked_fill(ignored, 0)[..., None])[..., 0].masked_fill(ignored, 0.0)
+    logprob = logprob * torch.where(ignored | ((tokens >= 0) & (tokens < V)), 1.0, float("nan"))
+    logprob = logprob.masked_fill(ignored, 0.0)
     p = lp.exp()
     entropy = -(p * lp.masked_fill(p == 0, 0.0)).sum(-1)
     return (logprob, entropy) if ids is None else (logprob, entropy, lp.gather(-1, ids))
@@ -139,7 +142,7 @@ def token_loss(logits, labels, ignore_index=-100):
 
 
 def _plain_loss(logits, labels, ignore_index):
-    return (F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), labels.reshape(-1), ignore_index=ignore_index),)
+    return (-_plain_logprobs(logits, labels, None, ignore_index)[0].sum() / (labels != ignore_index).sum(),)
 
 
 class _TokenLoss(torch.autograd.Function):
@@ -175,6 +178,8 @@ def embed_tokens(ids, weight, scale=1.0, padding_idx=None):
         raise ValueError(f"embed_tokens: the weight must be [vocabulary, width], got {tuple(weight.shape)}")
     if ids.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"embed_tokens: ids must be int64 or int32, got {ids.dtype}")
+    if isinstance(scale, torch.Tensor):
+        raise ValueError("embed_tokens: the scale must be a number (a tensor's gradient would be lost)")
     V = weight.shape[0]
     if padding_idx is None:
         padding_idx = -1

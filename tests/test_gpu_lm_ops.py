@@ -362,6 +362,22 @@ def test_embed_ids_of_any_shape_padding_and_impossible_ids():
     assert torch.equal(small.cpu(), w[[1, 3]])
 
 
+def test_embed_gradient_past_the_caches():
+    """A gradient of 135 MB in rows of whole lines, and in rows that are not."""
+    for V, D, dtype in ((66000, 1024, BF), (66001, 1023, BF), (33000, 1024, F32)):
+        ids = _randint(V, 200, 300)
+        ids[::2] = V - 1 - ids[::2]
+        dy = _randn(1, 300, D).to(dtype)
+        w = torch.empty(V, D, dtype=dtype, device="cuda").requires_grad_(True)
+        (dw,) = torch.autograd.grad(_ops().embed_tokens(ids.cuda(), w, padding_idx=5), [w], dy.cuda())
+        rows = torch.unique(ids)
+        at = torch.searchsorted(rows, ids)
+        pad = int(torch.searchsorted(rows, 5)) if 5 in rows else -1
+        lm.assert_within(dw.cpu()[rows], *lm.embed_grad(at, dy.double(), len(rows), 1.0, pad, dtype), "dw")
+        dw[rows.cuda()] = 0
+        assert not dw.any()
+
+
 def test_embed_recorded_backward():
     ids = torch.tensor([2, 0, 2, 1, -5]).cuda()
     w = _randn(1, 4, 6).cuda().requires_grad_(True)
@@ -476,6 +492,24 @@ def test_residual_norm_gradient_of_some_inputs():
         ref = lm.residual(t["x"].double(), t["y"].double(), t["weight"].double(), None, None, 1.0, 1e-6, d_s.double(), d_h.double())
         for g in grads:
             lm.assert_within(g, ref["x"][0], lm.rounded(*ref["x"], F32), "plain")
+
+
+def test_residual_norm_gradients_of_one_tensor_and_of_leaves():
+    """x and y one tensor; the plain join's gradients of two leaves are tensors of their own."""
+    t, d_s, d_h = _join_inputs(5, 72, F32, False, False)
+    x, w = t["x"].cuda().requires_grad_(True), t["weight"].cuda()
+    for scale in (1.0, 0.5):
+        (dx,) = torch.autograd.grad(_ops().residual_norm(x, x, w, scale=scale), [x], [d_s.cuda(), d_h.cuda()])
+        ref = lm.residual(t["x"].double(), t["x"].double(), t["weight"].double(), None, None, scale, 1e-6, d_s.double(), d_h.double())
+        total = ref["x"][0] + ref["y"][0]
+        err = sum(lm.rounded(*ref[n], F32) for n in ("x", "y"))
+        lm.assert_within(dx, total, lm.rounded(total, err, F32), "x twice")
+    y = t["y"].cuda().requires_grad_(True)
+    s, h = _ops().residual_norm(x, y, w)
+    (s.sum() + h.sum()).backward()
+    kept = y.grad.clone()
+    x.grad.zero_()
+    assert torch.equal(y.grad, kept) and kept.abs().sum() > 0
 
 
 def test_residual_norm_recorded_backward():

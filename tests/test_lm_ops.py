@@ -123,6 +123,8 @@ def test_embed_refuses():
             ops.embed_tokens(ids, bad)
     with pytest.raises(ValueError, match="int64 or int32"):
         ops.embed_tokens(ids.float(), w)
+    with pytest.raises(ValueError, match="scale"):
+        ops.embed_tokens(ids, w, scale=torch.tensor(2.0, requires_grad=True))
     for pad in (5, -6):
         with pytest.raises(ValueError, match="padding_idx"):
             ops.embed_tokens(ids, w, padding_idx=pad)
@@ -139,6 +141,8 @@ def test_residual_norm_refuses():
     for bad in (torch.tensor(1.0), x[:, :0]):
         with pytest.raises(ValueError, match="width"):
             ops.residual_norm(bad, bad, w)
+    with pytest.raises(ValueError, match="scale"):
+        ops.residual_norm(x, x, w, scale=torch.tensor(0.5, requires_grad=True))
     for y in (x[:2], x.half()):
         with pytest.raises(ValueError, match="y must be"):
             ops.residual_norm(x, y, w)
@@ -149,3 +153,21 @@ def test_residual_norm_refuses():
             ops.residual_norm(x, x, bad)
         with pytest.raises(ValueError, match="post_weight must be"):
             ops.residual_norm(x, x, w, post_weight=bad)
+
+
+def test_recorded_backward_of_impossible_tokens_stays_off_the_table():
+    """The torch operations behind a recorded backward pass never index with a
+    token outside the vocabulary."""
+    from cyclic_flow_attention.ops.vocab import _plain_logprobs, _plain_loss
+
+    x = torch.randn(4, 6, requires_grad=True)
+    tokens = torch.tensor([2, 6, -1, -100])
+    logprob, entropy = _plain_logprobs(x, tokens, None, -100)
+    want = torch.log_softmax(x.double(), -1)
+    assert abs(logprob[0].item() - want[0, 2].item()) < 1e-6 and logprob[1:3].isnan().all() and logprob[3] == 0
+    assert (entropy.double() + (want.exp() * want).sum(-1)).abs().max() < 1e-6
+    assert _plain_loss(x, tokens, -100)[0].isnan()
+    kept = torch.tensor([2, -100, 0, -100])
+    loss = _plain_loss(x, kept, -100)[0]
+    assert abs(loss.item() + (want[0, 2] + want[2, 0]).item() / 2) < 1e-6
+    assert _plain_loss(x, torch.full((4,), -100), -100)[0].isnan()
