@@ -94,23 +94,38 @@ __device__ __forceinline__ void put_top(const LogprobParams& p, long long r, int
     p.top_logprobs[r * p.k + rank] = (key_value(key) - a.m) - ls;
 }
 
-// One workgroup of NT threads to a row (rows beyond the grid in turn), tiles of
-// NT * LP_NV vectors of it in registers: a row of one tile is read from memory
+// Rows of a workgroup whose rows take NT threads each: a wave's rows share one.
+constexpr int rows_of(int NT) { return NT == 64 ? 4 : 1; }
+
+// What the threads of a row wrote to LDS or memory, its other threads see.
+template <int NT>
+__device__ __forceinline__ void row_sync() {
+    if (NT == 64) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        __syncthreads();
+    }
+}
+
+// NT threads to a row (rows beyond the grid in turn), tiles of NT * LP_NV
+// vectors of it in registers: a row of one tile is read from memory
 // once, also for its alternatives. With PARTS, to part blockIdx.y of a row, whose
 // sums and alternatives go to the workspace for logprobs_join_kernel.
 template <class E, int NT, bool TOP, bool PARTS>
-__global__ __launch_bounds__(NT) void logprobs_kernel(LogprobParams p) {
-    constexpr int N = RowVec<E>::N, W = NT / 64;
+__global__ __launch_bounds__(NT * rows_of(NT)) void logprobs_kernel(LogprobParams p) {
+    constexpr int N = RowVec<E>::N, W = NT / 64, RW = rows_of(NT), CAP = LP_CAP / RW;
     __shared__ RowSums red[W];
     __shared__ float best_s[TOP ? W : 1][64];
-    __shared__ uint64_t cand[TOP ? LP_CAP : 1];
+    __shared__ uint64_t cand_s[RW][TOP ? CAP : 1];
     __shared__ uint64_t next_s[TOP ? W : 1];
-    __shared__ float thr_s;
-    __shared__ int count_s;
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    __shared__ float thr_s[RW];
+    __shared__ int count_s[RW];
+    const int tid = threadIdx.x % NT, lane = tid & 63, wv = tid >> 6, sub = threadIdx.x / NT;
+    uint64_t* cand = cand_s[sub];
     const int c0 = PARTS ? blockIdx.y * p.part : 0, cols = PARTS ? min(p.part, p.V - c0) : p.V;
     const int nvec = cols / N, tail = cols - nvec * N;
-    for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    for (long long r = (long long)blockIdx.x * RW + sub; r < p.rows; r += (long long)gridDim.x * RW) {
         const E* x = row_of<E>(p, r) + c0;
         const long long t = p.tokens[r];
         const bool ignored = t == p.ignore;
@@ -213,31 +228,31 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobParams p) {
                     for (int w = 1; w < W; w++) best = fmaxf(best, best_s[w][lane]);
                     const float thr = kth_largest(best, p.k);
                     if (lane == 0) {
-                        thr_s = thr;
-                        count_s = 0;
+                        thr_s[sub] = thr;
+                        count_s[sub] = 0;
                     }
                 }
-                __syncthreads();
-                const float thr = thr_s;
+                row_sync<NT>();
+                const float thr = thr_s[sub];
                 const auto hold = [&](float e, int i) {
-                    const int at = atomicAdd(&count_s, 1);
-                    if (at < LP_CAP) cand[at] = order_key(e, i);
+                    const int at = atomicAdd(&count_s[sub], 1);
+                    if (at < CAP) cand[at] = order_key(e, i);
                 };
                 each(thr, [&](float e, int i) {
                     if (e >= thr) hold(e, i);
                 });
-                __syncthreads();
-                n = count_s;
-                if (n > LP_CAP) {  // many equal elements: all above them, and those of the lowest columns
-                    __syncthreads();
-                    if (tid == 0) count_s = 0;
-                    __syncthreads();
+                row_sync<NT>();
+                n = count_s[sub];
+                if (n > CAP) {  // many equal elements: all above them, and those of the lowest columns
+                    row_sync<NT>();
+                    if (tid == 0) count_s[sub] = 0;
+                    row_sync<NT>();
                     each(thr, [&](float e, int i) {
-                        if (e > thr || (e == thr && i < c0 + LP_CAP / 2)) hold(e, i);
+                        if (e > thr || (e == thr && i < c0 + CAP / 2)) hold(e, i);
                     });
-                    __syncthreads();
-                    n = count_s;
-                    if (n < p.k || n > LP_CAP) n = -1;
+                    row_sync<NT>();
+                    n = count_s[sub];
+                    if (n < p.k || n > CAP) n = -1;
                 }
             }
             if (n >= 0) {
@@ -260,16 +275,18 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobParams p) {
                         const uint64_t o = __shfl_xor(next, d);
                         next = o > next ? o : next;
                     }
-                    __syncthreads();
-                    if (lane == 0) next_s[wv] = next;
-                    __syncthreads();
-                    for (int w = 0; w < W; w++) next = next_s[w] > next ? next_s[w] : next;
+                    if (W > 1) {
+                        __syncthreads();
+                        if (lane == 0) next_s[wv] = next;
+                        __syncthreads();
+                        for (int w = 0; w < W; w++) next = next_s[w] > next ? next_s[w] : next;
+                    }
                     if (tid == 0) put(rank, next);
                     below = next;
                 }
             }
         }
-        if (W > 1 || TOP) __syncthreads();  // the shared arrays are free for the next row
+        if (W > 1 || TOP) row_sync<NT>();  // the shared arrays are free for the next row
     }
 }
 
@@ -345,17 +362,17 @@ __global__ __launch_bounds__(1024) void loss_mean_kernel(LogprobParams p) {
     }
 }
 
-// The gradient of the columns [c0, c1) of a row by a workgroup: blockIdx.y's
+// The gradient of the columns [c0, c1) of a row by NT threads: blockIdx.y's
 // share of the row, whole vectors.
-constexpr int LG_NT = 256, LG_NV = 4;
+constexpr int LG_NV = 4;
 
-template <class E, bool ENTROPY>
-__global__ __launch_bounds__(LG_NT) void logprobs_grad_kernel(LogprobParams p, int share) {
-    constexpr int N = RowVec<E>::N;
-    const int tid = threadIdx.x;
+template <class E, int NT, bool ENTROPY>
+__global__ __launch_bounds__(256) void logprobs_grad_kernel(LogprobParams p, int share) {
+    constexpr int N = RowVec<E>::N, RW = 256 / NT;
+    const int tid = threadIdx.x % NT;
     const int c0 = blockIdx.y * share, c1 = min(c0 + share, p.V);
     const int nvec = (c1 - c0) / N, tail = c1 - c0 - nvec * N;
-    for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    for (long long r = (long long)blockIdx.x * RW + threadIdx.x / NT; r < p.rows; r += (long long)gridDim.x * RW) {
         const E* x = row_of<E>(p, r) + c0;
         E* dx = static_cast<E*>(p.dx) + r * p.V + c0;
         const long long t = p.tokens[r];
@@ -376,7 +393,7 @@ __global__ __launch_bounds__(LG_NT) void logprobs_grad_kernel(LogprobParams p, i
         if (!any) {
 #pragma unroll
             for (int c = 0; c < N; c++) o[c] = (E)0.f;
-            for (int i = tid; i < nvec; i += LG_NT) store_row(dx + (size_t)i * N, o);
+            for (int i = tid; i < nvec; i += NT) store_row(dx + (size_t)i * N, o);
             if (tid < tail) dx[nvec * N + tid] = (E)0.f;
             continue;
         }
@@ -387,13 +404,13 @@ __global__ __launch_bounds__(LG_NT) void logprobs_grad_kernel(LogprobParams p, i
             const float q = fast_exp2(l);
             return ENTROPY ? q * fmaf(fmaxf(l, kNothing), b, a) : q * a;
         };
-        for (int i0 = 0; i0 < nvec; i0 += LG_NT * LG_NV) {
+        for (int i0 = 0; i0 < nvec; i0 += NT * LG_NV) {
             typename RowVec<E>::type v[LG_NV];
 #pragma unroll
-            for (int j = 0; j < LG_NV; j++) v[j] = load_row(x + (size_t)min(i0 + j * LG_NT + tid, nvec - 1) * N);
+            for (int j = 0; j < LG_NV; j++) v[j] = load_row(x + (size_t)min(i0 + j * NT + tid, nvec - 1) * N);
 #pragma unroll
             for (int j = 0; j < LG_NV; j++) {
-                const int i = i0 + j * LG_NT + tid;
+                const int i = i0 + j * NT + tid;
                 if (i < nvec) {
 #pragma unroll
                     for (int c = 0; c < N; c++) o[c] = (E)grad((float)v[j][c]);
@@ -402,7 +419,7 @@ __global__ __launch_bounds__(LG_NT) void logprobs_grad_kernel(LogprobParams p, i
             }
         }
         if (tid < tail) dx[nvec * N + tid] = (E)grad((float)x[nvec * N + tid]);
-        __syncthreads();  // the elements that outputs read themselves are written again
+        row_sync<NT>();  // the elements that outputs read themselves are written again
         if (tid <= k) {
             const auto index = [&](int j) { return j == 0 ? t : p.top_ids[r * p.k + j - 1]; };
             const auto cot = [&](int j) { return j == 0 ? dlp : p.d_top[r * p.k + j - 1]; };
@@ -429,11 +446,23 @@ int row_parts(long long rows, int V, int size) {
 
 template <class E, int NT>
 void launch_rows(const LogprobParams& p, hipStream_t stream) {
-    const dim3 grid((unsigned)min(p.rows, (long long)LOGPROBS_MAX_GRID));
+    const dim3 grid((unsigned)min((p.rows + rows_of(NT) - 1) / rows_of(NT), (long long)LOGPROBS_MAX_GRID));
+    const dim3 block(NT * rows_of(NT));
     if (p.k > 0)
-        hipLaunchKernelGGL((logprobs_kernel<E, NT, true, false>), grid, dim3(NT), 0, stream, p);
+        hipLaunchKernelGGL((logprobs_kernel<E, NT, true, false>), grid, block, 0, stream, p);
     else
-        hipLaunchKernelGGL((logprobs_kernel<E, NT, false, false>), grid, dim3(NT), 0, stream, p);
+        hipLaunchKernelGGL((logprobs_kernel<E, NT, false, false>), grid, block, 0, stream, p);
+}
+
+template <class E, int NT>
+void launch_grad(const LogprobParams& p, int shares, hipStream_t stream) {
+    constexpr int N = RowVec<E>::N, RW = 256 / NT;
+    const int share = ((p.V + shares - 1) / shares + N - 1) / N * N;
+    const dim3 grid((unsigned)min((p.rows + RW - 1) / RW, (long long)LOGPROBS_MAX_GRID), (unsigned)((p.V + share - 1) / share));
+    if (p.d_entropy)
+        hipLaunchKernelGGL((logprobs_grad_kernel<E, NT, true>), grid, dim3(256), 0, stream, p, share);
+    else
+        hipLaunchKernelGGL((logprobs_grad_kernel<E, NT, false>), grid, dim3(256), 0, stream, p, share);
 }
 
 template <class E>
@@ -454,15 +483,14 @@ template <class E>
 void launch(const LogprobParams& p, bool grad, hipStream_t stream) {
     constexpr int N = RowVec<E>::N;
     if (grad) {
-        const long long shares = min((1024 + p.rows - 1) / p.rows, (long long)(p.V + LG_NT * N - 1) / (LG_NT * N));
-        const int share = (int)(((p.V + shares - 1) / shares + N - 1) / N * N);
-        const dim3 grid((unsigned)min(p.rows, (long long)LOGPROBS_MAX_GRID), (unsigned)((p.V + share - 1) / share));
-        if (p.d_entropy)
-            hipLaunchKernelGGL((logprobs_grad_kernel<E, true>), grid, dim3(LG_NT), 0, stream, p, share);
-        else
-            hipLaunchKernelGGL((logprobs_grad_kernel<E, false>), grid, dim3(LG_NT), 0, stream, p, share);
+        if (p.V <= 64 * LG_NV * N)
+            launch_grad<E, 64>(p, 1, stream);
+        else  // few rows shared out to about four workgroups of a compute unit
+            launch_grad<E, 256>(p, (int)min((1024 + p.rows - 1) / p.rows, (long long)(p.V + 256 * N - 1) / (256 * N)), stream);
     } else if (p.V <= 64 * LP_NV * N) {
         launch_rows<E, 64>(p, stream);
+    } else if (p.V <= 128 * LP_NV * N) {
+        launch_rows<E, 128>(p, stream);
     } else if (p.V <= 256 * LP_NV * N || p.rows >= 512) {
         launch_rows<E, 256>(p, stream);
     } else if (const int parts = row_parts(p.rows, p.V, sizeof(E)); parts > 1) {
