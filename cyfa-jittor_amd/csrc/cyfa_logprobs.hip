@@ -438,20 +438,19 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogprobParams p, int
 }
 
 // Parts of a row, a workgroup each: those of its tiles, where the rows leave
-// compute units idle and have more than one.
+// compute units idle and have four tiles or more. us on MI355X for rows of
+// 131072 bf16 logits, with no and with 20 alternatives, in four parts with their
+// join, and as one: 1 row 9.9 / 12.3, 11.9 / 17.7; 64 rows 11.3 / 14.2, 13.5 /
+// 18.5; 128 rows 15.3 / 22.8, 13.5 / 19.2. Two tiles gain less than their join's launch costs.
 int row_parts(long long rows, int V, int size) {
     const long long tile = 1024 * LP_NV * (16 / size), tiles = (V + tile - 1) / tile;
-    return (int)max(1ll, min(min(tiles, 256 / rows), (long long)LP_PARTS));
+    return tiles < 4 || rows > 64 ? 1 : (int)min(min(tiles, 256 / rows), (long long)LP_PARTS);
 }
 
-template <class E, int NT>
+template <class E, int NT, bool TOP>
 void launch_rows(const LogprobParams& p, hipStream_t stream) {
     const dim3 grid((unsigned)min((p.rows + rows_of(NT) - 1) / rows_of(NT), (long long)LOGPROBS_MAX_GRID));
-    const dim3 block(NT * rows_of(NT));
-    if (p.k > 0)
-        hipLaunchKernelGGL((logprobs_kernel<E, NT, true, false>), grid, block, 0, stream, p);
-    else
-        hipLaunchKernelGGL((logprobs_kernel<E, NT, false, false>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((logprobs_kernel<E, NT, TOP, false>), grid, dim3(NT * rows_of(NT)), 0, stream, p);
 }
 
 template <class E, int NT>
@@ -487,24 +486,33 @@ void launch(const LogprobParams& p, bool grad, hipStream_t stream) {
             launch_grad<E, 64>(p, 1, stream);
         else  // few rows shared out to about four workgroups of a compute unit
             launch_grad<E, 256>(p, (int)min((1024 + p.rows - 1) / p.rows, (long long)(p.V + 256 * N - 1) / (256 * N)), stream);
-    } else if (p.V <= 64 * LP_NV * N) {
-        launch_rows<E, 64>(p, stream);
-    } else if (p.V <= 128 * LP_NV * N) {
-        launch_rows<E, 128>(p, stream);
-    } else if (p.V <= 256 * LP_NV * N || p.rows >= 512) {
-        launch_rows<E, 256>(p, stream);
-    } else if (const int parts = row_parts(p.rows, p.V, sizeof(E)); parts > 1) {
-        launch_parts<E>(p, parts, stream);
-    } else {
-        launch_rows<E, 1024>(p, stream);
+        return;
     }
+    // Threads of a row, by us on MI355X (bf16; no / 20 alternatives):
+    //   2048 columns   32768 rows: 64 threads 27 / 61, 256 57 / 171;  1024 rows: 3.7 / 8.3, 4.4 / 8.2
+    //   4096           16384 rows: 25 / 50, 34 / 94;                   1024 rows: 4.3 / 10.7, 4.8 / 9.0
+    //   8192           1024 rows: 6.4 / 15.1, 5.6 / 10.3
+    //   32000          1 row: 256 threads 5.0 / 10.4, 1024 5.7 / 7.9;  256 rows: 6.3 / 12.6, 7.2 / 10.1;
+    //                  512 rows: 8.8 / 15.9, 11.2 / 18.6;              8192 rows: 94 / 154, 137 / 279
+    // A row's own steps (its reductions, the search for alternatives) take the
+    // time where rows are short or few: few threads a row share a workgroup, or
+    // many, one row to a compute unit, search its columns.
+    const int parts = row_parts(p.rows, p.V, sizeof(E));
+    if (parts > 1)
+        launch_parts<E>(p, parts, stream);
+    else if (p.V <= 128 * LP_NV * N)
+        p.k > 0 ? launch_rows<E, 64, true>(p, stream) : launch_rows<E, 64, false>(p, stream);
+    else if (p.k > 0 && p.rows <= 256 && p.V > 256 * LP_NV * N)
+        launch_rows<E, 1024, true>(p, stream);
+    else
+        p.k > 0 ? launch_rows<E, 256, true>(p, stream) : launch_rows<E, 256, false>(p, stream);
 }
 
 }  // namespace
 
 // Bytes of the parts' sums and keys, 0 where rows are not shared out.
 size_t logprobs_workspace_bytes(long long rows, int V, int k, int size) {
-    if (rows <= 0 || rows >= 512) return 0;
+    if (rows <= 0) return 0;
     const int parts = row_parts(rows, V, size);
     return parts > 1 ? (size_t)((rows * parts * 3 + 1) / 2 * 2) * 4 + (size_t)rows * parts * k * 8 : 0;
 }

@@ -979,7 +979,7 @@ def logit_rows(logits):
 
 def _logprobs_workspace(args, dtype, dev):
     """The call's workspace, set in args; the caller keeps it until the launch."""
-    if args.rows >= 512:  # (rows enough for the compute units: none)
+    if args.rows > 64 or args.V <= 32768:  # (rows enough for the compute units, or short ones: none)
         return None
     n = int(load_library().cyfa_logprobs_workspace_bytes(args.rows, args.V, args.k, LM_DTYPES[dtype]))
     if n == 0:
