@@ -4,6 +4,12 @@
 // The gradient sorts the positions by id, each id's positions in their order,
 // and adds each id's rows of dy in that order in fp32: no atomics on sums, so
 // two backward passes give the same bits, and the result is rounded once.
+//
+// us on MI355X for 16384 positions of natural frequencies, 1024 bf16 columns and
+// 32000 ids: the lookup 10.4 (33.5 MB written, the 10 MB of different rows read),
+// the gradient 43 in three launches for 33.5 MB read and 65.5 written: the sort
+// 16, the shared ids' chunks 5, the rows 21 (4.7 TB/s). Adding the positions by
+// atomics, zeroing and rounding an fp32 table took 200.
 #include "cyfa_internal.h"
 #include "cyfa_rows.h"
 
@@ -41,6 +47,11 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedParams p) {
 // of the positions behind those of the waves before it. Ids outside [0, V) count
 // nowhere.
 //   slot(v) = (v mod G) range + v / G;  offsets[slot] .. offsets[slot + 1]: where v's positions lie in order
+// Every workgroup reading every id costs less than passes of a radix sort would
+// in launches: on MI355X 300 positions take 6.5 us, 4096 10, 16384 11.5 (16 where
+// one workgroup's ids are a fifteenth of them, whose wave-by-wave placing then
+// takes the time), 32768 21 (30). Up to 16384 positions stay in registers between
+// counting and placing.
 constexpr int ES_NT = 1024, ES_WAVES = ES_NT / 64, ES_U = 16;
 constexpr int ES_RANGE = 512;  // most ids of a workgroup: 33 KB of LDS
 
@@ -139,7 +150,9 @@ __global__ __launch_bounds__(ES_NT) void embed_sort_kernel(EmbedParams p) {
 }
 
 // Adds dy's rows of the sorted positions [s, e) (the same in every lane) in
-// order, the columns of one vector of this lane, EG_U rows' loads in flight.
+// order, the columns of one vector of this lane, EG_U rows' loads in flight (the
+// 16384 positions above: the chunks 11.5 us with 4, 5.3 with 8 and 16; the rows
+// 24.8, 21.4 and 24.8).
 constexpr int EG_U = 8;
 
 template <class E>
@@ -159,7 +172,8 @@ __device__ __forceinline__ void add_rows(const EmbedParams& p, const E* dy, int 
 
 // An id with many positions is shared out: every EMBED_CHUNK sorted positions
 // that all hold one id are added by a wave of embed_part_kernel, and
-// embed_grad_kernel adds the id's chunks and what is left at both ends.
+// embed_grad_kernel adds the id's chunks and what is left at both ends (chunks of
+// 64 took 13.6 us for the 5 of 32: a wave's rows come eight at a time).
 //
 // Columns of a wave: 64 vectors; the last, ragged vector of a row is read and
 // written ending at the row's end, so that it overlaps the one before it

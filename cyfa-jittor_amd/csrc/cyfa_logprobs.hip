@@ -7,7 +7,17 @@
 //          outputs that read x_i itself,  p_i = e^(x_i - m) / S,
 //          A = -(sum of the cotangents of logprob and of the alternatives)
 // One pass over the row each way: the forward keeps m, log S and the entropy of
-// each row for the gradient, in fp32 as every sum here.
+// each row for the gradient, in fp32 as every sum here. (lse = m + log S alone
+// would round away the low bits of log S beside a large m, and p with them.)
+//
+// Bound by the memory's rate where rows are many: an element costs ten VALU
+// instructions and one exponential at a quarter of their rate, two thirds of the
+// time of its bytes. On MI355X 16384 x 32000 bf16 rows (1.05 GB) take 177 us
+// forward (5.9 TB/s; a copy of 1 GiB moves 5.1), their loss with three labels of
+// ten ignored 129 us (those rows are not read), its gradient 322 us (5.5 TB/s of
+// 0.73 GB read and 1.05 written). The plain chain of fp32 operations took 7.35 ms
+// and, with the gradient, 5.2 ms. Few rows are bound by the latency of a row's
+// own steps: one row of 32000 with five alternatives 8 us, 64 rows with twenty 10.
 #include "cyfa_internal.h"
 #include "cyfa_rows.h"
 
@@ -17,9 +27,10 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;
-constexpr int LP_CAP = 1024;            // candidates for the alternatives held in LDS
-constexpr int LP_PARTS = 16;             // most parts of a row
-constexpr int LP_NV = 4;                // vectors of a thread in a tile of a row
+constexpr float kNothing = -200.f;  // the exponent (of 2) of what counts nothing: 0 times minus infinity would be a NaN
+constexpr int LP_CAP = 1024;        // candidates for the alternatives held in LDS
+constexpr int LP_PARTS = 16;        // most parts of a row
+constexpr int LP_NV = 4;            // vectors of a thread in a tile of a row: 64 bytes in flight
 
 // The order of the alternatives as an unsigned key: larger values first (a NaN
 // largest, as torch.topk has it; -0 equals +0), then the lower index.
@@ -46,13 +57,10 @@ struct RowSums {
 __device__ __forceinline__ void rescale(RowSums& a, float m) {
     const float d = (a.m - m) * kLog2e;  // m is finite or +inf, never below a.m
     const float f = fast_exp2(d);
-    a.s1 = f * (a.s1 + fmaxf(d, -200.f) * a.s);
+    a.s1 = f * (a.s1 + fmaxf(d, kNothing) * a.s);
     a.s *= f;
     a.m = m;
 }
-
-// The exponent of an element that counts nothing: 0 times minus infinity would be a NaN.
-constexpr float kNothing = -200.f;
 
 template <class E>
 __device__ __forceinline__ const E* row_of(const LogprobParams& p, long long r) {
@@ -363,7 +371,10 @@ __global__ __launch_bounds__(1024) void loss_mean_kernel(LogprobParams p) {
 }
 
 // The gradient of the columns [c0, c1) of a row by NT threads: blockIdx.y's
-// share of the row, whole vectors.
+// share of the row, whole vectors. Rows up to 2048 bf16 columns take a wave each
+// (2^28 logits in rows of 2048: 185 us on MI355X, 285 with a workgroup to a row;
+// in rows of 256, 510 and 1790). The elements that outputs read themselves are
+// stored a second time, by one thread each, rather than looked for at every element.
 constexpr int LG_NV = 4;
 
 template <class E, int NT, bool ENTROPY>
