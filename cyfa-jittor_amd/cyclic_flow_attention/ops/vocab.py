@@ -1,7 +1,7 @@
 """The vocabulary's two ends of a causal language model on the gfx950 HIP path:
 the scaled embedding lookup, and log probabilities of tokens with their mean as
 the training loss (the reference's nn.Embedding and cross_entropy_loss,
-models/cyfa/modeling_cyfa.py:59-66, 101-106 of Chyxx/CyFA-Jittor v0.1.2).
+models/cyfa/modeling_cyfa.py:63-71, 96-108 of Chyxx/CyFA-Jittor v0.1.2).
 
 Each computes in fp32 whatever the dtype (bf16, fp16 or fp32) and rounds its
 results once. Where an input requires a gradient the call is recorded for

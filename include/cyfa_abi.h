@@ -593,7 +593,7 @@ int cyfa_gates(const void *abd, long long abd_row, const float *dt_bias, const f
  * NaN. grad 1 reads stats, entropy (with d_entropy), top_ids (with d_top) and
  * count (with d_loss) as grad 0 left them and writes dx [rows, V], contiguous;
  * rows whose cotangents are all zero become zero without reading x. No
- * counterpart in the reference but the loss (models/cyfa/modeling_cyfa.py:101-106). */
+ * counterpart in the reference but the loss (models/cyfa/modeling_cyfa.py:96-108). */
 typedef struct CyfaLogprobArgs {
     long long rows, inner;        /* inner > 0 */
     long long outer_stride, row_stride;
@@ -623,7 +623,7 @@ int cyfa_logprobs(const CyfaLogprobArgs *args, int dtype, int grad, void *hip_st
  * and rounded once; weight, out, dy, dweight CYFA_DTYPE_BF16, _F32 or _F16,
  * contiguous, any alignment. An id outside [0, V) gives a row of NaN and has no
  * gradient, nor has the id padding (-1: none). n <= 2^30, V <= 2^26, D <= 2^20. Replaces
- * nn.Embedding (models/cyfa/modeling_cyfa.py:59-66) and its adjoint. */
+ * nn.Embedding (models/cyfa/modeling_cyfa.py:63-71) and its adjoint. */
 typedef struct CyfaEmbedArgs {
     long long n, V;
     int D;
