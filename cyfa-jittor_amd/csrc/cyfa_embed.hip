@@ -254,10 +254,7 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(EmbedParams p) {
             typename RowVec<E>::type o;
 #pragma unroll
             for (int i = 0; i < N; i++) o[i] = (E)(acc[i] * p.scale);
-            if (STREAM)
-                __builtin_nontemporal_store(o, reinterpret_cast<typename RowVec<E>::type*>(out + at));
-            else
-                store_row(out + at, o);
+            store_row<E, STREAM>(out + at, o);
         } else {
             for (int i = 0; i < p.D; i++) {
                 float a = 0.f;

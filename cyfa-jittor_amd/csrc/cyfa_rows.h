@@ -14,16 +14,23 @@ struct RowVec {
     typedef E type __attribute__((ext_vector_type(16 / sizeof(E))));
 };
 
-template <class E>
+// PAST: of a 16-byte aligned vector that nothing reads again soon, past the caches.
+template <class E, bool PAST = false>
 __device__ __forceinline__ typename RowVec<E>::type load_row(const E* p) {
     typename RowVec<E>::type v;
-    __builtin_memcpy(&v, p, 16);
+    if (PAST)
+        v = __builtin_nontemporal_load(reinterpret_cast<const typename RowVec<E>::type*>(p));
+    else
+        __builtin_memcpy(&v, p, 16);
     return v;
 }
 
-template <class E>
+template <class E, bool PAST = false>
 __device__ __forceinline__ void store_row(E* p, const typename RowVec<E>::type& v) {
-    __builtin_memcpy(p, &v, 16);
+    if (PAST)
+        __builtin_nontemporal_store(v, reinterpret_cast<typename RowVec<E>::type*>(p));
+    else
+        __builtin_memcpy(p, &v, 16);
 }
 
 }  // namespace cyfa

@@ -1021,17 +1021,17 @@ def logprobs_grad(logits, tokens, k, ignore, stats, entropy, ids, d_logprob, d_e
     return dx
 
 
-def token_loss(logits, labels, ignore):
-    """(loss, what token_loss_grad needs): the mean of -logprob over the labels
-    (int64, contiguous) that are not ``ignore``."""
+def token_loss(logits, labels, ignore, stats=False):
+    """(loss, what token_loss_grad needs, with ``stats``): the mean of -logprob
+    over the labels (int64, contiguous) that are not ``ignore``."""
     dev = require_device(logits, labels)
     fields, logits = logit_rows(logits)
     rows = fields[0]
     loss = torch.empty((), dtype=torch.float32, device=dev)
     kept = torch.empty(3 * rows + 1, dtype=torch.float32, device=dev)  # stats, logprob, count
     at = kept.data_ptr()
-    args = CyfaLogprobArgs(*fields, tokens=labels.data_ptr(), ignore=ignore, stats=at, logprob=at + 8 * rows,
-                           loss=loss.data_ptr(), count=at + 12 * rows)
+    args = CyfaLogprobArgs(*fields, tokens=labels.data_ptr(), ignore=ignore, stats=at if stats else None,
+                           logprob=at + 8 * rows, loss=loss.data_ptr(), count=at + 12 * rows)
     workspace = _logprobs_workspace(args, logits.dtype, dev)  # noqa: F841 (alive until the launch)
     _lm_call("cyfa_logprobs", args, logits.dtype, 0, dev)
     return loss, kept

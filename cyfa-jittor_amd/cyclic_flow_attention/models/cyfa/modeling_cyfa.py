@@ -148,7 +148,8 @@ class CyclicFlowAttentionModel(nn.Module):
         """The embeddings of input_ids. A training step on the GPU looks them up
         with the gradient by sorted tokens (the same bits every time)."""
         e = self.embeddings
-        if (plain_module(e, nn.Embedding) and e.weight.requires_grad and e.weight.dtype in _native.LM_DTYPES
+        if (torch.is_grad_enabled() and plain_module(e, nn.Embedding) and e.weight.requires_grad
+                and e.weight.dtype in _native.LM_DTYPES
                 and e.max_norm is None and not e.sparse and not e.scale_grad_by_freq
                 and input_ids.dtype in (torch.int64, torch.int32) and input_ids.device == e.weight.device
                 and type(input_ids) is torch.Tensor and hip_autograd_ok(e.weight)):

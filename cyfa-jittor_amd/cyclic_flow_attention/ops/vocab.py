@@ -150,7 +150,7 @@ class _TokenLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, labels, ignore_index):
-        loss, kept = _native.token_loss(logits, labels, ignore_index)
+        loss, kept = _native.token_loss(logits, labels, ignore_index, stats=True)
         ctx.save_for_backward(logits, labels, kept)
         ctx.ignore_index = ignore_index
         return loss

@@ -629,3 +629,135 @@ def test_together_on_another_stream():
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- sizes and uses past the ordinary
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: their last rows as in calls of their own."""
+    ops = _ops()
+    rows, V = 70001, 32001
+    assert rows * V > 2**31
+    x = torch.zeros(rows, V, dtype=BF, device="cuda")
+    last = (_randn(1, 3, V) * 3).to(BF).cuda()
+    x[-3:] = last
+    tokens = torch.full((rows,), 5, device="cuda")
+    tokens[-3:] = torch.tensor([0, V - 1, 77])
+    x.requires_grad_(True)
+    got = ops.token_logprobs(x, tokens, top_k=3)
+    ends = last.cpu().double()
+    ref = lm.logprobs(ends, tokens[-3:].cpu(), 3)
+    for name, value in (("logprob", got.logprob), ("entropy", got.entropy), ("top", got.top_logprobs)):
+        lm.assert_within(value[-3:], *ref[name], name)
+    assert torch.equal(got.top_ids[-3:].cpu(), ref["ids"]) and got.top_ids[5].tolist() == [0, 1, 2]
+    d = torch.zeros(rows)
+    d[-3:] = torch.tensor([1.0, -2.0, 0.5])
+    (dx,) = torch.autograd.grad(got.logprob, [x], d.cuda())
+    lm.assert_within(dx[-3:], *lm.logprobs_grad(ends, tokens[-3:].cpu(), None, d[-3:].double(), None, None, BF), "dx")
+    assert not dx[:-3].any()
+    del x, dx, got
+
+    n, D = 70001, 32001
+    w = _randn(2, 3, D).to(BF).cuda().requires_grad_(True)
+    ids = torch.zeros(n, dtype=torch.int64, device="cuda")
+    ids[-2:] = torch.tensor([1, 2])
+    out = ops.embed_tokens(ids, w, padding_idx=0)
+    assert torch.equal(out[-2:], w[1:]) and torch.equal(out[-3], w[0])
+    dy = torch.zeros(n, D, dtype=BF, device="cuda")
+    dy[-2:] = _randn(3, 2, D).to(BF).cuda()
+    (dw,) = torch.autograd.grad(out, [w], dy)
+    assert torch.equal(dw[1:], dy[-2:]) and not dw[0].any()
+    del out, dy, dw
+
+    rows, D = 270001, 8001
+    assert rows * D > 2**31
+    t, d_s, d_h = _join_inputs(3, D, BF, False, False, seed=4)
+    x, y = (torch.zeros(rows, D, dtype=BF, device="cuda") for _ in range(2))
+    x[-3:], y[-3:] = t["x"], t["y"]
+    weight = t["weight"].cuda()
+    s, h = ops.residual_norm(x.requires_grad_(True), y, weight)
+    ref = lm.residual(*(v.double() for v in (t["x"], t["y"], t["weight"])), None, None, 1.0, 1e-6, d_s.double(), d_h.double())
+    lm.assert_within(s[-3:], ref["s"][0], lm.rounded(*ref["s"], BF), "s")
+    lm.assert_within(h[-3:], ref["h"][0], lm.rounded(*ref["h"], BF), "h")
+    dh = torch.zeros_like(y)
+    dh[-3:] = d_h
+    (dx,) = torch.autograd.grad(h, [x], dh)
+    ref = lm.residual(*(v.double() for v in (t["x"], t["y"], t["weight"])), None, None, 1.0, 1e-6, 0 * d_s.double(), d_h.double())
+    lm.assert_within(dx[-3:], ref["x"][0], lm.rounded(*ref["x"], BF), "dx")
+    assert not dx[:-3].any()
+
+
+@pytest.mark.parametrize("rows,V,dtype", [(2100, 32000, BF), (1100, 32000, F32), (40000, 2048, F16), (2100, 32004, BF)])
+def test_rows_past_the_caches(rows, V, dtype):
+    """Logits and gradients of 128 MiB or more, in whole lines and not: the same
+    bits as in calls of fewer rows, and the formulas' on some."""
+    ops = _ops()
+    x = (torch.randn(rows, V, device="cuda", generator=torch.Generator("cuda").manual_seed(V)) * 3).to(dtype)
+    assert x.numel() * x.element_size() >= 128 << 20
+    tokens = _randint(rows, V, rows).cuda()
+    with torch.no_grad():
+        plain = ops.token_logprobs(x, tokens)
+        plain_loss = ops.token_loss(x, tokens)
+    x.requires_grad_(True)
+    got = ops.token_logprobs(x, tokens)
+    loss = ops.token_loss(x, tokens)
+    assert torch.equal(plain.logprob, got.logprob) and torch.equal(plain.entropy, got.entropy) and torch.equal(plain_loss, loss)
+    d, e = _randn(1, rows), _randn(2, rows)
+    (dx,) = torch.autograd.grad([got.logprob, got.entropy], [x], [d.cuda(), e.cuda()])
+    (dl,) = torch.autograd.grad(loss, [x])
+    some = torch.tensor([0, 1, rows // 2, rows - 1])
+    xd, td = x.detach()[some.cuda()].cpu().double(), tokens.cpu()[some]
+    lm.assert_within(got.logprob[some.cuda()], *lm.logprobs(xd, td)["logprob"], "logprob")
+    lm.assert_within(dx[some.cuda()], *lm.logprobs_grad(xd, td, None, d[some].double(), e[some].double(), None, dtype), "dx")
+    lm.assert_within(dl[some.cuda()], *lm.logprobs_grad(xd, td, None, torch.full((4,), -1.0 / rows).double(), None, None, dtype), "dl")
+    for part in (slice(0, rows // 3), slice(rows // 3, rows // 2 + 7)):
+        own = x.detach()[part].clone().requires_grad_(True)
+        r = ops.token_logprobs(own, tokens[part])
+        (own_dx,) = torch.autograd.grad([r.logprob, r.entropy], [own], [d.cuda()[part], e.cuda()[part]])
+        assert torch.equal(own_dx, dx[part]) and torch.equal(r.logprob, got.logprob[part])
+
+
+def test_two_backward_passes_and_calls_of_two_threads():
+    """A retained graph gives the same gradients again, and calls of two threads on streams of their own do not meet."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    ids, labels, params = _tiny_inputs()
+    ops = _ops()
+
+    def gradients(stream):
+        with torch.cuda.stream(stream):
+            p = [t.cuda().requires_grad_(True) for t in params]
+            lab = labels.cuda()
+            loss = _tiny_lm(ids.cuda(), lab, *_unpack(p), ops=ops)
+            first = torch.autograd.grad(loss, p, retain_graph=True)
+            second = torch.autograd.grad(loss, p)
+            big = ops.token_logprobs(_randn(3, 2, 140000).cuda(), torch.tensor([5, 139999]).cuda(), top_k=5)
+            stream.synchronize()
+        return [loss.detach(), *first, *second, big.logprob, big.entropy, big.top_logprobs, big.top_ids]
+
+    want = gradients(torch.cuda.Stream())
+    k = len(params)
+    for a, b in zip(want[1:1 + k], want[1 + k:1 + 2 * k]):
+        assert torch.equal(a, b)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    with ThreadPoolExecutor(2) as pool:
+        for _ in range(3):
+            for got in pool.map(gradients, streams):
+                assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_inference_tensors_and_frozen_inputs():
+    ops = _ops()
+    with torch.inference_mode():
+        x = _randn(1, 4, 33).cuda()
+        t = torch.tensor([0, 1, 2, 32]).cuda()
+        lp = ops.token_logprobs(x, t, top_k=1)
+        loss = ops.token_loss(x, t)
+        e = ops.embed_tokens(t, x)
+        s, h = ops.residual_norm(x, x, torch.ones(33, device="cuda"))
+    assert abs(loss.item() + lp.logprob.mean().item()) < 1e-5
+    assert not (lp.logprob.requires_grad or e.requires_grad or s.requires_grad)
+    assert torch.equal(s, x + x) and h.shape == x.shape
+    frozen = ops.token_logprobs(x.clone(), t)  # grad mode, nothing to record
+    assert not frozen.logprob.requires_grad and torch.equal(frozen.logprob, lp.logprob)
