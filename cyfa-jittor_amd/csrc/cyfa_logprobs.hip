@@ -12,9 +12,9 @@
 //
 // Bound by the memory's rate where rows are many: an element costs ten VALU
 // instructions and one exponential at a quarter of their rate, two thirds of the
-// time of its bytes. On MI355X 16384 x 32000 bf16 rows (1.05 GB) take 177 us
-// forward (5.9 TB/s; a copy of 1 GiB moves 5.1), their loss with three labels of
-// ten ignored 129 us (those rows are not read), its gradient 322 us (5.5 TB/s of
+// time of its bytes. On MI355X 16384 x 32000 bf16 rows (1.05 GB) take 156 us
+// forward (6.7 TB/s; a copy of 1 GiB moves 5.1), their loss with three labels of
+// ten ignored 128 us (those rows are not read), its gradient 312 us (5.7 TB/s of
 // 0.73 GB read and 1.05 written). The plain chain of fp32 operations took 7.35 ms
 // and, with the gradient, 5.2 ms. Few rows are bound by the latency of a row's
 // own steps: one row of 32000 with five alternatives 8 us, 64 rows with twenty 10.
