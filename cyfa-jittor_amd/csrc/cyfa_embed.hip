@@ -7,8 +7,8 @@
 //
 // us on MI355X for 16384 positions of natural frequencies, 1024 bf16 columns and
 // 32000 ids: the lookup 10.4 (33.5 MB written, the 10 MB of different rows read),
-// the gradient 43 in three launches for 33.5 MB read and 65.5 written: the sort
-// 16, the shared ids' chunks 5, the rows 21 (4.7 TB/s). Adding the positions by
+// the gradient 40 in three launches for 33.5 MB read and 65.5 written: the sort
+// 14, the shared ids' chunks 5, the rows 21 (4.7 TB/s). Adding the positions by
 // atomics, zeroing and rounding an fp32 table took 200.
 #include "cyfa_internal.h"
 #include "cyfa_rows.h"
@@ -48,11 +48,13 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedParams p) {
 // nowhere.
 //   slot(v) = (v mod G) range + v / G;  offsets[slot] .. offsets[slot + 1]: where v's positions lie in order
 // Every workgroup reading every id costs less than passes of a radix sort would
-// in launches: on MI355X 300 positions take 6.5 us, 4096 10, 16384 11.5 (16 where
-// one workgroup's ids are a fifteenth of them, whose wave-by-wave placing then
-// takes the time), 32768 21 (30). Up to 16384 positions stay in registers between
-// counting and placing.
+// in launches: on MI355X 300 positions take 6.5 us, 4096 8, 16384 11 (14 where one
+// workgroup's ids are a fifteenth of them, 24 where all are one id: that
+// workgroup's placing takes the time; with the ids of a wave's positions always
+// told apart bit by bit 12, 16 and 27), 32768 19 (25, 47). Up to 16384 positions
+// stay in registers between counting and placing.
 constexpr int ES_NT = 1024, ES_WAVES = ES_NT / 64, ES_U = 16;
+constexpr int ES_FEW = 8;      // different ids of 64 positions that are matched one after another
 constexpr int ES_RANGE = 512;  // most ids of a workgroup: 33 KB of LDS
 
 __global__ __launch_bounds__(ES_NT) void embed_sort_kernel(EmbedParams p) {
@@ -96,11 +98,20 @@ __global__ __launch_bounds__(ES_NT) void embed_sort_kernel(EmbedParams p) {
                     if (here) atomicAdd(&own[id], 1);
                     continue;
                 }
-                uint64_t same = __ballot(here);
-                if (!same) continue;
-                for (int b = 1; b < range; b <<= 1) {  // the lanes with this lane's id, bit by bit
-                    const uint64_t bit = __ballot((id & b) != 0);
-                    same &= (id & b) ? bit : ~bit;
+                const uint64_t all = __ballot(here);
+                if (!all) continue;
+                uint64_t same = all, todo = range > 1 ? all : 0;  // same: the lanes with this lane's id
+                for (int i = 0; todo && i < ES_FEW; i++) {        // one id after another, while they are few
+                    const uint64_t m = __ballot(here && id == __builtin_amdgcn_readlane(id, __builtin_ctzll(todo)));
+                    if ((m >> lane) & 1) same = m;
+                    todo &= ~m;
+                }
+                if (todo) {  // many: bit by bit
+                    same = all;
+                    for (int b = 1; b < range; b <<= 1) {
+                        const uint64_t bit = __ballot((id & b) != 0);
+                        same &= (id & b) ? bit : ~bit;
+                    }
                 }
                 // (LDS serves a wave's accesses in order: the next step reads what this one wrote)
                 if (here) {

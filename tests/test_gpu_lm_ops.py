@@ -761,3 +761,14 @@ def test_inference_tensors_and_frozen_inputs():
     assert torch.equal(s, x + x) and h.shape == x.shape
     frozen = ops.token_logprobs(x.clone(), t)  # grad mode, nothing to record
     assert not frozen.logprob.requires_grad and torch.equal(frozen.logprob, lp.logprob)
+
+
+def test_embed_gradient_of_ids_that_share_a_remainder():
+    """Ids whose positions one workgroup of the sort places, few and many of them at a time."""
+    V, D, n = 60000, 8, 5000
+    for ids in (_randint(1, 200, n) * 256 + 3, _randint(2, 3, n) * 256, (torch.arange(n) % 230) * 256 + 255,
+                torch.where(_randint(3, 2, n) == 0, _randint(4, 230, n) * 256 + 7, torch.full((n,), 7))):
+        w = torch.zeros(V, D, device="cuda", requires_grad=True)
+        dy = _randn(5, n, D)
+        (dw,) = torch.autograd.grad(_ops().embed_tokens(ids.cuda(), w), [w], dy.cuda())
+        lm.assert_within(dw, *lm.embed_grad(ids, dy.double(), V, 1.0, -1, F32), "dw")
