@@ -7,8 +7,8 @@
 //
 // us on MI355X for 16384 positions of natural frequencies, 1024 bf16 columns and
 // 32000 ids: the lookup 10.4 (33.5 MB written, the 10 MB of different rows read),
-// the gradient 40 in three launches for 33.5 MB read and 65.5 written: the sort
-// 14, the shared ids' chunks 5, the rows 21 (4.7 TB/s). Adding the positions by
+// the gradient 37 in three launches for 33.5 MB read and 65.5 written: the sort
+// 14, the shared ids' chunks 5, the rows 18 (5.5 TB/s). Adding the positions by
 // atomics, zeroing and rounding an fp32 table took 200.
 #include "cyfa_internal.h"
 #include "cyfa_rows.h"
@@ -162,8 +162,8 @@ __global__ __launch_bounds__(ES_NT) void embed_sort_kernel(EmbedParams p) {
 
 // Adds dy's rows of the sorted positions [s, e) (the same in every lane) in
 // order, the columns of one vector of this lane, EG_U rows' loads in flight (the
-// 16384 positions above: the chunks 11.5 us with 4, 5.3 with 8 and 16; the rows
-// 24.8, 21.4 and 24.8).
+// 16384 positions above: the chunks 11.5 us with 4, 5.3 with 8 and 16; the rows,
+// by a first form of their kernel, 24.8, 21.4 and 24.8).
 constexpr int EG_U = 8;
 
 template <class E>
@@ -191,15 +191,17 @@ __device__ __forceinline__ void add_rows(const EmbedParams& p, const E* dy, int 
 // (the same values are stored twice), and rows below one vector go column by column.
 constexpr int EMBED_CHUNK = 32;
 constexpr size_t EMBED_STREAM = 128 << 20;
-constexpr int EMBED_GRID = 4096;  // workgroups, 8 of a compute unit at a time
+constexpr int EMBED_WAVES = 16384;  // 16 to a SIMD, where rows are taken in turn
 
 template <class E>
 __global__ __launch_bounds__(256) void embed_part_kernel(EmbedParams p) {
     constexpr int N = RowVec<E>::N;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int chunks = p.offsets[(long long)p.range << p.shift] / EMBED_CHUNK;
-    const int d = blockIdx.y * 64 * N + lane * N;
-    for (int c = blockIdx.x * 4 + wv; c < chunks; c += gridDim.x * 4) {
+    const int cols = (p.D + 64 * N - 1) / (64 * N), wave = blockIdx.x * 4 + wv, lines = gridDim.x * 4 / cols;
+    const int d = wave % cols * 64 * N + lane * N;
+    if (wave >= lines * cols) return;
+    for (int c = wave / cols; c < chunks; c += lines) {
         const int s = c * EMBED_CHUNK, e = s + EMBED_CHUNK;
         const long long id = p.ids[p.order[s]];
         if (id != p.ids[p.order[e - 1]] || id == p.padding || d >= p.D) continue;  // not one id's whole chunk
@@ -221,63 +223,81 @@ __global__ __launch_bounds__(256) void embed_part_kernel(EmbedParams p) {
     }
 }
 
-// STREAM: the gradient's lines, each written whole by one wave, go past the caches.
+// Columns [d, d + N) of the gradient's row v from its positions [s, e) in order.
+// STREAM: its lines, each written whole by one wave, go past the caches.
 template <class E, bool STREAM>
+__device__ __forceinline__ void embed_row(const EmbedParams& p, int v, int d, int s, int e) {
+    constexpr int N = RowVec<E>::N;
+    if (v == p.padding) e = s;
+    const int c0 = (s + EMBED_CHUNK - 1) / EMBED_CHUNK, c1 = e / EMBED_CHUNK;
+    const bool parts = c0 < c1;  // whole chunks [c0, c1) of this id
+    E* out = static_cast<E*>(p.dweight) + (long long)v * p.D;
+    if (p.D >= N) {
+        const int at = min(d, p.D - N);
+        const E* dy = static_cast<const E*>(p.dy) + at;
+        float acc[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) acc[i] = 0.f;
+        add_rows<E>(p, dy, s, parts ? c0 * EMBED_CHUNK : e, acc);
+        if (parts) {
+            for (int c = c0; c < c1; c += EG_U) {
+                float part[EG_U][N];
+#pragma unroll
+                for (int u = 0; u < EG_U; u++)
+                    __builtin_memcpy(part[u], p.part + (long long)min(c + u, c1 - 1) * p.D + at, sizeof(part[u]));
+#pragma unroll
+                for (int u = 0; u < EG_U; u++)
+                    if (c + u < c1)
+#pragma unroll
+                        for (int i = 0; i < N; i++) acc[i] += part[u][i];
+            }
+            add_rows<E>(p, dy, c1 * EMBED_CHUNK, e, acc);
+        }
+        typename RowVec<E>::type o;
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i] = (E)(acc[i] * p.scale);
+        store_row<E, STREAM>(out + at, o);
+    } else {
+        for (int i = 0; i < p.D; i++) {
+            float a = 0.f;
+            const E* dy = static_cast<const E*>(p.dy) + i;
+            for (int j = s; j < (parts ? c0 * EMBED_CHUNK : e); j++) a += (float)dy[(long long)p.order[j] * p.D];
+            if (parts) {
+                for (int c = c0; c < c1; c++) a += p.part[(long long)c * p.D + i];
+                for (int j = c1 * EMBED_CHUNK; j < e; j++) a += (float)dy[(long long)p.order[j] * p.D];
+            }
+            out[i] = (E)(a * p.scale);
+        }
+    }
+}
+
+__device__ __forceinline__ const int* embed_slot(const EmbedParams& p, int v) {
+    return p.offsets + ((long long)(v & ((1 << p.shift) - 1)) * p.range + (v >> p.shift));
+}
+
+// A wave for one piece of 64 vectors of a row, the waves along the rows and then
+// row after row, each with rows that lie the grid apart, or (ONCE) one row each.
+template <class E, bool ONCE, bool STREAM>
 __global__ __launch_bounds__(256) void embed_grad_kernel(EmbedParams p) {
     constexpr int N = RowVec<E>::N;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int d = blockIdx.y * 64 * N + lane * N, V = (int)p.V, waves = gridDim.x * 4;
-    const auto slot = [&](int v) {
-        v = min(v, V - 1);
-        return p.offsets + ((long long)(v & ((1 << p.shift) - 1)) * p.range + (v >> p.shift));
-    };
-    int v = blockIdx.x * 4 + wv;
-    int next_s = slot(v)[0], next_e = slot(v)[1];  // (the next row's positions are on their way while this one is added)
-    for (; v < V; v += waves) {
-        const int s = next_s, e = v == p.padding ? s : next_e;
-        next_s = slot(v + waves)[0];
-        next_e = slot(v + waves)[1];
-        if (d >= p.D) continue;
-        const int c0 = (s + EMBED_CHUNK - 1) / EMBED_CHUNK, c1 = e / EMBED_CHUNK;
-        const bool parts = c0 < c1;  // whole chunks [c0, c1) of this id
-        E* out = static_cast<E*>(p.dweight) + (long long)v * p.D;
-        if (p.D >= N) {
-            const int at = min(d, p.D - N);
-            const E* dy = static_cast<const E*>(p.dy) + at;
-            float acc[N];
-#pragma unroll
-            for (int i = 0; i < N; i++) acc[i] = 0.f;
-            add_rows<E>(p, dy, s, parts ? c0 * EMBED_CHUNK : e, acc);
-            if (parts) {
-                for (int c = c0; c < c1; c += EG_U) {
-                    float part[EG_U][N];
-#pragma unroll
-                    for (int u = 0; u < EG_U; u++)
-                        __builtin_memcpy(part[u], p.part + (long long)min(c + u, c1 - 1) * p.D + at, sizeof(part[u]));
-#pragma unroll
-                    for (int u = 0; u < EG_U; u++)
-                        if (c + u < c1)
-#pragma unroll
-                            for (int i = 0; i < N; i++) acc[i] += part[u][i];
-                }
-                add_rows<E>(p, dy, c1 * EMBED_CHUNK, e, acc);
-            }
-            typename RowVec<E>::type o;
-#pragma unroll
-            for (int i = 0; i < N; i++) o[i] = (E)(acc[i] * p.scale);
-            store_row<E, STREAM>(out + at, o);
-        } else {
-            for (int i = 0; i < p.D; i++) {
-                float a = 0.f;
-                const E* dy = static_cast<const E*>(p.dy) + i;
-                for (int j = s; j < (parts ? c0 * EMBED_CHUNK : e); j++) a += (float)dy[(long long)p.order[j] * p.D];
-                if (parts) {
-                    for (int c = c0; c < c1; c++) a += p.part[(long long)c * p.D + i];
-                    for (int j = c1 * EMBED_CHUNK; j < e; j++) a += (float)dy[(long long)p.order[j] * p.D];
-                }
-                out[i] = (E)(a * p.scale);
-            }
-        }
+    const int cols = (p.D + 64 * N - 1) / (64 * N), V = (int)p.V;
+    const long long wave = (long long)blockIdx.x * 4 + wv;
+    int v = (int)(wave / cols);
+    const int d = (int)(wave % cols) * 64 * N + lane * N, lines = gridDim.x * 4 / cols;
+    if (v >= (ONCE ? V : min(V, lines))) return;
+    int s = embed_slot(p, v)[0], e = embed_slot(p, v)[1];
+    if (ONCE) {
+        if (d < p.D) embed_row<E, STREAM>(p, v, d, s, e);
+        return;
+    }
+    while (v < V) {  // (the next row's positions are on their way while this one is added)
+        const int next = min(v + lines, V - 1);
+        const int next_s = embed_slot(p, next)[0], next_e = embed_slot(p, next)[1];
+        if (d < p.D) embed_row<E, STREAM>(p, v, d, s, e);
+        v += lines;
+        s = next_s;
+        e = next_e;
     }
 }
 
@@ -289,22 +309,24 @@ void launch(const EmbedParams& p, bool grad, hipStream_t stream) {
     }
     hipLaunchKernelGGL(embed_sort_kernel, dim3(1u << p.shift), dim3(ES_NT), (ES_WAVES * p.range + 2 * ES_WAVES) * sizeof(int),
                        stream, p);
-    // workgroups of four waves, a wave for 64 vectors of a row, the rows in turn
-    const int cols = (p.D + 64 * RowVec<E>::N - 1) / (64 * RowVec<E>::N);
-    const auto grid = [&](long long rows) {
-        return dim3((unsigned)max(1ll, min((rows + 3) / 4, (long long)EMBED_GRID / cols)), cols);
+    const int cols = (p.D + 64 * RowVec<E>::N - 1) / (64 * RowVec<E>::N);  // pieces of 64 vectors of a row
+    const auto grid = [&](long long rows, long long most) {
+        return dim3((unsigned)((min(rows * cols, max(most, (long long)cols)) + 3) / 4));
     };
-    const long long chunks = p.n / EMBED_CHUNK;
-    if (chunks) hipLaunchKernelGGL(embed_part_kernel<E>, grid(chunks), dim3(256), 0, stream, p);
-    // A gradient that the last-level cache cannot keep beside its inputs is
-    // streamed: 32000 x 2048 fp32 (262 MB) 54 us a launch, 74 through the caches;
-    // 131072 x 1024 bf16 55, 65. Rows off the 128-byte lines, which two waves write
-    // in part, lose by it (131072 x 1000 bf16 78, 68), and a gradient of 66 MB
-    // gains 1.5 us that its reader may pay.
-    if ((size_t)p.V * p.D * sizeof(E) >= EMBED_STREAM && p.D * sizeof(E) % 128 == 0 && (uintptr_t)p.dweight % 128 == 0)
-        hipLaunchKernelGGL((embed_grad_kernel<E, true>), grid(p.V), dim3(256), 0, stream, p);
+    if (const long long chunks = p.n / EMBED_CHUNK)
+        hipLaunchKernelGGL(embed_part_kernel<E>, grid(chunks, EMBED_WAVES), dim3(256), 0, stream, p);
+    // A gradient in whole lines that the last-level cache cannot keep is written in
+    // the order of memory, a wave for every piece, past the caches (fewer than 2^32
+    // threads); others by waves in turn. us on MI355X so, by a wave for every piece
+    // through the caches, and in turn: 86274 x 2048 fp32 with 2 positions 102, 119,
+    // 154 (a fill of it takes 103); 32000 x 2048 fp32 with 2999 42, 50, 54; 32000 x 1024
+    // bf16 with 16384 (66 MB) 17.6, 19.7, 18; 32000 x 1536 fp16 with 9 18.5, 20, 16;
+    // rows off the lines, 131072 x 1001 bf16 with 4000 52, 57, 47.
+    const bool lines = p.D * sizeof(E) % 128 == 0 && (uintptr_t)p.dweight % 128 == 0;
+    if ((size_t)p.V * p.D * sizeof(E) >= EMBED_STREAM && lines && p.V * cols < 1 << 26)
+        hipLaunchKernelGGL((embed_grad_kernel<E, true, true>), grid(p.V, p.V * cols), dim3(256), 0, stream, p);
     else
-        hipLaunchKernelGGL((embed_grad_kernel<E, false>), grid(p.V), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((embed_grad_kernel<E, false, false>), grid(p.V, EMBED_WAVES), dim3(256), 0, stream, p);
 }
 
 }  // namespace
