@@ -7,6 +7,7 @@ visible, every entry point raises.
 """
 
 import ctypes
+import functools
 import os
 from pathlib import Path
 
@@ -1054,10 +1055,14 @@ def embed(ids, weight, scale):
     dev = require_device(ids, weight)
     V, D = weight.shape
     out = torch.empty(ids.shape + (D,), dtype=weight.dtype, device=dev)
-    args = CyfaEmbedArgs(n=ids.numel(), V=V, D=D, ids=ids.data_ptr(), weight=weight.data_ptr(), scale=scale,
-                         out=out.data_ptr())
+    args = CyfaEmbedArgs(ids.numel(), V, D, ids.data_ptr(), weight.data_ptr(), scale, out.data_ptr())
     _lm_call("cyfa_embed", args, weight.dtype, 0, dev)
     return out
+
+
+@functools.lru_cache(64)
+def _embed_grad_bytes(n, V, D):
+    return int(load_library().cyfa_embed_grad_workspace_bytes(n, V, D))
 
 
 def embed_grad(ids, V, dy, scale, padding):
@@ -1066,10 +1071,10 @@ def embed_grad(ids, V, dy, scale, padding):
     D = dy.shape[-1]
     n = ids.numel()
     dw = torch.empty(V, D, dtype=dy.dtype, device=dev)
-    size = int(load_library().cyfa_embed_grad_workspace_bytes(n, V, D))
+    size = _embed_grad_bytes(n, V, D)
     workspace = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)  # alive until the launch
-    args = CyfaEmbedArgs(n=n, V=V, D=D, ids=ids.data_ptr(), scale=scale, padding=padding, dy=dy.data_ptr(),
-                         dweight=dw.data_ptr(), workspace=workspace.data_ptr(), workspace_bytes=size)
+    args = CyfaEmbedArgs(n, V, D, ids.data_ptr(), None, scale, None, padding, dy.data_ptr(), dw.data_ptr(),
+                         workspace.data_ptr(), size)
     _lm_call("cyfa_embed", args, dy.dtype, 1, dev)
     return dw
 
@@ -1082,10 +1087,15 @@ def residual_norm(x, y, weight, post, gate, scale, eps, stats=False):
     rows = x.numel() // D
     s, h = torch.empty_like(x), torch.empty_like(x)
     st = torch.empty(rows, 2, dtype=torch.float32, device=dev) if stats else None
-    args = CyfaResidualArgs(rows=rows, D=D, x=x.data_ptr(), y=y.data_ptr(), gate=ptr(gate), weight=weight.data_ptr(),
-                            post=ptr(post), scale=scale, eps=eps, s=s.data_ptr(), h=h.data_ptr(), stats=ptr(st))
+    args = CyfaResidualArgs(rows, D, x.data_ptr(), y.data_ptr(), ptr(gate), weight.data_ptr(), ptr(post), scale, eps,
+                            s.data_ptr(), h.data_ptr(), ptr(st))
     _lm_call("cyfa_residual_norm", args, x.dtype, 0, dev)
     return s, h, st
+
+
+@functools.lru_cache(64)
+def _residual_grad_bytes(rows, D):
+    return int(load_library().cyfa_residual_grad_workspace_bytes(rows, D))
 
 
 def residual_norm_grad(x, y, weight, post, gate, scale, eps, stats, d_s, d_h, needed):
@@ -1097,13 +1107,13 @@ def residual_norm_grad(x, y, weight, post, gate, scale, eps, stats, d_s, d_h, ne
     plain = post is None and gate is None and scale == 1.0  # dy is dx
     dx = torch.empty_like(x) if needed[0] or (plain and needed[1]) else None
     dy = torch.empty_like(x) if needed[1] and not plain else None
-    dw, dp = (torch.empty(D, dtype=torch.float32, device=dev) if n else None for n in needed[2:4])
+    dw = torch.empty(D, dtype=torch.float32, device=dev) if needed[2] else None
+    dp = torch.empty(D, dtype=torch.float32, device=dev) if needed[3] else None
     dg = torch.empty_like(x) if needed[4] else None
-    size = int(load_library().cyfa_residual_grad_workspace_bytes(rows, D))
+    size = _residual_grad_bytes(rows, D)
     workspace = torch.empty(size, dtype=torch.uint8, device=dev)  # alive until the launch
-    args = CyfaResidualArgs(rows=rows, D=D, x=x.data_ptr(), y=y.data_ptr(), gate=ptr(gate), weight=weight.data_ptr(),
-                            post=ptr(post), scale=scale, eps=eps, stats=stats.data_ptr(), d_s=ptr(d_s), d_h=ptr(d_h),
-                            dx=ptr(dx), dy=ptr(dy), dgate=ptr(dg), dweight=ptr(dw), dpost=ptr(dp),
-                            workspace=workspace.data_ptr(), workspace_bytes=size)
+    args = CyfaResidualArgs(rows, D, x.data_ptr(), y.data_ptr(), ptr(gate), weight.data_ptr(), ptr(post), scale, eps, None,
+                            None, stats.data_ptr(), ptr(d_s), ptr(d_h), ptr(dx), ptr(dy), ptr(dg), ptr(dw), ptr(dp),
+                            workspace.data_ptr(), size)
     _lm_call("cyfa_residual_norm", args, x.dtype, 1, dev)
     return dx if needed[0] else None, dx if plain and needed[1] else dy, dw, dp, dg

@@ -21,27 +21,33 @@ def residual_norm(x, y, weight, post_weight=None, gate=None, scale=1.0, eps=1e-6
     All in fp32, s and h rounded once (h is that of s before its rounding).
     Differentiable in every tensor; a backward pass that is itself recorded runs
     in torch operations."""
-    if x.dtype not in _native.LM_DTYPES:
-        raise NotImplementedError(f"residual_norm: x must be bf16, fp16 or fp32, got {x.dtype}")
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"residual_norm: x must be [..., width], got {tuple(x.shape)}")
-    D = x.shape[-1]
+    shape, dtype = x.shape, x.dtype
+    if dtype not in _native.LM_DTYPES:
+        raise NotImplementedError(f"residual_norm: x must be bf16, fp16 or fp32, got {dtype}")
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"residual_norm: x must be [..., width], got {tuple(shape)}")
+    D = shape[-1]
     if D > _native.RESIDUAL_MAX_D:
         raise NotImplementedError(f"residual_norm: at most {_native.RESIDUAL_MAX_D} columns, got {D}")
     for name, t in (("y", y), ("gate", gate)):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
-            raise ValueError(f"residual_norm: {name} must be {tuple(x.shape)} {x.dtype}, got {tuple(t.shape)} {t.dtype}")
+        if t is not None and (t.shape != shape or t.dtype != dtype):
+            raise ValueError(f"residual_norm: {name} must be {tuple(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}")
     for name, t in (("weight", weight), ("post_weight", post_weight)):
-        if t is not None and (tuple(t.shape) != (D,) or not t.dtype.is_floating_point):
+        if t is not None and (t.dim() != 1 or t.shape[0] != D or not t.dtype.is_floating_point):
             raise ValueError(f"residual_norm: {name} must be a float tensor of shape ({D},), got {tuple(t.shape)} {t.dtype}")
     if isinstance(scale, torch.Tensor):
         raise ValueError("residual_norm: the scale must be a number (a tensor's gradient would be lost)")
-    given = (x.contiguous(), y.contiguous(), weight.float().contiguous(),
-             None if post_weight is None else post_weight.float().contiguous(),
-             None if gate is None else gate.contiguous())
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
-        return _ResidualNorm.apply(*given, float(scale), float(eps))
-    return _native.residual_norm(*given, float(scale), float(eps))[:2]
+    scale, eps = float(scale), float(eps)
+    x, y, weight = x.contiguous(), y.contiguous(), weight.float().contiguous()
+    if post_weight is not None:
+        post_weight = post_weight.float().contiguous()
+    if gate is not None:
+        gate = gate.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or y.requires_grad or weight.requires_grad
+                                    or (post_weight is not None and post_weight.requires_grad)
+                                    or (gate is not None and gate.requires_grad)):
+        return _ResidualNorm.apply(x, y, weight, post_weight, gate, scale, eps)
+    return _native.residual_norm(x, y, weight, post_weight, gate, scale, eps)[:2]
 
 
 def _plain(x, y, weight, post, gate, scale, eps):
@@ -70,8 +76,11 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def backward(ctx, d_s, d_h):
         *inputs, stats = ctx.saved_tensors
-        needed = ctx.needs_input_grad[:5]
+        needed = ctx.needs_input_grad
         if _recorded(d_s, d_h):
-            return _torch_backward(lambda *a: _plain(*a, *ctx.args), inputs, needed, (d_s, d_h)) + (None, None)
-        d_s, d_h = (None if t is None else t.contiguous() for t in (d_s, d_h))
+            return _torch_backward(lambda *a: _plain(*a, *ctx.args), inputs, needed[:5], (d_s, d_h)) + (None, None)
+        if d_s is not None:
+            d_s = d_s.contiguous()
+        if d_h is not None:
+            d_h = d_h.contiguous()
         return _native.residual_norm_grad(*inputs, *ctx.args, stats, d_s, d_h, needed) + (None, None)

@@ -17,6 +17,10 @@ import torch.nn.functional as F
 from .. import _native
 
 
+_peek = torch._C._functorch.peek_interpreter_stack
+_is_batched = torch._C._functorch.is_legacy_batchedtensor
+
+
 class TokenLogprobs(NamedTuple):
     """token_logprobs' results; the last two are None without alternatives."""
 
@@ -67,10 +71,10 @@ def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
 
 def _recorded(*cotangents):
     """Whether this backward pass is itself recorded, or batched (vmap)."""
-    if torch.is_grad_enabled() or torch._C._functorch.peek_interpreter_stack() is not None:
+    if torch.is_grad_enabled() or _peek() is not None:
         return True
     for t in cotangents:
-        if t is not None and torch._C._functorch.is_legacy_batchedtensor(t):
+        if t is not None and _is_batched(t):
             return True
     return False
 
