@@ -370,13 +370,13 @@ __global__ __launch_bounds__(1024) void loss_mean_kernel(LogprobParams p) {
     }
 }
 
+constexpr int LG_NV = 4;  // vectors of a thread in flight
+
 // The gradient of the columns [c0, c1) of a row by NT threads: blockIdx.y's
 // share of the row, whole vectors. Rows up to 2048 bf16 columns take a wave each
 // (2^28 logits in rows of 2048: 185 us on MI355X, 285 with a workgroup to a row;
 // in rows of 256, 510 and 1790). The elements that outputs read themselves are
 // stored a second time, by one thread each, rather than looked for at every element.
-constexpr int LG_NV = 4;
-
 //
 // The rows are taken from the last to the first: those that the forward read last
 // are in the caches still. A gradient of 128 MiB or more in whole lines goes past
@@ -553,14 +553,14 @@ size_t logprobs_workspace_bytes(long long rows, int V, int k, int size) {
 }
 
 void launch_logprobs(const LogprobParams& p, int dtype, bool grad, hipStream_t stream) {
-    if (p.rows == 0)
-        ;
-    else if (dtype == 0)
-        launch<bf16_t>(p, grad, stream);
-    else if (dtype == 1)
-        launch<float>(p, grad, stream);
-    else
-        launch<f16_t>(p, grad, stream);
+    if (p.rows > 0) {
+        if (dtype == 0)
+            launch<bf16_t>(p, grad, stream);
+        else if (dtype == 1)
+            launch<float>(p, grad, stream);
+        else
+            launch<f16_t>(p, grad, stream);
+    }
     if (!grad && p.loss) hipLaunchKernelGGL(loss_mean_kernel, dim3(1), dim3(1024), 0, stream, p);
 }
 
