@@ -183,9 +183,9 @@ __global__ __launch_bounds__(block_of(T)) void residual_norm_kernel(ResidualPara
 }
 
 // Workgroups of p.rows_wg rows; each leaves its sums for dweight and dpost in
-// part [workgroup][2][D], which residual_sum_kernel adds. The weights stay in
-// LDS (rows of a wave) or in registers; two waves per SIMD have to fit, so that
-// one's loads cover the other's arithmetic.
+// part [workgroup][2][D], which residual_sum_kernel adds (one workgroup alone, as
+// the gradients). The weights stay in LDS (rows of a wave) or in registers; two
+// waves per SIMD have to fit, so that one's loads cover the other's arithmetic.
 template <class E, int VN, int T, int J, bool POST, bool GATE>
 __global__ __launch_bounds__(block_of(T), 2) void residual_grad_kernel(ResidualParams p) {
     constexpr int RW = block_of(T) / T, C = J * T * VN;
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(block_of(T), 2) void residual_grad_kernel(ResidualP
         if (p.dy) cols.store(static_cast<E*>(p.dy) + o, d);
     }
     const auto leave = [&](float (&v)[J][VN], int which) {
-        float* out = p.part + ((long long)blockIdx.x * 2 + which) * p.D;
+        float* out = gridDim.x == 1 ? (which ? p.dpost : p.dweight) : p.part + ((long long)blockIdx.x * 2 + which) * p.D;
         if (RW == 1) {
             cols.store(out, v);
             return;
@@ -382,7 +382,13 @@ void launch(ResidualParams p, bool grad, hipStream_t stream) {
         hipLaunchKernelGGL((residual_norm_kernel<E, VN, T, J>), dim3((unsigned)min(groups, 1ll << 20)), block, 0, stream, p);
         return;
     }
-    p.rows_wg = grad_rows(p.rows);
+    // Up to four rows for every T threads of a workgroup: one workgroup alone, whose
+    // sums are the gradients. us on MI355X so and by several workgroups and
+    // their sums: 1024 bf16 columns, 4 rows 5.0 and 9.0, 16 rows 10.2 and 9.5 (13.3
+    // and 15.6 with the host's work for the launches), 64 rows 30 and 10; 4096
+    // columns, 4 rows 10.5 and 14.5, 16 rows 35 and 14.7.
+    constexpr int few = 4 * block_of(T) / T;
+    p.rows_wg = p.rows <= few ? few : grad_rows(p.rows);
     const int n = (int)((p.rows + p.rows_wg - 1) / p.rows_wg);
     if (n && p.post && p.gate)
         hipLaunchKernelGGL((residual_grad_kernel<E, VN, T, J, true, true>), dim3(n), block, 0, stream, p);
@@ -392,7 +398,8 @@ void launch(ResidualParams p, bool grad, hipStream_t stream) {
         hipLaunchKernelGGL((residual_grad_kernel<E, VN, T, J, false, true>), dim3(n), block, 0, stream, p);
     else if (n)
         hipLaunchKernelGGL((residual_grad_kernel<E, VN, T, J, false, false>), dim3(n), block, 0, stream, p);
-    if (p.dweight || p.dpost) hipLaunchKernelGGL(residual_sum_kernel, dim3((p.D + 31) / 32, 2), dim3(1024), 0, stream, p, n);
+    if (n != 1 && (p.dweight || p.dpost))
+        hipLaunchKernelGGL(residual_sum_kernel, dim3((p.D + 31) / 32, 2), dim3(1024), 0, stream, p, n);
 }
 
 // Threads of a row and vectors of each: up to 16 elements a thread, the most that

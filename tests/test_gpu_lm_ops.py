@@ -420,7 +420,7 @@ def _check_join(t, d_s, d_h, scale, eps, dtype, call=None):
     (1, 1, F32, 1.0), (3, 3, F32, 0.5), (2, 7, BF, 1.0), (5, 8, BF, 1.0), (4, 9, F16, -0.5), (3, 64, F32, 1.0), (65, 100, BF, 1.0),
     (2, 257, F32, 2.0), (9, 512, F16, 1.0), (5, 513, BF, 0.5), (1, 1024, BF, 1.0), (3, 1001, F32, 1.0), (2, 1536, BF, 1.0),
     (600, 40, BF, 1.0), (3, 2048, F32, 1.0), (4, 2049, BF, 1.0), (2, 5000, F16, 1.0), (2, 8192, F32, 1.0), (3, 8191, BF, 0.25),
-    (2100, 36, F32, 1.0)])
+    (2100, 36, F32, 1.0), (16, 520, BF, 1.0), (17, 520, BF, 1.0), (4, 3000, F32, 0.5), (5, 3000, F32, 0.5)])
 def test_residual_norm(rows, D, dtype, scale, post, gate):
     t, d_s, d_h = _join_inputs(rows, D, dtype, post, gate, seed=D)
     _check_join(t, d_s, d_h, scale, 1e-6, dtype)
