@@ -849,9 +849,10 @@ int cyfa_embed(const CyfaEmbedArgs* a, int dtype, int grad, void* hip_stream) {
     p.dweight = a->dweight;
     if (grad) {
         if (!a->dweight) return fail(CYFA_ERR_VALUE, "%s: null dweight", what);
-        if (!a->workspace || a->workspace_bytes < cyfa::embed_workspace(&p, a->n, a->V, a->D, a->workspace))
-            return fail(CYFA_ERR_WORKSPACE, "%s: workspace of %zu bytes", what, a->workspace ? a->workspace_bytes : (size_t)0);
-        if (!aligned(a->workspace, 256)) return fail(CYFA_ERR_ALIGN, "%s: workspace needs 256-byte alignment", what);
+        const size_t need = cyfa::embed_workspace(&p, a->n, a->V, a->D, a->workspace);
+        if (need && (!a->workspace || a->workspace_bytes < need))
+            return fail(CYFA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
+        if (need && !aligned(a->workspace, 256)) return fail(CYFA_ERR_ALIGN, "%s: workspace needs 256-byte alignment", what);
     }
     cyfa::launch_embed(p, dtype, grad != 0, (hipStream_t)hip_stream);
     return check_launch(what);

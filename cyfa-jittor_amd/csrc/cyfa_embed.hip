@@ -190,6 +190,7 @@ __device__ __forceinline__ void add_rows(const EmbedParams& p, const E* dy, int 
 // written ending at the row's end, so that it overlaps the one before it
 // (the same values are stored twice), and rows below one vector go column by column.
 constexpr int EMBED_CHUNK = 32;
+constexpr int EMBED_FEW = 64;  // positions that a wave's lanes hold
 constexpr size_t EMBED_STREAM = 128 << 20;
 constexpr int EMBED_WAVES = 16384;  // 16 to a SIMD, where rows are taken in turn
 
@@ -301,20 +302,64 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(EmbedParams p) {
     }
 }
 
+// The gradient from at most EMBED_FEW positions, unsorted, in one launch: a wave
+// holds every id, one in each lane, and finds the positions of a row by comparing.
+// us on MI355X so and sorted: 64 positions, 32000 x 1024 bf16 10.6 and 21 (all of one
+// id 14 and 21.5), 512 x 256 2.6 and 12.5; 30, 131072 x 1001 35 and 42.
+template <class E, bool STREAM>
+__global__ __launch_bounds__(256) void embed_few_kernel(EmbedParams p) {
+    constexpr int N = RowVec<E>::N;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = (int)p.n;
+    const int cols = (p.D + 64 * N - 1) / (64 * N), V = (int)p.V;
+    const int wave = blockIdx.x * 4 + wv, lines = gridDim.x * 4 / cols, d = wave % cols * 64 * N + lane * N;
+    if (wave >= lines * cols) return;
+    const long long id = lane < n ? p.ids[lane] : -1;
+    for (int v = wave / cols; v < V; v += lines) {
+        uint64_t at = __ballot(id == v && v != p.padding);  // the row's positions
+        if (d >= p.D) continue;
+        E* out = static_cast<E*>(p.dweight) + (long long)v * p.D;
+        if (p.D >= N) {
+            const int col = min(d, p.D - N);
+            float acc[N];
+#pragma unroll
+            for (int i = 0; i < N; i++) acc[i] = 0.f;
+            for (int left = __popcll(at); left > 0; left -= EG_U) {
+                typename RowVec<E>::type y[EG_U];
+#pragma unroll
+                for (int u = 0; u < EG_U; u++) {  // (the last position again where there are fewer)
+                    y[u] = load_row(static_cast<const E*>(p.dy) + (long long)__builtin_ctzll(at) * p.D + col);
+                    if (u + 1 < left) at &= at - 1;
+                }
+#pragma unroll
+                for (int u = 0; u < EG_U; u++)
+                    if (u < left)
+#pragma unroll
+                        for (int i = 0; i < N; i++) acc[i] += (float)y[u][i];
+            }
+            typename RowVec<E>::type o;
+#pragma unroll
+            for (int i = 0; i < N; i++) o[i] = (E)(acc[i] * p.scale);
+            store_row<E, STREAM>(out + col, o);
+        } else {
+            for (int i = 0; i < p.D; i++) {
+                float a = 0.f;
+                for (uint64_t m = at; m; m &= m - 1) a += (float)static_cast<const E*>(p.dy)[(long long)__builtin_ctzll(m) * p.D + i];
+                out[i] = (E)(a * p.scale);
+            }
+        }
+    }
+}
+
 template <class E>
 void launch(const EmbedParams& p, bool grad, hipStream_t stream) {
     if (!grad) {
         hipLaunchKernelGGL(embed_kernel<E>, dim3((unsigned)min((p.n + 3) / 4, 1ll << 20)), dim3(256), 0, stream, p);
         return;
     }
-    hipLaunchKernelGGL(embed_sort_kernel, dim3(1u << p.shift), dim3(ES_NT), (ES_WAVES * p.range + 2 * ES_WAVES) * sizeof(int),
-                       stream, p);
     const int cols = (p.D + 64 * RowVec<E>::N - 1) / (64 * RowVec<E>::N);  // pieces of 64 vectors of a row
     const auto grid = [&](long long rows, long long most) {
         return dim3((unsigned)((min(rows * cols, max(most, (long long)cols)) + 3) / 4));
     };
-    if (const long long chunks = p.n / EMBED_CHUNK)
-        hipLaunchKernelGGL(embed_part_kernel<E>, grid(chunks, EMBED_WAVES), dim3(256), 0, stream, p);
     // A gradient in whole lines that the last-level cache cannot keep is written in
     // the order of memory, a wave for every piece, past the caches (fewer than 2^32
     // threads); others by waves in turn. us on MI355X so, by a wave for every piece
@@ -323,16 +368,30 @@ void launch(const EmbedParams& p, bool grad, hipStream_t stream) {
     // bf16 with 16384 (66 MB) 17.6, 19.7, 18; 32000 x 1536 fp16 with 9 18.5, 20, 16;
     // rows off the lines, 131072 x 1001 bf16 with 4000 52, 57, 47.
     const bool lines = p.D * sizeof(E) % 128 == 0 && (uintptr_t)p.dweight % 128 == 0;
-    if ((size_t)p.V * p.D * sizeof(E) >= EMBED_STREAM && lines && p.V * cols < 1 << 26)
-        hipLaunchKernelGGL((embed_grad_kernel<E, true, true>), grid(p.V, p.V * cols), dim3(256), 0, stream, p);
+    const bool streamed = (size_t)p.V * p.D * sizeof(E) >= EMBED_STREAM && lines && p.V * cols < 1 << 26;
+    const dim3 rows = grid(p.V, streamed ? p.V * cols : EMBED_WAVES);
+    if (p.n <= EMBED_FEW) {
+        if (streamed)
+            hipLaunchKernelGGL((embed_few_kernel<E, true>), rows, dim3(256), 0, stream, p);
+        else
+            hipLaunchKernelGGL((embed_few_kernel<E, false>), rows, dim3(256), 0, stream, p);
+        return;
+    }
+    hipLaunchKernelGGL(embed_sort_kernel, dim3(1u << p.shift), dim3(ES_NT), (ES_WAVES * p.range + 2 * ES_WAVES) * sizeof(int),
+                       stream, p);
+    hipLaunchKernelGGL(embed_part_kernel<E>, grid(p.n / EMBED_CHUNK, EMBED_WAVES), dim3(256), 0, stream, p);
+    if (streamed)
+        hipLaunchKernelGGL((embed_grad_kernel<E, true, true>), rows, dim3(256), 0, stream, p);
     else
-        hipLaunchKernelGGL((embed_grad_kernel<E, false, false>), grid(p.V, EMBED_WAVES), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((embed_grad_kernel<E, false, false>), rows, dim3(256), 0, stream, p);
 }
 
 }  // namespace
 
 // offsets int [slots + 1], order int [n], part fp32 [n / chunk, D], each 256-byte aligned
+// (nothing for the few positions that are not sorted)
 size_t embed_workspace(EmbedParams* p, long long n, long long V, int D, void* base) {
+    if (n <= EMBED_FEW) return 0;
     const auto up = [](size_t b) { return (b + 255) / 256 * 256; };
     int shift = 8;  // a workgroup of the sort for each of 256 compute units, more for many ids
     while ((V + (1ll << shift) - 1) >> shift > ES_RANGE) shift++;

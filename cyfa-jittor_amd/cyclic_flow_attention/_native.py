@@ -1072,9 +1072,9 @@ def embed_grad(ids, V, dy, scale, padding):
     n = ids.numel()
     dw = torch.empty(V, D, dtype=dy.dtype, device=dev)
     size = _embed_grad_bytes(n, V, D)
-    workspace = torch.empty(max(size, 1), dtype=torch.uint8, device=dev)  # alive until the launch
+    workspace = torch.empty(size, dtype=torch.uint8, device=dev) if size else None  # alive until the launch
     args = CyfaEmbedArgs(n, V, D, ids.data_ptr(), None, scale, None, padding, dy.data_ptr(), dw.data_ptr(),
-                         workspace.data_ptr(), size)
+                         ptr(workspace), size)
     _lm_call("cyfa_embed", args, dy.dtype, 1, dev)
     return dw
 

@@ -634,7 +634,7 @@ typedef struct CyfaEmbedArgs {
     long long padding;
     const void *dy;               /* grad 1: [n, D] */
     void *dweight;                /* grad 1: [V, D], every row written */
-    void *workspace;              /* grad 1: cyfa_embed_grad_workspace_bytes(n, V, D) bytes, 256-byte aligned */
+    void *workspace;              /* grad 1: cyfa_embed_grad_workspace_bytes(n, V, D) bytes (0 for few positions), 256-byte aligned */
     size_t workspace_bytes;
 } CyfaEmbedArgs;
 

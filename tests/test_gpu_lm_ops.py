@@ -312,7 +312,8 @@ def test_loss_recorded_backward():
 @pytest.mark.parametrize("n,V,D,dtype,scale", [
     (1, 1, 1, F32, 1.0), (3, 5, 3, BF, 2.0), (64, 32, 7, F16, 1.0), (65, 300, 8, BF, 0.5), (129, 3, 33, F32, 1.0),
     (1000, 1000, 100, BF, 32.0), (700, 2, 513, F16, 1.0), (4097, 513, 64, F32, 1.0), (200, 1500, 1024, BF, 1.0),
-    (1025, 140000, 16, BF, 1.0), (37, 64, 2050, F32, 3.0)])
+    (1025, 140000, 16, BF, 1.0), (37, 64, 2050, F32, 3.0), (64, 90, 1000, BF, 1.0), (65, 90, 1000, BF, 1.0), (64, 3, 5, F16, 2.0),
+    (65, 7, 3, F32, 1.0), (9, 70000, 1024, BF, 1.0)])
 def test_embed(n, V, D, dtype, scale):
     w = _randn(n, V, D).to(dtype)
     ids = (_randint(V, V, n).double() ** 2 / V).long()  # low ids come up more often
