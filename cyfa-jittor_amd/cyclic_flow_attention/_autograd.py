@@ -1,0 +1,40 @@
+"""What the autograd functions of the layers and of the operators share: which
+backward passes run in torch operations, and how."""
+
+import torch
+
+_peek = torch._C._functorch.peek_interpreter_stack
+_is_batched = torch._C._functorch.is_legacy_batchedtensor
+
+
+def through_torch(*cotangents):
+    """Whether a backward pass has to run in torch operations: one that is
+    itself recorded (``create_graph=True``), or batched over several cotangents
+    (vmap). A cotangent may be None."""
+    if torch.is_grad_enabled() or _peek() is not None:
+        return True
+    for t in cotangents:
+        if t is not None and _is_batched(t):
+            return True
+    return False
+
+
+def torch_grads(fn, inputs, needed, cotangents):
+    """Gradients of fn(*inputs) (a tensor or a tuple of them) by autograd, None
+    where ``needed`` is false, recorded when this backward pass is.
+
+    fn is differentiated at aliases of the inputs: one input may have been
+    computed from another (a block's output from the residual it joins) or be
+    the same tensor, and a gradient of the inputs themselves would follow, and
+    free, the caller's graph between them."""
+    recorded = torch.is_grad_enabled()
+    with torch.enable_grad():
+        aliases = [t.view_as(t) if n else t for t, n in zip(inputs, needed)]
+        outs = fn(*aliases)
+        pairs = [(o, c) for o, c in zip(outs if isinstance(outs, tuple) else (outs,), cotangents) if c is not None]
+        wanted = [t for t, n in zip(aliases, needed) if n]
+        if not pairs or not wanted:
+            return tuple(torch.zeros_like(t) if n else None for t, n in zip(inputs, needed))
+        outs, cots = zip(*pairs)
+        grads = iter(torch.autograd.grad(outs, wanted, cots, create_graph=recorded, allow_unused=True))
+    return tuple(next(grads) if n else None for n in needed)

@@ -11,6 +11,7 @@ import torch
 from torch.autograd import forward_ad
 
 from .. import _native
+from .._autograd import through_torch, torch_grads
 
 
 def hip_autograd_ok(*tensors):
@@ -27,23 +28,6 @@ def hip_autograd_ok(*tensors):
             and torch._C._functorch.peek_interpreter_stack() is None and forward_ad._current_level < 0
             and not torch.compiler.is_compiling() and not torch.jit.is_tracing()
             and torch._C._len_torch_dispatch_stack() == 0)
-
-
-def _through_torch(*cotangents):
-    """Whether a backward pass has to run in torch operations: one that is
-    itself recorded, or batched over several cotangents (vmap)."""
-    return (torch.is_grad_enabled() or torch._C._functorch.peek_interpreter_stack() is not None
-            or any(torch._C._functorch.is_legacy_batchedtensor(t) for t in cotangents))
-
-
-def _torch_grads(fn, inputs, needed, dy):
-    """Gradients of fn(*inputs) by autograd, themselves recorded when this
-    backward pass is."""
-    recorded = torch.is_grad_enabled()
-    with torch.enable_grad():
-        wanted = [t for t, n in zip(inputs, needed) if n]
-        grads = iter(torch.autograd.grad(fn(*inputs), wanted, dy, create_graph=recorded, allow_unused=True))
-    return tuple(next(grads) if n else None for n in needed)
 
 
 def short_conv(x, weight, bias, cache, general):
@@ -68,8 +52,8 @@ class ShortConv(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias, cache = ctx.saved_tensors
         needed = ctx.needs_input_grad[:4]
-        if _through_torch(dy):
-            return _torch_grads(ctx.general, (x, weight, bias, cache), needed, dy) + (None,)
+        if through_torch(dy):
+            return torch_grads(ctx.general, (x, weight, bias, cache), needed, (dy,)) + (None,)
         grads = _native.short_conv_grad(x, weight, cache, _native.aligned_rows(dy), needed)
         return (*grads, None)
 
@@ -96,8 +80,8 @@ class GatedNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, gate = ctx.saved_tensors
         needed = ctx.needs_input_grad[:3]
-        if _through_torch(dy):
-            return _torch_grads(ctx.general, (x, weight, gate), needed, dy) + (None,) * 3
+        if through_torch(dy):
+            return torch_grads(ctx.general, (x, weight, gate), needed, (dy,)) + (None,) * 3
         return (*_native.norm_grad(x, weight, gate, *ctx.args, _native.aligned_rows(dy), needed), None, None, None)
 
 
@@ -128,8 +112,8 @@ class Gates(torch.autograd.Function):
         *inputs, abd = ctx.saved_tensors
         x, wa, wb, _, wd, _, dt_bias, A_log = inputs
         needed = ctx.needs_input_grad[:8]
-        if _through_torch(dg, dbeta, ddelta):
-            return _torch_grads(ctx.general, inputs, needed, (dg, dbeta, ddelta)) + (None,)
+        if through_torch(dg, dbeta, ddelta):
+            return torch_grads(ctx.general, inputs, needed, (dg, dbeta, ddelta)) + (None,)
         grads = _native.gates_grad(x, wa, wb, wd, dt_bias, A_log, abd, dg.contiguous(), dbeta.contiguous(),
                                    ddelta.contiguous(), needed[0])
         return tuple(t if n else None for t, n in zip(grads, needed)) + (None,)
@@ -177,8 +161,8 @@ class Projections(torch.autograd.Function):
     def backward(ctx, dq, dk, dv, dgate):
         *inputs, y = ctx.saved_tensors
         needed = ctx.needs_input_grad[:13]
-        if _through_torch(dq, dk, dv, dgate):
-            return _torch_grads(ctx.general, inputs, needed, (dq, dk, dv, dgate)) + (None,)
+        if through_torch(dq, dk, dv, dgate):
+            return torch_grads(ctx.general, inputs, needed, (dq, dk, dv, dgate)) + (None,)
         x, wq, wk, wv, wg, w2, _, cq, ck, cv = inputs[:10]
         widths = [w.shape[0] for w in (wq, wk, wv)]
         n = sum(widths)

@@ -6,7 +6,7 @@ v0.1.2, with the two options the reference's blocks leave out)."""
 import torch
 
 from .. import _native
-from .vocab import _recorded, _torch_backward
+from .._autograd import through_torch, torch_grads
 
 
 def residual_norm(x, y, weight, post_weight=None, gate=None, scale=1.0, eps=1e-6):
@@ -77,8 +77,8 @@ class _ResidualNorm(torch.autograd.Function):
     def backward(ctx, d_s, d_h):
         *inputs, stats = ctx.saved_tensors
         needed = ctx.needs_input_grad
-        if _recorded(d_s, d_h):
-            return _torch_backward(lambda *a: _plain(*a, *ctx.args), inputs, needed[:5], (d_s, d_h)) + (None, None)
+        if through_torch(d_s, d_h):
+            return torch_grads(lambda *a: _plain(*a, *ctx.args), inputs, needed[:5], (d_s, d_h)) + (None, None)
         if d_s is not None:
             d_s = d_s.contiguous()
         if d_h is not None:

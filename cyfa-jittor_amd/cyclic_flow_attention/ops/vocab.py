@@ -15,10 +15,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import _native
-
-
-_peek = torch._C._functorch.peek_interpreter_stack
-_is_batched = torch._C._functorch.is_legacy_batchedtensor
+from .._autograd import through_torch, torch_grads
 
 
 class TokenLogprobs(NamedTuple):
@@ -69,30 +66,6 @@ def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
     return TokenLogprobs(*_native.logprobs(logits, tokens, top_k, int(ignore_index))[:4])
 
 
-def _recorded(*cotangents):
-    """Whether this backward pass is itself recorded, or batched (vmap)."""
-    if torch.is_grad_enabled() or _peek() is not None:
-        return True
-    for t in cotangents:
-        if t is not None and _is_batched(t):
-            return True
-    return False
-
-
-def _torch_backward(fn, inputs, needed, cotangents):
-    """Gradients of fn(*inputs) in torch operations, recorded when this
-    backward pass is."""
-    recorded = torch.is_grad_enabled()
-    with torch.enable_grad():
-        pairs = [(o, c) for o, c in zip(fn(*inputs), cotangents) if c is not None]
-        wanted = [t for t, n in zip(inputs, needed) if n]
-        if not pairs or not wanted:
-            return tuple(torch.zeros_like(t) if n else None for t, n in zip(inputs, needed))
-        outs, cots = zip(*pairs)
-        grads = iter(torch.autograd.grad(outs, wanted, cots, create_graph=recorded, allow_unused=True))
-    return tuple(next(grads) if n else None for n in needed)
-
-
 def _plain_logprobs(logits, tokens, ids, ignore_index):
     """(logprob, entropy, top_logprobs) in torch operations."""
     lp = F.log_softmax(logits.float(), -1)
@@ -125,8 +98,8 @@ class _TokenLogprobs(torch.autograd.Function):
         logits, tokens, stats, entropy, ids = ctx.saved_tensors
         top_k, ignore_index = ctx.args
         cots = (d_logprob, d_entropy, d_top)
-        if _recorded(*cots):
-            return _torch_backward(lambda x: _plain_logprobs(x, tokens, ids, ignore_index), (logits,), (True,),
+        if through_torch(*cots):
+            return torch_grads(lambda x: _plain_logprobs(x, tokens, ids, ignore_index), (logits,), (True,),
                                    cots) + (None,) * 3
         cots = [None if c is None else c.contiguous() for c in cots]
         return _native.logprobs_grad(logits, tokens, top_k, ignore_index, stats, entropy, ids, *cots), None, None, None
@@ -162,8 +135,8 @@ class _TokenLoss(torch.autograd.Function):
     @staticmethod
     def backward(ctx, d_loss):
         logits, labels, kept = ctx.saved_tensors
-        if _recorded(d_loss):
-            return _torch_backward(lambda x: _plain_loss(x, labels, ctx.ignore_index), (logits,), (True,),
+        if through_torch(d_loss):
+            return torch_grads(lambda x: _plain_loss(x, labels, ctx.ignore_index), (logits,), (True,),
                                    (d_loss,)) + (None, None)
         return _native.token_loss_grad(logits, labels, ctx.ignore_index, kept, d_loss.contiguous()), None, None
 
@@ -211,7 +184,7 @@ class _EmbedTokens(torch.autograd.Function):
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
         V, scale, padding_idx = ctx.args
-        if _recorded(dy):  # (linear in dy)
+        if through_torch(dy):  # (linear in dy)
             kept = ((ids >= 0) & (ids < V) & (ids != padding_idx)).reshape(-1, 1)
             rows = torch.where(kept, dy.float().reshape(-1, dy.shape[-1]) * scale, 0.0)
             dw = rows.new_zeros(V, dy.shape[-1]).index_add(0, ids.reshape(-1).clamp(0, V - 1), rows)

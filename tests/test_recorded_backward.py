@@ -1,0 +1,103 @@
+"""Backward passes that are themselves recorded, or batched over cotangents, run
+in torch operations: their gradients where one input was computed from another,
+with the forward kernels' results formed by stand-ins (no GPU compute)."""
+
+import pytest
+import torch
+
+from cyclic_flow_attention import _native, ops
+from cyclic_flow_attention.layers import autograd as layer_autograd
+from cyclic_flow_attention.ops.residual import _plain
+
+
+@pytest.fixture
+def stand_ins(monkeypatch):
+    """The forward launches in torch operations; the adjoint kernels may not be called."""
+    def residual_norm(x, y, weight, post, gate, scale, eps, stats=False):
+        s, h = _plain(x, y, weight, post, gate, scale, eps)
+        return s, h, torch.zeros(x.shape[0], 2) if stats else None
+
+    def norm_train(x, weight, gate, eps, prescale):
+        assert prescale == 1.0
+        return _norm(x, weight, gate, eps)
+
+    def launch(*args, **kwargs):
+        raise AssertionError("an adjoint kernel was called")
+
+    monkeypatch.setattr(_native, "residual_norm", residual_norm)
+    monkeypatch.setattr(_native, "norm_train", norm_train)
+    for name in ("residual_norm_grad", "norm_grad"):
+        monkeypatch.setattr(_native, name, launch)
+
+
+def _norm(x, weight, gate, eps):
+    y = x * (x.square().mean(-1, keepdim=True) + eps).rsqrt() * weight
+    return y if gate is None else y * torch.sigmoid(gate)
+
+
+def _randn(seed, *shape):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed))
+
+
+# y and gate as functions of x; fp32 through two reductions of 24 terms: 2^-18 of the largest value
+DEPENDENT = {"y of x": (torch.tanh, None), "y is x": (lambda x: x, None), "gate of x": (lambda x: 2 * x, torch.sin),
+             "gate of y": (torch.tanh, torch.tanh)}
+
+
+@pytest.mark.parametrize("case", DEPENDENT)
+def test_join_of_a_block_computed_from_its_residual(stand_ins, case):
+    make_y, make_gate = DEPENDENT[case]
+    x0, w0, p0 = _randn(1, 5, 24), 1 + 0.1 * _randn(2, 24), 1 + 0.1 * _randn(3, 24)
+    cots = [_randn(4, 5, 24), _randn(5, 5, 24)]
+    results = []
+    for dtype in (torch.float32, torch.float64):
+        x, w, p = (t.to(dtype).requires_grad_(True) for t in (x0, w0, p0))
+        y = make_y(x)
+        gate = None if make_gate is None else make_gate(y if case == "gate of y" else x)
+        join = ops.residual_norm if dtype == torch.float32 else lambda a, b, c, d, g, s, e: _plain_double(a, b, c, d, g, s, e)
+        s, h = join(x, y, w, p, gate, 0.5, 1e-3)
+        grads = torch.autograd.grad([s, h], [x, w, p], [c.to(dtype) for c in cots], create_graph=True)
+        again = torch.autograd.grad(sum(g.square().sum() for g in grads), [x, w, p])
+        results.append([*grads, *again])
+    for got, want in zip(*results):
+        assert (got.double() - want).abs().max() <= 2.0**-18 * want.abs().max(), case
+
+
+def _plain_double(x, y, weight, post, gate, scale, eps):
+    b = y * (y.square().mean(-1, keepdim=True) + eps).rsqrt() * post
+    s = x + scale * (b if gate is None else b * torch.sigmoid(gate))
+    return s, s * (s.square().mean(-1, keepdim=True) + eps).rsqrt() * weight
+
+
+def test_batched_cotangents_leave_the_graph_before_the_join(stand_ins):
+    x, w = _randn(1, 5, 24).requires_grad_(True), _randn(2, 24)
+    cots = _randn(3, 3, 5, 24)
+    s, h = ops.residual_norm(x, torch.tanh(x), w)
+    (batched,) = torch.autograd.grad(h, [x], cots, is_grads_batched=True, retain_graph=True)
+    again = torch.autograd.grad(h, [x], cots, is_grads_batched=True)[0]  # the graph of tanh is still there
+    z = x.detach().double().requires_grad_(True)
+    t = z + torch.tanh(z)
+    ref = t * (t.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w
+    for i in range(3):
+        (want,) = torch.autograd.grad(ref, [z], cots[i].double(), retain_graph=True)
+        assert (batched[i].double() - want).abs().max() <= 2.0**-18 * want.abs().max()
+    assert torch.equal(batched, again)
+
+
+@pytest.mark.parametrize("gate_of", [torch.sin, lambda x: x])
+def test_norm_whose_gate_was_computed_from_its_input(stand_ins, gate_of):
+    def general(x, weight, gate):
+        return _norm(x, weight, gate, 1e-3)
+
+    results = []
+    for dtype in (torch.float32, torch.float64):
+        x = _randn(1, 5, 24).to(dtype).requires_grad_(True)
+        w = _randn(2, 24).to(dtype)
+        if dtype == torch.float32:
+            y = layer_autograd.rms_norm(x, w, gate_of(x), 1e-3, 1.0, general)
+        else:
+            y = general(x, w, gate_of(x))
+        (dx,) = torch.autograd.grad(y, [x], _randn(3, 5, 24).to(dtype), create_graph=True)
+        results.append([dx, torch.autograd.grad(dx.square().sum(), [x])[0]])
+    for got, want in zip(*results):
+        assert (got.double() - want).abs().max() <= 2.0**-18 * want.abs().max()
