@@ -21,7 +21,8 @@ def through_torch(*cotangents):
 
 def torch_grads(fn, inputs, needed, cotangents):
     """Gradients of fn(*inputs) (a tensor or a tuple of them) by autograd, None
-    where ``needed`` is false, recorded when this backward pass is.
+    where ``needed`` is false and zeros where no given cotangent reaches an
+    input, as the adjoint kernels give them; recorded when this backward pass is.
 
     fn is differentiated at aliases of the inputs: one input may have been
     computed from another (a block's output from the residual it joins) or be
@@ -31,10 +32,12 @@ def torch_grads(fn, inputs, needed, cotangents):
     with torch.enable_grad():
         aliases = [t.view_as(t) if n else t for t, n in zip(inputs, needed)]
         outs = fn(*aliases)
-        pairs = [(o, c) for o, c in zip(outs if isinstance(outs, tuple) else (outs,), cotangents) if c is not None]
+        pairs = [(o, c) for o, c in zip(outs if isinstance(outs, tuple) else (outs,), cotangents)
+                 if c is not None and o.requires_grad]
         wanted = [t for t, n in zip(aliases, needed) if n]
-        if not pairs or not wanted:
-            return tuple(torch.zeros_like(t) if n else None for t, n in zip(inputs, needed))
-        outs, cots = zip(*pairs)
-        grads = iter(torch.autograd.grad(outs, wanted, cots, create_graph=recorded, allow_unused=True))
+        grads = [None] * len(wanted)
+        if pairs and wanted:
+            outs, cots = zip(*pairs)
+            grads = torch.autograd.grad(outs, wanted, cots, create_graph=recorded, allow_unused=True)
+        grads = iter([torch.zeros_like(t) if g is None else g for t, g in zip(wanted, grads)])
     return tuple(next(grads) if n else None for n in needed)

@@ -101,3 +101,16 @@ def test_norm_whose_gate_was_computed_from_its_input(stand_ins, gate_of):
         results.append([dx, torch.autograd.grad(dx.square().sum(), [x])[0]])
     for got, want in zip(*results):
         assert (got.double() - want).abs().max() <= 2.0**-18 * want.abs().max()
+
+
+def test_inputs_that_no_cotangent_reaches(stand_ins):
+    """s does not depend on the next norm's weight: zeros, as the kernels give."""
+    x0, w0 = _randn(1, 5, 24), _randn(2, 24)
+    for x_grad in (False, True):
+        x, w = x0.clone().requires_grad_(x_grad), w0.clone().requires_grad_(True)
+        s, _ = ops.residual_norm(x, 2 * x0, w)
+        wanted = [x, w] if x_grad else [w]
+        grads = torch.autograd.grad(s, wanted, torch.ones_like(s), create_graph=True)
+        assert not grads[-1].any()
+        if x_grad:
+            assert torch.equal(grads[0], torch.ones_like(s))
