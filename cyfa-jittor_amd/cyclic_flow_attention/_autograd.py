@@ -7,16 +7,21 @@ _peek = torch._C._functorch.peek_interpreter_stack
 _is_batched = torch._C._functorch.is_legacy_batchedtensor
 
 
-def through_torch(*cotangents):
-    """Whether a backward pass has to run in torch operations: one that is
-    itself recorded (``create_graph=True``), or batched over several cotangents
-    (vmap). A cotangent may be None."""
-    if torch.is_grad_enabled() or _peek() is not None:
+def batched(*cotangents):
+    """Whether this backward pass runs over several cotangents at once (vmap). A
+    cotangent may be None."""
+    if _peek() is not None:
         return True
     for t in cotangents:
         if t is not None and _is_batched(t):
             return True
     return False
+
+
+def through_torch(*cotangents):
+    """Whether a backward pass has to run in torch operations: one that is
+    itself recorded (``create_graph=True``), or batched."""
+    return torch.is_grad_enabled() or batched(*cotangents)
 
 
 def torch_grads(fn, inputs, needed, cotangents):

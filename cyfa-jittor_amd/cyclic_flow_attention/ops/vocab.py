@@ -15,7 +15,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import _native
-from .._autograd import through_torch, torch_grads
+from .._autograd import batched, through_torch, torch_grads
 
 
 class TokenLogprobs(NamedTuple):
@@ -79,6 +79,19 @@ def _plain_logprobs(logits, tokens, ids, ignore_index):
     return (logprob, entropy) if ids is None else (logprob, entropy, lp.gather(-1, ids))
 
 
+def _live_rows(logits, tokens, ignore_index, d_logprob, d_entropy, d_top):
+    """[..., 1]: rows that have probabilities or that a cotangent other than
+    zero reaches; the others get a gradient of zeros, whatever they hold."""
+    live = logits.detach().float().logsumexp(-1).isfinite()
+    if d_logprob is not None:
+        live = live | ((d_logprob != 0) & (tokens != ignore_index))
+    if d_entropy is not None:
+        live = live | (d_entropy != 0)
+    if d_top is not None:
+        live = live | (d_top != 0).any(-1)
+    return live[..., None]
+
+
 class _TokenLogprobs(torch.autograd.Function):
     """token_logprobs with its gradient: keeps the logits and, of each row, the
     maximum, the log of the sum and the entropy."""
@@ -99,8 +112,17 @@ class _TokenLogprobs(torch.autograd.Function):
         top_k, ignore_index = ctx.args
         cots = (d_logprob, d_entropy, d_top)
         if through_torch(*cots):
-            return torch_grads(lambda x: _plain_logprobs(x, tokens, ids, ignore_index), (logits,), (True,),
-                                   cots) + (None,) * 3
+            live = _live_rows(logits, tokens, ignore_index, *cots)
+
+            def plain(x):
+                return _plain_logprobs(x, tokens, ids, ignore_index)
+
+            if batched(*cots):
+                (dx,) = torch_grads(plain, (logits,), (True,), cots)
+                dx = torch.where(live, dx, 0.0)
+            else:  # (other rows stay out of the higher derivatives too)
+                (dx,) = torch_grads(lambda x: plain(torch.where(live, x, 0.0)), (logits,), (True,), cots)
+            return dx, None, None, None
         cots = [None if c is None else c.contiguous() for c in cots]
         return _native.logprobs_grad(logits, tokens, top_k, ignore_index, stats, entropy, ids, *cots), None, None, None
 
@@ -119,7 +141,10 @@ def token_loss(logits, labels, ignore_index=-100):
 
 
 def _plain_loss(logits, labels, ignore_index):
-    return (-_plain_logprobs(logits, labels, None, ignore_index)[0].sum() / (labels != ignore_index).sum(),)
+    """token_loss in torch operations; rows of ignored labels are not read."""
+    kept = labels != ignore_index
+    logits = torch.where(kept[..., None], logits, 0.0)
+    return (-_plain_logprobs(logits, labels, None, ignore_index)[0].sum() / kept.sum(),)
 
 
 class _TokenLoss(torch.autograd.Function):
@@ -136,8 +161,7 @@ class _TokenLoss(torch.autograd.Function):
     def backward(ctx, d_loss):
         logits, labels, kept = ctx.saved_tensors
         if through_torch(d_loss):
-            return torch_grads(lambda x: _plain_loss(x, labels, ctx.ignore_index), (logits,), (True,),
-                                   (d_loss,)) + (None, None)
+            return torch_grads(lambda x: _plain_loss(x, labels, ctx.ignore_index), (logits,), (True,), (d_loss,)) + (None, None)
         return _native.token_loss_grad(logits, labels, ctx.ignore_index, kept, d_loss.contiguous()), None, None
 
 

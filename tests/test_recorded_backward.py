@@ -8,6 +8,7 @@ import torch
 from cyclic_flow_attention import _native, ops
 from cyclic_flow_attention.layers import autograd as layer_autograd
 from cyclic_flow_attention.ops.residual import _plain
+from cyclic_flow_attention.ops.vocab import _plain_logprobs, _plain_loss
 
 
 @pytest.fixture
@@ -21,12 +22,22 @@ def stand_ins(monkeypatch):
         assert prescale == 1.0
         return _norm(x, weight, gate, eps)
 
+    def logprobs(logits, tokens, k, ignore, stats=False):
+        ids = logits.topk(k, -1).indices if k else None
+        out = _plain_logprobs(logits, tokens, ids, ignore)
+        return (*out, *(() if k else (None,)), ids, torch.zeros(logits.shape[:-1] + (2,)) if stats else None)
+
+    def token_loss(logits, labels, ignore, stats=False):
+        return _plain_loss(logits, labels, ignore)[0], torch.zeros(1)
+
     def launch(*args, **kwargs):
         raise AssertionError("an adjoint kernel was called")
 
     monkeypatch.setattr(_native, "residual_norm", residual_norm)
     monkeypatch.setattr(_native, "norm_train", norm_train)
-    for name in ("residual_norm_grad", "norm_grad"):
+    monkeypatch.setattr(_native, "logprobs", logprobs)
+    monkeypatch.setattr(_native, "token_loss", token_loss)
+    for name in ("residual_norm_grad", "norm_grad", "logprobs_grad", "token_loss_grad"):
         monkeypatch.setattr(_native, name, launch)
 
 
@@ -114,3 +125,69 @@ def test_inputs_that_no_cotangent_reaches(stand_ins):
         assert not grads[-1].any()
         if x_grad:
             assert torch.equal(grads[0], torch.ones_like(s))
+
+
+INF, NAN = float("inf"), float("nan")
+
+
+def test_rows_without_probabilities_that_no_cotangent_reaches(stand_ins):
+    """Zeros, whatever the row holds; the other rows' gradients as ever."""
+    x0 = _randn(1, 6, 9)
+    x0[0], x0[1, 2], x0[2, 3], x0[3, 4:] = -INF, NAN, INF, -INF
+    tokens = torch.tensor([0, 1, 2, 3, -100, 5])
+    keep = torch.tensor([0.0, 0.0, 0.0, 1.0, 1.0, 0.0])
+    cots = [keep * _randn(2, 6), (keep * _randn(3, 6)), keep[:, None] * _randn(4, 6, 2)]
+    x = x0.clone().requires_grad_(True)
+    got = ops.token_logprobs(x, tokens, top_k=2)
+    (dx,) = torch.autograd.grad(got[:3], [x], cots, create_graph=True)
+    z = x0[3:5].double().requires_grad_(True)
+    want = _plain_logprobs(z, tokens[3:5], got.top_ids[3:5], -100)
+    (dz,) = torch.autograd.grad(want, [z], [c[3:5].double() for c in cots])
+    assert not dx[:3].any() and not dx[5].any() and (dx[3:5] - dz).abs().max() <= 2.0**-18 * dz.abs().max()
+    for i in range(3):  # one that a cotangent reaches
+        (dx,) = torch.autograd.grad(got[:2], [x], [torch.eye(6)[i], torch.zeros(6)], create_graph=True)
+        assert dx[i].isnan().all() and not dx[[r for r in range(6) if r != i]].any()
+    ignored = tokens.masked_fill(tokens == 0, -100)  # the first row's label is ignored
+    (dx,) = torch.autograd.grad(ops.token_logprobs(x, ignored).logprob, [x], torch.eye(6)[0], create_graph=True)
+    assert not dx.any()
+
+
+def test_loss_beside_rows_without_probabilities(stand_ins):
+    x0 = _randn(1, 4, 9)
+    x0[0], x0[1, 2] = -INF, NAN
+    labels = torch.tensor([-100, -100, 3, 8])
+    x, z = x0.clone().requires_grad_(True), x0[2:].double().requires_grad_(True)
+    (dx,) = torch.autograd.grad(ops.token_loss(x, labels), [x], create_graph=True)
+    (dz,) = torch.autograd.grad(torch.nn.functional.cross_entropy(z, labels[2:]), [z])
+    assert not dx[:2].any() and (dx[2:] - dz).abs().max() <= 2.0**-18 * dz.abs().max()
+
+
+def test_derivative_with_respect_to_cotangents_of_zero(stand_ins):
+    """The forward derivative as the adjoint of the adjoint at cotangents of zero."""
+    x, u = _randn(1, 3, 9).requires_grad_(True), _randn(2, 3, 9)
+    v = torch.zeros(3, requires_grad=True)
+    tokens = torch.tensor([1, 2, 8])
+    (dx,) = torch.autograd.grad(ops.token_logprobs(x, tokens).logprob, [x], v, create_graph=True)
+    (got,) = torch.autograd.grad(dx, [v], u)
+    p = x.detach().double().softmax(-1)
+    want = u.double().gather(1, tokens[:, None])[:, 0] - (p * u).sum(-1)
+    assert (got - want).abs().max() <= 2.0**-18 * want.abs().max()
+
+
+def test_batched_cotangents_of_log_probabilities(stand_ins):
+    x = _randn(1, 4, 9)
+    x[1] = -INF
+    x.requires_grad_(True)
+    tokens = torch.tensor([0, 1, -100, 8])
+    got = ops.token_logprobs(x, tokens, top_k=2)[:3]
+    cots = [_randn(i, 5, *o.shape) for i, o in enumerate(got)]
+    for c in cots:
+        c[:, 1] = 0
+    batched = torch.autograd.grad(got, [x], cots, is_grads_batched=True, retain_graph=True)[0]
+    for i in range(5):
+        (one,) = torch.autograd.grad(got, [x], [c[i] for c in cots], create_graph=True)
+        assert (batched[i] - one).abs().max() <= 2.0**-20 * one.abs().max() and not one[1].any()
+    loss = ops.token_loss(x, tokens.masked_fill(torch.arange(4) == 1, -100))
+    batched = torch.autograd.grad(loss, [x], torch.tensor([1.0, -2.0]), is_grads_batched=True, retain_graph=True)[0]
+    (one,) = torch.autograd.grad(loss, [x], create_graph=True)
+    assert torch.equal(batched, torch.stack([one, -2 * one]))
