@@ -1,10 +1,28 @@
 """What the autograd functions of the layers and of the operators share: which
-backward passes run in torch operations, and how."""
+calls and which backward passes run in torch operations, and how."""
 
 import torch
+from torch.autograd import forward_ad
 
 _peek = torch._C._functorch.peek_interpreter_stack
 _is_batched = torch._C._functorch.is_legacy_batchedtensor
+
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def kernel_ok(*tensors):
+    """Whether a call with these tensors (or Nones) may go to a kernel, of which
+    torch sees nothing: plain tensors, and no torch.func transform, forward-mode
+    derivative, tracing, compiling or dispatch mode (make_fx, operation
+    counters), each of which would lose what the kernel computes."""
+    if torch.compiler.is_compiling():
+        return False
+    for t in tensors:
+        if t is not None and type(t) not in _PLAIN:
+            return False
+    return (_peek() is None and forward_ad._current_level < 0 and not torch.jit.is_tracing()
+            and torch._C._len_torch_dispatch_stack() == 0)
 
 
 def batched(*cotangents):

@@ -8,26 +8,19 @@ higher derivatives stay available.
 """
 
 import torch
-from torch.autograd import forward_ad
 
 from .. import _native
-from .._autograd import through_torch, torch_grads
+from .._autograd import kernel_ok, through_torch, torch_grads
 
 
 def hip_autograd_ok(*tensors):
-    """Whether a call that records gradients may take these functions: plain
-    tensors of one GPU, and nothing that has to see the torch operations
-    themselves (torch.func transforms, forward-mode derivatives, tracing or
-    compiling, dispatch modes, which make_fx and operation counters are, autocast)."""
+    """Whether a call that records gradients may take these functions: tensors
+    of one GPU, no autocast, and nothing that has to see the torch operations
+    themselves (kernel_ok)."""
     given = [t for t in tensors if t is not None]
-    if not all(type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda for t in given):
+    if not kernel_ok(*given) or not all(t.is_cuda and t.device == given[0].device for t in given):
         return False
-    if any(t.device != given[0].device for t in given):
-        return False
-    return (torch.is_grad_enabled() and not torch.is_autocast_enabled("cuda")
-            and torch._C._functorch.peek_interpreter_stack() is None and forward_ad._current_level < 0
-            and not torch.compiler.is_compiling() and not torch.jit.is_tracing()
-            and torch._C._len_torch_dispatch_stack() == 0)
+    return torch.is_grad_enabled() and not torch.is_autocast_enabled("cuda")
 
 
 def short_conv(x, weight, bias, cache, general):

@@ -6,7 +6,7 @@ v0.1.2, with the two options the reference's blocks leave out)."""
 import torch
 
 from .. import _native
-from .._autograd import through_torch, torch_grads
+from .._autograd import kernel_ok, through_torch, torch_grads
 
 
 def residual_norm(x, y, weight, post_weight=None, gate=None, scale=1.0, eps=1e-6):
@@ -19,7 +19,9 @@ def residual_norm(x, y, weight, post_weight=None, gate=None, scale=1.0, eps=1e-6
     s is the next residual, h the next block's input. x, y and gate share one
     shape and dtype (bf16, fp16 or fp32), the weights are [D], D at most 8192.
     All in fp32, s and h rounded once (h is that of s before its rounding).
-    Differentiable in every tensor; a backward pass that is itself recorded runs
+    Differentiable in every tensor; a backward pass that is itself recorded, and
+    a call that torch has to see (torch.func transforms, forward-mode
+    derivatives, tracing, compiling, dispatch modes, subclasses of tensors), run
     in torch operations."""
     shape, dtype = x.shape, x.dtype
     if dtype not in _native.LM_DTYPES:
@@ -43,6 +45,9 @@ def residual_norm(x, y, weight, post_weight=None, gate=None, scale=1.0, eps=1e-6
         post_weight = post_weight.float().contiguous()
     if gate is not None:
         gate = gate.contiguous()
+    if not kernel_ok(x, y, weight, post_weight, gate):
+        _native.require_device(x, y, weight, post_weight, gate)
+        return _plain(x, y, weight, post_weight, gate, scale, eps)
     if torch.is_grad_enabled() and (x.requires_grad or y.requires_grad or weight.requires_grad
                                     or (post_weight is not None and post_weight.requires_grad)
                                     or (gate is not None and gate.requires_grad)):

@@ -6,7 +6,9 @@ models/cyfa/modeling_cyfa.py:63-71, 96-108 of Chyxx/CyFA-Jittor v0.1.2).
 Each computes in fp32 whatever the dtype (bf16, fp16 or fp32) and rounds its
 results once. Where an input requires a gradient the call is recorded for
 autograd and its backward runs as HIP kernels too; a backward pass that is
-itself recorded (``create_graph=True``) runs in torch operations.
+itself recorded (``create_graph=True``) runs in torch operations, and so does a
+call that torch has to see (torch.func transforms, forward-mode derivatives,
+tracing, compiling, dispatch modes, subclasses of tensors).
 """
 
 from typing import NamedTuple
@@ -15,7 +17,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import _native
-from .._autograd import batched, through_torch, torch_grads
+from .._autograd import batched, kernel_ok, through_torch, torch_grads
 
 
 class TokenLogprobs(NamedTuple):
@@ -61,6 +63,10 @@ def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
         raise ValueError(f"token_logprobs: top_k must be in [0, {logits.shape[-1]}], got {top_k}")
     if top_k > _native.LOGPROBS_MAX_TOP:
         raise NotImplementedError(f"token_logprobs: at most {_native.LOGPROBS_MAX_TOP} alternatives, got {top_k}")
+    if not kernel_ok(logits, tokens):
+        _native.require_device(logits, tokens)
+        ids = logits.detach().sort(dim=-1, descending=True, stable=True).indices[..., :top_k] if top_k else None
+        return TokenLogprobs(*_plain_logprobs(logits, tokens, ids, int(ignore_index)), *(() if top_k else (None,)), ids)
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top_k, int(ignore_index)))
     return TokenLogprobs(*_native.logprobs(logits, tokens, top_k, int(ignore_index))[:4])
@@ -135,6 +141,9 @@ def token_loss(logits, labels, ignore_index=-100):
     logits; rows of ignored labels get zeros. The labels are those of the rows
     as they are (a causal model shifts them: label t is the token after t)."""
     labels = _check_logits("token_loss", logits, labels, "labels")
+    if not kernel_ok(logits, labels):
+        _native.require_device(logits, labels)
+        return _plain_loss(logits, labels, int(ignore_index))[0]
     if torch.is_grad_enabled() and logits.requires_grad:
         return _TokenLoss.apply(logits, labels, int(ignore_index))
     return _native.token_loss(logits, labels, int(ignore_index))[0]
@@ -190,9 +199,20 @@ def embed_tokens(ids, weight, scale=1.0, padding_idx=None):
         padding_idx = int(padding_idx) % V
     ids = ids.to(torch.int64).contiguous()
     weight = weight.contiguous()
+    if not kernel_ok(ids, weight):
+        _native.require_device(ids, weight)
+        return _plain_embed(ids, weight, float(scale), padding_idx)
     if torch.is_grad_enabled() and weight.requires_grad:
         return _EmbedTokens.apply(ids, weight, float(scale), padding_idx)
     return _native.embed(ids, weight, float(scale))
+
+
+def _plain_embed(ids, weight, scale, padding_idx):
+    """embed_tokens in torch operations."""
+    V = weight.shape[0]
+    rows = weight.float()[ids.clamp(0, V - 1)]
+    rows = torch.where((ids == padding_idx)[..., None], rows.detach(), rows) * scale
+    return torch.where(((ids >= 0) & (ids < V))[..., None], rows, float("nan")).to(weight.dtype)
 
 
 class _EmbedTokens(torch.autograd.Function):

@@ -1,5 +1,6 @@
 """Recorded and batched backward passes of the joins between a model's blocks,
-where one input was computed from another."""
+where one input was computed from another, and forward-mode derivatives and
+traces of the operators around the blocks."""
 
 import pytest
 import torch
@@ -59,3 +60,33 @@ def test_model_gradients_of_a_recorded_pass(monkeypatch):
     for name, a, b, c in zip(params, got, want, plain):
         for other in (b, c):  # fp32 sums in another order through two layers
             assert (a.double() - other.double()).norm() <= 2e-5 * other.double().norm() + 1e-12, name
+
+
+def test_forward_mode_derivatives_and_traces():
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x, d = _randn(1, 5, 40).cuda(), _randn(2, 5, 40).cuda()
+    t, w = torch.tensor([1, 39, 0, 7, 7]).cuda(), torch.ones(40, device="cuda")
+
+    def calls(x):
+        r = ops.token_logprobs(x, t, top_k=3)
+        return (r.logprob, r.entropy, r.top_logprobs, ops.token_loss(x, t), ops.embed_tokens(t % 5, x),
+                *ops.residual_norm(x, 2 * x, w))
+
+    h = 2.0**-7
+    with torch.no_grad():
+        high, low, at = calls(x + h * d), calls(x - h * d), calls(x)  # the kernels
+        with forward_ad.dual_level():
+            outs = [forward_ad.unpack_dual(o) for o in calls(forward_ad.make_dual(x, d))]
+        traced = make_fx(calls)(_randn(3, 5, 40).cuda())(x)
+        ids = [ops.token_logprobs(x + e * d, t, top_k=3).top_ids for e in (h, -h)]
+    for i, (a, b, c, o, g) in enumerate(zip(high, low, at, outs, traced)):
+        off = (o.tangent - (a - b) / (2 * h)).abs()
+        if i == 2:  # (alternatives that change places between the two points: their quotient is no derivative)
+            assert (ids[0] != ids[1]).sum() == 2
+            off = off[ids[0] == ids[1]]
+        # third derivatives of order ten times h^2, fp32 values of order ten over h
+        assert off.max() <= 20 * h * h + 60 * 2.0**-24 / h
+        assert (o.primal - c).abs().max() <= 2.0**-18 * (1 + c.abs().max())
+        assert (g - c).abs().max() <= 2.0**-18 * (1 + c.abs().max())
