@@ -12,6 +12,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from ... import _native
+from ..._autograd import kernel_ok
 from ...layers.autograd import hip_autograd_ok
 from ...layers.cyfa import CyclicFlowAttention, FusedWeight, RMSNorm, inference_fast_path, plain_module
 from ...ops.residual import residual_norm
@@ -250,20 +251,23 @@ class CyclicFlowAttentionForCausalLM(nn.Module):
             logits = _native.linear(hidden, self.lm_head.weight)
         else:
             logits = self.lm_head(hidden)
-        loss = None
-        if labels is not None:
-            if (logits.dtype in _native.LM_DTYPES and logits.dim() == 3 and labels.dtype == torch.int64
-                    and type(labels) is torch.Tensor and labels.shape == logits.shape[:2] and labels.device == logits.device
-                    and (hip_autograd_ok(logits) or inference_fast_path(logits))):
-                # labels shifted instead of logits: the gradient is written once, in place
-                loss = token_loss(logits, F.pad(labels[:, 1:], (0, 1), value=-100))
-            else:
-                loss = F.cross_entropy(
-                    logits[:, :-1].float().reshape(-1, self.config.vocab_size),
-                    labels[:, 1:].reshape(-1),
-                    ignore_index=-100,
-                )
+        loss = None if labels is None else self._loss(logits, labels)
         return {"logits": logits, "loss": loss, "cache": cache}
+
+    def _loss(self, logits, labels):
+        """The mean cross entropy of logits [B, T, V] against the next labels, on
+        the HIP path with and without gradients."""
+        recorded = torch.is_grad_enabled() and logits.requires_grad
+        if (logits.dtype in _native.LM_DTYPES and logits.dim() == 3 and labels.dtype == torch.int64
+                and labels.shape == logits.shape[:2] and labels.device == logits.device
+                and logits.is_cuda and kernel_ok(logits, labels) and (not recorded or hip_autograd_ok(logits))):
+            # labels shifted instead of logits: the gradient is written once, in place
+            return token_loss(logits, F.pad(labels[:, 1:], (0, 1), value=-100))
+        return F.cross_entropy(
+            logits[:, :-1].float().reshape(-1, self.config.vocab_size),
+            labels[:, 1:].reshape(-1),
+            ignore_index=-100,
+        )
 
     @torch.no_grad()
     def score(self, input_ids, top_k=0, attention_mask=None):

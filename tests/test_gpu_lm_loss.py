@@ -1,0 +1,49 @@
+"""The model's loss on the HIP path: every dtype with and without gradients, and
+what may happen to the logits before the backward pass."""
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from cyclic_flow_attention import CyclicFlowAttentionConfig, CyclicFlowAttentionForCausalLM, _native
+
+pytestmark = pytest.mark.gpu
+
+V = 301
+
+
+def _model(dtype):
+    torch.manual_seed(3)
+    config = CyclicFlowAttentionConfig(hidden_size=256, num_heads=1, head_dim=256, num_hidden_layers=1, vocab_size=V,
+                                       intermediate_size=512, num_slots=128)
+    model = CyclicFlowAttentionForCausalLM(config).cuda()
+    return model if dtype == torch.float32 else model.to(dtype) if dtype == torch.float16 else model.to_bfloat16()
+
+
+def _ids(B=2, T=40):
+    return torch.randint(0, V, (B, T), generator=torch.Generator().manual_seed(1)).cuda()
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    n = []
+    call = _native.token_loss
+    monkeypatch.setattr(_native, "token_loss", lambda *args, **kwargs: n.append(1) or call(*args, **kwargs))
+    return n
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_loss_without_gradients_of_every_dtype(launches, dtype):
+    model, ids = _model(dtype), _ids()
+    labels = ids.clone()
+    labels[1, 30:] = -100
+    for context in (torch.no_grad(), torch.inference_mode()):
+        with context:
+            out = model(ids, labels=labels)
+        want = F.cross_entropy(out["logits"][:, :-1].double().reshape(-1, V), labels[:, 1:].reshape(-1))
+        assert abs(out["loss"].item() - want.item()) <= 2.0**-18 * want.item()
+        with context:
+            labels[0, 3] = V  # as in a training step
+            assert model(ids, labels=labels)["loss"].isnan()
+        labels[0, 3] = 5
+    assert len(launches) == 4
