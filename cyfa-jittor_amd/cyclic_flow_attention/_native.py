@@ -944,7 +944,10 @@ def gates(abd, dt_bias, A_log):
 
 # The element types of the operators around a model's blocks (CYFA_DTYPE_*).
 LM_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
-LOGPROBS_MAX_TOP = 32
+# Their largest sizes: alternatives, vocabulary; ids, rows and columns of an
+# embedding's gradient; columns of a join.
+LOGPROBS_MAX_TOP, LOGPROBS_MAX_V = 32, 1 << 28
+EMBED_MAX_N, EMBED_MAX_V, EMBED_MAX_D = 1 << 30, 1 << 26, 1 << 20
 RESIDUAL_MAX_D = 8192
 
 

@@ -151,6 +151,8 @@ class CyclicFlowAttentionModel(nn.Module):
         e = self.embeddings
         if (torch.is_grad_enabled() and plain_module(e, nn.Embedding) and e.weight.requires_grad
                 and e.weight.dtype in _native.LM_DTYPES
+                and e.weight.shape[0] <= _native.EMBED_MAX_V and e.weight.shape[1] <= _native.EMBED_MAX_D
+                and input_ids.numel() <= _native.EMBED_MAX_N
                 and e.max_norm is None and not e.sparse and not e.scale_grad_by_freq
                 and input_ids.dtype in (torch.int64, torch.int32) and input_ids.device == e.weight.device
                 and type(input_ids) is torch.Tensor and hip_autograd_ok(e.weight)):
@@ -260,7 +262,8 @@ class CyclicFlowAttentionForCausalLM(nn.Module):
         recorded = torch.is_grad_enabled() and logits.requires_grad
         if (logits.dtype in _native.LM_DTYPES and logits.dim() == 3 and labels.dtype == torch.int64
                 and labels.shape == logits.shape[:2] and labels.device == logits.device
-                and logits.is_cuda and kernel_ok(logits, labels) and (not recorded or hip_autograd_ok(logits))):
+                and logits.shape[-1] <= _native.LOGPROBS_MAX_V and logits.is_cuda and kernel_ok(logits, labels)
+                and (not recorded or hip_autograd_ok(logits))):
             # labels shifted instead of logits: the gradient is written once, in place
             return token_loss(logits, F.pad(labels[:, 1:], (0, 1), value=-100))
         return F.cross_entropy(

@@ -47,3 +47,21 @@ def test_loss_without_gradients_of_every_dtype(launches, dtype):
             assert model(ids, labels=labels)["loss"].isnan()
         labels[0, 3] = 5
     assert len(launches) == 4
+
+
+def test_sizes_past_the_operators_keep_the_torch_operations(launches, monkeypatch):
+    model, ids = _model(torch.float32), _ids()
+    want = model(ids, labels=ids)["loss"]
+    grads = torch.autograd.grad(want, [model.model.embeddings.weight])
+    assert len(launches) == 1
+    monkeypatch.setattr(_native, "LOGPROBS_MAX_V", V - 1)
+    embeds = []
+    for name, largest in (("EMBED_MAX_V", V - 1), ("EMBED_MAX_D", 255), ("EMBED_MAX_N", 79)):
+        with monkeypatch.context() as m:
+            m.setattr(_native, name, largest)
+            m.setattr(_native, "embed", lambda *args: embeds.append(1))
+            loss = model(ids, labels=ids)["loss"]
+            (got,) = torch.autograd.grad(loss, [model.model.embeddings.weight])
+        assert abs(loss.item() - want.item()) <= 2.0**-16 * want.item()
+        assert (got - grads[0]).norm() <= 2e-5 * grads[0].norm()
+    assert len(launches) == 1 and not embeds

@@ -171,3 +171,17 @@ def test_recorded_backward_of_impossible_tokens_stays_off_the_table():
     loss = _plain_loss(x, kept, -100)[0]
     assert abs(loss.item() + (want[0, 2] + want[2, 0]).item() / 2) < 1e-6
     assert _plain_loss(x, torch.full((4,), -100), -100)[0].isnan()
+
+
+def test_largest_sizes_are_the_librarys():
+    lib = _native.load_library()
+    size = lib.cyfa_embed_grad_workspace_bytes
+    N, V, D = _native.EMBED_MAX_N, _native.EMBED_MAX_V, _native.EMBED_MAX_D
+    assert min(size(N, 5, 1), size(65, V, 1), size(65, 5, D)) > 0
+    assert size(N + 1, 5, 1) == size(65, V + 1, 1) == size(65, 5, D + 1) == 0
+    size = lib.cyfa_logprobs_workspace_bytes
+    V, k = _native.LOGPROBS_MAX_V, _native.LOGPROBS_MAX_TOP
+    assert size(1, V, k, 0) > 0 and size(1, V + 1, k, 0) == size(1, V, k + 1, 0) == 0
+    call = _caller("cyfa_residual_norm", _native.CyfaResidualArgs, dict(
+        rows=0, D=1, x=0x10000, y=0x20000, weight=0x30000, s=0x40000, h=0x50000))
+    assert call(0, D=_native.RESIDUAL_MAX_D) == _native.CYFA_OK and call(0, D=_native.RESIDUAL_MAX_D + 1) == UNSUPPORTED
