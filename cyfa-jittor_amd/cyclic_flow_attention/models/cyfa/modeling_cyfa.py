@@ -261,7 +261,7 @@ class CyclicFlowAttentionForCausalLM(nn.Module):
         the HIP path with and without gradients."""
         recorded = torch.is_grad_enabled() and logits.requires_grad
         if (logits.dtype in _native.LM_DTYPES and logits.dim() == 3 and labels.dtype == torch.int64
-                and labels.shape == logits.shape[:2] and labels.device == logits.device
+                and labels.shape == logits.shape[:2] and labels.shape[1] > 0 and labels.device == logits.device
                 and logits.shape[-1] <= _native.LOGPROBS_MAX_V and logits.is_cuda and kernel_ok(logits, labels)
                 and (not recorded or hip_autograd_ok(logits))):
             # labels shifted instead of logits: the gradient is written once, in place

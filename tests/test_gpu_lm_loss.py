@@ -65,3 +65,10 @@ def test_sizes_past_the_operators_keep_the_torch_operations(launches, monkeypatc
         assert abs(loss.item() - want.item()) <= 2.0**-16 * want.item()
         assert (got - grads[0]).norm() <= 2e-5 * grads[0].norm()
     assert len(launches) == 1 and not embeds
+
+
+def test_loss_of_no_tokens(launches):
+    model = _model(torch.float32)
+    logits = torch.zeros(2, 0, V, device="cuda", requires_grad=True)
+    loss = model._loss(logits, torch.zeros(2, 0, dtype=torch.int64, device="cuda"))
+    assert loss.isnan() and torch.autograd.grad(loss, [logits])[0].shape == logits.shape and not launches
