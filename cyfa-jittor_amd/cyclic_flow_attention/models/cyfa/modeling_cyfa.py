@@ -6,6 +6,7 @@ names, and the bf16 precision policy of ``to_bfloat16``.
 """
 
 import math
+from contextlib import nullcontext
 
 import torch
 import torch.nn.functional as F
@@ -14,7 +15,7 @@ from torch import nn
 from ... import _native
 from ..._autograd import kernel_ok
 from ...layers.autograd import hip_autograd_ok
-from ...layers.cyfa import CyclicFlowAttention, FusedWeight, RMSNorm, inference_fast_path, plain_module
+from ...layers.cyfa import CyclicFlowAttention, FusedWeight, RMSNorm, inference_fast_path, plain_linear, plain_module
 from ...ops.residual import residual_norm
 from ...ops.vocab import embed_tokens, token_logprobs, token_loss
 
@@ -110,6 +111,32 @@ def join_norm(x, y, norm):
         return residual_norm(x, y, norm.weight, eps=norm.eps)
     s = x + y
     return s, norm(s)
+
+
+def editable_logits(hidden, head):
+    """A context for the loss of the logits head(hidden), whose caller may edit
+    them in place before the backward pass, as where the loss keeps a copy: the
+    loss keeps the logits themselves, and a backward pass that finds them edited
+    forms them again. (Saved-tensor hooks of the caller's own stay in charge.)"""
+    hooks = torch._C._autograd
+    if not hooks._saved_tensors_hooks_is_enabled() or hooks._top_saved_tensors_default_hooks(False) is not None:
+        return nullcontext()
+    source = [hidden.detach(), head.weight.detach(), None if head.bias is None else head.bias.detach()]
+    versions = [t._version for t in source if t is not None]
+
+    def pack(t):
+        return t.detach(), t._version
+
+    def unpack(kept):
+        t, version = kept
+        if t._version == version:
+            return t
+        if versions != [s._version for s in source if s is not None]:
+            raise RuntimeError("the model's logits, and what they were computed from, have been edited in place since its loss")
+        with torch.no_grad():
+            return F.linear(*source)
+
+    return torch.autograd.graph.saved_tensors_hooks(pack, unpack)
 
 
 class CyFABlock(nn.Module):
@@ -253,19 +280,20 @@ class CyclicFlowAttentionForCausalLM(nn.Module):
             logits = _native.linear(hidden, self.lm_head.weight)
         else:
             logits = self.lm_head(hidden)
-        loss = None if labels is None else self._loss(logits, labels)
+        loss = None if labels is None else self._loss(hidden, logits, labels)
         return {"logits": logits, "loss": loss, "cache": cache}
 
-    def _loss(self, logits, labels):
-        """The mean cross entropy of logits [B, T, V] against the next labels, on
-        the HIP path with and without gradients."""
+    def _loss(self, hidden, logits, labels):
+        """The mean cross entropy of logits [B, T, V] (lm_head's of hidden)
+        against the next labels, on the HIP path with and without gradients."""
         recorded = torch.is_grad_enabled() and logits.requires_grad
         if (logits.dtype in _native.LM_DTYPES and logits.dim() == 3 and labels.dtype == torch.int64
                 and labels.shape == logits.shape[:2] and labels.shape[1] > 0 and labels.device == logits.device
                 and logits.shape[-1] <= _native.LOGPROBS_MAX_V and logits.is_cuda and kernel_ok(logits, labels)
-                and (not recorded or hip_autograd_ok(logits))):
-            # labels shifted instead of logits: the gradient is written once, in place
-            return token_loss(logits, F.pad(labels[:, 1:], (0, 1), value=-100))
+                and (not recorded or (hip_autograd_ok(logits) and plain_linear(self.lm_head)))):
+            with editable_logits(hidden, self.lm_head) if recorded else nullcontext():
+                # labels shifted instead of logits: the gradient is written once, in place
+                return token_loss(logits, F.pad(labels[:, 1:], (0, 1), value=-100))
         return F.cross_entropy(
             logits[:, :-1].float().reshape(-1, self.config.vocab_size),
             labels[:, 1:].reshape(-1),
