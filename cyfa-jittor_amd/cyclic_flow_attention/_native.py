@@ -981,11 +981,14 @@ def logit_rows(logits):
     return (rows, logits.shape[1], logits.stride(0), logits.stride(1), V, logits.data_ptr()), logits
 
 
+@functools.lru_cache(64)
+def _logprobs_bytes(rows, V, k, dtype):
+    return int(load_library().cyfa_logprobs_workspace_bytes(rows, V, k, dtype))
+
+
 def _logprobs_workspace(args, dtype, dev):
     """The call's workspace, set in args; the caller keeps it until the launch."""
-    if args.rows > 64 or args.V <= 32768:  # (rows enough for the compute units, or short ones: none)
-        return None
-    n = int(load_library().cyfa_logprobs_workspace_bytes(args.rows, args.V, args.k, LM_DTYPES[dtype]))
+    n = _logprobs_bytes(args.rows, args.V, args.k, LM_DTYPES[dtype])
     if n == 0:
         return None
     workspace = torch.empty(n, dtype=torch.uint8, device=dev)

@@ -185,3 +185,20 @@ def test_largest_sizes_are_the_librarys():
     call = _caller("cyfa_residual_norm", _native.CyfaResidualArgs, dict(
         rows=0, D=1, x=0x10000, y=0x20000, weight=0x30000, s=0x40000, h=0x50000))
     assert call(0, D=_native.RESIDUAL_MAX_D) == _native.CYFA_OK and call(0, D=_native.RESIDUAL_MAX_D + 1) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("rows,V,k", [(1, 100, 3), (65, 1 << 20, 0), (64, 32768, 5), (3, 1 << 20, 7)])
+def test_workspaces_are_what_the_library_asks_for(monkeypatch, rows, V, k):
+    """Whatever the rule by which it shares rows out."""
+    class Library:
+        @staticmethod
+        def cyfa_logprobs_workspace_bytes(*asked):
+            assert asked == (rows, V, k, 1)
+            return 768
+
+    _native._logprobs_bytes.cache_clear()
+    monkeypatch.setattr(_native, "load_library", Library)
+    args = _native.CyfaLogprobArgs(rows=rows, V=V, k=k)
+    workspace = _native._logprobs_workspace(args, torch.float32, torch.device("cpu"))
+    _native._logprobs_bytes.cache_clear()
+    assert workspace.numel() == args.workspace_bytes == 768 and args.workspace == workspace.data_ptr()
