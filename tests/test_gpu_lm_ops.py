@@ -773,3 +773,20 @@ def test_embed_gradient_of_ids_that_share_a_remainder():
         dy = _randn(5, n, D)
         (dw,) = torch.autograd.grad(_ops().embed_tokens(ids.cuda(), w), [w], dy.cuda())
         lm.assert_within(dw, *lm.embed_grad(ids, dy.double(), V, 1.0, -1, F32), "dw")
+
+
+@pytest.mark.parametrize("n", [16384, 16385, 20011, 33000])
+def test_embed_gradient_of_many_mixed_ids(n):
+    """More positions than the sort keeps between counting and placing, with
+    several ids to a workgroup: of a whole vocabulary, of few ids, and of ids
+    that share a remainder, few and many of them at a time."""
+    V, D = 5000, 24
+    same = torch.where(_randint(5, 2, n) == 0, _randint(6, 19, n) * 256 + 7, torch.full((n,), 7))
+    impossible = torch.where(_randint(7, 3, n) == 0, torch.tensor(V), _randint(8, V, n))
+    for ids in (_randint(1, V, n), (_randint(2, V, n).double() ** 3 / V**2).long(), _randint(3, 19, n) * 256 + 3, same, impossible):
+        w = torch.zeros(V, D, device="cuda", requires_grad=True)
+        dy = _randn(9, n, D)
+        out = _ops().embed_tokens(ids.cuda(), w, padding_idx=11)
+        (dw,) = torch.autograd.grad(out, [w], dy.cuda(), retain_graph=True)
+        lm.assert_within(dw, *lm.embed_grad(ids, dy.double(), V, 1.0, 11, F32), "dw")
+        assert torch.equal(dw, torch.autograd.grad(out, [w], dy.cuda())[0])
