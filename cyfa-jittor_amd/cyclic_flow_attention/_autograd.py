@@ -4,11 +4,11 @@ calls and which backward passes run in torch operations, and how."""
 import torch
 from torch.autograd import forward_ad
 
+# (looked up once: a small call's time is the host's)
 _peek = torch._C._functorch.peek_interpreter_stack
 _is_batched = torch._C._functorch.is_legacy_batchedtensor
-
-
-_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_compiling, _tracing, _modes = torch.compiler.is_compiling, torch._C._is_tracing, torch._C._len_torch_dispatch_stack
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, type(None)))
 
 
 def kernel_ok(*tensors):
@@ -16,13 +16,12 @@ def kernel_ok(*tensors):
     torch sees nothing: plain tensors, and no torch.func transform, forward-mode
     derivative, tracing, compiling or dispatch mode (make_fx, operation
     counters), each of which would lose what the kernel computes."""
-    if torch.compiler.is_compiling():
+    if _compiling() or _peek() is not None or forward_ad._current_level >= 0 or _tracing() or _modes():
         return False
     for t in tensors:
-        if t is not None and type(t) not in _PLAIN:
+        if type(t) not in _PLAIN:
             return False
-    return (_peek() is None and forward_ad._current_level < 0 and not torch.jit.is_tracing()
-            and torch._C._len_torch_dispatch_stack() == 0)
+    return True
 
 
 def batched(*cotangents):
