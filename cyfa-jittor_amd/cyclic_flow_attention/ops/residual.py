@@ -40,9 +40,9 @@ def residual_norm(x, y, weight, post_weight=None, gate=None, scale=1.0, eps=1e-6
     if isinstance(scale, torch.Tensor):
         raise ValueError("residual_norm: the scale must be a number (a tensor's gradient would be lost)")
     scale, eps = float(scale), float(eps)
-    x, y, weight = x.contiguous(), y.contiguous(), weight.float().contiguous()
+    x, y, weight = x.contiguous(), y.contiguous(), _fp32(weight)
     if post_weight is not None:
-        post_weight = post_weight.float().contiguous()
+        post_weight = _fp32(post_weight)
     if gate is not None:
         gate = gate.contiguous()
     if not kernel_ok(x, y, weight, post_weight, gate):
@@ -53,6 +53,10 @@ def residual_norm(x, y, weight, post_weight=None, gate=None, scale=1.0, eps=1e-6
                                     or (gate is not None and gate.requires_grad)):
         return _ResidualNorm.apply(x, y, weight, post_weight, gate, scale, eps)
     return _native.residual_norm(x, y, weight, post_weight, gate, scale, eps)[:2]
+
+
+def _fp32(t):
+    return t.contiguous() if t.dtype is torch.float32 else t.float().contiguous()
 
 
 def _plain(x, y, weight, post, gate, scale, eps):

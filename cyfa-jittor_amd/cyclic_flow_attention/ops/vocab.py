@@ -38,7 +38,11 @@ def _check_logits(what, logits, tokens, name):
         raise ValueError(f"{what}: {name} must have shape {tuple(logits.shape[:-1])}, got {tuple(tokens.shape)}")
     if tokens.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"{what}: {name} must be int64 or int32, got {tokens.dtype}")
-    return tokens.to(torch.int64).contiguous()
+    return _int64(tokens)
+
+
+def _int64(t):
+    return t.contiguous() if t.dtype is torch.int64 else t.to(torch.int64).contiguous()
 
 
 def token_logprobs(logits, tokens, top_k=0, ignore_index=-100):
@@ -197,7 +201,7 @@ def embed_tokens(ids, weight, scale=1.0, padding_idx=None):
         raise ValueError(f"embed_tokens: padding_idx must be in [-{V}, {V}), got {padding_idx}")
     else:
         padding_idx = int(padding_idx) % V
-    ids = ids.to(torch.int64).contiguous()
+    ids = _int64(ids)
     weight = weight.contiguous()
     if not kernel_ok(ids, weight):
         _native.require_device(ids, weight)
