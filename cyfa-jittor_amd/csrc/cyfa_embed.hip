@@ -2,8 +2,9 @@
 // and its gradient dweight[v] = scale sum_{i: ids[i] = v} dy[i].
 //
 // The gradient sorts the positions by id, each id's positions in their order,
-// and adds each id's rows of dy in that order in fp32: no atomics on sums, so
-// two backward passes give the same bits, and the result is rounded once.
+// and adds each id's rows of dy in fp32 by a rule that the ids alone fix (in that
+// order, chunks of 32 by themselves; below): no atomics on sums, so two backward
+// passes give the same bits, and the result is rounded once.
 //
 // us on MI355X for 16384 positions of natural frequencies, 1024 bf16 columns and
 // 32000 ids: the lookup 10.4 (33.5 MB written, the 10 MB of different rows read),
@@ -51,8 +52,9 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedParams p) {
 // in launches: on MI355X 300 positions take 6.5 us, 4096 8, 16384 11 (14 where one
 // workgroup's ids are a fifteenth of them, 24 where all are one id: that
 // workgroup's placing takes the time; with the ids of a wave's positions always
-// told apart bit by bit 12, 16 and 27), 32768 19 (25, 47). Up to 16384 positions
-// stay in registers between counting and placing.
+// told apart bit by bit 12, 16 and 27), 32768 19 (25, 47), 131072 of natural
+// frequencies 81, nearly half of that gradient's 176: every workgroup reads them
+// all. Up to 16384 positions stay in registers between counting and placing.
 constexpr int ES_NT = 1024, ES_WAVES = ES_NT / 64, ES_U = 16;
 constexpr int ES_FEW = 8;      // different ids of 64 positions that are matched one after another
 constexpr int ES_RANGE = 512;  // most ids of a workgroup: 33 KB of LDS
@@ -183,8 +185,10 @@ __device__ __forceinline__ void add_rows(const EmbedParams& p, const E* dy, int 
 
 // An id with many positions is shared out: every EMBED_CHUNK sorted positions
 // that all hold one id are added by a wave of embed_part_kernel, and
-// embed_grad_kernel adds the id's chunks and what is left at both ends (chunks of
-// 64 took 13.6 us for the 5 of 32: a wave's rows come eight at a time).
+// embed_grad_kernel adds the rows before them, the chunks and the rows after them
+// (chunks of 64 took 13.6 us for the 5 of 32: a wave's rows come eight at a time).
+// The cuts are those of all sorted positions, so that an id's last bits also
+// depend on how many positions the ids before it hold.
 //
 // Columns of a wave: 64 vectors; the last, ragged vector of a row is read and
 // written ending at the row's end, so that it overlaps the one before it
@@ -224,7 +228,7 @@ __global__ __launch_bounds__(256) void embed_part_kernel(EmbedParams p) {
     }
 }
 
-// Columns [d, d + N) of the gradient's row v from its positions [s, e) in order.
+// Columns [d, d + N) of the gradient's row v from its sorted positions [s, e).
 // STREAM: its lines, each written whole by one wave, go past the caches.
 template <class E, bool STREAM>
 __device__ __forceinline__ void embed_row(const EmbedParams& p, int v, int d, int s, int e) {

@@ -402,11 +402,16 @@ void launch(ResidualParams p, bool grad, hipStream_t stream) {
         hipLaunchKernelGGL(residual_sum_kernel, dim3((p.D + 31) / 32, 2), dim3(1024), 0, stream, p, n);
 }
 
-// Threads of a row and vectors of each: up to 16 elements a thread, the most that
-// the gradient keeps in registers with two waves per SIMD, and a wave to a row as
-// far as that goes (16384 x 1024 bf16 with output norm and gate, a wave against a
-// workgroup to a row: forward 28 and 37 us, gradient 52 and 81). fp32 rows past
-// 4096 columns have 16 in four vectors and spill a little.
+// Threads of a row and vectors of each: up to 16 elements a thread, and a wave to
+// a row as far as that goes (16384 x 1024 bf16 with output norm and gate, a wave
+// against a workgroup to a row: forward 28 and 37 us, gradient 52 and 81). The
+// gradient keeps them in registers with two waves per SIMD up to 4096 columns.
+// Past those, where the threads of a workgroup hold a row and its weights, it does
+// not: with output norm and gate 36 bytes a lane of 16-bit rows go to scratch,
+// 292 of fp32 rows (24 with the output norm alone, 36 with the gate alone). us on
+// MI355X with both, forward and gradient: 2^24 bf16 elements in rows of 1024 28.5
+// and 52.5, of 4096 28.4 and 53.5, of 8192 28.9 and 68.8; 2^23 fp32 elements in
+// rows of 4096 26.9 and 55.4, of 8192 27.3 and 106.5.
 template <class E>
 void launch_type(const ResidualParams& p, bool grad, hipStream_t stream) {
     constexpr int N = 16 / sizeof(E);

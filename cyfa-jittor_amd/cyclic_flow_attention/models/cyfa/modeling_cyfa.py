@@ -104,7 +104,7 @@ class GatedMLP(nn.Module):
 def join_norm(x, y, norm):
     """(x + y, norm(x + y)): the residual add between two halves of a block and
     the norm after it. A training step on the GPU runs both, and their adjoint,
-    as one residual_norm launch each."""
+    as one residual_norm launch each, which norms the sum before its rounding."""
     if (x.dtype in _native.LM_DTYPES and x.shape == y.shape and x.dtype == y.dtype and 0 < x.shape[-1] <= _native.RESIDUAL_MAX_D
             and plain_module(norm, RMSNorm) and tuple(norm.weight.shape) == x.shape[-1:]
             and hip_autograd_ok(x, y, norm.weight)):
@@ -207,7 +207,8 @@ class CyclicFlowAttentionModel(nn.Module):
         if x.numel() // x.shape[-1] <= _native.LINEAR_ROWS_MAX and attention_mask is None:
             # bf16 decode steps: each pre-norm runs inside the projection after
             # it, each residual add inside the projection before it (x + y, as
-            # CyFABlock.forward, bit for bit)
+            # CyFABlock.forward without gradients, bit for bit; a training step
+            # norms the sum before its rounding, see join_norm)
             # (a small-batch step's decode kernel reads the weights that follow
             # it into the caches: the block's MLP, then the next layer's input
             # projection, the first layer's after the last)
@@ -224,7 +225,7 @@ class CyclicFlowAttentionModel(nn.Module):
                 new.append(s)
             return self.norm(x), (new if use_cache else None)
         # bf16 prefill: each residual add runs inside the following norm kernel
-        # (x + y and residual + mlp, as CyFABlock.forward, bit for bit)
+        # (x + y and residual + mlp, as CyFABlock.forward without gradients, bit for bit)
         pending = None
         for i, layer in enumerate(self.layers):
             h = layer.attn_norm(x) if pending is None else None

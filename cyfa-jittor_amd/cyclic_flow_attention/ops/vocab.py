@@ -182,9 +182,9 @@ def embed_tokens(ids, weight, scale=1.0, padding_idx=None):
     """scale weight[ids]: rows of ``weight`` [V, D] for integer ``ids`` [...],
     [..., D] in the weight's dtype. An id outside [0, V) gives a row of NaN.
 
-    The gradient of the weight is dense and adds each id's cotangents in the
-    order of the positions, in fp32 and rounded once, so that two backward
-    passes give the same bits; the row of ``padding_idx`` (negative: from the
+    The gradient of the weight is dense and adds each id's cotangents in fp32,
+    in an association that the ids alone fix, and rounds once, so that two
+    backward passes give the same bits; the row of ``padding_idx`` (negative: from the
     end) and ids outside [0, V) get none."""
     if weight.dtype not in _native.LM_DTYPES:
         raise NotImplementedError(f"embed_tokens: the weight must be bf16, fp16 or fp32, got {weight.dtype}")

@@ -619,8 +619,8 @@ size_t cyfa_logprobs_workspace_bytes(long long rows, int V, int k, int dtype);
 int cyfa_logprobs(const CyfaLogprobArgs *args, int dtype, int grad, void *hip_stream);
 
 /* The embedding lookup out[i] = scale weight[ids[i]] (grad 0) and its gradient
- * dweight[v] = scale sum of dy[i] over ids[i] = v, i in order (grad 1), in f32
- * and rounded once; weight, out, dy, dweight CYFA_DTYPE_BF16, _F32 or _F16,
+ * dweight[v] = scale sum of dy[i] over ids[i] = v (grad 1), in f32, in an
+ * association that the ids alone fix, and rounded once; weight, out, dy, dweight CYFA_DTYPE_BF16, _F32 or _F16,
  * contiguous, any alignment. An id outside [0, V) gives a row of NaN and has no
  * gradient, nor has the id padding (-1: none). n <= 2^30, V <= 2^26, D <= 2^20. Replaces
  * nn.Embedding (models/cyfa/modeling_cyfa.py:63-71) and its adjoint. */
