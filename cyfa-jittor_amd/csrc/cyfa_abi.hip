@@ -133,6 +133,153 @@ extern "C" {
 
 int cyfa_abi_version(void) { return CYFA_ABI_VERSION; }
 
+int cyfa_adjust_logits(const CyfaAdjustArgs* a, int dtype, int grad, void* hip_stream) {
+    const char* what = "cyfa_adjust_logits";
+    if (!a) return fail(CYFA_ERR_VALUE, "%s: null args", what);
+    if (dtype < CYFA_DTYPE_BF16 || dtype > CYFA_DTYPE_F16) return fail(CYFA_ERR_VALUE, "%s: dtype %d", what, dtype);
+    if (a->rows < 0 || a->inner <= 0 || a->V <= 0 || a->L < 0 || a->n_tokens < 0)
+        return fail(CYFA_ERR_VALUE, "%s: rows=%lld inner=%lld V=%d L=%lld n_tokens=%d", what, a->rows, a->inner, a->V, a->L, a->n_tokens);
+    if (a->V > cyfa::LOGPROBS_MAX_V || a->L > 0x7fffffff) return fail(CYFA_ERR_UNSUPPORTED, "%s: V=%d L=%lld", what, a->V, a->L);
+    if (a->n_tokens > cyfa::ADJUST_MAX_TOKENS)
+        return fail(CYFA_ERR_UNSUPPORTED, "%s: %d of at most %d token biases", what, a->n_tokens, cyfa::ADJUST_MAX_TOKENS);
+    const int size = dtype == CYFA_DTYPE_F32 ? 4 : 2;
+    if (!aligned(a->x, size) || !aligned(a->dy, size) || !aligned(a->y, size) || !aligned(a->history, a->wide ? 8 : 4))
+        return fail(CYFA_ERR_ALIGN, "%s: tensors need their element's alignment", what);
+    const void* words4[] = {a->repetitions, a->presences, a->frequencies, a->bias, a->token_values};
+    for (const void* ptr : words4)
+        if (!aligned(ptr, 4)) return fail(CYFA_ERR_ALIGN, "%s: f32 tensors need 4-byte alignment", what);
+    const void* words8[] = {a->lengths, a->prompts, a->token_ids};
+    for (const void* ptr : words8)
+        if (!aligned(ptr, 8)) return fail(CYFA_ERR_ALIGN, "%s: int64 tensors need 8-byte alignment", what);
+    if (a->rows == 0) return CYFA_OK;
+    if (!a->x || !a->y || (grad && !a->dy) || (a->L > 0 && !a->history) || (a->n_tokens > 0 && (!a->token_ids || !a->token_values)))
+        return fail(CYFA_ERR_VALUE, "%s: null required pointer", what);
+    cyfa::AdjustParams p{};
+    p.rows = a->rows;
+    p.inner = a->inner;
+    p.V = a->V;
+    p.x = a->x;
+    p.x_outer = a->x_outer;
+    p.x_row = a->x_row;
+    p.history = a->history;
+    p.h_outer = a->h_outer;
+    p.h_row = a->h_row;
+    p.L = a->L;
+    p.wide = a->wide;
+    p.lengths = a->lengths;
+    p.prompts = a->prompts;
+    p.repetition = a->repetition;
+    p.presence = a->presence;
+    p.frequency = a->frequency;
+    p.repetitions = a->repetitions;
+    p.presences = a->presences;
+    p.frequencies = a->frequencies;
+    p.bias = a->bias;
+    p.b_outer = a->b_outer;
+    p.b_row = a->b_row;
+    p.token_ids = a->token_ids;
+    p.ti_outer = a->ti_outer;
+    p.ti_row = a->ti_row;
+    p.token_values = a->token_values;
+    p.tv_outer = a->tv_outer;
+    p.tv_row = a->tv_row;
+    p.n_tokens = a->n_tokens;
+    p.allowed = a->allowed;
+    p.a_outer = a->a_outer;
+    p.a_row = a->a_row;
+    p.packed = a->packed;
+    p.dy = a->dy;
+    p.y = a->y;
+    p.y_outer = a->y_outer;
+    p.y_row = a->y_row;
+    cyfa::launch_adjust(p, dtype, grad != 0, (hipStream_t)hip_stream);
+    return check_launch(what);
+}
+
+int cyfa_sample_tokens(const CyfaSampleArgs* a, int dtype, int grad, void* hip_stream) {
+    const char* what = "cyfa_sample_tokens";
+    if (!a) return fail(CYFA_ERR_VALUE, "%s: null args", what);
+    if (dtype < CYFA_DTYPE_BF16 || dtype > CYFA_DTYPE_F16) return fail(CYFA_ERR_VALUE, "%s: dtype %d", what, dtype);
+    if (grad) return fail(CYFA_ERR_VALUE, "%s: a choice has no gradient", what);
+    if (a->rows < 0 || a->inner <= 0 || a->V <= 0)
+        return fail(CYFA_ERR_VALUE, "%s: rows=%lld inner=%lld V=%d", what, a->rows, a->inner, a->V);
+    if (a->V > cyfa::LOGPROBS_MAX_V) return fail(CYFA_ERR_UNSUPPORTED, "%s: V=%d", what, a->V);
+    const int size = dtype == CYFA_DTYPE_F32 ? 4 : 2;
+    if (!aligned(a->x, size)) return fail(CYFA_ERR_ALIGN, "%s: tensors need their element's alignment", what);
+    const void* words4[] = {a->uniform, a->temperatures, a->top_ps, a->min_ps, a->logprob};
+    for (const void* ptr : words4)
+        if (!aligned(ptr, 4)) return fail(CYFA_ERR_ALIGN, "%s: f32 tensors need 4-byte alignment", what);
+    const void* words8[] = {a->uniform64, a->top_ks, a->ids};
+    for (const void* ptr : words8)
+        if (!aligned(ptr, 8)) return fail(CYFA_ERR_ALIGN, "%s: int64 and f64 tensors need 8-byte alignment", what);
+    if (a->rows == 0) return CYFA_OK;
+    if (!a->x || !a->ids || !a->logprob || (!a->uniform && !a->uniform64)) return fail(CYFA_ERR_VALUE, "%s: null required pointer", what);
+    cyfa::SampleParams p{};
+    p.rows = a->rows;
+    p.inner = a->inner;
+    p.outer_stride = a->outer_stride;
+    p.row_stride = a->row_stride;
+    p.V = a->V;
+    p.x = a->x;
+    p.uniform = a->uniform;
+    p.uniform64 = a->uniform64;
+    p.temperature = a->temperature;
+    p.top_p = a->top_p;
+    p.min_p = a->min_p;
+    p.top_k = a->top_k;
+    p.temperatures = a->temperatures;
+    p.top_ps = a->top_ps;
+    p.min_ps = a->min_ps;
+    p.top_ks = a->top_ks;
+    p.ids = a->ids;
+    p.logprob = a->logprob;
+    cyfa::launch_sample(p, dtype, (hipStream_t)hip_stream);
+    return check_launch(what);
+}
+
+int cyfa_distill_loss(const CyfaDistillArgs* a, int dtype, int grad, void* hip_stream) {
+    const char* what = "cyfa_distill_loss";
+    if (!a) return fail(CYFA_ERR_VALUE, "%s: null args", what);
+    if (dtype < CYFA_DTYPE_BF16 || dtype > CYFA_DTYPE_F16) return fail(CYFA_ERR_VALUE, "%s: dtype %d", what, dtype);
+    if (a->rows < 0 || a->inner <= 0 || a->V <= 0 || a->k <= 0)
+        return fail(CYFA_ERR_VALUE, "%s: rows=%lld inner=%lld V=%d k=%d", what, a->rows, a->inner, a->V, a->k);
+    if (!(a->temperature >= 1e-30f) || !isfinite(a->temperature) || (a->tail && a->temperature != 1.f))
+        return fail(CYFA_ERR_VALUE, "%s: temperature %g", what, (double)a->temperature);
+    if (a->k > cyfa::DISTILL_MAX_K) return fail(CYFA_ERR_UNSUPPORTED, "%s: k=%d of at most %d tokens", what, a->k, cyfa::DISTILL_MAX_K);
+    if (a->V > (a->tail ? cyfa::DISTILL_MAX_TAIL_V : cyfa::LOGPROBS_MAX_V))
+        return fail(CYFA_ERR_UNSUPPORTED, "%s: V=%d tail=%d", what, a->V, a->tail);
+    const int size = dtype == CYFA_DTYPE_F32 ? 4 : 2;
+    if (!aligned(a->x, size) || !aligned(a->dx, size) || !aligned(a->ids, 8))
+        return fail(CYFA_ERR_ALIGN, "%s: tensors need their element's alignment", what);
+    const void* words4[] = {a->values, a->weights, a->kept, a->loss, a->total, a->d_loss};
+    for (const void* ptr : words4)
+        if (!aligned(ptr, 4)) return fail(CYFA_ERR_ALIGN, "%s: f32 tensors need 4-byte alignment", what);
+    if (!a->total || (grad ? !a->d_loss : !a->loss)) return fail(CYFA_ERR_VALUE, "%s: null loss", what);
+    if (a->rows > 0 && (!a->x || !a->ids || !a->values || !a->kept || (grad && !a->dx)))
+        return fail(CYFA_ERR_VALUE, "%s: null required pointer", what);
+    if (a->rows == 0 && grad) return CYFA_OK;
+    cyfa::DistillParams p{};
+    p.rows = a->rows;
+    p.inner = a->inner;
+    p.outer_stride = a->outer_stride;
+    p.row_stride = a->row_stride;
+    p.V = a->V;
+    p.x = a->x;
+    p.k = a->k;
+    p.ids = a->ids;
+    p.values = a->values;
+    p.weights = a->weights;
+    p.temperature = a->temperature;
+    p.tail = a->tail;
+    p.kept = a->kept;
+    p.loss = a->loss;
+    p.total = a->total;
+    p.d_loss = a->d_loss;
+    p.dx = a->dx;
+    cyfa::launch_distill(p, dtype, grad != 0, (hipStream_t)hip_stream);
+    return check_launch(what);
+}
+
 const char* cyfa_last_error(void) { return g_error; }
 
 size_t cyfa_chunk_workspace_bytes(int B, int T, int H, int K, int V, int M, int C) {

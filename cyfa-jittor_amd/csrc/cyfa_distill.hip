@@ -1,0 +1,358 @@
+// cyfa_distill.hip -- the divergence of a student's distribution from a teacher's
+// that is known at its k most probable tokens, and the gradient. For a row x [V]
+// of the student's logits, q = softmax(x / T), the teacher's entries (id_i, t_i),
+// those with an id outside [0, V) or t_i = -inf left out:
+//   p_i = softmax(t / T)_i over the row's entries          loss = sum p_i (log p_i - log q_id)
+//   dx_j = (q_j - sum of p_i over id_i = j) / T
+// or, with the tail, T = 1, p_i = e^t_i and the rest of either mass as one more
+// outcome, p_r = 1 - sum p_i, q_r = sum of q_j over the columns of no entry:
+//   loss = sum p_i (log p_i - log q_id) + p_r (log p_r - log q_r)
+//   dx_j = q_j P - sum of p_i over id_i = j, P = sum p_i + p_r,  at the entries' columns
+//   dx_j = (q_j / q_r) (q_r P - p_r)                             elsewhere
+// One pass over the row each way, sums in fp32; what the teacher's few entries
+// give is formed in double (1 - sum p_i cancels). The columns of no entry keep a
+// maximum and a sum of their own with the tail: taken as the difference of the
+// row's sum and the entries', a small rest would be lost.
+#include "cyfa_internal.h"
+#include "cyfa_rows.h"
+
+namespace cyfa {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLowest = -3.402823466e38f;
+constexpr int DS_NV = 4;  // vectors of a thread in flight
+
+// What the forward keeps of a row for the gradient.
+struct DistillRow {
+    float m, ls;        // of all columns: the maximum, log2 of the sum of 2^((x - m) c)
+    float rm, rls;      // of the columns of no entry (with the tail; else of all)
+    float rest, entry;  // what multiplies the softmax of the columns of no entry, of the entries
+    float norm;         // p_i = 2^(t_i c - norm)
+    float weight;       // of the row in the mean, 0 without entries
+    float loss, pad;
+};
+static_assert(sizeof(DistillRow) == DISTILL_ROW_FLOATS * 4, "DISTILL_ROW_FLOATS");
+
+// Whether an entry counts.
+__device__ __forceinline__ bool counts(long long id, float t, int V) { return id >= 0 && id < V && t != -INFINITY; }
+
+template <int NT>
+__device__ __forceinline__ void row_sync() {
+    if (NT == 64) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        __syncthreads();
+    }
+}
+
+constexpr int rows_of(int NT) { return NT == 64 ? 4 : 1; }
+
+// A maximum and a sum of 2^((x - m) c) of a set of elements.
+struct Sum {
+    float m, s;
+};
+
+__device__ __forceinline__ void rescale(Sum& a, float m, float c) {
+    a.s *= fast_exp2((a.m - m) * c);
+    a.m = m;
+}
+
+__device__ __forceinline__ void join(Sum& a, Sum b, float c) {
+    const float m = fmaxf(a.m, b.m);
+    rescale(a, m, c);
+    rescale(b, m, c);
+    a.s += b.s;
+}
+
+// NT threads to a row.
+template <class E, int NT, bool TAIL>
+__global__ __launch_bounds__(NT * rows_of(NT)) void distill_kernel(DistillParams p) {
+    constexpr int N = RowVec<E>::N, W = NT / 64, RW = rows_of(NT);
+    extern __shared__ uint32_t entries_s[];  // TAIL: a bit for each column of an entry, p.words words a row
+    __shared__ Sum red[RW][W];
+    const int tid = threadIdx.x % NT, lane = tid & 63, wv = tid >> 6, sub = threadIdx.x / NT;
+    uint32_t* bits = entries_s + (size_t)sub * p.words;
+    const float c = kLog2e / p.temperature;
+    for (long long r = (long long)blockIdx.x * RW + sub; r < p.rows; r += (long long)gridDim.x * RW) {
+        const E* x = static_cast<const E*>(p.x) + (r / p.inner) * p.outer_stride + (r % p.inner) * p.row_stride;
+        const long long* ids = p.ids + r * p.k;
+        const float* t = p.values + r * p.k;
+        bool any = false;
+        for (int i = lane; i < p.k; i += 64) any |= counts(ids[i], t[i], p.V);
+        const float weight = __any(any) ? (p.weights ? p.weights[r] : 1.f) : 0.f;
+        DistillRow* keep = reinterpret_cast<DistillRow*>(p.kept) + r;
+        if (weight == 0.f) {  // (nothing of the row counts; the same in every wave)
+            if (tid == 0) {
+                keep->weight = 0.f;
+                keep->loss = 0.f;
+            }
+            continue;
+        }
+        if (TAIL) {
+            row_sync<NT>();
+            for (int i = tid; i < p.words; i += NT) bits[i] = 0;
+            row_sync<NT>();
+            for (int i = tid; i < p.k; i += NT)
+                if (counts(ids[i], t[i], p.V)) atomicOr(&bits[ids[i] >> 5], 1u << (ids[i] & 31));
+            row_sync<NT>();
+        }
+        const auto entry_bits = [&](int col) { return TAIL ? bits[col >> 5] >> (col & 31) : 0u; };
+        const int nvec = p.V / N, tail = p.V - nvec * N;
+        Sum a = {kLowest, 0.f};
+        float best = -INFINITY;
+        const float last = tid < tail && !(entry_bits(nvec * N + tid) & 1) ? (float)x[nvec * N + tid] : -INFINITY;
+        for (int v0 = 0; v0 < nvec; v0 += NT * DS_NV) {
+            typename RowVec<E>::type v[DS_NV];
+#pragma unroll
+            for (int j = 0; j < DS_NV; j++) v[j] = load_row(x + (size_t)min(v0 + j * NT + tid, nvec - 1) * N);
+            float e[DS_NV][N];
+#pragma unroll
+            for (int j = 0; j < DS_NV; j++) {
+                const int i = v0 + j * NT + tid;
+                const uint32_t skip = TAIL && i < nvec ? entry_bits(i * N) : 0;
+#pragma unroll
+                for (int k = 0; k < N; k++) {
+                    e[j][k] = i < nvec && !(TAIL && (skip >> k & 1)) ? (float)v[j][k] : -INFINITY;
+                    best = fmaxf(best, e[j][k]);
+                }
+            }
+            rescale(a, fmaxf(a.m, best), c);
+#pragma unroll
+            for (int j = 0; j < DS_NV; j++)
+#pragma unroll
+                for (int k = 0; k < N; k++) a.s += fast_exp2((e[j][k] - a.m) * c);
+        }
+        rescale(a, fmaxf(a.m, fmaxf(best, last)), c);
+        a.s += fast_exp2((last - a.m) * c);
+        const float m = wave_max(a.m);
+        rescale(a, m, c);
+        a.s = wave_sum(a.s);
+        if (W > 1) {
+            if (lane == 0) red[sub][wv] = a;
+            __syncthreads();
+            a = red[sub][0];
+#pragma unroll 3
+            for (int w = 1; w < W; w++) join(a, red[sub][w], c);
+        }
+        if (wv == 0) {
+            // The entries, a lane each: the student's logits there, the teacher's masses.
+            Sum b = {kLowest, 0.f};
+            float tmax = -INFINITY;
+            for (int i = lane; i < p.k; i += 64)
+                if (counts(ids[i], t[i], p.V)) {
+                    tmax = fmaxf(tmax, t[i]);
+                    if (TAIL) {  // (a column counts once)
+                        bool first = true;
+                        for (int j = 0; j < i; j++) first &= ids[j] != ids[i] || t[j] == -INFINITY;
+                        if (first) {
+                            const float e = (float)x[ids[i]];
+                            const float bm = fmaxf(b.m, e);
+                            rescale(b, bm, c);
+                            b.s += fast_exp2((e - b.m) * c);
+                        }
+                    }
+                }
+            Sum all = a;
+            if (TAIL) {
+                const float bm = wave_max(b.m);
+                rescale(b, bm, c);
+                b.s = wave_sum(b.s);
+                join(all, b, c);
+            }
+            const float ls = log2f(all.s), rls = log2f(a.s);
+            tmax = wave_max(tmax);
+            const double T = p.temperature;
+            double mass = 0.;
+            for (int i = lane; i < p.k; i += 64)
+                if (counts(ids[i], t[i], p.V)) mass += exp(TAIL ? (double)t[i] : ((double)t[i] - tmax) / T);
+            mass = wave_sum(mass);
+            const double lognorm = TAIL ? 0. : (double)tmax / T + log(mass);
+            double loss = 0.;
+            for (int i = lane; i < p.k; i += 64)
+                if (counts(ids[i], t[i], p.V)) {
+                    const double lp = (double)t[i] / T - lognorm;
+                    const float lq = ((float)x[ids[i]] - all.m) / p.temperature - kLn2 * ls;
+                    loss += exp(lp) * (lp - (double)lq);
+                }
+            loss = wave_sum(loss);
+            DistillRow row;
+            row.m = all.m;
+            row.ls = ls;
+            row.rm = a.s == 0.f ? 0.f : a.m;  // (no column of no entry but -inf: a softmax of zeros)
+            row.rls = a.s == 0.f ? 0.f : rls;
+            row.rest = row.entry = 1.f;
+            row.norm = (float)(lognorm * 1.4426950408889634);
+            row.weight = weight;
+            row.pad = 0.f;
+            if (TAIL) {
+                // the rest, where the student has any
+                const double pr = a.s > 0.f ? fmax(0., 1. - mass) : 0.;
+                const double lqr = (double)(a.m - all.m) + (double)kLn2 * ((double)rls - (double)ls);
+                if (pr > 0.) loss += pr * (log(pr) - lqr);
+                row.entry = (float)(mass + pr);
+                row.rest = (float)(exp(lqr) * (mass + pr) - pr);
+            }
+            row.loss = (float)loss;
+            if (lane == 0) *keep = row;
+        }
+        if (W > 1) __syncthreads();  // the shared arrays are free for the next row
+    }
+}
+
+// The weighted mean over the rows, one workgroup, in double and in a fixed order.
+__global__ __launch_bounds__(1024) void distill_mean_kernel(DistillParams p) {
+    __shared__ double sums[2][16];
+    constexpr int U = 8;
+    double s = 0., n = 0.;
+    const DistillRow* row = reinterpret_cast<const DistillRow*>(p.kept);
+    for (long long r0 = threadIdx.x; r0 < p.rows; r0 += 1024 * U) {
+        float w[U], l[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long long r = min(r0 + 1024 * u, p.rows - 1);
+            w[u] = row[r].weight;
+            l[u] = row[r].loss;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (r0 + 1024 * u < p.rows && w[u] != 0.f) {
+                s += (double)w[u] * (double)l[u];
+                n += (double)w[u];
+            }
+    }
+    s = wave_sum(s);
+    n = wave_sum(n);
+    if ((threadIdx.x & 63) == 0) {
+        sums[0][threadIdx.x >> 6] = s;
+        sums[1][threadIdx.x >> 6] = n;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = n = 0.;
+        for (int w = 0; w < 16; w++) {
+            s += sums[0][w];
+            n += sums[1][w];
+        }
+        *p.loss = (float)(s / n);
+        *p.total = (float)n;
+    }
+}
+
+// The gradient of the columns [c0, c1) of a row by NT threads: blockIdx.y's
+// share of the row, whole vectors. The entries' columns are stored a second
+// time, by one thread each.
+template <class E, int NT>
+__global__ __launch_bounds__(256) void distill_grad_kernel(DistillParams p, int share) {
+    constexpr int N = RowVec<E>::N, RW = 256 / NT;
+    const int tid = threadIdx.x % NT;
+    const int c0 = blockIdx.y * share, c1 = min(c0 + share, p.V);
+    const int nvec = (c1 - c0) / N, tail = c1 - c0 - nvec * N;
+    const float c = kLog2e / p.temperature;
+    for (long long i = (long long)blockIdx.x * RW + threadIdx.x / NT; i < p.rows; i += (long long)gridDim.x * RW) {
+        const long long r = p.rows - 1 - i;
+        const E* x = static_cast<const E*>(p.x) + (r / p.inner) * p.outer_stride + (r % p.inner) * p.row_stride + c0;
+        E* dx = static_cast<E*>(p.dx) + r * p.V + c0;
+        const DistillRow* keep = reinterpret_cast<const DistillRow*>(p.kept) + r;
+        const float weight = keep->weight;
+        const float g = weight == 0.f ? 0.f : *p.d_loss * weight / *p.total / p.temperature;
+        typename RowVec<E>::type o;
+        if (g == 0.f) {
+#pragma unroll
+            for (int k = 0; k < N; k++) o[k] = (E)0.f;
+            for (int j = tid; j < nvec; j += NT) store_row(dx + (size_t)j * N, o);
+            if (tid < tail) dx[nvec * N + tid] = (E)0.f;
+            continue;
+        }
+        const DistillRow row = *keep;
+        const float a = g * row.rest;
+        const auto grad = [&](float e) { return a * fast_exp2((e - row.rm) * c - row.rls); };
+        for (int i0 = 0; i0 < nvec; i0 += NT * DS_NV) {
+            typename RowVec<E>::type v[DS_NV];
+#pragma unroll
+            for (int j = 0; j < DS_NV; j++) v[j] = load_row(x + (size_t)min(i0 + j * NT + tid, nvec - 1) * N);
+#pragma unroll
+            for (int j = 0; j < DS_NV; j++) {
+                const int at = i0 + j * NT + tid;
+                if (at < nvec) {
+#pragma unroll
+                    for (int k = 0; k < N; k++) o[k] = (E)grad((float)v[j][k]);
+                    store_row(dx + (size_t)at * N, o);
+                }
+            }
+        }
+        if (tid < tail) dx[nvec * N + tid] = (E)grad((float)x[nvec * N + tid]);
+        row_sync<NT>();  // the entries' columns are written again
+        const long long* ids = p.ids + r * p.k;
+        const float* t = p.values + r * p.k;
+        for (int j = tid; j < p.k; j += NT) {
+            const long long id = ids[j];
+            bool first = id >= c0 && id < c1 && t[j] != -INFINITY;
+            float sum = 0.f;
+            if (first)
+                for (int l = 0; l < p.k; l++)
+                    if (ids[l] == id && t[l] != -INFINITY) {
+                        if (l < j) first = false;
+                        sum += fast_exp2(t[l] * c - row.norm);
+                    }
+            if (first) {
+                const float q = fast_exp2(((float)x[id - c0] - row.m) * c - row.ls);
+                dx[id - c0] = (E)(g * (q * row.entry - sum));
+            }
+        }
+        row_sync<NT>();
+    }
+}
+
+template <class E, int NT>
+void launch_rows(DistillParams p, hipStream_t stream) {
+    const dim3 grid((unsigned)min((p.rows + rows_of(NT) - 1) / rows_of(NT), (long long)LOGPROBS_MAX_GRID)), block(NT * rows_of(NT));
+    if (p.tail) {
+        p.words = (p.V + 31) / 32;
+        hipLaunchKernelGGL((distill_kernel<E, NT, true>), grid, block, (size_t)p.words * 4 * rows_of(NT), stream, p);
+    } else {
+        hipLaunchKernelGGL((distill_kernel<E, NT, false>), grid, block, 0, stream, p);
+    }
+}
+
+template <class E, int NT>
+void launch_grad(const DistillParams& p, int shares, hipStream_t stream) {
+    constexpr int N = RowVec<E>::N, RW = 256 / NT;
+    const int share = ((p.V + shares - 1) / shares + N - 1) / N * N;
+    const dim3 grid((unsigned)min((p.rows + RW - 1) / RW, (long long)LOGPROBS_MAX_GRID), (unsigned)((p.V + share - 1) / share));
+    hipLaunchKernelGGL((distill_grad_kernel<E, NT>), grid, dim3(256), 0, stream, p, share);
+}
+
+template <class E>
+void launch(const DistillParams& p, bool grad, hipStream_t stream) {
+    constexpr int N = RowVec<E>::N;
+    const bool narrow = p.V <= 64 * DS_NV * N;
+    if (grad) {
+        if (narrow)
+            launch_grad<E, 64>(p, 1, stream);
+        else  // few rows shared out to about four workgroups of a compute unit
+            launch_grad<E, 256>(p, (int)min((1024 + p.rows - 1) / p.rows, (long long)(p.V + 256 * N - 1) / (256 * N)), stream);
+    } else if (narrow) {
+        launch_rows<E, 64>(p, stream);
+    } else {
+        launch_rows<E, 256>(p, stream);
+    }
+}
+
+}  // namespace
+
+void launch_distill(const DistillParams& p, int dtype, bool grad, hipStream_t stream) {
+    if (p.rows > 0) {
+        if (dtype == 0)
+            launch<bf16_t>(p, grad, stream);
+        else if (dtype == 1)
+            launch<float>(p, grad, stream);
+        else
+            launch<f16_t>(p, grad, stream);
+    }
+    if (!grad) hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, stream, p);
+}
+
+}  // namespace cyfa

@@ -610,4 +610,78 @@ constexpr int RESIDUAL_MAX_D = 8192;
 size_t residual_workspace_bytes(long long rows, int D);
 void launch_residual_norm(const ResidualParams& p, int dtype, bool grad, hipStream_t stream);
 
+// Logits with penalties for the tokens of a row's history, biases and a mask,
+// and the gradient (cyfa_adjust.hip). Row r of a tensor lies at
+// (r / inner) outer + (r % inner) row elements.
+struct AdjustParams {
+    long long rows, inner;
+    int V;
+    const void* x;
+    long long x_outer, x_row;
+    const void* history;         // [rows, L] int64 (wide) or int32; tokens outside [0, V) are passed over
+    long long h_outer, h_row, L;
+    int wide;
+    const long long *lengths, *prompts;  // nullable [rows]: tokens of the history, those of its prompt
+    float repetition, presence, frequency;
+    const float *repetitions, *presences, *frequencies;  // nullable [rows], in place of the numbers
+    const float* bias;           // nullable [rows, V]
+    long long b_outer, b_row;
+    const long long* token_ids;  // [rows, n_tokens], the same token several times adds up
+    long long ti_outer, ti_row;
+    const float* token_values;
+    long long tv_outer, tv_row;
+    int n_tokens;
+    const void* allowed;         // nullable [rows, V] bytes, or (packed) a bit a column; strides in bytes
+    long long a_outer, a_row;
+    int packed;
+    const void* dy;              // gradient: [rows, V]
+    void* y;                     // may be x, with its strides; gradient: dx
+    long long y_outer, y_row;
+    int cols;                    // of a slice, set by the launcher
+    long long jobs;
+};
+constexpr int ADJUST_MAX_TOKENS = 1024;
+void launch_adjust(const AdjustParams& p, int dtype, bool grad, hipStream_t stream);
+
+// The choice of a token from each row of logits (cyfa_sample.hip).
+struct SampleParams {
+    long long rows, inner;
+    long long outer_stride, row_stride;
+    int V;
+    const void* x;
+    const float* uniform;        // [rows], or
+    const double* uniform64;
+    double temperature, top_p, min_p;
+    long long top_k;
+    const float *temperatures, *top_ps, *min_ps;  // nullable [rows], in place of the numbers
+    const long long* top_ks;
+    long long* ids;              // [rows]
+    float* logprob;              // [rows]
+    double one;                  // the integer of weight 1, set by the launcher
+};
+void launch_sample(SampleParams p, int dtype, hipStream_t stream);
+
+// The divergence from a teacher's most probable tokens, and the gradient
+// (cyfa_distill.hip).
+struct DistillParams {
+    long long rows, inner;
+    long long outer_stride, row_stride;
+    int V;
+    const void* x;
+    int k;
+    const long long* ids;        // [rows, k]
+    const float* values;         // [rows, k]
+    const float* weights;        // nullable [rows]
+    float temperature;
+    int tail;
+    float* kept;                 // [rows, DISTILL_ROW_FLOATS]
+    float *loss, *total;         // [1]: the weighted mean, the weights' sum
+    const float* d_loss;         // gradient: [1]
+    void* dx;                    // gradient: [rows, V]
+    int words;                   // set by the launcher
+};
+constexpr int DISTILL_ROW_FLOATS = 10, DISTILL_MAX_K = 256;
+constexpr int DISTILL_MAX_TAIL_V = 1 << 19;  // a bit a column in 64 KiB of LDS
+void launch_distill(const DistillParams& p, int dtype, bool grad, hipStream_t stream);
+
 }  // namespace cyfa

@@ -12,6 +12,8 @@ from .models.cyfa import (
     CyclicFlowAttentionModel,
 )
 
+from .sampling import Sampler, Sampling
+
 __version__ = "0.1.2"
 
 __all__ = [
@@ -19,4 +21,6 @@ __all__ = [
     "CyclicFlowAttentionConfig",
     "CyclicFlowAttentionForCausalLM",
     "CyclicFlowAttentionModel",
+    "Sampler",
+    "Sampling",
 ]

@@ -15,7 +15,7 @@ import torch
 import torch.nn.functional as F
 
 LIB_PATH = Path(os.environ.get("CYFA_LIB", Path(__file__).with_name("libcyfa_hip.so")))
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 CYFA_OK = 0
 CYFA_ERR_VALUE = -1
@@ -207,6 +207,41 @@ class CyfaResidualArgs(ctypes.Structure):
     ]
 
 
+class CyfaAdjustArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_longlong), ("inner", ctypes.c_longlong), ("V", _c_int),
+        ("x", _c_void_p), ("x_outer", ctypes.c_longlong), ("x_row", ctypes.c_longlong),
+        ("history", _c_void_p), ("h_outer", ctypes.c_longlong), ("h_row", ctypes.c_longlong), ("L", ctypes.c_longlong),
+        ("wide", _c_int), ("lengths", _c_void_p), ("prompts", _c_void_p),
+        ("repetition", _c_float), ("presence", _c_float), ("frequency", _c_float),
+        ("repetitions", _c_void_p), ("presences", _c_void_p), ("frequencies", _c_void_p),
+        ("bias", _c_void_p), ("b_outer", ctypes.c_longlong), ("b_row", ctypes.c_longlong),
+        ("token_ids", _c_void_p), ("ti_outer", ctypes.c_longlong), ("ti_row", ctypes.c_longlong),
+        ("token_values", _c_void_p), ("tv_outer", ctypes.c_longlong), ("tv_row", ctypes.c_longlong), ("n_tokens", _c_int),
+        ("allowed", _c_void_p), ("a_outer", ctypes.c_longlong), ("a_row", ctypes.c_longlong), ("packed", _c_int),
+        ("dy", _c_void_p), ("y", _c_void_p), ("y_outer", ctypes.c_longlong), ("y_row", ctypes.c_longlong),
+    ]
+
+
+class CyfaSampleArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_longlong), ("inner", ctypes.c_longlong), ("outer_stride", ctypes.c_longlong),
+        ("row_stride", ctypes.c_longlong), ("V", _c_int), ("x", _c_void_p), ("uniform", _c_void_p), ("uniform64", _c_void_p),
+        ("temperature", ctypes.c_double), ("top_p", ctypes.c_double), ("min_p", ctypes.c_double), ("top_k", ctypes.c_longlong),
+        ("temperatures", _c_void_p), ("top_ps", _c_void_p), ("min_ps", _c_void_p), ("top_ks", _c_void_p),
+        ("ids", _c_void_p), ("logprob", _c_void_p),
+    ]
+
+
+class CyfaDistillArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_longlong), ("inner", ctypes.c_longlong), ("outer_stride", ctypes.c_longlong),
+        ("row_stride", ctypes.c_longlong), ("V", _c_int), ("x", _c_void_p), ("k", _c_int), ("ids", _c_void_p),
+        ("values", _c_void_p), ("weights", _c_void_p), ("temperature", _c_float), ("tail", _c_int), ("kept", _c_void_p),
+        ("loss", _c_void_p), ("total", _c_void_p), ("d_loss", _c_void_p), ("dx", _c_void_p),
+    ]
+
+
 # Every symbol include/cyfa_abi.h declares, with its ctypes signature.
 SIGNATURES = {
     "cyfa_chunk_fwd": (_c_int, [ctypes.POINTER(CyfaChunkArgs), _c_void_p]),
@@ -248,6 +283,9 @@ SIGNATURES = {
     "cyfa_embed": (_c_int, [ctypes.POINTER(CyfaEmbedArgs), _c_int, _c_int, _c_void_p]),
     "cyfa_residual_grad_workspace_bytes": (_c_size_t, [ctypes.c_longlong, _c_int]),
     "cyfa_residual_norm": (_c_int, [ctypes.POINTER(CyfaResidualArgs), _c_int, _c_int, _c_void_p]),
+    "cyfa_adjust_logits": (_c_int, [ctypes.POINTER(CyfaAdjustArgs), _c_int, _c_int, _c_void_p]),
+    "cyfa_sample_tokens": (_c_int, [ctypes.POINTER(CyfaSampleArgs), _c_int, _c_int, _c_void_p]),
+    "cyfa_distill_loss": (_c_int, [ctypes.POINTER(CyfaDistillArgs), _c_int, _c_int, _c_void_p]),
     "cyfa_last_error": (ctypes.c_char_p, []),
     "cyfa_abi_version": (_c_int, []),
 }
@@ -1123,3 +1161,130 @@ def residual_norm_grad(x, y, weight, post, gate, scale, eps, stats, d_s, d_h, ne
                             workspace.data_ptr(), size)
     _lm_call("cyfa_residual_norm", args, x.dtype, 1, dev)
     return dx if needed[0] else None, dx if plain and needed[1] else dy, dw, dp, dg
+
+
+# The largest sizes of the operators on a model's logits (CYFA_ADJUST_MAX_TOKENS,
+# CYFA_DISTILL_MAX_K): token biases of a row; tokens of a teacher; the vocabulary
+# beside a teacher's tail. Floats a row that distill_loss keeps for its gradient.
+ADJUST_MAX_TOKENS, DISTILL_MAX_K, DISTILL_MAX_TAIL_V, DISTILL_ROW_FLOATS = 1024, 256, 1 << 19, 10
+
+
+def leading_strides(t):
+    """(outer, row) strides of t [rows..., n], its rows contiguous: row r of the
+    flattened leading dimensions at (r / inner) outer + (r % inner) row, inner
+    the last of them; and the tensor they describe: t, or a copy."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    if t.dim() == 1:
+        return (0, 0), t
+    if t.dim() == 2:
+        return (0, t.stride(0)), t
+    if t.dim() > 3:
+        t = t.reshape(-1, *t.shape[-2:])
+    return (t.stride(0), t.stride(1)), t
+
+
+def adjust(logits, out, history, lengths, prompts, penalties, bias, tokens, allowed, dy=None):
+    """Writes logits [..., V] with the penalties for history's tokens, biases and
+    mask into out (the logits themselves, or of their shape), or with dy
+    (contiguous) the gradient of the logits. history [..., L] int64 or int32,
+    bias [..., V] fp32, tokens ([..., n] int64, [..., n] fp32) and allowed
+    [..., V] bool or [..., words] int32 have the logits' leading shape (expanded
+    views are read in place), lengths and prompts are int64 contiguous, each of
+    the three penalties a number or fp32 contiguous; all of them may be None."""
+    dev = logits.device
+    V = logits.shape[-1]
+    (xo, xr), x = leading_strides(logits)
+    (yo, yr), y = ((xo, xr), x) if out is logits else leading_strides(out)
+    args = CyfaAdjustArgs(logits.numel() // V, logits.shape[-2] if logits.dim() > 1 else 1, V, x.data_ptr(), xo, xr)
+    args.inner = max(args.inner, 1)
+    args.y, args.y_outer, args.y_row = y.data_ptr(), yo, yr
+    kept = [x, y]  # alive until the launch
+    if history is not None and history.shape[-1] > 0:
+        (args.h_outer, args.h_row), history = leading_strides(history)
+        args.history, args.L, args.wide = history.data_ptr(), history.shape[-1], history.dtype is torch.int64
+        args.lengths, args.prompts = ptr(lengths), ptr(prompts)
+        kept.append(history)
+    for name, v in zip(("repetition", "presence", "frequency"), penalties):
+        if isinstance(v, torch.Tensor):
+            setattr(args, name[:-1] + "ies" if name == "frequency" else name + "s", v.data_ptr())
+        else:
+            setattr(args, name, v)
+    if bias is not None:
+        (args.b_outer, args.b_row), bias = leading_strides(bias)
+        args.bias = bias.data_ptr()
+        kept.append(bias)
+    if tokens is not None and tokens[0].shape[-1] > 0:
+        (args.ti_outer, args.ti_row), ids = leading_strides(tokens[0])
+        (args.tv_outer, args.tv_row), values = leading_strides(tokens[1])
+        args.token_ids, args.token_values, args.n_tokens = ids.data_ptr(), values.data_ptr(), ids.shape[-1]
+        kept += [ids, values]
+    if allowed is not None:
+        (ao, ar), allowed = leading_strides(allowed)
+        args.packed = allowed.dtype is torch.int32
+        size = 4 if args.packed else 1
+        args.allowed, args.a_outer, args.a_row = allowed.data_ptr(), ao * size, ar * size
+        kept.append(allowed)
+    args.dy = ptr(dy)
+    _lm_call("cyfa_adjust_logits", args, logits.dtype, 0 if dy is None else 1, dev)
+
+
+def sample(logits, uniform, temperature, top_k, top_p, min_p):
+    """(ids int64, logprob fp32) [...] of logits [..., V]; uniform [...] fp32 or
+    fp64 contiguous; each option a number or contiguous [...] (fp32, top_k int64)."""
+    dev = logits.device
+    fields, logits = logit_rows(logits)
+    ids = torch.empty(uniform.shape, dtype=torch.int64, device=dev)
+    logprob = torch.empty(uniform.shape, dtype=torch.float32, device=dev)
+    args = CyfaSampleArgs(*fields, ids=ids.data_ptr(), logprob=logprob.data_ptr())
+    if uniform.dtype is torch.float32:
+        args.uniform = uniform.data_ptr()
+    else:
+        args.uniform64 = uniform.data_ptr()
+    if isinstance(temperature, torch.Tensor):
+        args.temperatures = temperature.data_ptr()
+    else:
+        args.temperature = temperature
+    if isinstance(top_k, torch.Tensor):
+        args.top_ks = top_k.data_ptr()
+    else:
+        args.top_k = top_k
+    if isinstance(top_p, torch.Tensor):
+        args.top_ps = top_p.data_ptr()
+    else:
+        args.top_p = top_p
+    if isinstance(min_p, torch.Tensor):
+        args.min_ps = min_p.data_ptr()
+    else:
+        args.min_p = min_p
+    _lm_call("cyfa_sample_tokens", args, logits.dtype, 0, dev)
+    return ids, logprob
+
+
+def distill_loss(logits, ids, values, weights, temperature, tail):
+    """(loss, what distill_loss_grad needs): ids int64 and values fp32 [..., k],
+    weights fp32 [...] or None, all contiguous."""
+    dev = logits.device
+    fields, logits = logit_rows(logits)
+    rows = fields[0]
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    kept = torch.empty(rows * DISTILL_ROW_FLOATS + 1, dtype=torch.float32, device=dev)
+    at = kept.data_ptr()
+    args = CyfaDistillArgs(*fields, k=ids.shape[-1], ids=ids.data_ptr(), values=values.data_ptr(), weights=ptr(weights),
+                           temperature=temperature, tail=tail, kept=at, loss=loss.data_ptr(),
+                           total=at + 4 * rows * DISTILL_ROW_FLOATS)
+    _lm_call("cyfa_distill_loss", args, logits.dtype, 0, dev)
+    return loss, kept
+
+
+def distill_loss_grad(logits, ids, values, weights, temperature, tail, kept, d_loss):
+    """The gradient of logits from the loss's cotangent (fp32, on the device)."""
+    dev = logits.device
+    dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    fields, logits = logit_rows(logits)
+    at = kept.data_ptr()
+    args = CyfaDistillArgs(*fields, k=ids.shape[-1], ids=ids.data_ptr(), values=values.data_ptr(), weights=ptr(weights),
+                           temperature=temperature, tail=tail, kept=at, total=at + 4 * fields[0] * DISTILL_ROW_FLOATS,
+                           d_loss=d_loss.data_ptr(), dx=dx.data_ptr())
+    _lm_call("cyfa_distill_loss", args, dx.dtype, 1, dev)
+    return dx

@@ -5,11 +5,17 @@
 from a seeded numpy generator); ``generate_batch`` runs right-padded prompts
 through one masked prefill and then greedy decode steps, each row stopping on
 its own. Both return token ids as Python lists, as the reference does; the
-model runs on whatever device holds its parameters.
+model runs on whatever device holds its parameters. With a ``Sampling`` both
+choose their tokens on the model's GPU, with penalties, biases, masks, top-k and
+min-p besides.
 """
 
 import numpy as np
 import torch
+
+from .sampling import Sampler, Sampling
+
+__all__ = ["Sampling", "generate", "generate_batch"]
 
 
 def _device(model):
@@ -30,22 +36,29 @@ def _nucleus(logits, temperature, top_p, rng):
 
 
 @torch.no_grad()
-def generate(model, ids, max_new_tokens=64, eos_token_id=None, temperature=0.0, top_p=1.0, seed=42, on_token=None):
+def generate(model, ids, max_new_tokens=64, eos_token_id=None, temperature=0.0, top_p=1.0, seed=42, on_token=None,
+             sampling=None):
     """New tokens after the prompt ``ids`` (a list of ints). Stops after
     max_new_tokens, on eos_token_id (which is kept), or when
     on_token(generated) returns true. ValueError for an empty prompt, a
-    negative length or temperature, or top_p outside (0, 1]."""
+    negative length or temperature, or top_p outside (0, 1]. ``sampling`` (a
+    Sampling) in place of temperature, top_p and seed."""
     if not ids or max_new_tokens < 0 or temperature < 0 or not 0 < top_p <= 1:
         raise ValueError("Invalid prompt or sampling options")
+    if sampling is not None and (temperature, top_p, seed) != (0.0, 1.0, 42):
+        raise ValueError("temperature, top_p and seed are the Sampling's own")
     model.eval()
     dev = _device(model)
     rng = np.random.default_rng(seed)
+    sampler = None if sampling is None else Sampler(sampling, torch.tensor([list(ids)], dtype=torch.long, device=dev), max_new_tokens)
     current, cache, generated = list(ids), None, []
     for _ in range(max_new_tokens):
         result = model(torch.tensor([current], dtype=torch.long, device=dev), cache=cache, use_cache=True)
         cache = result["cache"]
         last = result["logits"][0, -1]
-        if temperature == 0:
+        if sampler is not None:
+            token = int(sampler.next(last[None], [generated]))
+        elif temperature == 0:
             # greedy: the first largest logit, found on the device (one index
             # crosses to the host, not the row); NaN counts as largest, as in
             # numpy's argmax of the same values
@@ -62,8 +75,9 @@ def generate(model, ids, max_new_tokens=64, eos_token_id=None, temperature=0.0, 
 
 
 @torch.no_grad()
-def generate_batch(model, prompts, max_new_tokens=48, eos_token_id=None, on_token=None):
-    """Greedy continuations of several prompts at once. The prompts are
+def generate_batch(model, prompts, max_new_tokens=48, eos_token_id=None, on_token=None, sampling=None):
+    """Continuations of several prompts at once, greedy or with ``sampling`` (a
+    Sampling). The prompts are
     right-padded to a multiple of 64 tokens and run through one prefill with
     an attention mask (pads leave the state and the conv cache unchanged);
     each row's first token comes from the logits at its last prompt token.
@@ -85,8 +99,9 @@ def generate_batch(model, prompts, max_new_tokens=48, eos_token_id=None, on_toke
     hidden, cache = model.model(ids.to(dev), use_cache=True, attention_mask=mask.to(dev))
     last = hidden[torch.arange(len(prompts), device=dev), (lengths - 1).to(dev)]
     logits = model.lm_head(last)
+    sampler = None if sampling is None else Sampler(sampling, ids.to(dev), max_new_tokens, lengths)
     for step in range(max_new_tokens):
-        tokens = logits.argmax(-1)
+        tokens = logits.argmax(-1) if sampler is None else sampler.next(logits, generated)
         for row, token in enumerate(tokens.tolist()):
             if finished[row]:
                 continue

@@ -5,6 +5,7 @@ pre-norm attention + SwiGLU MLP blocks, torch-checkpoint-compatible parameter
 names, and the bf16 precision policy of ``to_bfloat16``.
 """
 
+import copy
 import math
 from contextlib import nullcontext
 
@@ -16,8 +17,10 @@ from ... import _native
 from ..._autograd import kernel_ok
 from ...layers.autograd import hip_autograd_ok
 from ...layers.cyfa import CyclicFlowAttention, FusedWeight, RMSNorm, inference_fast_path, plain_linear, plain_module
+from ...ops.distill import distill_loss
 from ...ops.residual import residual_norm
 from ...ops.vocab import embed_tokens, token_logprobs, token_loss
+from ...sampling import Sampler
 
 
 def mlp_width(config):
@@ -317,6 +320,26 @@ class CyclicFlowAttentionForCausalLM(nn.Module):
             tokens = tokens.masked_fill(attention_mask[:, 1:] == 0, -100)
         return token_logprobs(logits[:, :-1], tokens, top_k=top_k)
 
+    def distill(self, input_ids, top_ids, top_logprobs, temperature=1.0, tail=False, attention_mask=None):
+        """The mean divergence of this model's predictions of the tokens input_ids
+        [B, T] after the first from a teacher's, known at its most probable tokens:
+        top_ids and top_logprobs [B, T - 1, k] as the teacher's score(input_ids,
+        top_k=k) gives them (ops.distill_loss; a GPU model). With a right-padding
+        attention_mask [B, T], padded tokens do not count. Differentiable."""
+        B, T = input_ids.shape
+        if top_ids.shape[:-1] != (B, T - 1) or top_ids.shape != top_logprobs.shape:
+            raise ValueError(f"distill: the teacher's tokens must be [{B}, {T - 1}, k], got {tuple(top_ids.shape)} {tuple(top_logprobs.shape)}")
+        hidden, _ = self.model(input_ids, attention_mask=attention_mask)
+        if inference_fast_path(hidden):
+            logits = _native.linear(hidden, self.lm_head.weight)
+        else:
+            logits = self.lm_head(hidden)
+        if attention_mask is not None:
+            top_ids = top_ids.masked_fill(attention_mask[:, 1:, None] == 0, -100)
+        # a row of no tokens at the end instead of shorter logits: the gradient is written once, in place
+        return distill_loss(logits, F.pad(top_ids, (0, 0, 0, 1), value=-100), F.pad(top_logprobs, (0, 0, 0, 1)),
+                            temperature=temperature, tail=tail)
+
     def to_bfloat16(self):
         for name, p in self.named_parameters():
             if not any(s in name for s in FP32_PARAMETERS):
@@ -324,24 +347,30 @@ class CyclicFlowAttentionForCausalLM(nn.Module):
         return self
 
     @torch.no_grad()
-    def graphed_decoder(self, cache, tokens):
-        """A GraphedDecodeStep continuing from a prefill cache and the last tokens [B, 1]."""
-        return GraphedDecodeStep(self, cache, tokens)
+    def graphed_decoder(self, cache, tokens, sampler=None):
+        """A GraphedDecodeStep continuing from a prefill cache and the last tokens
+        [B, 1], greedy or with a sampling.Sampler that holds the tokens so far."""
+        return GraphedDecodeStep(self, cache, tokens, sampler)
 
     @torch.no_grad()
-    def generate(self, input_ids, max_new_tokens=32, eos_token_id=None):
-        """Greedy decoding with the constant-size state (modeling_cyfa.py:142-158).
+    def generate(self, input_ids, max_new_tokens=32, eos_token_id=None, sampling=None):
+        """Decoding with the constant-size state (modeling_cyfa.py:142-158), greedy
+        or with ``sampling`` (a sampling.Sampling without a function of the tokens).
 
-        The argmax stays on the device; tokens are copied to the host once at
+        The choice stays on the device; tokens are copied to the host once at
         the end (the reference synchronises every step)."""
         self.eval()
+        sampler = None if sampling is None else Sampler(sampling, input_ids, max_new_tokens)
+        if sampler is not None and callable(sampling.allowed):
+            raise ValueError("generate: masks that follow the tokens are generation.generate_batch's")
         tokens = [input_ids]
         cache = None
         current = input_ids
         for _ in range(max_new_tokens):
             result = self(current, cache=cache, use_cache=True)
             cache = result["cache"]
-            current = result["logits"][:, -1:].argmax(-1)
+            last = result["logits"][:, -1:]
+            current = last.argmax(-1) if sampler is None else sampler.next(last[:, 0])[:, None]
             tokens.append(current)
             if eos_token_id is not None and bool((current == eos_token_id).all()):
                 break
@@ -361,11 +390,12 @@ def _clone_cache(c):
 
 
 class GraphedDecodeStep:
-    """One greedy decode step of the whole model, captured as HIP graphs.
+    """One decode step of the whole model, captured as HIP graphs.
 
     A step reads the token buffer, runs every layer's one-token path, writes
     the new recurrent states and conv histories, and stores the argmax token
-    in the token buffer for the next replay. Two caches alternate: the step
+    (or that of a sampling.Sampler, which keeps it and counts its room) in the
+    token buffer for the next replay. Two caches alternate: the step
     captured from cache 0 writes cache 1 and the other one back, so that no
     decode kernel updates a state in place (which lets it run several
     workgroups per (batch, head) at small batches; see decode_next on the
@@ -376,10 +406,13 @@ class GraphedDecodeStep:
     token (generation.py:23-62).
     """
 
-    def __init__(self, model, cache, tokens):
+    def __init__(self, model, cache, tokens, sampler=None):
         if not torch.cuda.is_available() or not tokens.is_cuda:
             raise ValueError("graphed decoding needs the model and tokens on a GPU")
+        if sampler is not None and callable(sampler.sampling.allowed):
+            raise ValueError("graphed decoding has no masks that follow the tokens")
         self.model = model
+        self.sampler = sampler
         self.tokens = tokens.detach().clone()
         first = [_clone_cache(c) for c in cache]
         self._caches = (first, [_clone_cache(c) for c in first])
@@ -393,7 +426,10 @@ class GraphedDecodeStep:
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):
-                model(self.tokens.clone(), cache=scratch, use_cache=True)
+                out = model(self.tokens.clone(), cache=scratch, use_cache=True)
+                if sampler is not None:
+                    copy.deepcopy(sampler).choose(out["logits"][:, -1])
+                del out
             torch.cuda.current_stream().wait_stream(side)
             del scratch
             for parity in (0, 1):
@@ -401,6 +437,8 @@ class GraphedDecodeStep:
                 for attn, nxt in zip(layers, dst):
                     attn.decode_next = nxt
                 graph = torch.cuda.CUDAGraph()
+                if sampler is not None:
+                    graph.register_generator_state(sampler.generator)
                 with torch.cuda.graph(graph):
                     out = model(self.tokens, cache=src, use_cache=True)
                     for d, o in zip(dst, out["cache"]):  # layers off the fused path return new tensors
@@ -411,7 +449,9 @@ class GraphedDecodeStep:
                             if a.data_ptr() != b.data_ptr():
                                 a.copy_(b)
                     last = out["logits"][:, -1:]
-                    if inference_fast_path(last):
+                    if sampler is not None:
+                        self.tokens.copy_(sampler.choose(last[:, 0])[:, None])
+                    elif inference_fast_path(last):
                         _native.argmax_rows(last, out=self.tokens)  # straight into the token buffer
                     else:
                         self.tokens.copy_(last.argmax(-1))
@@ -433,6 +473,8 @@ class GraphedDecodeStep:
         return self._logits[1 - self._parity]
 
     def step(self):
+        if self.sampler is not None:
+            self.sampler.take()
         self.graphs[self._parity].replay()
         self._parity ^= 1
         return self.tokens

@@ -3,8 +3,11 @@
 causal language model's blocks."""
 
 from .chunk import chunk_cyfa
+from .distill import distill_loss
 from .fused_recurrent import fused_recurrent_cyfa
 from .residual import residual_norm
+from .sampling import SampledTokens, adjust_logits, sample_tokens
 from .vocab import TokenLogprobs, embed_tokens, token_logprobs, token_loss
 
-__all__ = ["TokenLogprobs", "chunk_cyfa", "embed_tokens", "fused_recurrent_cyfa", "residual_norm", "token_logprobs", "token_loss"]
+__all__ = ["SampledTokens", "TokenLogprobs", "adjust_logits", "chunk_cyfa", "distill_loss", "embed_tokens",
+           "fused_recurrent_cyfa", "residual_norm", "sample_tokens", "token_logprobs", "token_loss"]

@@ -1,0 +1,109 @@
+"""The choice of the next tokens of a batch of sequences, on the model's GPU:
+penalties, biases and masks on the logits, then temperature, top-k, top-p and
+min-p (ops.adjust_logits, ops.sample_tokens), with the sequences' tokens kept on
+the device. (generation.py:23-62 of Chyxx/CyFA-Jittor v0.1.2 chooses on the
+host, by temperature and top-p alone.)"""
+
+import copy
+from dataclasses import dataclass
+
+import torch
+
+from .ops.sampling import adjust_logits, sample_tokens
+
+
+@dataclass(frozen=True)
+class Sampling:
+    """How tokens are chosen. Numbers are for every sequence, tensors [B] for
+    each; their meaning is that of ops.adjust_logits and ops.sample_tokens.
+    ``bias``: a float tensor [V] or [B, V]; ``token_bias``: a dict {token: value};
+    ``allowed``: a mask (bool [V] or [B, V], or int32 words of bits), or in
+    generate and generate_batch a function of the sequences' new tokens so far
+    (a list of lists) that returns one, or None. ``seed``: of the batch's random
+    numbers."""
+
+    temperature: float | torch.Tensor = 1.0
+    top_k: int | torch.Tensor = 0
+    top_p: float | torch.Tensor = 1.0
+    min_p: float | torch.Tensor = 0.0
+    repetition: float | torch.Tensor = 1.0
+    presence: float | torch.Tensor = 0.0
+    frequency: float | torch.Tensor = 0.0
+    bias: torch.Tensor | None = None
+    token_bias: dict | None = None
+    allowed: object = None
+    seed: int = 42
+
+
+class Sampler:
+    """Chooses the next tokens of B sequences under a ``Sampling`` and keeps their
+    tokens: ``prompts`` [B, T], of which the first ``lengths`` [B] (all without)
+    count, and up to ``room`` tokens more. Its calls can be captured into a HIP
+    graph (GraphedDecodeStep does), where ``generator`` has to be registered and
+    the caller counts the replays with ``take``."""
+
+    def __init__(self, sampling, prompts, room, lengths=None):
+        if prompts.dim() != 2 or prompts.dtype not in (torch.int64, torch.int32) or room < 0:
+            raise ValueError("a Sampler needs prompts [B, T] of int64 or int32 tokens and room for no fewer than 0 more")
+        dev, (B, T) = prompts.device, prompts.shape
+        self.sampling, self.room = sampling, room
+        self.history = torch.full((B, T + room), -1, dtype=torch.int64, device=dev)
+        self.history[:, :T] = prompts
+        if lengths is None:
+            lengths = torch.full((B,), T, dtype=torch.int64, device=dev)
+        self.prompt_lengths = lengths.to(device=dev, dtype=torch.int64).clone()
+        self.lengths = self.prompt_lengths.clone()
+        self.generator = torch.Generator(device=dev).manual_seed(sampling.seed)
+
+        def here(v):
+            return v.to(dev) if isinstance(v, torch.Tensor) else v
+
+        s = sampling
+        self._choice = dict(temperature=here(s.temperature), top_k=here(s.top_k), top_p=here(s.top_p), min_p=here(s.min_p))
+        self._penalties = dict(repetition=here(s.repetition), presence=here(s.presence), frequency=here(s.frequency))
+        self._bias = here(s.bias)
+        self._allowed = here(s.allowed)
+        self._token_bias = None
+        if s.token_bias:
+            self._token_bias = (torch.tensor(list(s.token_bias), dtype=torch.int64, device=dev),
+                                torch.tensor([float(v) for v in s.token_bias.values()], device=dev))
+        self._penalised = any(isinstance(v, torch.Tensor) or v != none for v, none in
+                              zip((s.repetition, s.presence, s.frequency), (1.0, 0.0, 0.0)))
+
+    def __deepcopy__(self, memo):
+        """A Sampler of its own state (the random numbers' among it), for a trial run."""
+        other = copy.copy(self)
+        other.history, other.lengths = self.history.clone(), self.lengths.clone()
+        other.generator = torch.Generator(device=self.generator.device)
+        other.generator.set_state(self.generator.get_state())
+        return other
+
+    def take(self):
+        """Counts one token of every sequence; ValueError where there is no room for it."""
+        if self.room <= 0:
+            raise ValueError("the Sampler has no room for more tokens")
+        self.room -= 1
+
+    @torch.no_grad()
+    def choose(self, logits, allowed=None):
+        """The next tokens [B] for logits [B, V], kept as the sequences' last; the
+        caller has counted them (``take``). ``allowed`` in place of the Sampling's."""
+        if allowed is None:
+            allowed = self._allowed if isinstance(self._allowed, torch.Tensor) else None
+        else:
+            allowed = allowed.to(logits.device)
+        if self._penalised or self._bias is not None or self._token_bias is not None or allowed is not None:
+            given = (self.history, self.lengths, self.prompt_lengths) if self._penalised else (None, None, None)
+            logits = adjust_logits(logits, *given, **self._penalties, bias=self._bias, token_bias=self._token_bias, allowed=allowed)
+        uniform = torch.rand(logits.shape[0], device=logits.device, generator=self.generator)
+        ids = sample_tokens(logits, uniform, **self._choice).ids
+        at = self.lengths.clamp(max=self.history.shape[1] - 1)[:, None]
+        self.history.scatter_(1, at, ids[:, None])
+        self.lengths.add_(1)
+        return ids
+
+    def next(self, logits, generated=None):
+        """take and choose, with a mask from the Sampling's function of ``generated``."""
+        self.take()
+        allowed = self.sampling.allowed
+        return self.choose(logits, allowed(generated) if callable(allowed) and not isinstance(allowed, torch.Tensor) else None)

@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define CYFA_ABI_VERSION 17
+#define CYFA_ABI_VERSION 18
 
 enum {
     CYFA_OK = 0,
@@ -665,6 +665,112 @@ typedef struct CyfaResidualArgs {
 
 size_t cyfa_residual_grad_workspace_bytes(long long rows, int D);
 int cyfa_residual_norm(const CyfaResidualArgs *args, int dtype, int grad, void *hip_stream);
+
+/* Logits as a sampler wants them (grad 0) and the gradient (grad 1), for rows x
+ * of V columns (CYFA_DTYPE_BF16, _F32 or _F16). Row r of a tensor with strides
+ * lies at (r / inner) outer + (r % inner) row elements, any alignment. With n the
+ * occurrences of column j in the row's history[0 .. length) and c those from
+ * position prompt on:
+ *   y = x > 0 ? x / repetition : x repetition     where n > 0
+ *   y -= c frequency + presence                   where c > 0
+ *   y += bias_j + sum of the token values of j
+ *   y = -inf                                      where j is not allowed
+ *   dx = dy (n > 0 ? (x > 0 ? 1 / repetition : repetition) : 1), 0 where j is not allowed
+ * in f32, rounded once. Lengths are clamped to [0, L]; tokens outside [0, V) are
+ * passed over. y may be x, with the same strides. No counterpart in the
+ * reference, whose generation samples the logits as they are (generation.py:23-62). */
+typedef struct CyfaAdjustArgs {
+    long long rows, inner;        /* inner > 0 */
+    int V;                        /* at most 2^28 */
+    const void *x;
+    long long x_outer, x_row;
+    const void *history;          /* L > 0: [rows, L], int64 (wide) or int32 */
+    long long h_outer, h_row;
+    long long L;                  /* below 2^31 */
+    int wide;
+    const long long *lengths;     /* nullable [rows]: L */
+    const long long *prompts;     /* nullable [rows]: 0 */
+    float repetition, presence, frequency;
+    const float *repetitions, *presences, *frequencies; /* nullable [rows], in place of the numbers */
+    const float *bias;            /* nullable f32 [rows, V] */
+    long long b_outer, b_row;
+    const long long *token_ids;   /* n_tokens > 0: [rows, n_tokens] */
+    long long ti_outer, ti_row;
+    const float *token_values;
+    long long tv_outer, tv_row;
+    int n_tokens;                 /* at most CYFA_ADJUST_MAX_TOKENS */
+    const void *allowed;          /* nullable [rows, V] bytes, 0: not allowed; or (packed) a bit a column, the lowest */
+    long long a_outer, a_row;     /* of a byte first; strides in bytes */
+    int packed;
+    const void *dy;               /* grad 1: [rows, V], contiguous */
+    void *y;                      /* grad 1: dx */
+    long long y_outer, y_row;
+} CyfaAdjustArgs;
+
+#define CYFA_ADJUST_MAX_TOKENS 1024
+int cyfa_adjust_logits(const CyfaAdjustArgs *args, int dtype, int grad, void *hip_stream);
+
+/* The choice of a token from each row of logits x (rows as CyfaLogprobArgs has
+ * them) with a number u in [0, 1) for each. With w_j = e^((x_j - max) / T), in the
+ * order of falling x, the lower index first, kept are the first top_k (0 or V and
+ * more: all), of those the ones before which less than top_p of their mass lies
+ * (1 and more: all; the first is always kept), of those the ones with w >= min_p.
+ * ids[r] is the first kept column, in the order of the columns, at which the
+ * running mass of the kept passes u times their mass; logprob[r] the logarithm of
+ * its share of that mass. T = 0: the first largest, logprob 0. A row that holds a
+ * NaN or +inf, or nothing but -inf, has no probabilities: its first largest (a
+ * NaN before all others), logprob NaN. Weights are held as multiples of 2^-46 of
+ * the largest (2^(ceil(log2 V) - 62) past 2^16 columns) and added up exactly. Replaces the host-side
+ * choice of generation.py:23-62; min_p and top_k have no counterpart there. grad
+ * has to be 0. */
+typedef struct CyfaSampleArgs {
+    long long rows, inner;        /* inner > 0 */
+    long long outer_stride, row_stride;
+    int V;                        /* at most 2^28 */
+    const void *x;
+    const float *uniform;         /* [rows], or */
+    const double *uniform64;
+    double temperature, top_p, min_p;
+    long long top_k;
+    const float *temperatures, *top_ps, *min_ps; /* nullable [rows], in place of the numbers */
+    const long long *top_ks;
+    long long *ids;               /* [rows] */
+    float *logprob;               /* [rows] */
+} CyfaSampleArgs;
+
+int cyfa_sample_tokens(const CyfaSampleArgs *args, int dtype, int grad, void *hip_stream);
+
+/* The divergence of q = softmax(x / T) (rows of logits as CyfaLogprobArgs has
+ * them) from a teacher's distribution known at k tokens of each row, entries
+ * (ids, values), those with an id outside [0, V) or a value of -inf left out:
+ *   tail 0: p = softmax(values / T) over the entries, l = sum p (log p - log q_id)
+ *   tail 1 (T = 1): p = e^values, l = the same + p_r (log p_r - log q_r), with
+ *     p_r = max(0, 1 - sum p), q_r = the sum of q over the columns of no entry
+ *     (nothing where those are all -inf)
+ *   loss = sum of weights l / sum of weights, over the rows with an entry and a weight other than 0
+ * and the logits' gradient (grad 1), contiguous, from kept and total as grad 0
+ * left them; rows that do not count get zeros. Equal ids add up. No counterpart in the reference. */
+typedef struct CyfaDistillArgs {
+    long long rows, inner;        /* inner > 0 */
+    long long outer_stride, row_stride;
+    int V;                        /* at most 2^28; with the tail, 2^19 */
+    const void *x;
+    int k;                        /* 1 .. CYFA_DISTILL_MAX_K */
+    const long long *ids;         /* [rows, k] */
+    const float *values;          /* [rows, k] */
+    const float *weights;         /* nullable [rows]: 1 */
+    float temperature;
+    int tail;
+    float *kept;                  /* [rows, CYFA_DISTILL_ROW_FLOATS] */
+    float *loss;                  /* grad 0: [1] */
+    float *total;                 /* [1] */
+    const float *d_loss;          /* grad 1: [1] */
+    void *dx;                     /* grad 1: [rows, V] */
+} CyfaDistillArgs;
+
+#define CYFA_DISTILL_MAX_K 256
+#define CYFA_DISTILL_ROW_FLOATS 10
+int cyfa_distill_loss(const CyfaDistillArgs *args, int dtype, int grad, void *hip_stream);
 
 /* Thread-local message of the last failing call (never NULL). No reference
  * counterpart: Jittor reports kernel errors as C++ exceptions. */
