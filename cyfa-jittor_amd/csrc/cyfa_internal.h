@@ -657,7 +657,7 @@ struct SampleParams {
     const long long* top_ks;
     long long* ids;              // [rows]
     float* logprob;              // [rows]
-    int bits;                    // weights are multiples of 2^-bits, set by the launcher
+    double unit;                 // 2^(52 - bits): weights are multiples of 2^-bits; set by the launcher
     long long first;             // row of a launch's first workgroup, set by the launcher
 };
 void launch_sample(SampleParams p, int dtype, hipStream_t stream);

@@ -88,33 +88,44 @@ __device__ __forceinline__ float kth_largest(float x, int k) {
     return -wave_max(rank < k ? -x : -INFINITY);
 }
 
+// An element in fp32. (Of a bf16 by its bits: the compiler takes the largest of
+// converted bf16 as a bf16, with a rounding and another conversion for each.)
+__device__ __forceinline__ float wide(float x) { return x; }
+__device__ __forceinline__ float wide(f16_t x) { return (float)x; }
+__device__ __forceinline__ float wide(bf16_t x) {
+    return __builtin_bit_cast(float, (uint32_t)__builtin_bit_cast(uint16_t, x) << 16);
+}
+
 // A row's settings.
 struct Choice {
     double m;       // the maximum
     double c;       // log2 e / T
-    int bits;       // weights are multiples of 2^-bits
+    double least;   // a distance to the maximum whose weight is nothing
+    double unit;    // 2^(52 - bits): weights are multiples of 2^-bits
+    double k[10];   // kExp2, in scalar registers
 };
 
-// 2^((x - m) c) as an integer multiple of 2^-bits: 2^n times the polynomial of
-// degree 10 that meets 2^f at the Chebyshev points of [-1/2, 1/2] (off by at most
-// 3.2e-16 of it); adding 2^52 rounds to an integer in the low bits.
+// The coefficients of the polynomial of degree 10 that meets 2^f at the Chebyshev
+// points of [-1/2, 1/2] (off by at most 3.2e-16 of it), but for the first, 1.
+constexpr int SM_DEGREE = 10;
+__device__ constexpr double kExp2[SM_DEGREE] = {0.69314718055995,       0.24022650695910097,   0.05550410866444772,    0.009618129107606888,
+                                                0.0013333558230164974,  0.0001540353044173605, 1.5252657260200837e-05, 1.321544258792169e-06,
+                                                1.0208690299958306e-07, 7.072585949269223e-09};
+
+// 2^((x - m) c) as an integer multiple of 2^-bits, without a branch: adding 1.5
+// 2^52 leaves the exponent's whole part n in the low bits; 2^n is put into the
+// exponent of the polynomial of the rest; adding 2^(52 - bits) rounds to an integer
+// in the low bits.
 __device__ __forceinline__ u64 weight(const Choice& ch, float x) {
-    const double t = ((double)x - ch.m) * ch.c;
-    if (!(t > -48.)) return 0;
-    const double n = rint(t), f = t - n;
-    double y = 7.072585949269223e-09;
-    y = fma(y, f, 1.0208690299958306e-07);
-    y = fma(y, f, 1.321544258792169e-06);
-    y = fma(y, f, 1.5252657260200837e-05);
-    y = fma(y, f, 0.0001540353044173605);
-    y = fma(y, f, 0.0013333558230164974);
-    y = fma(y, f, 0.009618129107606888);
-    y = fma(y, f, 0.05550410866444772);
-    y = fma(y, f, 0.24022650695910097);
-    y = fma(y, f, 0.69314718055995);
+    const double d = fmax((double)x - ch.m, ch.least);
+    const double shifted = fma(d, ch.c, 0x1.8p52), f = fma(d, ch.c, 0x1.8p52 - shifted);
+    double y = ch.k[SM_DEGREE - 1];
+#pragma unroll
+    for (int i = SM_DEGREE - 2; i >= 0; i--) y = fma(y, f, ch.k[i]);
     y = fma(y, f, 1.0);
-    y = ldexp(y, (int)n + ch.bits);
-    return __builtin_bit_cast(u64, y + 0x1p52) & 0xfffffffffffffull;
+    i32x2 bits = __builtin_bit_cast(i32x2, y);
+    bits[1] += __builtin_bit_cast(i32x2, shifted)[0] << 20;
+    return __builtin_bit_cast(u64, __builtin_bit_cast(double, bits) + ch.unit) & 0xfffffffffffffull;
 }
 
 // Rows of up to ROW bytes in LDS; ROW = 0: of any length, read anew for each pass.
@@ -169,9 +180,9 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         return v;
     };
     const auto largest = [&](const Piece& v) {
-        float top = (float)v[0];
+        float top = wide(v[0]);
 #pragma unroll
-        for (int c = 1; c < P; c++) top = fmaxf(top, (float)v[c]);
+        for (int c = 1; c < P; c++) top = fmaxf(top, wide(v[c]));
         return top;
     };
     // f(element, column) of this thread's elements in pieces that reach ``from``
@@ -181,7 +192,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
             const Piece v = piece(i);
             if (largest(v) >= from)
 #pragma unroll
-                for (int c = 0; c < P; c++) f((float)v[c], i * P + c);
+                for (int c = 0; c < P; c++) f(wide(v[c]), i * P + c);
         }
     };
     // ---- the maximum, the least finite element, what no distribution holds
@@ -202,7 +213,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
                 if (ROW) row_s[i] = v[j];
 #pragma unroll
                 for (int c = 0; c < N; c++) {
-                    const float e = (float)v[j][c];
+                    const float e = wide(v[j][c]);
                     bad |= e != e;
                     best = fmaxf(best, e);
                     least = fminf(least, e > -INFINITY ? e : INFINITY);
@@ -238,7 +249,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
                 const Piece v = piece(i);
 #pragma unroll
                 for (int c = 0; c < P; c++)
-                    if ((float)v[c] != (float)v[c]) at = min(at, (unsigned)(i * P + c));
+                    if (wide(v[c]) != wide(v[c])) at = min(at, (unsigned)(i * P + c));
             }
         for (int d = 32; d > 0; d >>= 1) at = min(at, (unsigned)__shfl_xor((int)at, d));
         __syncthreads();
@@ -253,8 +264,14 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     }
     Choice ch;
     ch.m = best;
-    ch.c = fmin(kLog2eD / T, 1e300);  // (0 times it stays 0)
-    ch.bits = p.bits;
+    ch.c = fmax(fmin(kLog2eD / T, 1e300), 1e-300);  // (0 times it stays 0, -inf times it -inf)
+    ch.least = -60. / ch.c;
+    ch.unit = p.unit;
+#pragma unroll
+    for (int i = 0; i < SM_DEGREE; i++) {
+        ch.k[i] = kExp2[i];
+        asm("" : "+s"(ch.k[i]));  // (as literals each would be moved to the sum's registers before its product)
+    }
     float lowest = -INFINITY;  // the least fp32 value that min_p keeps; the largest is always kept
     if (min_p > 0.) {
         const double border = fmin(ch.m, ch.m + T * log(min_p));
@@ -379,16 +396,23 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         const float inv = span > 0.f ? (float)BINS / span : 0.f;
         const auto bin_of = [&](float e) { return (int)fminf((m - e) * inv, (float)(BINS - 1)); };
         clear();
-        each(from, [&](float e, int i) {
-            if (e >= from && order_key(e, i) >= base) {
-                if (MASS) {  // (the count of the bin that matters is that of the list)
-                    const u64 we = weight(ch, e);
-                    if (we) atomicAdd(&mass_s[bin_of(e)], we);
-                } else {
-                    atomicAdd(&count_s[bin_of(e)], 1u);
-                }
+        if (MASS && base == 0) {  // (the count of the bin that matters is that of the list)
+#pragma unroll 1
+            for (int i = tid; i < npiece; i += NT) {
+                const Piece v = piece(i);
+#pragma unroll
+                for (int c = 0; c < P; c++) atomicAdd(&mass_s[bin_of(wide(v[c]))], weight(ch, wide(v[c])));
             }
-        });
+        } else {
+            each(from, [&](float e, int i) {
+                if (e >= from && order_key(e, i) >= base) {
+                    if (MASS)
+                        atomicAdd(&mass_s[bin_of(e)], weight(ch, e));
+                    else
+                        atomicAdd(&count_s[bin_of(e)], 1u);
+                }
+            });
+        }
         __syncthreads();
         total = scan_bins();
         find_border(0, 0);
@@ -430,8 +454,10 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
             wa = found_mass;
             n = found_n;
         };
-        each(from, [&](float e, int i) {
-            if (e >= from && bin_of(e) == bin) {
+        // (no element of the bin lies more than its lower end and a bin for the roundings below the maximum)
+        const float low = bin == BINS - 1 || !(inv > 0.f) ? from : fmaxf(from, m - (float)(bin + 2) / inv);
+        each(low, [&](float e, int i) {
+            if (e >= low && bin_of(e) == bin) {
                 const u64 key = order_key(e, i);
                 if (key >= base) {
                     const int at = atomicAdd(&held_s, 1);
@@ -497,12 +523,12 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
             const u64 key = list_s[tid];
             unsigned before = ca;
             u64 mass = wa;
-#pragma unroll 4
-            for (int i = 0; i < (int)n; i++)
-                if (list_s[i] > key) {
-                    before++;
-                    if (MASS) mass += list_w[i];
-                }
+#pragma unroll 8
+            for (int i = 0; i < (int)n; i++) {
+                const bool first = list_s[i] > key;
+                before += first;
+                if (MASS) mass += first ? list_w[i] : 0;
+            }
             if (!dropped(before, mass, total)) atomicMin(&found_key, key);
         }
         __syncthreads();
@@ -519,12 +545,15 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     // ---- the draw: a wave to a run of the row's pieces
     const int run = (npiece + W - 1) / W, begin = min(wv * run, npiece), end = min(begin + run, npiece);
     const bool every = base == 0;
-    const auto kept_weight = [&](float e, int i) { return every || (e >= from && order_key(e, i) >= base) ? weight(ch, e) : 0; };
+    const auto kept = [&](float e, int i) { return every || (e >= from && order_key(e, i) >= base); };
     const auto piece_weight = [&](const Piece& v, int i) {
         u64 s = 0;
         if (largest(v) >= from)
 #pragma unroll
-            for (int c = 0; c < P; c++) s += kept_weight((float)v[c], i * P + c);
+            for (int c = 0; c < P; c++) {
+                const u64 w = weight(ch, wide(v[c]));
+                s += kept(wide(v[c]), i * P + c) ? w : 0;
+            }
         return s;
     };
     u64 sum = 0;
@@ -550,8 +579,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
                 if (mass <= target && target < mass + s) {  // (one lane)
 #pragma unroll 1
                     for (int c = 0; c < P; c++) {
-                        const float e = (float)(ROW ? reinterpret_cast<const E*>(row_s)[i * P + c] : x[(size_t)i * P + c]);
-                        const u64 w = kept_weight(e, i * P + c);
+                        const float e = wide(ROW ? reinterpret_cast<const E*>(row_s)[i * P + c] : x[(size_t)i * P + c]);
+                        const u64 w = kept(e, i * P + c) ? weight(ch, e) : 0;
                         mass += w;
                         if (mass > target) {
                             put(i * P + c, w, total);
@@ -592,7 +621,7 @@ void launch(const SampleParams& p, hipStream_t stream) {
 void launch_sample(SampleParams p, int dtype, hipStream_t stream) {
     int bits = 0;  // of the number of columns
     while ((1ll << bits) < p.V) bits++;
-    p.bits = bits > 16 ? 62 - bits : 46;
+    p.unit = (double)(1ull << (52 - (bits > 16 ? 62 - bits : 46)));
     if (dtype == 0)
         launch<bf16_t>(p, stream);
     else if (dtype == 1)
