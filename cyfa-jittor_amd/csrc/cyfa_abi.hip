@@ -196,6 +196,10 @@ int cyfa_adjust_logits(const CyfaAdjustArgs* a, int dtype, int grad, void* hip_s
     return check_launch(what);
 }
 
+size_t cyfa_sample_workspace_bytes(long long rows, int V) {
+    return rows <= 0 || V <= 0 || V > cyfa::LOGPROBS_MAX_V ? 0 : cyfa::sample_workspace_bytes(rows, V);
+}
+
 int cyfa_sample_tokens(const CyfaSampleArgs* a, int dtype, int grad, void* hip_stream) {
     const char* what = "cyfa_sample_tokens";
     if (!a) return fail(CYFA_ERR_VALUE, "%s: null args", what);
@@ -213,6 +217,10 @@ int cyfa_sample_tokens(const CyfaSampleArgs* a, int dtype, int grad, void* hip_s
     for (const void* ptr : words8)
         if (!aligned(ptr, 8)) return fail(CYFA_ERR_ALIGN, "%s: int64 and f64 tensors need 8-byte alignment", what);
     if (a->rows == 0) return CYFA_OK;
+    const size_t need = cyfa::sample_workspace_bytes(a->rows, a->V);
+    if (need && (!a->workspace || a->workspace_bytes < need))
+        return fail(CYFA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
+    if (need && !aligned(a->workspace, 16)) return fail(CYFA_ERR_ALIGN, "%s: workspace needs 16-byte alignment", what);
     if (!a->x || !a->ids || !a->logprob || (!a->uniform && !a->uniform64)) return fail(CYFA_ERR_VALUE, "%s: null required pointer", what);
     cyfa::SampleParams p{};
     p.rows = a->rows;
@@ -233,6 +241,7 @@ int cyfa_sample_tokens(const CyfaSampleArgs* a, int dtype, int grad, void* hip_s
     p.top_ks = a->top_ks;
     p.ids = a->ids;
     p.logprob = a->logprob;
+    p.stats = a->workspace;
     cyfa::launch_sample(p, dtype, (hipStream_t)hip_stream);
     return check_launch(what);
 }

@@ -658,8 +658,15 @@ struct SampleParams {
     long long* ids;              // [rows]
     float* logprob;              // [rows]
     double unit;                 // 2^(52 - bits): weights are multiples of 2^-bits; set by the launcher
-    long long first;             // row of a launch's first workgroup, set by the launcher
+    void* stats;                 // sample_workspace_bytes, 16-byte aligned
+    unsigned long long* part_mass;  // the rest is set by the launcher
+    unsigned* part_count;
+    int part, parts;             // columns of a part of a row, parts of a row
+    long long first;             // row of a launch's first workgroup
 };
+constexpr int SAMPLE_PARTS = 64;         // most parts of a row
+constexpr int SAMPLE_PART_COLS = 2048;   // fewest columns of a part
+size_t sample_workspace_bytes(long long rows, int V);
 void launch_sample(SampleParams p, int dtype, hipStream_t stream);
 
 // The divergence from a teacher's most probable tokens, and the gradient

@@ -15,11 +15,16 @@
 // A workgroup to a row, which it keeps in LDS where it fits. A prefix is found by
 // counting: the elements, or their mass, by bins of their distance to the
 // maximum; the bin in which the prefix ends gives its elements to a list, whose
-// keys are binned again until few enough are left to rank each against each. A
-// top_k of at most 64, the usual one, needs no bins: a value that at least k
-// elements reach and seldom many more is the k-th largest of the largest elements
-// of 64 sets of threads, and the few that reach it are ranked, cut and drawn from
-// by one wave.
+// keys are binned again until few enough are left to rank each against each.
+// Masses are counted for runs of the row apart, so that the run that holds the
+// token is known from the bins and its weights alone are formed again. A top_k of
+// at most 64, the usual one, needs no bins: a value that at least k elements reach
+// and seldom many more is the k-th largest of the largest elements of 64 sets of
+// threads, and the few that reach it are ranked, cut and drawn from by one wave.
+//
+// Few rows are shared out: a workgroup to each part of a row finds its maximum, a
+// second launch counts the parts' bins, and a third, a workgroup to a row, goes on
+// from there with the parts as runs.
 #include <type_traits>
 
 #include "cyfa_internal.h"
@@ -33,7 +38,8 @@ typedef unsigned long long u64;
 
 constexpr double kLog2eD = 1.4426950408889634;
 constexpr int SM_FEW = 128;   // elements ranked each against each by a thread each
-constexpr int SM_TOP = 64;    // largest top_k that one wave handles
+constexpr int SM_TOP = 128;   // largest top_k that one wave handles
+constexpr int SM_ROW = 129024;  // bytes of the longest rows in LDS
 
 __device__ __forceinline__ uint32_t value_key(float x) {
     x += 0.f;  // -0 equals +0
@@ -88,6 +94,19 @@ __device__ __forceinline__ float kth_largest(float x, int k) {
     return -wave_max(rank < k ? -x : -INFINITY);
 }
 
+// The same of 128 values, two of each lane.
+__device__ __forceinline__ float kth_largest(float x, float y, int k) {
+    const uint32_t a = (value_key(x) & ~127u) | (uint32_t)(threadIdx.x & 63), b = (value_key(y) & ~127u) | 64u | (uint32_t)(threadIdx.x & 63);
+    int ra = 0, rb = 0;
+#pragma unroll 8
+    for (int i = 0; i < 64; i++) {
+        const uint32_t oa = (uint32_t)__builtin_amdgcn_readlane((int)a, i), ob = (uint32_t)__builtin_amdgcn_readlane((int)b, i);
+        ra += (oa > a) + (ob > a);
+        rb += (oa > b) + (ob > b);
+    }
+    return -wave_max(fmaxf(ra < k ? -x : -INFINITY, rb < k ? -y : -INFINITY));
+}
+
 // An element in fp32. (Of a bf16 by its bits: the compiler takes the largest of
 // converted bf16 as a bf16, with a rounding and another conversion for each.)
 __device__ __forceinline__ float wide(float x) { return x; }
@@ -128,30 +147,176 @@ __device__ __forceinline__ u64 weight(const Choice& ch, float x) {
     return __builtin_bit_cast(u64, __builtin_bit_cast(double, bits) + ch.unit) & 0xfffffffffffffull;
 }
 
-// Rows of up to ROW bytes in LDS; ROW = 0: of any length, read anew for each pass.
-// Passes over the row take it in pieces of 8 bytes: of whole vectors the compiler
-// holds eight exponentials' operands at a time, and spills them.
-template <class E, int NT, int ROW>
+// What one launch finds of a part of a row for the next.
+struct PartStats {
+    float best, least;  // the maximum, the least finite element
+    int bad;            // a NaN is there
+    int pad;
+};
+
+constexpr int SM_BINS = 512;  // bins of a part
+
+// The bins: of the distance to the maximum, over that of the least element or
+// what the temperature leaves of it, whichever is less.
+struct Bins {
+    float m, inv, last;
+    __device__ __forceinline__ Bins(float m, float least, double T, int bins) : m(m), last((float)(bins - 1)) {
+        const float span = fminf(m - least, 40.f * fmaxf((float)T, 1.f));
+        inv = span > 0.f ? (float)bins / span : 0.f;
+    }
+    __device__ __forceinline__ int of(float e) const { return (int)fminf((m - e) * inv, last); }
+};
+
+template <class E>
+__device__ __forceinline__ const E* row_of(const SampleParams& p, long long r) {
+    return static_cast<const E*>(p.x) + (r / p.inner) * p.outer_stride + (r % p.inner) * p.row_stride;
+}
+
+__device__ __forceinline__ Choice choice_of(const SampleParams& p, float m, double T) {
+    Choice ch;
+    ch.m = m;
+    ch.c = fmax(fmin(kLog2eD / T, 1e300), 1e-300);  // (0 times it stays 0, -inf times it -inf)
+    ch.least = -60. / ch.c;
+    ch.unit = p.unit;
+#pragma unroll
+    for (int i = 0; i < SM_DEGREE; i++) {
+        ch.k[i] = kExp2[i];
+        asm("" : "+s"(ch.k[i]));  // (as literals each would be moved to the sum's registers before its product)
+    }
+    return ch;
+}
+
+// This part of a row: maximum, least finite element, NaN. Parts are whole vectors.
+template <class E>
+__global__ __launch_bounds__(256) void sample_stats_kernel(SampleParams p) {
+    constexpr int N = RowVec<E>::N;
+    __shared__ float red[2][4];
+    __shared__ int bad_s[4];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const long long r = blockIdx.x;
+    const int c0 = blockIdx.y * p.part, cols = min(p.part, p.V - c0), nvec = cols / N, tail = cols - nvec * N;
+    const E* x = row_of<E>(p, r) + c0;
+    float best = -INFINITY, least = INFINITY;
+    bool bad = false;
+    const auto add = [&](E v) {
+        const float e = wide(v);
+        bad |= e != e;
+        best = fmaxf(best, e);
+        least = fminf(least, e > -INFINITY ? e : INFINITY);
+    };
+#pragma unroll 2
+    for (int i = tid; i < nvec; i += 256) {
+        const typename RowVec<E>::type v = load_row(x + (size_t)i * N);
+#pragma unroll
+        for (int c = 0; c < N; c++) add(v[c]);
+    }
+    if (tid < tail) add(x[nvec * N + tid]);
+    best = wave_max(best);
+    least = -wave_max(-least);
+    bad = __any(bad);
+    if (lane == 0) {
+        red[0][wv] = best;
+        red[1][wv] = least;
+        bad_s[wv] = bad;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < 4; w++) {
+            best = fmaxf(best, red[0][w]);
+            least = fminf(least, red[1][w]);
+            bad |= bad_s[w] != 0;
+        }
+        static_cast<PartStats*>(p.stats)[r * gridDim.y + blockIdx.y] = {best, least, bad, 0};
+    }
+}
+
+// A row's maximum, least element and NaN from those of its parts, in every lane.
+__device__ __forceinline__ PartStats join_parts(const SampleParams& p, long long r, int parts) {
+    PartStats a = {-INFINITY, INFINITY, 0, 0};
+    for (int i = threadIdx.x & 63; i < parts; i += 64) {
+        const PartStats b = static_cast<const PartStats*>(p.stats)[r * parts + i];
+        a.best = fmaxf(a.best, b.best);
+        a.least = fminf(a.least, b.least);
+        a.bad |= b.bad;
+    }
+    a.best = wave_max(a.best);
+    a.least = -wave_max(-a.least);
+    a.bad = __any(a.bad);
+    return a;
+}
+
+// The counts and masses of a part's bins.
+template <class E>
+__global__ __launch_bounds__(256) void sample_bins_kernel(SampleParams p) {
+    constexpr int N = RowVec<E>::N, P = N / 2;
+    typedef E Piece __attribute__((ext_vector_type(P)));
+    __shared__ u64 mass_s[SM_BINS];
+    __shared__ unsigned count_s[SM_BINS];
+    const int tid = threadIdx.x;
+    const long long r = blockIdx.x;
+    const int c0 = blockIdx.y * p.part, cols = min(p.part, p.V - c0), npiece = cols / P, tail = cols - npiece * P;
+    const double T = p.temperatures ? (double)p.temperatures[r] : p.temperature;
+    const PartStats a = join_parts(p, r, gridDim.y);
+    if (a.bad || a.best == INFINITY || a.best == -INFINITY || !(T > 0.)) return;  // (no bins are read)
+    const E* x = row_of<E>(p, r) + c0;
+    const Choice ch = choice_of(p, a.best, T);
+    const Bins bins(a.best, a.least, T, SM_BINS);
+    for (int b = tid; b < SM_BINS; b += 256) {
+        mass_s[b] = 0;
+        count_s[b] = 0;
+    }
+    __syncthreads();
+    const auto add = [&](E v) {
+        const int b = bins.of(wide(v));
+        atomicAdd(&count_s[b], 1u);
+        atomicAdd(&mass_s[b], weight(ch, wide(v)));
+    };
+#pragma unroll 1
+    for (int i = tid; i < npiece; i += 256) {
+        Piece v;
+        __builtin_memcpy(&v, x + (size_t)i * P, 8);
+#pragma unroll
+        for (int c = 0; c < P; c++) add(v[c]);
+    }
+    if (tid < tail) add(x[npiece * P + tid]);
+    __syncthreads();
+    const long long at = (r * gridDim.y + blockIdx.y) * SM_BINS;
+    for (int b = tid; b < SM_BINS; b += 256) {
+        p.part_mass[at + b] = mass_s[b];
+        p.part_count[at + b] = count_s[b];
+    }
+}
+
+// The rows of a launch, a workgroup each. Rows of up to ROW bytes lie in LDS; ROW =
+// 0: of any length, read anew for each pass. PARTS: what the two launches before
+// found of the row's p.parts parts (ROW = 0).
+// Passes that form weights take the row in pieces of 8 bytes: of whole vectors the
+// compiler holds eight exponentials' operands at a time, and spills them.
+template <class E, int NT, int ROW, bool PARTS>
 __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     typedef typename RowVec<E>::type Vec;
-    constexpr int N = RowVec<E>::N, P = N / 2, W = NT / 64, BINS = NT > 512 ? 512 : NT;
+    constexpr int N = RowVec<E>::N, P = N / 2, W = NT / 64, BINS = NT > SM_BINS ? SM_BINS : NT;
+    constexpr int RUNS = PARTS ? SAMPLE_PARTS : ROW > 65536 ? 2 : W > 8 ? 8 : W;  // PARTS: at most
     typedef E Piece __attribute__((ext_vector_type(P)));
     __shared__ Vec row_s[ROW ? ROW / 16 : 1];
+    __shared__ u64 run_s[PARTS ? 1 : RUNS][BINS];  // masses of the runs' bins
     __shared__ u64 mass_s[BINS];
     __shared__ unsigned count_s[BINS];
-    __shared__ u64 list_s[NT];
+    __shared__ u64 list_s[NT], all_s[NT];
     __shared__ u64 list_w[SM_FEW];
     __shared__ u64 red_s[2][W];
+    __shared__ u64 runs_s[RUNS];  // masses of the kept in the runs
     __shared__ float redf_s[2][W], thr_s;
     __shared__ unsigned redu_s[W];
-    __shared__ u64 found_mass, found_key;
+    __shared__ u64 found_mass, found_key, found_kept;
     __shared__ unsigned found_count, found_n;
-    __shared__ int found_bin, held_s;
-    float* const sets_s = reinterpret_cast<float*>(list_s);  // [W][64], until the list is used
+    __shared__ int found_bin, held_s, vecs_s;
+    float* const sets_s = reinterpret_cast<float*>(all_s);  // [W][64], until the list is used
+    int* const near_s = reinterpret_cast<int*>(mass_s);     // [2 BINS], while no bins are counted
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const int full = p.V / N, nvec = (p.V + N - 1) / N, npiece = (p.V + P - 1) / P;
     const long long r = p.first + blockIdx.x;
-    const E* x = static_cast<const E*>(p.x) + (r / p.inner) * p.outer_stride + (r % p.inner) * p.row_stride;
+    const E* x = row_of<E>(p, r);
     const double T = p.temperatures ? (double)p.temperatures[r] : p.temperature;
     const double top_p = p.top_ps ? (double)p.top_ps[r] : p.top_p;
     const double min_p = p.min_ps ? (double)p.min_ps[r] : p.min_p;
@@ -179,26 +344,29 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         }
         return v;
     };
-    const auto largest = [&](const Piece& v) {
-        float top = wide(v[0]);
-#pragma unroll
-        for (int c = 1; c < P; c++) top = fmaxf(top, wide(v[c]));
-        return top;
-    };
-    // f(element, column) of this thread's elements in pieces that reach ``from``
+    // f(element, column) of this thread's elements in vectors that reach ``from``
     const auto each = [&](float from, auto&& f) {
 #pragma unroll 1
-        for (int i = tid; i < npiece; i += NT) {
-            const Piece v = piece(i);
-            if (largest(v) >= from)
+        for (int i = tid; i < nvec; i += NT) {
+            const Vec v = ROW ? row_s[i] : from_memory(i);
+            float top = wide(v[0]);
 #pragma unroll
-                for (int c = 0; c < P; c++) f(wide(v[c]), i * P + c);
+            for (int c = 1; c < N; c++) top = fmaxf(top, wide(v[c]));
+            if (top >= from)
+#pragma unroll
+                for (int c = 0; c < N; c++) f(wide(v[c]), i * N + c);
         }
     };
     // ---- the maximum, the least finite element, what no distribution holds
     float best = -INFINITY, least = INFINITY;
     bool bad = false;
-    {
+    if (tid == 0) held_s = 0;
+    if (PARTS) {
+        const PartStats a = join_parts(p, r, p.parts);
+        best = a.best;
+        least = a.least;
+        bad = a.bad;
+    } else {
         constexpr int U = 4;  // vectors of a thread in flight
         for (int i0 = tid; i0 < nvec; i0 += NT * U) {
             Vec v[U];
@@ -220,37 +388,32 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
                 }
             }
         }
+        sets_s[wv * 64 + lane] = best;
+        best = wave_max(best);
+        least = -wave_max(-least);
+        bad = __any(bad);
+        if (lane == 0) {
+            redf_s[0][wv] = best;
+            redf_s[1][wv] = least;
+            redu_s[wv] = bad;
+        }
     }
-    const float own_best = best;
-    best = wave_max(best);
-    least = -wave_max(-least);
-    bad = __any(bad);
-    sets_s[wv * 64 + lane] = own_best;
-    if (lane == 0) {
-        redf_s[0][wv] = best;
-        redf_s[1][wv] = least;
-        redu_s[wv] = bad;
-    }
-    if (tid == 0) held_s = 0;
     __syncthreads();
-    for (int w = 0; w < W; w++) {
-        best = fmaxf(best, redf_s[0][w]);
-        least = fminf(least, redf_s[1][w]);
-        bad |= redu_s[w] != 0;
-    }
+    if (!PARTS)
+        for (int w = 0; w < W; w++) {
+            best = fmaxf(best, redf_s[0][w]);
+            least = fminf(least, redf_s[1][w]);
+            bad |= redu_s[w] != 0;
+        }
     const bool none = bad || best == INFINITY || best == -INFINITY;
     if (none || !(T > 0.)) {  // the first of the largest, a NaN before all
         unsigned at = 0xffffffffu;
-        each(-INFINITY, [&](float e, int i) {
-            if (e == best && !bad) at = min(at, (unsigned)i);
-        });
-        if (bad)
-            for (int i = tid; i < npiece; i += NT) {
-                const Piece v = piece(i);
+        for (int i = tid; i < npiece; i += NT) {
+            const Piece v = piece(i);
 #pragma unroll
-                for (int c = 0; c < P; c++)
-                    if (wide(v[c]) != wide(v[c])) at = min(at, (unsigned)(i * P + c));
-            }
+            for (int c = 0; c < P; c++)
+                if (bad ? wide(v[c]) != wide(v[c]) : wide(v[c]) == best) at = min(at, (unsigned)(i * P + c));
+        }
         for (int d = 32; d > 0; d >>= 1) at = min(at, (unsigned)__shfl_xor((int)at, d));
         __syncthreads();
         if (lane == 0) redu_s[wv] = at;
@@ -262,16 +425,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         }
         return;
     }
-    Choice ch;
-    ch.m = best;
-    ch.c = fmax(fmin(kLog2eD / T, 1e300), 1e-300);  // (0 times it stays 0, -inf times it -inf)
-    ch.least = -60. / ch.c;
-    ch.unit = p.unit;
-#pragma unroll
-    for (int i = 0; i < SM_DEGREE; i++) {
-        ch.k[i] = kExp2[i];
-        asm("" : "+s"(ch.k[i]));  // (as literals each would be moved to the sum's registers before its product)
-    }
+    const Choice ch = choice_of(p, best, T);
     float lowest = -INFINITY;  // the least fp32 value that min_p keeps; the largest is always kept
     if (min_p > 0.) {
         const double border = fmin(ch.m, ch.m + T * log(min_p));
@@ -289,12 +443,16 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     u64 base = 0;          // kept so far: keys from here on
     float from = -INFINITY;  // its value
     const bool cut_k = top_k > 0 && top_k < p.V, cut_p = top_p < 1.;
-    if (cut_k && top_k <= SM_TOP) {
+    if (!PARTS && cut_k && top_k <= SM_TOP) {
         const int k = (int)top_k;
-        if (wv == 0) {
-            float most = sets_s[lane];
-            for (int w = 1; w < W; w++) most = fmaxf(most, sets_s[w * 64 + lane]);
-            const float thr = kth_largest(most, k);
+        if (wv == 0) {  // (of one set of threads a lane, or, past 64, of two)
+            float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int w = 0; w < W; w += 2) {
+                most[0] = fmaxf(most[0], sets_s[w * 64 + lane]);
+                most[1] = fmaxf(most[1], sets_s[(w + 1) * 64 + lane]);
+            }
+            const float thr = k <= 64 ? kth_largest(fmaxf(most[0], most[1]), k) : kth_largest(most[0], most[1], k);
             if (lane == 0) thr_s = thr;
         }
         __syncthreads();
@@ -307,32 +465,44 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         });
         __syncthreads();
         const int n = held_s;
-        if (n <= 2 * SM_FEW && n <= NT) {
-            u64 key = 0;
-            int rank = SM_TOP;
-            if (tid < n) {
-                key = list_s[tid];
-                rank = 0;
-#pragma unroll 8
-                for (int i = 0; i < n; i++) rank += list_s[i] > key;
+        if (n <= 4 * SM_FEW && n <= NT) {
+            for (int at = tid / 8; at < n; at += NT / 8) {  // eight threads to one
+                const u64 key = list_s[at];
+                int rank = 0;
+#pragma unroll 4
+                for (int i = tid & 7; i < n; i += 8) rank += list_s[i] > key;
+#pragma unroll
+                for (int d = 4; d > 0; d >>= 1) rank += __shfl_xor(rank, d);
+                if ((tid & 7) == 0 && rank < k) all_s[rank] = key;
             }
             __syncthreads();
-            if (rank < k) list_s[rank] = key;
-            __syncthreads();
-            if (wv == 0) {  // a lane to each of the k, in their order
-                key = lane < k ? list_s[lane] : 0;
-                const float e = key_value(key);
-                u64 w = lane < k ? weight(ch, e) : 0;
-                const u64 sum = wave_scan(w), all = lane_u64(sum, 63);
-                const bool keep = lane == 0 || (lane < k && e >= lowest && !(cut_p && (double)(sum - w) >= top_p * (double)all));
-                const int kept = __popcll(__ballot(keep));
-                const u64 total = lane_u64(sum, kept - 1), target = mass_at(total);
-                u64 upto = 0;  // the mass of the kept up to this one by index
-                for (int i = 0; i < kept; i++) {
-                    const u64 other = lane_u64(key, i), ow = lane_u64(w, i);
-                    if ((uint32_t)other >= (uint32_t)key) upto += ow;
+            if (wv == 0) {  // a lane to each of the first 64 and to each of the second
+                u64 keys[2], w[2], sum[2], before = 0;
+                float e[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    keys[h] = lane + 64 * h < k ? all_s[lane + 64 * h] : 0;
+                    e[h] = key_value(keys[h]);
+                    w[h] = lane + 64 * h < k ? weight(ch, e[h]) : 0;
+                    sum[h] = before + wave_scan(w[h]);
+                    before = lane_u64(sum[h], 63);
                 }
-                if (lane < kept && upto > target && upto - w <= target) put(key_index(key), w, total);
+                int kept = 0;
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    kept += __popcll(__ballot((lane == 0 && h == 0) || (lane + 64 * h < k && e[h] >= lowest &&
+                                                                        !(cut_p && (double)(sum[h] - w[h]) >= top_p * (double)before))));
+                const u64 total = kept > 64 ? lane_u64(sum[1], kept - 65) : lane_u64(sum[0], kept - 1), target = mass_at(total);
+                u64 upto[2] = {0, 0};  // the mass of the kept up to these by index
+                const auto pass = [&](u64 other, u64 ow) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) upto[h] += (uint32_t)other >= (uint32_t)keys[h] ? ow : 0;
+                };
+                for (int i = 0; i < min(kept, 64); i++) pass(lane_u64(keys[0], i), lane_u64(w[0], i));
+                for (int i = 64; i < kept; i++) pass(lane_u64(keys[1], i - 64), lane_u64(w[1], i - 64));
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (lane + 64 * h < kept && upto[h] > target && upto[h] - w[h] <= target) put(key_index(keys[h]), w[h], total);
             }
             return;
         }
@@ -340,46 +510,70 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         base = order_key(thr, 0x7fffffff);
         __syncthreads();
     }
+    const Bins bins(best, least, T, BINS);
+    // The runs of the row: their masses by bins, whether they have been counted.
+    const int runs = PARTS ? p.parts : RUNS;
+    const int run_len = PARTS ? p.part / P : (npiece + RUNS - 1) / RUNS;  // pieces of a run
+    bool counted = PARTS;
+    const auto run_mass = [&](int run, int b) -> u64 { return PARTS ? p.part_mass[(r * runs + run) * BINS + b] : run_s[PARTS ? 0 : run][b]; };
+    u64 total = 0;      // the mass of what the last search looked at
+    int k_bin = BINS;   // PARTS: the bin in which top_k ends,
+    u64 k_mass = 0;     // and the mass of its kept elements
+    int in_all = -1;    // elements of the last border's bin in all_s, where it holds them
+    // The values of a bin, but for their rounding: those within half of mid.
+    const auto near_bin = [&](int bin, float& mid, float& half) {
+        mid = 0.f;
+        half = INFINITY;
+        if (bin < BINS - 1 && bins.inv > 0.f) {
+            const float width = 1.f / bins.inv, low = best - (float)(bin + 1) * width * (1.f + 0x1p-20f);
+            const float high = best - (float)bin * width * (1.f - 0x1p-20f);
+            mid = 0.5f * low + 0.5f * high;
+            half = fmaxf(high - mid, mid - low);  // (roundings keep the order of differences from mid)
+        }
+    };
     // Lowers what is kept to the longest prefix that ``dropped`` (elements
-    // before, mass before, all mass) does not end; MASS: it asks for the mass.
+    // before, mass before, all mass) does not end. MASS: it asks for the mass.
     const auto search = [&](auto with_mass, auto&& dropped) {
-        constexpr bool MASS = decltype(with_mass)::value;
-        // a bin's count and mass to those before it; the total mass
+        constexpr bool MASS = decltype(with_mass)::value, BOTH = MASS || PARTS;
+        // a bin's count and mass to those before it
         unsigned c, cb;
-        u64 w, wb, total;
+        u64 w, wb;
         const auto scan_bins = [&]() {
-            c = tid < BINS ? count_s[tid] : 0;
-            w = MASS && tid < BINS ? mass_s[tid] : 0;
-            const u64 cs = wave_scan(c), ws = MASS ? wave_scan(w) : 0;
+            const u64 cs = wave_scan(c), ws = BOTH ? wave_scan(w) : 0;
             if (lane == 63) {
                 red_s[0][wv] = cs;
                 red_s[1][wv] = ws;
             }
             __syncthreads();
-            u64 cbase = 0, wbase = 0, wt = 0;
+            u64 cbase = 0, wbase = 0, all = 0;
             for (int i = 0; i < BINS / 64; i++) {
                 if (i < wv) cbase += red_s[0][i];
-                if (MASS && i < wv) wbase += red_s[1][i];
-                if (MASS) wt += red_s[1][i];
+                if (BOTH && i < wv) wbase += red_s[1][i];
+                if (BOTH) all += red_s[1][i];
             }
             cb = (unsigned)(cbase + cs - c);
             wb = wbase + ws - w;
-            return wt;
+            return all;
         };
         const auto clear = [&]() {
             if (tid < BINS) {
                 count_s[tid] = 0;
-                if (MASS) mass_s[tid] = 0;
+                if (BOTH) mass_s[tid] = 0;
             }
             if (tid == 0) {
                 held_s = 0;
+                vecs_s = 0;
                 found_bin = -1;
             }
             __syncthreads();
         };
         const auto hit = [&](int b, float e) {
             atomicAdd(&count_s[b], 1u);
-            if (MASS) atomicAdd(&mass_s[b], weight(ch, e));
+            if (BOTH) atomicAdd(&mass_s[b], weight(ch, e));
+        };
+        const auto read_bins = [&]() {
+            c = tid < BINS ? count_s[tid] : 0;
+            w = BOTH && tid < BINS ? mass_s[tid] : 0;
         };
         // the bin in which the prefix ends, known to all
         const auto find_border = [&](unsigned ca, u64 wa) {
@@ -391,35 +585,64 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
             }
             __syncthreads();
         };
-        // bins of the distance to the maximum, over the least element's or what the temperature leaves of it
-        const float m = (float)ch.m, span = fminf(m - fmaxf(least, from), 40.f * fmaxf((float)T, 1.f));
-        const float inv = span > 0.f ? (float)BINS / span : 0.f;
-        const auto bin_of = [&](float e) { return (int)fminf((m - e) * inv, (float)(BINS - 1)); };
+        if (!PARTS && MASS)
+            for (int b = tid; b < RUNS * BINS; b += NT) run_s[0][b] = 0;
         clear();
-        if (MASS && base == 0) {  // (the count of the bin that matters is that of the list)
-#pragma unroll 1
-            for (int i = tid; i < npiece; i += NT) {
-                const Piece v = piece(i);
-#pragma unroll
-                for (int c = 0; c < P; c++) atomicAdd(&mass_s[bin_of(wide(v[c]))], weight(ch, wide(v[c])));
+        if (PARTS) {
+            c = 0;
+            w = 0;
+            if (tid < BINS)
+#pragma unroll 4
+                for (int i = 0; i < runs; i++) {
+                    c += p.part_count[(r * runs + i) * BINS + tid];
+                    w += run_mass(i, tid);
+                }
+            if (tid >= k_bin) {  // past the first top_k
+                c = 0;
+                w = tid == k_bin ? k_mass : 0;
             }
+        } else if (MASS) {  // (the count of the bin that matters is that of the list)
+            counted = true;
+            const int run = wv * RUNS / W, begin = run * run_len, end = min(begin + run_len, npiece);
+            constexpr int STEP = NT / RUNS;
+            if (base == 0) {
+#pragma unroll 1
+                for (int i = begin + tid % STEP; i < end; i += STEP) {
+                    const Piece v = piece(i);
+#pragma unroll
+                    for (int c = 0; c < P; c++) atomicAdd(&run_s[PARTS ? 0 : run][bins.of(wide(v[c]))], weight(ch, wide(v[c])));
+                }
+            } else {
+#pragma unroll 1
+                for (int i = begin + tid % STEP; i < end; i += STEP) {
+                    const Piece v = piece(i);
+#pragma unroll
+                    for (int c = 0; c < P; c++) {
+                        const float e = wide(v[c]);
+                        if (e >= from && order_key(e, i * P + c) >= base) atomicAdd(&run_s[PARTS ? 0 : run][bins.of(e)], weight(ch, e));
+                    }
+                }
+            }
+            __syncthreads();
+            c = 0;
+            w = 0;
+            if (tid < BINS)
+#pragma unroll
+                for (int i = 0; i < RUNS; i++) w += run_s[PARTS ? 0 : i][tid];
         } else {
             each(from, [&](float e, int i) {
-                if (e >= from && order_key(e, i) >= base) {
-                    if (MASS)
-                        atomicAdd(&mass_s[bin_of(e)], weight(ch, e));
-                    else
-                        atomicAdd(&count_s[bin_of(e)], 1u);
-                }
+                if (e >= from && order_key(e, i) >= base) atomicAdd(&count_s[bins.of(e)], 1u);
             });
+            __syncthreads();
+            read_bins();
         }
-        __syncthreads();
         total = scan_bins();
         find_border(0, 0);
         const int bin = found_bin;
         if (bin < 0) return;  // nothing is dropped
         unsigned ca = found_count, n;
         u64 wa = found_mass;
+        const u64 above = wa;
         u64 lo = 0, hi = 0;  // the keys of the undecided, once they are known
         const auto range = [&](u64 low, u64 high) {
             for (int d = 32; d > 0; d >>= 1) {
@@ -454,29 +677,64 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
             wa = found_mass;
             n = found_n;
         };
-        // (no element of the bin lies more than its lower end and a bin for the roundings below the maximum)
-        const float low = bin == BINS - 1 || !(inv > 0.f) ? from : fmaxf(from, m - (float)(bin + 2) / inv);
-        each(low, [&](float e, int i) {
-            if (e >= low && bin_of(e) == bin) {
-                const u64 key = order_key(e, i);
-                if (key >= base) {
-                    const int at = atomicAdd(&held_s, 1);
-                    if (at < NT) list_s[at] = key;
-                }
-            }
-        });
-        __syncthreads();
-        n = (unsigned)held_s;
-        if (n > NT) {  // too many for the list: bins of their keys
-            u64 low = ~0ull, high = 0;
+        // f(key) of the bin's elements
+        const auto in_bin = [&](auto&& f) {
             each(from, [&](float e, int i) {
-                if (e >= from && bin_of(e) == bin) {
+                if (e >= from && bins.of(e) == bin) {
                     const u64 key = order_key(e, i);
-                    if (key >= base) {
-                        low = key < low ? key : low;
-                        high = key > high ? key : high;
+                    if (key >= base) f(key);
+                }
+            });
+        };
+        const auto hold = [&](u64 key) {
+            const int at = atomicAdd(&held_s, 1);
+            if (at < NT) all_s[at] = key;
+        };
+        // The vectors that hold some of them first: a wave's next 512 elements hold
+        // one or two, and would all be looked at by themselves for those.
+        float mid, half;
+        near_bin(bin, mid, half);
+#pragma unroll 2
+        for (int i = tid; i < nvec; i += NT) {
+            const Vec v = ROW ? row_s[i] : from_memory(i);
+            float near = INFINITY;
+#pragma unroll
+            for (int c = 0; c < N; c++) near = fminf(near, fabsf(wide(v[c]) - mid));
+            if (near <= half) {
+                const int at = atomicAdd(&vecs_s, 1);
+                if (at < 2 * BINS) near_s[at] = i;
+            }
+        }
+        __syncthreads();
+        const int vecs = vecs_s;
+        if (vecs <= 2 * BINS) {
+            for (int at = tid; at < vecs; at += NT) {
+                const int i = near_s[at];
+                const Vec v = ROW ? row_s[i] : from_memory(i);
+#pragma unroll
+                for (int c = 0; c < N; c++) {
+                    const float e = wide(v[c]);
+                    if (e >= from && bins.of(e) == bin) {
+                        const u64 key = order_key(e, i * N + c);
+                        if (key >= base) hold(key);
                     }
                 }
+            }
+        } else {
+            in_bin(hold);
+        }
+        __syncthreads();
+        n = (unsigned)held_s;
+        in_all = n > NT ? -1 : (int)n;
+        if (n <= NT) {
+            if (tid < (int)n) list_s[tid] = all_s[tid];
+            __syncthreads();
+        }
+        if (n > NT) {  // too many for the list: bins of their keys
+            u64 low = ~0ull, high = 0;
+            in_bin([&](u64 key) {
+                low = key < low ? key : low;
+                high = key > high ? key : high;
             });
             range(low, high);
             while (n > NT) {
@@ -487,6 +745,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
                     if (key >= lo && key <= hi) hit((int)((hi - key) >> shift), e);
                 });
                 __syncthreads();
+                read_bins();
                 scan_bins();
                 find_border(ca, wa);
                 if (found_bin < 0) return;  // (never: the bins add up to what was undecided)
@@ -509,6 +768,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
             const int b = (int)((hi - key) >> shift);
             if (tid < (int)n) hit(b, key_value(key));
             __syncthreads();
+            read_bins();
             scan_bins();
             find_border(ca, wa);
             if (found_bin < 0) return;
@@ -516,39 +776,94 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
             narrow(shift);
             __syncthreads();
         }
-        if (tid == 0) found_key = ~0ull;
-        if (MASS && tid < (int)n) list_w[tid] = weight(ch, key_value(list_s[tid]));
+        if (tid == 0) {
+            found_key = ~0ull;
+            found_kept = wa - above;
+        }
+        if (BOTH && tid < (int)n) list_w[tid] = weight(ch, key_value(list_s[tid]));
         __syncthreads();
-        if (tid < (int)n) {
-            const u64 key = list_s[tid];
-            unsigned before = ca;
-            u64 mass = wa;
-#pragma unroll 8
-            for (int i = 0; i < (int)n; i++) {
+        // each against each, eight threads to one
+        for (int at = tid / 8; at < (int)n; at += NT / 8) {
+            const u64 key = list_s[at];
+            unsigned before = 0;
+            u64 mass = 0;
+#pragma unroll 4
+            for (int i = tid & 7; i < (int)n; i += 8) {
                 const bool first = list_s[i] > key;
                 before += first;
-                if (MASS) mass += first ? list_w[i] : 0;
+                if (BOTH) mass += first ? list_w[i] : 0;
             }
-            if (!dropped(before, mass, total)) atomicMin(&found_key, key);
+#pragma unroll
+            for (int d = 4; d > 0; d >>= 1) {
+                before += __shfl_xor(before, d);
+                if (BOTH) mass += __shfl_xor(mass, d);
+            }
+            if ((tid & 7) == 0 && !dropped(ca + before, wa + mass, total)) {
+                atomicMin(&found_key, key);
+                if (BOTH) atomicAdd(&found_kept, list_w[at]);
+            }
         }
         __syncthreads();
         base = found_key;
         from = key_value(base);
+        if (PARTS) {
+            k_bin = bin;
+            k_mass = found_kept;
+        }
         __syncthreads();
     };
     if (cut_k) search(std::false_type{}, [&](unsigned before, u64, u64) { return before >= top_k; });
-    if (cut_p) search(std::true_type{}, [&](unsigned, u64 mass, u64 total) { return mass > 0 && (double)mass >= top_p * (double)total; });
+    if (cut_p) search(std::true_type{}, [&](unsigned, u64 mass, u64 all) { return mass > 0 && (double)mass >= top_p * (double)all; });
     if (lowest > from) {
+        in_all = -1;
         from = lowest;
         base = order_key(lowest, 0x7fffffff);
     }
-    // ---- the draw: a wave to a run of the row's pieces
-    const int run = (npiece + W - 1) / W, begin = min(wv * run, npiece), end = min(begin + run, npiece);
+    // ---- the draw: the runs' masses from their bins, the run of the token a wave to a part of it
     const bool every = base == 0;
-    const auto kept = [&](float e, int i) { return every || (e >= from && order_key(e, i) >= base); };
-    const auto piece_weight = [&](const Piece& v, int i) {
+    const auto kept = [&](float e, int i) { return every || e > from || (e == from && order_key(e, i) >= base); };
+    int begin = 0, end = npiece;
+    u64 passed = 0, target = 0;
+    if (counted) {
+        const int border = every ? BINS : bins.of(from);
+        for (int run = wv; run < runs; run += W) {
+            u64 s = 0;
+            for (int b = lane; b < border; b += 64) s += run_mass(run, b);
+            s = wave_add(s);
+            if (lane == 0) runs_s[run] = s;
+        }
+        __syncthreads();
+        if (!every) {  // the kept ones of the border's bin
+            const auto add = [&](u64 key) {
+                if (key >= base && key_index(key) < p.V) atomicAdd(&runs_s[key_index(key) / P / run_len], weight(ch, key_value(key)));
+            };
+            if (in_all >= 0) {
+                if (tid < in_all) add(all_s[tid]);
+            } else {
+                each(from, [&](float e, int i) {
+                    if (e >= from && bins.of(e) == border) add(order_key(e, i));
+                });
+            }
+            __syncthreads();
+        }
+        total = 0;
+        for (int i = 0; i < runs; i++) total += runs_s[i];
+        target = mass_at(total);
+        int run = 0;
+        while (run < runs - 1 && passed + runs_s[run] <= target) passed += runs_s[run++];
+        begin = run * run_len;
+        end = min(begin + run_len, npiece);
+    }
+    const int len = (end - begin + W - 1) / W;
+    begin = min(begin + wv * len, end);
+    end = min(begin + len, end);
+    const auto piece_weight = [&](int i) {
+        const Piece v = piece(i);
+        float top = wide(v[0]);
+#pragma unroll
+        for (int c = 1; c < P; c++) top = fmaxf(top, wide(v[c]));
         u64 s = 0;
-        if (largest(v) >= from)
+        if (top >= from)
 #pragma unroll
             for (int c = 0; c < P; c++) {
                 const u64 w = weight(ch, wide(v[c]));
@@ -558,21 +873,21 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     };
     u64 sum = 0;
 #pragma unroll 1
-    for (int i = begin + lane; i < end; i += 64) sum += piece_weight(piece(i), i);
+    for (int i = begin + lane; i < end; i += 64) sum += piece_weight(i);
     sum = wave_add(sum);
     if (lane == 0) red_s[0][wv] = sum;
     __syncthreads();
-    u64 total = 0, passed = 0;
-    for (int w = 0; w < W; w++) {
-        total += red_s[0][w];
-        if (w < wv) passed += red_s[0][w];
+    if (!counted) {
+        total = 0;
+        for (int w = 0; w < W; w++) total += red_s[0][w];
+        target = mass_at(total);
     }
-    const u64 target = mass_at(total);
+    for (int w = 0; w < wv; w++) passed += red_s[0][w];
     if (passed <= target && target < passed + sum) {  // (one wave)
 #pragma unroll 1
         for (int i0 = begin; i0 < end; i0 += 64) {
             const int i = i0 + lane;
-            const u64 s = i < end ? piece_weight(piece(i), i) : 0;
+            const u64 s = i < end ? piece_weight(i) : 0;
             const u64 upto = wave_scan(s), all = lane_u64(upto, 63);
             if (passed + all > target) {
                 u64 mass = passed + upto - s;
@@ -599,24 +914,50 @@ template <class E, int NT, int ROW>
 void launch_rows(SampleParams p, hipStream_t stream) {
     for (p.first = 0; p.first < p.rows; p.first += LOGPROBS_MAX_GRID) {
         const dim3 grid((unsigned)min(p.rows - p.first, (long long)LOGPROBS_MAX_GRID));
-        hipLaunchKernelGGL((sample_kernel<E, NT, ROW>), grid, dim3(NT), 0, stream, p);
+        hipLaunchKernelGGL((sample_kernel<E, NT, ROW, false>), grid, dim3(NT), 0, stream, p);
     }
 }
 
+// Parts of a row, 1 where it is not shared out.
+int row_parts(long long rows, int V) {
+    const int parts = (int)min(256 / max(rows, 1ll), (long long)SAMPLE_PARTS);
+    return min(parts, V / SAMPLE_PART_COLS);
+}
+
 template <class E>
-void launch(const SampleParams& p, hipStream_t stream) {
+void launch(SampleParams p, hipStream_t stream) {
+    constexpr int N = RowVec<E>::N;
     const size_t bytes = ((size_t)p.V * sizeof(E) + 15) / 16 * 16;
-    if (bytes <= 16384)
+    const int parts = row_parts(p.rows, p.V);
+    if (parts > 1) {
+        p.part = ((p.V + parts - 1) / parts + N - 1) / N * N;
+        p.parts = (p.V + p.part - 1) / p.part;
+        const size_t all = (size_t)p.rows * parts;
+        p.part_mass = (u64*)((char*)p.stats + all * sizeof(PartStats));
+        p.part_count = (unsigned*)(p.part_mass + all * SM_BINS);
+        p.first = 0;
+        const dim3 grid((unsigned)p.rows, (unsigned)p.parts);
+        hipLaunchKernelGGL(sample_stats_kernel<E>, grid, dim3(256), 0, stream, p);
+        hipLaunchKernelGGL(sample_bins_kernel<E>, grid, dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((sample_kernel<E, 1024, 0, true>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
+    } else if (bytes <= 16384) {
         launch_rows<E, 256, 16384>(p, stream);
-    else if (bytes <= 65536)
+    } else if (bytes <= 65536) {
         launch_rows<E, 1024, 65536>(p, stream);
-    else if (bytes <= 131072)
-        launch_rows<E, 1024, 131072>(p, stream);
-    else
+    } else if (bytes <= SM_ROW) {
+        launch_rows<E, 1024, SM_ROW>(p, stream);
+    } else {
         launch_rows<E, 1024, 0>(p, stream);
+    }
 }
 
 }  // namespace
+
+// Bytes of the parts' statistics and bins, 0 where rows are not shared out.
+size_t sample_workspace_bytes(long long rows, int V) {
+    const int parts = rows > 0 ? row_parts(rows, V) : 1;
+    return parts > 1 ? (size_t)rows * parts * (sizeof(PartStats) + SM_BINS * 12) : 0;
+}
 
 void launch_sample(SampleParams p, int dtype, hipStream_t stream) {
     int bits = 0;  // of the number of columns

@@ -229,7 +229,7 @@ class CyfaSampleArgs(ctypes.Structure):
         ("row_stride", ctypes.c_longlong), ("V", _c_int), ("x", _c_void_p), ("uniform", _c_void_p), ("uniform64", _c_void_p),
         ("temperature", ctypes.c_double), ("top_p", ctypes.c_double), ("min_p", ctypes.c_double), ("top_k", ctypes.c_longlong),
         ("temperatures", _c_void_p), ("top_ps", _c_void_p), ("min_ps", _c_void_p), ("top_ks", _c_void_p),
-        ("ids", _c_void_p), ("logprob", _c_void_p),
+        ("ids", _c_void_p), ("logprob", _c_void_p), ("workspace", _c_void_p), ("workspace_bytes", _c_size_t),
     ]
 
 
@@ -284,6 +284,7 @@ SIGNATURES = {
     "cyfa_residual_grad_workspace_bytes": (_c_size_t, [ctypes.c_longlong, _c_int]),
     "cyfa_residual_norm": (_c_int, [ctypes.POINTER(CyfaResidualArgs), _c_int, _c_int, _c_void_p]),
     "cyfa_adjust_logits": (_c_int, [ctypes.POINTER(CyfaAdjustArgs), _c_int, _c_int, _c_void_p]),
+    "cyfa_sample_workspace_bytes": (_c_size_t, [ctypes.c_longlong, _c_int]),
     "cyfa_sample_tokens": (_c_int, [ctypes.POINTER(CyfaSampleArgs), _c_int, _c_int, _c_void_p]),
     "cyfa_distill_loss": (_c_int, [ctypes.POINTER(CyfaDistillArgs), _c_int, _c_int, _c_void_p]),
     "cyfa_last_error": (ctypes.c_char_p, []),
@@ -1229,6 +1230,11 @@ def adjust(logits, out, history, lengths, prompts, penalties, bias, tokens, allo
     _lm_call("cyfa_adjust_logits", args, logits.dtype, 0 if dy is None else 1, dev)
 
 
+@functools.lru_cache(64)
+def _sample_bytes(rows, V):
+    return int(load_library().cyfa_sample_workspace_bytes(rows, V))
+
+
 def sample(logits, uniform, temperature, top_k, top_p, min_p):
     """(ids int64, logprob fp32) [...] of logits [..., V]; uniform [...] fp32 or
     fp64 contiguous; each option a number or contiguous [...] (fp32, top_k int64)."""
@@ -1257,6 +1263,10 @@ def sample(logits, uniform, temperature, top_k, top_p, min_p):
         args.min_ps = min_p.data_ptr()
     else:
         args.min_p = min_p
+    n = _sample_bytes(args.rows, args.V)
+    if n:
+        workspace = torch.empty(n, dtype=torch.uint8, device=dev)  # alive until the launch
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), n
     _lm_call("cyfa_sample_tokens", args, logits.dtype, 0, dev)
     return ids, logprob
 

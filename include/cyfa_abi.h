@@ -736,8 +736,11 @@ typedef struct CyfaSampleArgs {
     const long long *top_ks;
     long long *ids;               /* [rows] */
     float *logprob;               /* [rows] */
+    void *workspace;              /* cyfa_sample_workspace_bytes(rows, V) bytes, 16-byte aligned; */
+    size_t workspace_bytes;       /* few rows of many columns alone need one */
 } CyfaSampleArgs;
 
+size_t cyfa_sample_workspace_bytes(long long rows, int V);
 int cyfa_sample_tokens(const CyfaSampleArgs *args, int dtype, int grad, void *hip_stream);
 
 /* The divergence of q = softmax(x / T) (rows of logits as CyfaLogprobArgs has
