@@ -12,7 +12,8 @@
 // past 2^16 columns, so that a row's sum fits 64), and integers add up the same
 // in any order. Weights below half of that step count nothing.
 //
-// A workgroup to a row, which it keeps in LDS where it fits. A prefix is found by
+// A workgroup to a row, whose passes find it in the L2 (rows held in LDS took as
+// long: 13.6 us against 14.0 for 256 rows of 32000 bf16). A prefix is found by
 // counting: the elements, or their mass, by bins of their distance to the
 // maximum; the bin in which the prefix ends gives its elements to a list, whose
 // keys are binned again until few enough are left to rank each against each.
@@ -37,9 +38,8 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr double kLog2eD = 1.4426950408889634;
-constexpr int SM_FEW = 128;   // elements ranked each against each by a thread each
+constexpr int SM_FEW = 512;   // elements ranked each against each, by eight threads each
 constexpr int SM_TOP = 128;   // largest top_k that one wave handles
-constexpr int SM_ROW = 129024;  // bytes of the longest rows in LDS
 
 __device__ __forceinline__ uint32_t value_key(float x) {
     x += 0.f;  // -0 equals +0
@@ -82,6 +82,19 @@ __device__ __forceinline__ u64 lane_u64(u64 x, int lane) {
 
 // The sum over the lanes, in every lane.
 __device__ __forceinline__ u64 wave_add(u64 x) { return lane_u64(wave_scan(x), 63); }
+
+// The largest of the lanes, in every lane: as wave_max.
+__device__ __forceinline__ u64 wave_most(u64 x) {
+    const auto most = [](u64 a, u64 b) { return a > b ? a : b; };
+    const auto moved = [](u64 x, auto step) {
+        return __builtin_bit_cast(u64, dpp_mov<decltype(step)::value>(__builtin_bit_cast(double, x)));
+    };
+    x = most(x, moved(x, std::integral_constant<int, 0xB1>{}));
+    x = most(x, moved(x, std::integral_constant<int, 0x4E>{}));
+    x = most(x, moved(x, std::integral_constant<int, 0x141>{}));
+    x = most(x, moved(x, std::integral_constant<int, 0x140>{}));
+    return most(most(lane_u64(x, 0), lane_u64(x, 16)), most(lane_u64(x, 32), lane_u64(x, 48)));
+}
 
 // The k-th largest of the 64 lanes' values x (no NaN), but for an order of the
 // last 6 bits: ranked as integers in the values' order with the lane in place
@@ -149,7 +162,7 @@ __device__ __forceinline__ u64 weight(const Choice& ch, float x) {
 
 // What one launch finds of a part of a row for the next.
 struct PartStats {
-    float best, least;  // the maximum, the least finite element
+    float best, least;  // the maximum, the least element
     int bad;            // a NaN is there
     int pad;
 };
@@ -186,7 +199,7 @@ __device__ __forceinline__ Choice choice_of(const SampleParams& p, float m, doub
     return ch;
 }
 
-// This part of a row: maximum, least finite element, NaN. Parts are whole vectors.
+// This part of a row: maximum, least element, NaN. Parts are whole vectors.
 template <class E>
 __global__ __launch_bounds__(256) void sample_stats_kernel(SampleParams p) {
     constexpr int N = RowVec<E>::N;
@@ -199,10 +212,8 @@ __global__ __launch_bounds__(256) void sample_stats_kernel(SampleParams p) {
     float best = -INFINITY, least = INFINITY;
     bool bad = false;
     const auto add = [&](E v) {
-        const float e = wide(v);
-        bad |= e != e;
-        best = fmaxf(best, e);
-        least = fminf(least, e > -INFINITY ? e : INFINITY);
+        best = __builtin_elementwise_maximum(best, wide(v));  // (a NaN stays)
+        least = __builtin_elementwise_minimum(least, wide(v));
     };
 #pragma unroll 2
     for (int i = tid; i < nvec; i += 256) {
@@ -211,9 +222,9 @@ __global__ __launch_bounds__(256) void sample_stats_kernel(SampleParams p) {
         for (int c = 0; c < N; c++) add(v[c]);
     }
     if (tid < tail) add(x[nvec * N + tid]);
+    bad = __any(best != best);
     best = wave_max(best);
     least = -wave_max(-least);
-    bad = __any(bad);
     if (lane == 0) {
         red[0][wv] = best;
         red[1][wv] = least;
@@ -287,25 +298,23 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(SampleParams p) {
     }
 }
 
-// The rows of a launch, a workgroup each. Rows of up to ROW bytes lie in LDS; ROW =
-// 0: of any length, read anew for each pass. PARTS: what the two launches before
-// found of the row's p.parts parts (ROW = 0).
+// The rows of a launch, a workgroup each. PARTS: with what the two launches before
+// found of the row's p.parts parts.
 // Passes that form weights take the row in pieces of 8 bytes: of whole vectors the
 // compiler holds eight exponentials' operands at a time, and spills them.
-template <class E, int NT, int ROW, bool PARTS>
+template <class E, int NT, bool PARTS>
 __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     typedef typename RowVec<E>::type Vec;
     constexpr int N = RowVec<E>::N, P = N / 2, W = NT / 64, BINS = NT > SM_BINS ? SM_BINS : NT;
-    constexpr int RUNS = PARTS ? SAMPLE_PARTS : ROW > 65536 ? 2 : W > 8 ? 8 : W;  // PARTS: at most
+    constexpr int RUNS = W > 8 ? 8 : W;
     typedef E Piece __attribute__((ext_vector_type(P)));
-    __shared__ Vec row_s[ROW ? ROW / 16 : 1];
     __shared__ u64 run_s[PARTS ? 1 : RUNS][BINS];  // masses of the runs' bins
     __shared__ u64 mass_s[BINS];
     __shared__ unsigned count_s[BINS];
     __shared__ u64 list_s[NT], all_s[NT];
-    __shared__ u64 list_w[SM_FEW];
+    __shared__ u64 list_w[SM_FEW < NT ? SM_FEW : NT];
     __shared__ u64 red_s[2][W];
-    __shared__ u64 runs_s[RUNS];  // masses of the kept in the runs
+    __shared__ u64 runs_s[PARTS ? SAMPLE_PARTS : W];  // masses of the kept in the runs
     __shared__ float redf_s[2][W], thr_s;
     __shared__ unsigned redu_s[W];
     __shared__ u64 found_mass, found_key, found_kept;
@@ -335,7 +344,6 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     };
     const auto piece = [&](int i) {
         Piece v;
-        if (ROW) return reinterpret_cast<const Piece*>(row_s)[i];
         if ((i + 1) * P <= p.V) {
             __builtin_memcpy(&v, x + (size_t)i * P, 8);
         } else {
@@ -348,7 +356,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     const auto each = [&](float from, auto&& f) {
 #pragma unroll 1
         for (int i = tid; i < nvec; i += NT) {
-            const Vec v = ROW ? row_s[i] : from_memory(i);
+            const Vec v = from_memory(i);
             float top = wide(v[0]);
 #pragma unroll
             for (int c = 1; c < N; c++) top = fmaxf(top, wide(v[c]));
@@ -357,11 +365,12 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
                 for (int c = 0; c < N; c++) f(wide(v[c]), i * N + c);
         }
     };
-    // ---- the maximum, the least finite element, what no distribution holds
+    // ---- the maximum, the least element, what no distribution holds
     float best = -INFINITY, least = INFINITY;
     bool bad = false;
+    const bool cut_k = top_k > 0 && top_k < p.V, cut_p = top_p < 1., few = cut_k && top_k <= SM_TOP;
     if (tid == 0) held_s = 0;
-    if (PARTS) {
+    if (PARTS && !few) {
         const PartStats a = join_parts(p, r, p.parts);
         best = a.best;
         least = a.least;
@@ -378,20 +387,17 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
                 const int i = i0 + j * NT;
                 if (i >= nvec) continue;
                 if (i == full) v[j] = from_memory(i);
-                if (ROW) row_s[i] = v[j];
 #pragma unroll
                 for (int c = 0; c < N; c++) {
-                    const float e = wide(v[j][c]);
-                    bad |= e != e;
-                    best = fmaxf(best, e);
-                    least = fminf(least, e > -INFINITY ? e : INFINITY);
+                    best = __builtin_elementwise_maximum(best, wide(v[j][c]));  // (a NaN stays)
+                    least = __builtin_elementwise_minimum(least, wide(v[j][c]));
                 }
             }
         }
         sets_s[wv * 64 + lane] = best;
+        bad = __any(best != best);
         best = wave_max(best);
         least = -wave_max(-least);
-        bad = __any(bad);
         if (lane == 0) {
             redf_s[0][wv] = best;
             redf_s[1][wv] = least;
@@ -399,7 +405,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         }
     }
     __syncthreads();
-    if (!PARTS)
+    if (!PARTS || few)
         for (int w = 0; w < W; w++) {
             best = fmaxf(best, redf_s[0][w]);
             least = fminf(least, redf_s[1][w]);
@@ -442,8 +448,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     };
     u64 base = 0;          // kept so far: keys from here on
     float from = -INFINITY;  // its value
-    const bool cut_k = top_k > 0 && top_k < p.V, cut_p = top_p < 1.;
-    if (!PARTS && cut_k && top_k <= SM_TOP) {
+    if (few) {
         const int k = (int)top_k;
         if (wv == 0) {  // (of one set of threads a lane, or, past 64, of two)
             float most[2] = {-INFINITY, -INFINITY};
@@ -465,7 +470,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         });
         __syncthreads();
         const int n = held_s;
-        if (n <= 4 * SM_FEW && n <= NT) {
+        if (n <= min(SM_FEW, NT)) {
             for (int at = tid / 8; at < n; at += NT / 8) {  // eight threads to one
                 const u64 key = list_s[at];
                 int rank = 0;
@@ -512,8 +517,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     }
     const Bins bins(best, least, T, BINS);
     // The runs of the row: their masses by bins, whether they have been counted.
-    const int runs = PARTS ? p.parts : RUNS;
-    const int run_len = PARTS ? p.part / P : (npiece + RUNS - 1) / RUNS;  // pieces of a run
+    int runs = PARTS ? p.parts : RUNS;
+    int run_len = PARTS ? p.part / P : (npiece + RUNS - 1) / RUNS;  // pieces of a run
     bool counted = PARTS;
     const auto run_mass = [&](int run, int b) -> u64 { return PARTS ? p.part_mass[(r * runs + run) * BINS + b] : run_s[PARTS ? 0 : run][b]; };
     u64 total = 0;      // the mass of what the last search looked at
@@ -645,11 +650,8 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         const u64 above = wa;
         u64 lo = 0, hi = 0;  // the keys of the undecided, once they are known
         const auto range = [&](u64 low, u64 high) {
-            for (int d = 32; d > 0; d >>= 1) {
-                const u64 a = __shfl_xor(low, d), b = __shfl_xor(high, d);
-                low = a < low ? a : low;
-                high = b > high ? b : high;
-            }
+            low = ~wave_most(~low);
+            high = wave_most(high);
             __syncthreads();
             if (lane == 0) {
                 red_s[0][wv] = low;
@@ -696,7 +698,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         near_bin(bin, mid, half);
 #pragma unroll 2
         for (int i = tid; i < nvec; i += NT) {
-            const Vec v = ROW ? row_s[i] : from_memory(i);
+            const Vec v = from_memory(i);
             float near = INFINITY;
 #pragma unroll
             for (int c = 0; c < N; c++) near = fminf(near, fabsf(wide(v[c]) - mid));
@@ -710,7 +712,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         if (vecs <= 2 * BINS) {
             for (int at = tid; at < vecs; at += NT) {
                 const int i = near_s[at];
-                const Vec v = ROW ? row_s[i] : from_memory(i);
+                const Vec v = from_memory(i);
 #pragma unroll
                 for (int c = 0; c < N; c++) {
                     const float e = wide(v[c]);
@@ -760,7 +762,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
             });
             __syncthreads();
         }
-        while (n > SM_FEW) {  // a thread to each of the list
+        while (n > SM_FEW) {  // (a thread to each of the list)
             const u64 key = tid < (int)n ? list_s[tid] : 0;
             range(tid < (int)n ? key : ~0ull, key);
             const int shift = shift_of();
@@ -819,12 +821,30 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         from = lowest;
         base = order_key(lowest, 0x7fffffff);
     }
-    // ---- the draw: the runs' masses from their bins, the run of the token a wave to a part of it
+    // ---- the draw: the runs' masses, those of a wave each of the run of the token, that wave
     const bool every = base == 0;
     const auto kept = [&](float e, int i) { return every || e > from || (e == from && order_key(e, i) >= base); };
-    int begin = 0, end = npiece;
-    u64 passed = 0, target = 0;
-    if (counted) {
+    const auto piece_weight = [&](int i) {
+        const Piece v = piece(i);
+        float top = wide(v[0]);
+#pragma unroll
+        for (int c = 1; c < P; c++) top = fmaxf(top, wide(v[c]));
+        u64 s = 0;
+        if (top >= from)
+#pragma unroll
+            for (int c = 0; c < P; c++) {
+                const u64 w = weight(ch, wide(v[c]));
+                s += kept(wide(v[c]), i * P + c) ? w : 0;
+            }
+        return s;
+    };
+    const auto wave_mass = [&](int begin, int end) {
+        u64 s = 0;
+#pragma unroll 1
+        for (int i = begin + lane; i < end; i += 64) s += piece_weight(i);
+        return wave_add(s);
+    };
+    if (counted) {  // by bins
         const int border = every ? BINS : bins.of(from);
         for (int run = wv; run < runs; run += W) {
             u64 s = 0;
@@ -846,42 +866,27 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
             }
             __syncthreads();
         }
-        total = 0;
-        for (int i = 0; i < runs; i++) total += runs_s[i];
-        target = mass_at(total);
-        int run = 0;
-        while (run < runs - 1 && passed + runs_s[run] <= target) passed += runs_s[run++];
-        begin = run * run_len;
-        end = min(begin + run_len, npiece);
+    } else {
+        runs = W;
+        run_len = (npiece + W - 1) / W;
+        const int begin = min(wv * run_len, npiece);
+        const u64 s = wave_mass(begin, min(begin + run_len, npiece));
+        if (lane == 0) runs_s[wv] = s;
+        __syncthreads();
     }
+    total = 0;
+    for (int i = 0; i < runs; i++) total += runs_s[i];
+    const u64 target = mass_at(total);
+    u64 passed = 0;
+    int run = 0;
+    while (run < runs - 1 && passed + runs_s[run] <= target) passed += runs_s[run++];
+    int begin = min(run * run_len, npiece), end = min(begin + run_len, npiece);
     const int len = (end - begin + W - 1) / W;
     begin = min(begin + wv * len, end);
     end = min(begin + len, end);
-    const auto piece_weight = [&](int i) {
-        const Piece v = piece(i);
-        float top = wide(v[0]);
-#pragma unroll
-        for (int c = 1; c < P; c++) top = fmaxf(top, wide(v[c]));
-        u64 s = 0;
-        if (top >= from)
-#pragma unroll
-            for (int c = 0; c < P; c++) {
-                const u64 w = weight(ch, wide(v[c]));
-                s += kept(wide(v[c]), i * P + c) ? w : 0;
-            }
-        return s;
-    };
-    u64 sum = 0;
-#pragma unroll 1
-    for (int i = begin + lane; i < end; i += 64) sum += piece_weight(i);
-    sum = wave_add(sum);
+    const u64 sum = wave_mass(begin, end);
     if (lane == 0) red_s[0][wv] = sum;
     __syncthreads();
-    if (!counted) {
-        total = 0;
-        for (int w = 0; w < W; w++) total += red_s[0][w];
-        target = mass_at(total);
-    }
     for (int w = 0; w < wv; w++) passed += red_s[0][w];
     if (passed <= target && target < passed + sum) {  // (one wave)
 #pragma unroll 1
@@ -894,7 +899,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
                 if (mass <= target && target < mass + s) {  // (one lane)
 #pragma unroll 1
                     for (int c = 0; c < P; c++) {
-                        const float e = wide(ROW ? reinterpret_cast<const E*>(row_s)[i * P + c] : x[(size_t)i * P + c]);
+                        const float e = wide(x[(size_t)i * P + c]);
                         const u64 w = kept(e, i * P + c) ? weight(ch, e) : 0;
                         mass += w;
                         if (mass > target) {
@@ -910,25 +915,29 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     }
 }
 
-template <class E, int NT, int ROW>
+template <class E, int NT>
 void launch_rows(SampleParams p, hipStream_t stream) {
     for (p.first = 0; p.first < p.rows; p.first += LOGPROBS_MAX_GRID) {
         const dim3 grid((unsigned)min(p.rows - p.first, (long long)LOGPROBS_MAX_GRID));
-        hipLaunchKernelGGL((sample_kernel<E, NT, ROW, false>), grid, dim3(NT), 0, stream, p);
+        hipLaunchKernelGGL((sample_kernel<E, NT, false>), grid, dim3(NT), 0, stream, p);
     }
 }
 
-// Parts of a row, 1 where it is not shared out.
-int row_parts(long long rows, int V) {
-    const int parts = (int)min(256 / max(rows, 1ll), (long long)SAMPLE_PARTS);
-    return min(parts, V / SAMPLE_PART_COLS);
+// Parts of a row, 1 where it is not shared out: few wide rows, but for a top_k that
+// one wave handles (of which a call with a top_k for each row may hold some). us
+// on MI355X, bf16, one workgroup a row against parts: top_p 0.9, 16 rows of 32000
+// 21 / 22, of 50001 37 / 32, of 131072 62 / 40; 64 rows of 131072 62 / 59; 128 68 /
+// 94; whole distributions, 16 rows of 32000 16 / 15, of 50001 22 / 18; top_k 50, 16
+// rows of 131072 19 / 28.
+int row_parts(const SampleParams& p) {
+    if (p.V < SAMPLE_MIN_V || p.rows > SAMPLE_MAX_ROWS || p.rows <= 0 || (!p.top_ks && p.top_k > 0 && p.top_k <= SM_TOP)) return 1;
+    return min(p.V / SAMPLE_PART_COLS, SAMPLE_PARTS);
 }
 
 template <class E>
 void launch(SampleParams p, hipStream_t stream) {
     constexpr int N = RowVec<E>::N;
-    const size_t bytes = ((size_t)p.V * sizeof(E) + 15) / 16 * 16;
-    const int parts = row_parts(p.rows, p.V);
+    const int parts = row_parts(p);
     if (parts > 1) {
         p.part = ((p.V + parts - 1) / parts + N - 1) / N * N;
         p.parts = (p.V + p.part - 1) / p.part;
@@ -939,23 +948,29 @@ void launch(SampleParams p, hipStream_t stream) {
         const dim3 grid((unsigned)p.rows, (unsigned)p.parts);
         hipLaunchKernelGGL(sample_stats_kernel<E>, grid, dim3(256), 0, stream, p);
         hipLaunchKernelGGL(sample_bins_kernel<E>, grid, dim3(256), 0, stream, p);
-        hipLaunchKernelGGL((sample_kernel<E, 1024, 0, true>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
-    } else if (bytes <= 16384) {
-        launch_rows<E, 256, 16384>(p, stream);
-    } else if (bytes <= 65536) {
-        launch_rows<E, 1024, 65536>(p, stream);
-    } else if (bytes <= SM_ROW) {
-        launch_rows<E, 1024, SM_ROW>(p, stream);
+        hipLaunchKernelGGL((sample_kernel<E, 1024, true>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
+    } else if (p.V <= 8192) {
+        launch_rows<E, 256>(p, stream);
+    } else if (p.rows <= 256) {
+        launch_rows<E, 1024>(p, stream);
     } else {
-        launch_rows<E, 1024, 0>(p, stream);
+        launch_rows<E, 512>(p, stream);
     }
+    // Threads of a row by us on MI355X, bf16, 256 / 512 / 1024 threads:
+    //   4096 columns, 1024 rows: whole 14 / 18 / 33, top_k 50 15 / 20 / 34, top_p 0.9 20 / 29 / 52; 1 row: 7 / 7 / 8, 11 / 9 / 9, 12 / 12 / 13
+    //   16384, 1024 rows: top_k 21 / 25 / 40, top_p 46 / 46 / 70; 1 row: 15 / 11 / 10, 27 / 17 / 17
+    //   32000, 1024 rows: whole 62 / 54 / 66, top_k 33 / 35 / 48, top_p 0.95 79 / 74 / 95; 64 rows: top_p 41 / 27 / 24
+    //   50001 fp32, 1021 rows: whole 116 / 100 / 112, top_k 65 / 67 / 80, top_p 336 / 140 / 173
 }
 
 }  // namespace
 
 // Bytes of the parts' statistics and bins, 0 where rows are not shared out.
 size_t sample_workspace_bytes(long long rows, int V) {
-    const int parts = rows > 0 ? row_parts(rows, V) : 1;
+    SampleParams p{};
+    p.rows = rows;
+    p.V = V;
+    const int parts = row_parts(p);
     return parts > 1 ? (size_t)rows * parts * (sizeof(PartStats) + SM_BINS * 12) : 0;
 }
 
