@@ -139,7 +139,7 @@ int cyfa_adjust_logits(const CyfaAdjustArgs* a, int dtype, int grad, void* hip_s
     if (dtype < CYFA_DTYPE_BF16 || dtype > CYFA_DTYPE_F16) return fail(CYFA_ERR_VALUE, "%s: dtype %d", what, dtype);
     if (a->rows < 0 || a->inner <= 0 || a->V <= 0 || a->L < 0 || a->n_tokens < 0)
         return fail(CYFA_ERR_VALUE, "%s: rows=%lld inner=%lld V=%d L=%lld n_tokens=%d", what, a->rows, a->inner, a->V, a->L, a->n_tokens);
-    if (a->V > cyfa::LOGPROBS_MAX_V || a->L > 0x7fffffff) return fail(CYFA_ERR_UNSUPPORTED, "%s: V=%d L=%lld", what, a->V, a->L);
+    if (a->V > cyfa::LOGPROBS_MAX_V || a->L > cyfa::ADJUST_MAX_L) return fail(CYFA_ERR_UNSUPPORTED, "%s: V=%d L=%lld", what, a->V, a->L);
     if (a->n_tokens > cyfa::ADJUST_MAX_TOKENS)
         return fail(CYFA_ERR_UNSUPPORTED, "%s: %d of at most %d token biases", what, a->n_tokens, cyfa::ADJUST_MAX_TOKENS);
     const int size = dtype == CYFA_DTYPE_F32 ? 4 : 2;

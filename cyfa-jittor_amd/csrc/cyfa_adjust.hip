@@ -9,10 +9,13 @@
 //   dx = dy (n > 0 ? (x > 0 ? 1 / repetition : repetition) : 1), 0 where j is not allowed
 // in fp32, every product and sum rounded by itself, y rounded once.
 //
-// A workgroup takes a row's slice of columns: it counts the history's tokens that
+// A workgroup takes a row's slice of columns. It counts the history's tokens that
 // fall into the slice in LDS (a word a column: the top bit for any occurrence,
-// the others count those behind the prompt; integers, so that their order does
-// not matter), then passes over the slice once.
+// the low ones count those behind the prompt; integers, so that their order does
+// not matter) and lists the columns that it meets, whose results it forms one by
+// one; the slice itself is passed over as where nothing is repeated, and the
+// listed columns are stored a second time. So the pass reads no counts, and runs
+// at the memory's rate.
 #include "cyfa_internal.h"
 #include "cyfa_rows.h"
 
@@ -22,11 +25,22 @@ namespace {
 
 constexpr int AJ_NT = 256;
 constexpr int AJ_NV = 4;            // vectors of a thread in flight
-constexpr int AJ_COLS = 8192;       // most columns of a slice: 32 KiB of LDS, half as many where it holds the tokens' biases too
-constexpr uint32_t AJ_SEEN = 0x80000000u;
+constexpr int AJ_COLS = 8192;       // most columns of a slice: 48 KiB of LDS, half as many where it holds the tokens' biases too
+constexpr uint32_t AJ_SEEN = 0x80000000u, AJ_BIASED = 0x40000000u, AJ_MADE = 0x3fffffffu;
+
+// A slice's columns that the history or the tokens' biases name: counts [cols],
+// their list and its length.
+struct Touched {
+    uint32_t* counts;
+    uint16_t* list;
+    int* n;
+    __device__ __forceinline__ void met(uint32_t before, int c) const {
+        if (before == 0) list[atomicAdd(n, 1)] = (uint16_t)c;
+    }
+};
 
 template <class I>
-__device__ void count_tokens(const AdjustParams& p, const I* ids, long long n, long long prompt, int c0, int cols, uint32_t* counts) {
+__device__ void count_tokens(const I* ids, long long n, long long prompt, int c0, int cols, const Touched& touched) {
     constexpr int U = 8;
     for (long long i0 = threadIdx.x; i0 < n; i0 += AJ_NT * U) {
         I t[U];
@@ -35,12 +49,8 @@ __device__ void count_tokens(const AdjustParams& p, const I* ids, long long n, l
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const long long i = i0 + u * AJ_NT, c = (long long)t[u] - c0;
-            if (i < n && c >= 0 && c < cols) {
-                if (i < prompt)
-                    atomicOr(&counts[c], AJ_SEEN);
-                else
-                    atomicAdd(&counts[c], 1u);
-            }
+            if (i < n && c >= 0 && c < cols)  // (AJ_SEEN and a one: the count of what is behind the prompt, too)
+                touched.met(i < prompt ? atomicOr(&touched.counts[c], AJ_SEEN) : atomicAdd(&touched.counts[c], 1u), (int)c);
         }
     }
 }
@@ -48,40 +58,45 @@ __device__ void count_tokens(const AdjustParams& p, const I* ids, long long n, l
 template <class E, bool GRAD, bool TOKENS>
 __global__ __launch_bounds__(AJ_NT) void adjust_kernel(AdjustParams p) {
 #pragma clang fp contract(off)
+    typedef typename RowVec<E>::type Vec;
     constexpr int N = RowVec<E>::N;
-    extern __shared__ uint32_t lds[];
-    uint32_t* counts = lds;                                    // [p.cols] with a history
-    float* values = (float*)(lds + (p.L > 0 ? p.cols : 0));    // [p.cols] with the tokens' biases
+    extern __shared__ __align__(16) uint32_t lds[];
     __shared__ int ids_s[TOKENS ? ADJUST_MAX_TOKENS : 1];
     __shared__ float values_s[TOKENS ? ADJUST_MAX_TOKENS : 1];
+    __shared__ int listed_s;
     const int tid = threadIdx.x;
+    const bool history = p.L > 0, touches = history || TOKENS;
+    const Touched touched = {lds, reinterpret_cast<uint16_t*>(lds + p.cols * (TOKENS ? 2 : 1)), &listed_s};
+    float* values = reinterpret_cast<float*>(lds + p.cols);  // TOKENS: [cols], the tokens' biases
     const long long slices = (p.V + p.cols - 1) / p.cols;
-    for (long long job = blockIdx.x; job < p.jobs; job += gridDim.x) {
-        // The slices of a row, which read the same history, go to one XCD's L2
-        // (consecutive workgroups run on the eight XCDs in turn).
-        long long r, s;
-        if (p.rows >= 8) {
-            r = job / (8 * slices) * 8 + job % 8;
-            s = job / 8 % slices;
-            if (r >= p.rows) continue;
-        } else {
-            r = job / slices;
-            s = job % slices;
+    const long long job = p.first + blockIdx.x;
+    // The slices of a row, which read the same history, go to one XCD's L2
+    // (consecutive workgroups run on the eight XCDs in turn).
+    long long r, s;
+    if (p.rows >= 8) {
+        r = job / (8 * slices) * 8 + job % 8;
+        s = job / 8 % slices;
+        if (r >= p.rows) return;
+    } else {
+        r = job / slices;
+        s = job % slices;
+    }
+    const long long ro = r / p.inner, ri = r % p.inner;
+    const int c0 = (int)s * p.cols, cols = min(p.cols, p.V - c0);
+    const E* x = static_cast<const E*>(p.x) + ro * p.x_outer + ri * p.x_row + c0;
+    const E* from = GRAD ? static_cast<const E*>(p.dy) + r * p.V + c0 : x;
+    E* y = static_cast<E*>(p.y) + ro * p.y_outer + ri * p.y_row + c0;
+    const float* bias = !GRAD && p.bias ? p.bias + ro * p.b_outer + ri * p.b_row + c0 : nullptr;
+    const unsigned char* allowed =
+        p.allowed ? static_cast<const unsigned char*>(p.allowed) + ro * p.a_outer + ri * p.a_row + (p.packed ? c0 / 8 : c0) : nullptr;
+    const auto kept = [&](int c) { return !allowed || (p.packed ? (allowed[c >> 3] >> (c & 7) & 1) != 0 : allowed[c] != 0); };
+    if (touches) {
+        for (int c = tid * 4; c < p.cols; c += AJ_NT * 4) {
+            *reinterpret_cast<uint4*>(touched.counts + c) = uint4{0, 0, 0, 0};
+            if (TOKENS) *reinterpret_cast<float4*>(values + c) = float4{0.f, 0.f, 0.f, 0.f};
         }
-        const long long ro = r / p.inner, ri = r % p.inner;
-        const int c0 = (int)s * p.cols, cols = min(p.cols, p.V - c0);
-        const E* x = static_cast<const E*>(p.x) + ro * p.x_outer + ri * p.x_row + c0;
-        const E* dy = static_cast<const E*>(p.dy) + (GRAD ? r * p.V + c0 : 0);
-        E* y = static_cast<E*>(p.y) + ro * p.y_outer + ri * p.y_row + c0;
-        const float repetition = p.repetitions ? p.repetitions[r] : p.repetition;
-        const float presence = p.presences ? p.presences[r] : p.presence;
-        const float frequency = p.frequencies ? p.frequencies[r] : p.frequency;
-        const bool history = p.L > 0;
-        __syncthreads();  // the row before is done with the LDS
-        if (history)
-            for (int c = tid; c < p.cols; c += AJ_NT) counts[c] = 0;
+        if (tid == 0) listed_s = 0;
         if (TOKENS) {
-            for (int c = tid; c < p.cols; c += AJ_NT) values[c] = 0.f;
             const long long* ids = p.token_ids + ro * p.ti_outer + ri * p.ti_row;
             const float* v = p.token_values + ro * p.tv_outer + ri * p.tv_row;
             for (int i = tid; i < p.n_tokens; i += AJ_NT) {
@@ -92,12 +107,12 @@ __global__ __launch_bounds__(AJ_NT) void adjust_kernel(AdjustParams p) {
         }
         __syncthreads();
         if (history) {
-            const long long n = p.lengths ? max(0ll, min(p.L, p.lengths[r])) : p.L;
-            const long long prompt = p.prompts ? p.prompts[r] : 0;
+            const long long n = p.lengths ? max(0ll, min(p.L, p.lengths[r])) : p.L, prompt = p.prompts ? p.prompts[r] : 0;
+            const long long at = ro * p.h_outer + ri * p.h_row;
             if (p.wide)
-                count_tokens(p, static_cast<const long long*>(p.history) + ro * p.h_outer + ri * p.h_row, n, prompt, c0, cols, counts);
+                count_tokens(static_cast<const long long*>(p.history) + at, n, prompt, c0, cols, touched);
             else
-                count_tokens(p, static_cast<const int*>(p.history) + ro * p.h_outer + ri * p.h_row, n, prompt, c0, cols, counts);
+                count_tokens(static_cast<const int*>(p.history) + at, n, prompt, c0, cols, touched);
         }
         if (TOKENS)
             // the first entry of a token adds all of its entries, in their order
@@ -111,54 +126,84 @@ __global__ __launch_bounds__(AJ_NT) void adjust_kernel(AdjustParams p) {
                         if (j < i) first = false;
                         sum += values_s[j];
                     }
-                if (first) values[c] = sum;
+                if (first) {
+                    values[c] = sum;
+                    touched.met(atomicOr(&touched.counts[c], AJ_BIASED), c);
+                }
             }
         __syncthreads();
-        const float* bias = p.bias ? p.bias + ro * p.b_outer + ri * p.b_row + c0 : nullptr;
-        const unsigned char* allowed = p.allowed ? static_cast<const unsigned char*>(p.allowed) + ro * p.a_outer + ri * p.a_row : nullptr;
-        const auto one = [&](float e, int c, bool keep) {
-            const uint32_t w = history ? counts[c] : 0;
+        // the listed columns' results, in place of their counts
+        const float repetition = p.repetitions ? p.repetitions[r] : p.repetition;
+        const float presence = p.presences ? p.presences[r] : p.presence;
+        const float frequency = p.frequencies ? p.frequencies[r] : p.frequency;
+        for (int i = tid; i < listed_s; i += AJ_NT) {
+            const int c = touched.list[i];
+            const uint32_t w = touched.counts[c], made = w & AJ_MADE;
+            const float xc = (float)x[c];
+            float e;
             if (GRAD) {
-                if (w && e != 0.f) {
-                    const float xc = (float)x[c];
-                    e *= xc > 0.f ? 1.f / repetition : repetition;
-                }
-                return keep ? e : 0.f;
-            }
-            if (w) {
-                e = e > 0.f ? e / repetition : e * repetition;
-                const uint32_t made = w & ~AJ_SEEN;
+                e = (float)from[c];
+                if (e != 0.f) e *= xc > 0.f ? 1.f / repetition : repetition;
+                e = kept(c) ? e : 0.f;
+            } else {
+                e = xc;
+                if (made || (w & AJ_SEEN)) e = e > 0.f ? e / repetition : e * repetition;
                 if (made) e = e - ((float)made * frequency + presence);
+                if (bias) e = e + bias[c];
+                if (TOKENS && (w & AJ_BIASED)) e = e + values[c];
+                e = kept(c) ? e : -INFINITY;
             }
-            if (bias) e = e + bias[c];
-            if (TOKENS) e = e + values[c];
-            return keep ? e : -INFINITY;
-        };
-        const auto kept = [&](int c) {
-            if (!allowed) return true;
-            const int j = c0 + c;
-            return p.packed ? (allowed[j >> 3] >> (j & 7) & 1) != 0 : allowed[j] != 0;
-        };
-        const E* from = GRAD ? dy : x;
-        const int nvec = cols / N, tail = cols - nvec * N;
-        for (int i0 = 0; i0 < nvec; i0 += AJ_NT * AJ_NV) {
-            typename RowVec<E>::type v[AJ_NV];
+            touched.counts[c] = __builtin_bit_cast(uint32_t, e);
+        }
+        __syncthreads();  // (y may be x)
+    }
+    const int nvec = cols / N, tail = cols - nvec * N;
+    const float out = GRAD ? 0.f : -INFINITY;
+    for (int i0 = 0; i0 < nvec; i0 += AJ_NT * AJ_NV) {
+        Vec v[AJ_NV];
+        uint32_t keep[AJ_NV][N / 4];  // bytes or bits of the mask
 #pragma unroll
-            for (int j = 0; j < AJ_NV; j++) v[j] = load_row(from + (size_t)min(i0 + j * AJ_NT + tid, nvec - 1) * N);
+        for (int j = 0; j < AJ_NV; j++) v[j] = load_row(from + (size_t)min(i0 + j * AJ_NT + tid, nvec - 1) * N);
+        if (allowed)
 #pragma unroll
             for (int j = 0; j < AJ_NV; j++) {
-                const int i = i0 + j * AJ_NT + tid;
-                if (i < nvec) {
-                    typename RowVec<E>::type o;
+                const int c = min(i0 + j * AJ_NT + tid, nvec - 1) * N;
+                if (p.packed)
+                    keep[j][0] = allowed[c >> 3] >> (c & 7);
+                else
+                    __builtin_memcpy(keep[j], allowed + c, N);
+            }
 #pragma unroll
-                    for (int c = 0; c < N; c++) o[c] = (E)one((float)v[j][c], i * N + c, kept(i * N + c));
-                    store_row(y + (size_t)i * N, o);
+        for (int j = 0; j < AJ_NV; j++) {
+            const int i = i0 + j * AJ_NT + tid;
+            if (i >= nvec) continue;
+            if (bias) {
+                float b[N];
+                __builtin_memcpy(b, bias + (size_t)i * N, sizeof b);
+#pragma unroll
+                for (int c = 0; c < N; c++) v[j][c] = (E)((float)v[j][c] + b[c]);
+            }
+            if (allowed) {
+#pragma unroll
+                for (int c = 0; c < N; c++) {
+                    const bool k = p.packed ? (keep[j][0] >> c & 1) != 0 : (keep[j][c / 4] >> (c % 4 * 8) & 0xff) != 0;
+                    v[j][c] = k ? v[j][c] : (E)out;
                 }
             }
+            store_row(y + (size_t)i * N, v[j]);
         }
-        if (tid < tail) {
-            const int c = nvec * N + tid;
-            y[c] = (E)one((float)from[c], c, kept(c));
+    }
+    if (tid < tail) {
+        const int c = nvec * N + tid;
+        float e = (float)from[c];
+        if (bias) e = e + bias[c];
+        y[c] = (E)(kept(c) ? e : out);
+    }
+    if (touches) {
+        __syncthreads();  // the listed columns are stored again
+        for (int i = tid; i < listed_s; i += AJ_NT) {
+            const int c = touched.list[i];
+            y[c] = (E)__builtin_bit_cast(float, touched.counts[c]);
         }
     }
 }
@@ -170,15 +215,17 @@ void launch(AdjustParams p, bool grad, hipStream_t stream) {
     const bool tokens = !grad && p.n_tokens > 0;
     p.cols = (int)min(max((want + 31) / 32 * 32, 1024ll), (long long)(tokens ? AJ_COLS / 2 : AJ_COLS));
     const long long slices = (p.V + p.cols - 1) / p.cols;
-    p.jobs = (p.rows >= 8 ? (p.rows + 7) / 8 * 8 : p.rows) * slices;
-    const dim3 grid((unsigned)min(p.jobs, (long long)LOGPROBS_MAX_GRID));
-    const size_t lds = (size_t)p.cols * 4 * ((p.L > 0) + tokens);
-    if (grad)
-        hipLaunchKernelGGL((adjust_kernel<E, true, false>), grid, dim3(AJ_NT), lds, stream, p);
-    else if (tokens)
-        hipLaunchKernelGGL((adjust_kernel<E, false, true>), grid, dim3(AJ_NT), lds, stream, p);
-    else
-        hipLaunchKernelGGL((adjust_kernel<E, false, false>), grid, dim3(AJ_NT), lds, stream, p);
+    const long long jobs = (p.rows >= 8 ? (p.rows + 7) / 8 * 8 : p.rows) * slices;
+    const size_t lds = p.L > 0 || tokens ? (size_t)p.cols * (tokens ? 10 : 6) : 0;
+    for (p.first = 0; p.first < jobs; p.first += LOGPROBS_MAX_GRID) {
+        const dim3 grid((unsigned)min(jobs - p.first, (long long)LOGPROBS_MAX_GRID));
+        if (grad)
+            hipLaunchKernelGGL((adjust_kernel<E, true, false>), grid, dim3(AJ_NT), lds, stream, p);
+        else if (tokens)
+            hipLaunchKernelGGL((adjust_kernel<E, false, true>), grid, dim3(AJ_NT), lds, stream, p);
+        else
+            hipLaunchKernelGGL((adjust_kernel<E, false, false>), grid, dim3(AJ_NT), lds, stream, p);
+    }
 }
 
 }  // namespace

@@ -638,9 +638,10 @@ struct AdjustParams {
     void* y;                     // may be x, with its strides; gradient: dx
     long long y_outer, y_row;
     int cols;                    // of a slice, set by the launcher
-    long long jobs;
+    long long first;             // a launch's first slice, set by the launcher
 };
 constexpr int ADJUST_MAX_TOKENS = 1024;
+constexpr long long ADJUST_MAX_L = (1 << 30) - 1;  // a column's count leaves two bits of a word
 void launch_adjust(const AdjustParams& p, int dtype, bool grad, hipStream_t stream);
 
 // The choice of a token from each row of logits (cyfa_sample.hip).

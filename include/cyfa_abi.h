@@ -686,7 +686,7 @@ typedef struct CyfaAdjustArgs {
     long long x_outer, x_row;
     const void *history;          /* L > 0: [rows, L], int64 (wide) or int32 */
     long long h_outer, h_row;
-    long long L;                  /* below 2^31 */
+    long long L;                  /* below 2^30 */
     int wide;
     const long long *lengths;     /* nullable [rows]: L */
     const long long *prompts;     /* nullable [rows]: 0 */
