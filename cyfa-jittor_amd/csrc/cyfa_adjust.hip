@@ -48,11 +48,11 @@ __global__ __launch_bounds__(NT) void adjust_kernel(AdjustParams p) {
     typedef Counts<BITS> C;
     constexpr int N = RowVec<E>::N, U = 4;
     extern __shared__ __align__(16) uint32_t lds[];
-    __shared__ int ids_s[GRAD ? 1 : ADJUST_MAX_TOKENS];
-    __shared__ float values_s[GRAD ? 1 : ADJUST_MAX_TOKENS];
     __shared__ int listed_s;
-    const C counts = {lds};                                                      // [cols]
-    uint16_t* const list = reinterpret_cast<uint16_t*>(lds + p.cols / (32 / BITS));  // [min(cols, L)]
+    const C counts = {lds};                                                              // [cols]
+    int* const ids_s = reinterpret_cast<int*>(lds + p.cols / (32 / BITS));               // [n_tokens]
+    float* const values_s = reinterpret_cast<float*>(ids_s) + (GRAD ? 0 : p.n_tokens);   // [n_tokens]
+    uint16_t* const list = reinterpret_cast<uint16_t*>(values_s + (GRAD ? 0 : p.n_tokens));  // [min(cols, L)]
     const int tid = threadIdx.x;
     const bool tokens = !GRAD && p.n_tokens > 0, touches = p.L > 0 || tokens;
     const long long slices = (p.V + p.cols - 1) / p.cols;
@@ -254,7 +254,8 @@ template <class E, int NT, int BITS, bool GRAD>
 void launch_slices(AdjustParams p, long long cols, hipStream_t stream) {
     p.cols = (int)cols;
     const long long slices = (p.V + p.cols - 1) / p.cols, jobs = (p.rows >= 8 ? (p.rows + 7) / 8 * 8 : p.rows) * slices;
-    const size_t lds = p.L > 0 || p.n_tokens > 0 ? (size_t)cols * BITS / 8 + (size_t)min(cols, p.L) * 2 : 0;
+    const int tokens = GRAD ? 0 : p.n_tokens;
+    const size_t lds = p.L > 0 || tokens > 0 ? (size_t)cols * BITS / 8 + (size_t)tokens * 8 + (size_t)min(cols, p.L) * 2 : 0;
     for (p.first = 0; p.first < jobs; p.first += LOGPROBS_MAX_GRID) {
         const dim3 grid((unsigned)min(jobs - p.first, (long long)LOGPROBS_MAX_GRID));
         hipLaunchKernelGGL((adjust_kernel<E, NT, BITS, GRAD>), grid, dim3(NT), lds, stream, p);
@@ -263,14 +264,24 @@ void launch_slices(AdjustParams p, long long cols, hipStream_t stream) {
 
 template <class E, bool GRAD>
 void launch(const AdjustParams& p, hipStream_t stream) {
-    // Slices of a row so that some hundred workgroups fill the compute units.
-    const long long whole = (p.V + 31ll) / 32 * 32, want = (p.rows * p.V / 512 + 31) / 32 * 32;
+    // Columns of a slice and threads that take it, by us on MI355X (forward / gradient
+    // of bf16). Each slice reads the history; few large ones leave compute units idle:
+    //   4096 x 32000, 768 tokens: 256 threads, 4096 columns 130 / 147, 8192 123 / 160; 512, 8192 136 / 148,
+    //     16384 116 / 142 (stored past the caches 107 / 138 here, and no faster where a loss reads the results);
+    //     1024, 32000 120 / 140
+    //   256 x 50001 fp16 with a mask, 6100 tokens: 512, 8192 40, 16384 46; 1024, 16704 40, 25024 36
+    //   64 x 32000 with a mask, 1500 tokens: 512, 8192 8.7, 16384 9.2; 1024, 25024 10.2
+    //   1024 x 4096, 380 tokens: 256, 4096 7.3; 512 9.4
+    const long long whole = (p.V + 31ll) / 32 * 32, slices = (whole + 32767) / 32768;
+    const bool many = p.rows * p.V >= 16384ll * 512;
     if (p.L > Counts<16>::MADE)
-        launch_slices<E, 256, 32, GRAD>(p, min(whole, min(max(want, 1024ll), 8192ll)), stream);
-    else if (want <= 8192 || whole <= 8192)
-        launch_slices<E, 256, 16, GRAD>(p, min(whole, max(want, 1024ll)), stream);
+        launch_slices<E, 512, 32, GRAD>(p, min(whole, 8192ll), stream);
+    else if (p.V <= 4096)
+        launch_slices<E, 256, 16, GRAD>(p, whole, stream);
+    else if (many && p.L >= 4096)
+        launch_slices<E, 1024, 16, GRAD>(p, (whole / slices + 31) / 32 * 32, stream);
     else
-        launch_slices<E, 1024, 16, GRAD>(p, min(whole, min(want, 32768ll)), stream);
+        launch_slices<E, 512, 16, GRAD>(p, min(whole, many ? 16384ll : 8192ll), stream);
 }
 
 }  // namespace

@@ -96,7 +96,8 @@ def _adjust_ref(x, kw, allowed, dy=None):
     (1, 1, 1, F32, True, False, 0, ""), (2, 7, 9, BF, True, True, 3, "bool"), (3, 33, 2, F16, False, False, 2, "bits"),
     (9, 257, 100, F32, False, True, 0, "bits"), (5, 1023, 700, BF, True, False, 9, "bool"), (20, 2051, 33, F16, True, True, 0, ""),
     (1, 32000, 513, BF, True, False, 17, "bits"), (3, 50001, 4097, F32, True, True, 300, "bool"), (9, 8193, 1, BF, False, True, 1, "bits"),
-    (70, 40000, 65, BF, True, True, 1024, "bits")])
+    (70, 40000, 65, BF, True, True, 1024, "bits"), (3, 9001, 20000, BF, True, False, 40, "bool"), (260, 33000, 40, F16, True, False, 2, ""),
+    (4, 300, 17000, F32, False, True, 0, "bits"), (129, 66001, 4100, BF, False, False, 3, "bits")])
 def test_adjust(rows, V, L, dtype, wide, bias, tokens, mask):
     x, kw, allowed = _adjust_case(V + L, rows, V, L, dtype, wide, bias, tokens, mask)
     dy = (_randn(V, rows, V)).to(dtype)
