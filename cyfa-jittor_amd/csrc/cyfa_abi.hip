@@ -260,10 +260,11 @@ int cyfa_distill_loss(const CyfaDistillArgs* a, int dtype, int grad, void* hip_s
     const int size = dtype == CYFA_DTYPE_F32 ? 4 : 2;
     if (!aligned(a->x, size) || !aligned(a->dx, size) || !aligned(a->ids, 8))
         return fail(CYFA_ERR_ALIGN, "%s: tensors need their element's alignment", what);
+    if (!aligned(a->parts, 8)) return fail(CYFA_ERR_ALIGN, "%s: f64 tensors need 8-byte alignment", what);
     const void* words4[] = {a->values, a->weights, a->kept, a->loss, a->total, a->d_loss};
     for (const void* ptr : words4)
         if (!aligned(ptr, 4)) return fail(CYFA_ERR_ALIGN, "%s: f32 tensors need 4-byte alignment", what);
-    if (!a->total || (grad ? !a->d_loss : !a->loss)) return fail(CYFA_ERR_VALUE, "%s: null loss", what);
+    if (!a->total || (grad ? !a->d_loss : !a->loss || !a->parts)) return fail(CYFA_ERR_VALUE, "%s: null loss", what);
     if (a->rows > 0 && (!a->x || !a->ids || !a->values || !a->kept || (grad && !a->dx)))
         return fail(CYFA_ERR_VALUE, "%s: null required pointer", what);
     if (a->rows == 0 && grad) return CYFA_OK;
@@ -283,6 +284,7 @@ int cyfa_distill_loss(const CyfaDistillArgs* a, int dtype, int grad, void* hip_s
     p.kept = a->kept;
     p.loss = a->loss;
     p.total = a->total;
+    p.parts = a->parts;
     p.d_loss = a->d_loss;
     p.dx = a->dx;
     cyfa::launch_distill(p, dtype, grad != 0, (hipStream_t)hip_stream);

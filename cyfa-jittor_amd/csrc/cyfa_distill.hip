@@ -10,9 +10,10 @@
 //   dx_j = q_j P - sum of p_i over id_i = j, P = sum p_i + p_r,  at the entries' columns
 //   dx_j = (q_j / q_r) (q_r P - p_r)                             elsewhere
 // One pass over the row each way, sums in fp32; what the teacher's few entries
-// give is formed in double (1 - sum p_i cancels). The columns of no entry keep a
-// maximum and a sum of their own with the tail: taken as the difference of the
-// row's sum and the entries', a small rest would be lost.
+// give is formed in double (1 - sum p_i cancels), by a wave a row in a launch of
+// its own: at the end of the row's pass three waves of four would wait for it. The
+// columns of no entry keep a maximum and a sum of their own with the tail: taken
+// as the difference of the row's sum and the entries', a small rest would be lost.
 #include "cyfa_internal.h"
 #include "cyfa_rows.h"
 
@@ -67,172 +68,214 @@ __device__ __forceinline__ void join(Sum& a, Sum b, float c) {
     a.s += b.s;
 }
 
-// NT threads to a row.
+__device__ __forceinline__ const void* row_at(const DistillParams& p, long long r, int size) {
+    return static_cast<const char*>(p.x) + ((r / p.inner) * p.outer_stride + (r % p.inner) * p.row_stride) * size;
+}
+
+// A row's weight in the mean, the same in every lane: 0 where nothing of it counts.
+__device__ __forceinline__ float row_weight(const DistillParams& p, long long r) {
+    bool any = false;
+    for (int i = threadIdx.x & 63; i < p.k; i += 64) any |= counts(p.ids[r * p.k + i], p.values[r * p.k + i], p.V);
+    return __any(any) ? (p.weights ? p.weights[r] : 1.f) : 0.f;
+}
+
+// The maximum and the sum of a row's columns (TAIL: of those of no entry), by NT threads.
 template <class E, int NT, bool TAIL>
-__global__ __launch_bounds__(NT * rows_of(NT)) void distill_kernel(DistillParams p) {
+__global__ __launch_bounds__(NT * rows_of(NT)) void distill_sums_kernel(DistillParams p) {
     constexpr int N = RowVec<E>::N, W = NT / 64, RW = rows_of(NT);
     extern __shared__ uint32_t entries_s[];  // TAIL: a bit for each column of an entry, p.words words a row
     __shared__ Sum red[RW][W];
     const int tid = threadIdx.x % NT, lane = tid & 63, wv = tid >> 6, sub = threadIdx.x / NT;
     uint32_t* bits = entries_s + (size_t)sub * p.words;
     const float c = kLog2e / p.temperature;
-    for (long long r = (long long)blockIdx.x * RW + sub; r < p.rows; r += (long long)gridDim.x * RW) {
-        const E* x = static_cast<const E*>(p.x) + (r / p.inner) * p.outer_stride + (r % p.inner) * p.row_stride;
-        const long long* ids = p.ids + r * p.k;
-        const float* t = p.values + r * p.k;
-        bool any = false;
-        for (int i = lane; i < p.k; i += 64) any |= counts(ids[i], t[i], p.V);
-        const float weight = __any(any) ? (p.weights ? p.weights[r] : 1.f) : 0.f;
+    const long long r = p.first + (long long)blockIdx.x * RW + sub;
+    if (r >= p.rows) return;  // (rows of a wave each share no barrier)
+    const E* x = static_cast<const E*>(row_at(p, r, sizeof(E)));
+    if (row_weight(p, r) == 0.f) return;
+    if (TAIL) {
+        for (int i = tid; i < p.words; i += NT) bits[i] = 0;
+        row_sync<NT>();
+        for (int i = tid; i < p.k; i += NT) {
+            const long long id = p.ids[r * p.k + i];
+            if (counts(id, p.values[r * p.k + i], p.V)) atomicOr(&bits[id >> 5], 1u << (id & 31));
+        }
+        row_sync<NT>();
+    }
+    const auto entry_bits = [&](int col) { return TAIL ? bits[col >> 5] >> (col & 31) : 0u; };
+    const int nvec = p.V / N, tail = p.V - nvec * N;
+    Sum a = {kLowest, 0.f};
+    float best = -INFINITY;
+    const float last = tid < tail && !(entry_bits(nvec * N + tid) & 1) ? wide(x[nvec * N + tid]) : -INFINITY;
+    for (int v0 = 0; v0 < nvec; v0 += NT * DS_NV) {
+        typename RowVec<E>::type v[DS_NV];
+        uint32_t skip[DS_NV];  // elements of entries, or past the end
+#pragma unroll
+        for (int j = 0; j < DS_NV; j++) v[j] = load_row(x + (size_t)min(v0 + j * NT + tid, nvec - 1) * N);
+#pragma unroll
+        for (int j = 0; j < DS_NV; j++) {
+            const int i = v0 + j * NT + tid;
+            skip[j] = i >= nvec ? ~0u : entry_bits(i * N);
+            if (TAIL) {
+#pragma unroll
+                for (int k = 0; k < N; k++) best = fmaxf(best, skip[j] >> k & 1 ? -INFINITY : wide(v[j][k]));
+            } else if (i < nvec) {
+#pragma unroll
+                for (int k = 0; k < N; k++) best = fmaxf(best, wide(v[j][k]));
+            }
+        }
+        rescale(a, fmaxf(a.m, best), c);
+#pragma unroll
+        for (int j = 0; j < DS_NV; j++) {
+            if (!TAIL && skip[j]) continue;
+#pragma unroll
+            for (int k = 0; k < N; k++) a.s += fast_exp2((TAIL && (skip[j] >> k & 1) ? -INFINITY : wide(v[j][k]) - a.m) * c);
+        }
+    }
+    rescale(a, fmaxf(a.m, fmaxf(best, last)), c);
+    a.s += fast_exp2((last - a.m) * c);
+    const float m = wave_max(a.m);
+    rescale(a, m, c);
+    a.s = wave_sum(a.s);
+    if (W > 1) {
+        if (lane == 0) red[sub][wv] = a;
+        __syncthreads();
+        a = red[sub][0];
+#pragma unroll 3
+        for (int w = 1; w < W; w++) join(a, red[sub][w], c);
+    }
+    if (tid == 0) {
         DistillRow* keep = reinterpret_cast<DistillRow*>(p.kept) + r;
-        if (weight == 0.f) {  // (nothing of the row counts; the same in every wave)
-            if (tid == 0) {
+        keep->rm = a.m;
+        keep->rls = a.s;
+    }
+}
+
+// The rows' losses and what the gradient needs, from those sums and the entries: a
+// wave to a row, rows beyond the grid in turn, and the workgroup's part of the mean.
+template <class E, bool TAIL>
+__global__ __launch_bounds__(256) void distill_rows_kernel(DistillParams p) {
+    constexpr int Q = DISTILL_MAX_K / 64;  // entries of a lane
+    __shared__ double part_s[2][4];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const float c = kLog2e / p.temperature;
+    const double T = p.temperature;
+    double part = 0., parts = 0.;
+    for (long long r = (long long)blockIdx.x * 4 + wv; r < p.rows; r += (long long)gridDim.x * 4) {
+        const float weight = row_weight(p, r);
+        DistillRow* keep = reinterpret_cast<DistillRow*>(p.kept) + r;
+        if (weight == 0.f) {
+            if (lane == 0) {
                 keep->weight = 0.f;
                 keep->loss = 0.f;
             }
             continue;
         }
-        if (TAIL) {
-            row_sync<NT>();
-            for (int i = tid; i < p.words; i += NT) bits[i] = 0;
-            row_sync<NT>();
-            for (int i = tid; i < p.k; i += NT)
-                if (counts(ids[i], t[i], p.V)) atomicOr(&bits[ids[i] >> 5], 1u << (ids[i] & 31));
-            row_sync<NT>();
-        }
-        const auto entry_bits = [&](int col) { return TAIL ? bits[col >> 5] >> (col & 31) : 0u; };
-        const int nvec = p.V / N, tail = p.V - nvec * N;
-        Sum a = {kLowest, 0.f};
-        float best = -INFINITY;
-        const float last = tid < tail && !(entry_bits(nvec * N + tid) & 1) ? (float)x[nvec * N + tid] : -INFINITY;
-        for (int v0 = 0; v0 < nvec; v0 += NT * DS_NV) {
-            typename RowVec<E>::type v[DS_NV];
+        const E* x = static_cast<const E*>(row_at(p, r, sizeof(E)));
+        const Sum a = {keep->rm, keep->rls};
+        int id[Q];  // -1: none
+        float t[Q], e[Q];
+        float tmax = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < DS_NV; j++) v[j] = load_row(x + (size_t)min(v0 + j * NT + tid, nvec - 1) * N);
-            float e[DS_NV][N];
-#pragma unroll
-            for (int j = 0; j < DS_NV; j++) {
-                const int i = v0 + j * NT + tid;
-                const uint32_t skip = TAIL && i < nvec ? entry_bits(i * N) : 0;
-#pragma unroll
-                for (int k = 0; k < N; k++) {
-                    e[j][k] = i < nvec && !(TAIL && (skip >> k & 1)) ? (float)v[j][k] : -INFINITY;
-                    best = fmaxf(best, e[j][k]);
+        for (int q = 0; q < Q; q++) {
+            const int i = q * 64 + lane;
+            id[q] = -1;
+            t[q] = e[q] = 0.f;
+            if (i < p.k) {
+                const long long at = p.ids[r * p.k + i];
+                t[q] = p.values[r * p.k + i];
+                if (counts(at, t[q], p.V)) {
+                    id[q] = (int)at;
+                    e[q] = wide(x[at]);
+                    tmax = fmaxf(tmax, t[q]);
                 }
             }
-            rescale(a, fmaxf(a.m, best), c);
-#pragma unroll
-            for (int j = 0; j < DS_NV; j++)
-#pragma unroll
-                for (int k = 0; k < N; k++) a.s += fast_exp2((e[j][k] - a.m) * c);
         }
-        rescale(a, fmaxf(a.m, fmaxf(best, last)), c);
-        a.s += fast_exp2((last - a.m) * c);
-        const float m = wave_max(a.m);
-        rescale(a, m, c);
-        a.s = wave_sum(a.s);
-        if (W > 1) {
-            if (lane == 0) red[sub][wv] = a;
-            __syncthreads();
-            a = red[sub][0];
-#pragma unroll 3
-            for (int w = 1; w < W; w++) join(a, red[sub][w], c);
-        }
-        if (wv == 0) {
-            // The entries, a lane each: the student's logits there, the teacher's masses.
+        Sum all = a;
+        if (TAIL) {  // the entries' columns, each once
+            bool again[Q] = {};
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+                for (int j = 0; j < min(64, p.k - q * 64); j++) {
+                    const int other = __builtin_amdgcn_readlane(id[q], j);
+#pragma unroll
+                    for (int o = 0; o < Q; o++) again[o] |= other == id[o] && q * 64 + j < o * 64 + lane;
+                }
             Sum b = {kLowest, 0.f};
-            float tmax = -INFINITY;
-            for (int i = lane; i < p.k; i += 64)
-                if (counts(ids[i], t[i], p.V)) {
-                    tmax = fmaxf(tmax, t[i]);
-                    if (TAIL) {  // (a column counts once)
-                        bool first = true;
-                        for (int j = 0; j < i; j++) first &= ids[j] != ids[i] || t[j] == -INFINITY;
-                        if (first) {
-                            const float e = (float)x[ids[i]];
-                            const float bm = fmaxf(b.m, e);
-                            rescale(b, bm, c);
-                            b.s += fast_exp2((e - b.m) * c);
-                        }
-                    }
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+                if (id[q] >= 0 && !again[q]) {
+                    rescale(b, fmaxf(b.m, e[q]), c);
+                    b.s += fast_exp2((e[q] - b.m) * c);
                 }
-            Sum all = a;
-            if (TAIL) {
-                const float bm = wave_max(b.m);
-                rescale(b, bm, c);
-                b.s = wave_sum(b.s);
-                join(all, b, c);
-            }
-            const float ls = log2f(all.s), rls = log2f(a.s);
-            tmax = wave_max(tmax);
-            const double T = p.temperature;
-            double mass = 0.;
-            for (int i = lane; i < p.k; i += 64)
-                if (counts(ids[i], t[i], p.V)) mass += exp(TAIL ? (double)t[i] : ((double)t[i] - tmax) / T);
-            mass = wave_sum(mass);
-            const double lognorm = TAIL ? 0. : (double)tmax / T + log(mass);
-            double loss = 0.;
-            for (int i = lane; i < p.k; i += 64)
-                if (counts(ids[i], t[i], p.V)) {
-                    const double lp = (double)t[i] / T - lognorm;
-                    const float lq = ((float)x[ids[i]] - all.m) / p.temperature - kLn2 * ls;
-                    loss += exp(lp) * (lp - (double)lq);
-                }
-            loss = wave_sum(loss);
-            DistillRow row;
-            row.m = all.m;
-            row.ls = ls;
-            row.rm = a.s == 0.f ? 0.f : a.m;  // (no column of no entry but -inf: a softmax of zeros)
-            row.rls = a.s == 0.f ? 0.f : rls;
-            row.rest = row.entry = 1.f;
-            row.norm = (float)(lognorm * 1.4426950408889634);
-            row.weight = weight;
-            row.pad = 0.f;
-            if (TAIL) {
-                // the rest, where the student has any
-                const double pr = a.s > 0.f ? fmax(0., 1. - mass) : 0.;
-                const double lqr = (double)(a.m - all.m) + (double)kLn2 * ((double)rls - (double)ls);
-                if (pr > 0.) loss += pr * (log(pr) - lqr);
-                row.entry = (float)(mass + pr);
-                row.rest = (float)(exp(lqr) * (mass + pr) - pr);
-            }
-            row.loss = (float)loss;
-            if (lane == 0) *keep = row;
+            const float bm = wave_max(b.m);
+            rescale(b, bm, c);
+            b.s = wave_sum(b.s);
+            join(all, b, c);
         }
-        if (W > 1) __syncthreads();  // the shared arrays are free for the next row
+        const float ls = log2f(all.s), rls = log2f(a.s);
+        tmax = wave_max(tmax);
+        double p_[Q], mass = 0.;
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            p_[q] = id[q] >= 0 ? exp(TAIL ? (double)t[q] : ((double)t[q] - tmax) / T) : 0.;
+            mass += p_[q];
+        }
+        mass = wave_sum(mass);
+        const double lognorm = TAIL ? 0. : (double)tmax / T + log(mass), scale = TAIL ? 1. : 1. / mass;
+        double loss = 0.;
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+            if (id[q] >= 0 && p_[q] != 0.) {
+                const float lq = (e[q] - all.m) / p.temperature - kLn2 * ls;
+                loss += p_[q] * scale * (((double)t[q] / T - lognorm) - (double)lq);
+            }
+        loss = wave_sum(loss);
+        DistillRow row;
+        row.m = all.m;
+        row.ls = ls;
+        row.rm = a.s == 0.f ? 0.f : a.m;  // (no column of no entry but -inf: a softmax of zeros)
+        row.rls = a.s == 0.f ? 0.f : rls;
+        row.rest = row.entry = 1.f;
+        row.norm = (float)(lognorm * 1.4426950408889634);
+        row.weight = weight;
+        row.pad = 0.f;
+        if (TAIL) {
+            // the rest, where the student has any
+            const double pr = a.s > 0.f ? fmax(0., 1. - mass) : 0.;
+            const double lqr = (double)(a.m - all.m) + (double)kLn2 * ((double)rls - (double)ls);
+            if (pr > 0.) loss += pr * (log(pr) - lqr);
+            row.entry = (float)(mass + pr);
+            row.rest = (float)(exp(lqr) * (mass + pr) - pr);
+        }
+        row.loss = (float)loss;
+        if (lane == 0) *keep = row;
+        part += (double)weight * (double)row.loss;
+        parts += (double)weight;
+    }
+    if (lane == 0) {
+        part_s[0][wv] = part;
+        part_s[1][wv] = parts;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const double* s = part_s[threadIdx.x];
+        p.parts[2 * blockIdx.x + threadIdx.x] = ((s[0] + s[1]) + s[2]) + s[3];
     }
 }
 
-// The weighted mean over the rows, one workgroup, in double and in a fixed order.
-__global__ __launch_bounds__(1024) void distill_mean_kernel(DistillParams p) {
-    __shared__ double sums[2][16];
-    constexpr int U = 8;
-    double s = 0., n = 0.;
-    const DistillRow* row = reinterpret_cast<const DistillRow*>(p.kept);
-    for (long long r0 = threadIdx.x; r0 < p.rows; r0 += 1024 * U) {
-        float w[U], l[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const long long r = min(r0 + 1024 * u, p.rows - 1);
-            w[u] = row[r].weight;
-            l[u] = row[r].loss;
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            if (r0 + 1024 * u < p.rows && w[u] != 0.f) {
-                s += (double)w[u] * (double)l[u];
-                n += (double)w[u];
-            }
-    }
-    s = wave_sum(s);
-    n = wave_sum(n);
+// The weighted mean over the rows from the workgroups' parts, in a fixed order.
+__global__ __launch_bounds__(DISTILL_PARTS) void distill_mean_kernel(DistillParams p, int parts) {
+    __shared__ double sums[2][DISTILL_PARTS / 64];
+    const bool is = (int)threadIdx.x < parts;
+    const double s = wave_sum(is ? p.parts[2 * threadIdx.x] : 0.), n = wave_sum(is ? p.parts[2 * threadIdx.x + 1] : 0.);
     if ((threadIdx.x & 63) == 0) {
         sums[0][threadIdx.x >> 6] = s;
         sums[1][threadIdx.x >> 6] = n;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-        s = n = 0.;
-        for (int w = 0; w < 16; w++) {
+        double s = 0., n = 0.;
+        for (int w = 0; w < DISTILL_PARTS / 64; w++) {
             s += sums[0][w];
             n += sums[1][w];
         }
@@ -243,8 +286,10 @@ __global__ __launch_bounds__(1024) void distill_mean_kernel(DistillParams p) {
 
 // The gradient of the columns [c0, c1) of a row by NT threads: blockIdx.y's
 // share of the row, whole vectors. The entries' columns are stored a second
-// time, by one thread each.
-template <class E, int NT>
+// time, by one thread each. The rows are taken from the last to the first: those
+// that the forward read last are in the caches still; a large gradient in whole
+// lines goes past them (STREAM).
+template <class E, int NT, bool STREAM>
 __global__ __launch_bounds__(256) void distill_grad_kernel(DistillParams p, int share) {
     constexpr int N = RowVec<E>::N, RW = 256 / NT;
     const int tid = threadIdx.x % NT;
@@ -253,7 +298,7 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillParams p, int 
     const float c = kLog2e / p.temperature;
     for (long long i = (long long)blockIdx.x * RW + threadIdx.x / NT; i < p.rows; i += (long long)gridDim.x * RW) {
         const long long r = p.rows - 1 - i;
-        const E* x = static_cast<const E*>(p.x) + (r / p.inner) * p.outer_stride + (r % p.inner) * p.row_stride + c0;
+        const E* x = static_cast<const E*>(row_at(p, r, sizeof(E))) + c0;
         E* dx = static_cast<E*>(p.dx) + r * p.V + c0;
         const DistillRow* keep = reinterpret_cast<const DistillRow*>(p.kept) + r;
         const float weight = keep->weight;
@@ -262,7 +307,7 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillParams p, int 
         if (g == 0.f) {
 #pragma unroll
             for (int k = 0; k < N; k++) o[k] = (E)0.f;
-            for (int j = tid; j < nvec; j += NT) store_row(dx + (size_t)j * N, o);
+            for (int j = tid; j < nvec; j += NT) store_row<E, STREAM>(dx + (size_t)j * N, o);
             if (tid < tail) dx[nvec * N + tid] = (E)0.f;
             continue;
         }
@@ -278,12 +323,12 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillParams p, int 
                 const int at = i0 + j * NT + tid;
                 if (at < nvec) {
 #pragma unroll
-                    for (int k = 0; k < N; k++) o[k] = (E)grad((float)v[j][k]);
-                    store_row(dx + (size_t)at * N, o);
+                    for (int k = 0; k < N; k++) o[k] = (E)grad(wide(v[j][k]));
+                    store_row<E, STREAM>(dx + (size_t)at * N, o);
                 }
             }
         }
-        if (tid < tail) dx[nvec * N + tid] = (E)grad((float)x[nvec * N + tid]);
+        if (tid < tail) dx[nvec * N + tid] = (E)grad(wide(x[nvec * N + tid]));
         row_sync<NT>();  // the entries' columns are written again
         const long long* ids = p.ids + r * p.k;
         const float* t = p.values + r * p.k;
@@ -298,7 +343,7 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillParams p, int 
                         sum += fast_exp2(t[l] * c - row.norm);
                     }
             if (first) {
-                const float q = fast_exp2(((float)x[id - c0] - row.m) * c - row.ls);
+                const float q = fast_exp2((wide(x[id - c0]) - row.m) * c - row.ls);
                 dx[id - c0] = (E)(g * (q * row.entry - sum));
             }
         }
@@ -307,14 +352,23 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillParams p, int 
 }
 
 template <class E, int NT>
-void launch_rows(DistillParams p, hipStream_t stream) {
-    const dim3 grid((unsigned)min((p.rows + rows_of(NT) - 1) / rows_of(NT), (long long)LOGPROBS_MAX_GRID)), block(NT * rows_of(NT));
-    if (p.tail) {
-        p.words = (p.V + 31) / 32;
-        hipLaunchKernelGGL((distill_kernel<E, NT, true>), grid, block, (size_t)p.words * 4 * rows_of(NT), stream, p);
-    } else {
-        hipLaunchKernelGGL((distill_kernel<E, NT, false>), grid, block, 0, stream, p);
+void launch_sums(DistillParams p, hipStream_t stream) {
+    constexpr int RW = rows_of(NT);
+    p.words = (p.V + 31) / 32;
+    for (p.first = 0; p.first < p.rows; p.first += (long long)LOGPROBS_MAX_GRID * RW) {
+        const dim3 grid((unsigned)min((p.rows - p.first + RW - 1) / RW, (long long)LOGPROBS_MAX_GRID)), block(NT * RW);
+        if (p.tail)
+            hipLaunchKernelGGL((distill_sums_kernel<E, NT, true>), grid, block, (size_t)p.words * 4 * RW, stream, p);
+        else
+            hipLaunchKernelGGL((distill_sums_kernel<E, NT, false>), grid, block, 0, stream, p);
     }
+}
+
+// Whether the gradient goes past the caches: 128 MiB or more, in rows of whole
+// 128-byte lines.
+template <class E>
+bool past_caches(const DistillParams& p) {
+    return p.V * sizeof(E) % 128 == 0 && (uintptr_t)p.dx % 128 == 0 && (size_t)p.rows * p.V * sizeof(E) >= (size_t)128 << 20;
 }
 
 template <class E, int NT>
@@ -322,8 +376,14 @@ void launch_grad(const DistillParams& p, int shares, hipStream_t stream) {
     constexpr int N = RowVec<E>::N, RW = 256 / NT;
     const int share = ((p.V + shares - 1) / shares + N - 1) / N * N;
     const dim3 grid((unsigned)min((p.rows + RW - 1) / RW, (long long)LOGPROBS_MAX_GRID), (unsigned)((p.V + share - 1) / share));
-    hipLaunchKernelGGL((distill_grad_kernel<E, NT>), grid, dim3(256), 0, stream, p, share);
+    if (past_caches<E>(p))
+        hipLaunchKernelGGL((distill_grad_kernel<E, NT, true>), grid, dim3(256), 0, stream, p, share);
+    else
+        hipLaunchKernelGGL((distill_grad_kernel<E, NT, false>), grid, dim3(256), 0, stream, p, share);
 }
+
+// Workgroups that the rows' losses are formed by.
+int parts_of(long long rows) { return (int)min((rows + 3) / 4, (long long)DISTILL_PARTS); }
 
 template <class E>
 void launch(const DistillParams& p, bool grad, hipStream_t stream) {
@@ -334,11 +394,14 @@ void launch(const DistillParams& p, bool grad, hipStream_t stream) {
             launch_grad<E, 64>(p, 1, stream);
         else  // few rows shared out to about four workgroups of a compute unit
             launch_grad<E, 256>(p, (int)min((1024 + p.rows - 1) / p.rows, (long long)(p.V + 256 * N - 1) / (256 * N)), stream);
-    } else if (narrow) {
-        launch_rows<E, 64>(p, stream);
-    } else {
-        launch_rows<E, 256>(p, stream);
+        return;
     }
+    narrow ? launch_sums<E, 64>(p, stream) : launch_sums<E, 256>(p, stream);
+    const dim3 grid((unsigned)parts_of(p.rows));
+    if (p.tail)
+        hipLaunchKernelGGL((distill_rows_kernel<E, true>), grid, dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL((distill_rows_kernel<E, false>), grid, dim3(256), 0, stream, p);
 }
 
 }  // namespace
@@ -352,7 +415,7 @@ void launch_distill(const DistillParams& p, int dtype, bool grad, hipStream_t st
         else
             launch<f16_t>(p, grad, stream);
     }
-    if (!grad) hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, stream, p);
+    if (!grad) hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(DISTILL_PARTS), 0, stream, p, parts_of(p.rows));
 }
 
 }  // namespace cyfa

@@ -33,4 +33,12 @@ __device__ __forceinline__ void store_row(E* p, const typename RowVec<E>::type& 
         __builtin_memcpy(p, &v, 16);
 }
 
+// An element in fp32. (Of a bf16 by its bits: the compiler takes the largest of
+// converted bf16 as a bf16, with a rounding and another conversion for each.)
+__device__ __forceinline__ float wide(float x) { return x; }
+__device__ __forceinline__ float wide(f16_t x) { return (float)x; }
+__device__ __forceinline__ float wide(bf16_t x) {
+    return __builtin_bit_cast(float, (uint32_t)__builtin_bit_cast(uint16_t, x) << 16);
+}
+
 }  // namespace cyfa

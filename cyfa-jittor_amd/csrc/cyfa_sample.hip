@@ -120,14 +120,6 @@ __device__ __forceinline__ float kth_largest(float x, float y, int k) {
     return -wave_max(fmaxf(ra < k ? -x : -INFINITY, rb < k ? -y : -INFINITY));
 }
 
-// An element in fp32. (Of a bf16 by its bits: the compiler takes the largest of
-// converted bf16 as a bf16, with a rounding and another conversion for each.)
-__device__ __forceinline__ float wide(float x) { return x; }
-__device__ __forceinline__ float wide(f16_t x) { return (float)x; }
-__device__ __forceinline__ float wide(bf16_t x) {
-    return __builtin_bit_cast(float, (uint32_t)__builtin_bit_cast(uint16_t, x) << 16);
-}
-
 // A row's settings.
 struct Choice {
     double m;       // the maximum

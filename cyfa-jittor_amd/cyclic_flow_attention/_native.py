@@ -238,7 +238,7 @@ class CyfaDistillArgs(ctypes.Structure):
         ("rows", ctypes.c_longlong), ("inner", ctypes.c_longlong), ("outer_stride", ctypes.c_longlong),
         ("row_stride", ctypes.c_longlong), ("V", _c_int), ("x", _c_void_p), ("k", _c_int), ("ids", _c_void_p),
         ("values", _c_void_p), ("weights", _c_void_p), ("temperature", _c_float), ("tail", _c_int), ("kept", _c_void_p),
-        ("loss", _c_void_p), ("total", _c_void_p), ("d_loss", _c_void_p), ("dx", _c_void_p),
+        ("loss", _c_void_p), ("total", _c_void_p), ("parts", _c_void_p), ("d_loss", _c_void_p), ("dx", _c_void_p),
     ]
 
 
@@ -1166,8 +1166,9 @@ def residual_norm_grad(x, y, weight, post, gate, scale, eps, stats, d_s, d_h, ne
 
 # The largest sizes of the operators on a model's logits (CYFA_ADJUST_MAX_TOKENS,
 # CYFA_DISTILL_MAX_K): token biases of a row; tokens of a teacher; the vocabulary
-# beside a teacher's tail. Floats a row that distill_loss keeps for its gradient.
-ADJUST_MAX_TOKENS, DISTILL_MAX_K, DISTILL_MAX_TAIL_V, DISTILL_ROW_FLOATS = 1024, 256, 1 << 19, 10
+# beside a teacher's tail. Floats a row that distill_loss keeps for its gradient;
+# parts of its mean.
+ADJUST_MAX_TOKENS, DISTILL_MAX_K, DISTILL_MAX_TAIL_V, DISTILL_ROW_FLOATS, DISTILL_PARTS = 1024, 256, 1 << 19, 10, 1024
 
 
 def leading_strides(t):
@@ -1278,11 +1279,12 @@ def distill_loss(logits, ids, values, weights, temperature, tail):
     fields, logits = logit_rows(logits)
     rows = fields[0]
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    kept = torch.empty(rows * DISTILL_ROW_FLOATS + 1, dtype=torch.float32, device=dev)
+    kept = torch.empty(rows * DISTILL_ROW_FLOATS + 2, dtype=torch.float32, device=dev)
+    parts = torch.empty(2 * DISTILL_PARTS, dtype=torch.float64, device=dev)  # alive until the launch
     at = kept.data_ptr()
     args = CyfaDistillArgs(*fields, k=ids.shape[-1], ids=ids.data_ptr(), values=values.data_ptr(), weights=ptr(weights),
                            temperature=temperature, tail=tail, kept=at, loss=loss.data_ptr(),
-                           total=at + 4 * rows * DISTILL_ROW_FLOATS)
+                           total=at + 4 * rows * DISTILL_ROW_FLOATS, parts=parts.data_ptr())
     _lm_call("cyfa_distill_loss", args, logits.dtype, 0, dev)
     return loss, kept
 

@@ -767,12 +767,14 @@ typedef struct CyfaDistillArgs {
     float *kept;                  /* [rows, CYFA_DISTILL_ROW_FLOATS] */
     float *loss;                  /* grad 0: [1] */
     float *total;                 /* [1] */
+    double *parts;                /* grad 0: [CYFA_DISTILL_PARTS, 2], scratch */
     const float *d_loss;          /* grad 1: [1] */
     void *dx;                     /* grad 1: [rows, V] */
 } CyfaDistillArgs;
 
 #define CYFA_DISTILL_MAX_K 256
 #define CYFA_DISTILL_ROW_FLOATS 10
+#define CYFA_DISTILL_PARTS 1024
 int cyfa_distill_loss(const CyfaDistillArgs *args, int dtype, int grad, void *hip_stream);
 
 /* Thread-local message of the last failing call (never NULL). No reference

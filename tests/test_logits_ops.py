@@ -70,7 +70,7 @@ def test_sample_validates_before_launch():
 def test_distill_validates_before_launch():
     call = _caller("cyfa_distill_loss", _native.CyfaDistillArgs, dict(
         rows=4, inner=4, row_stride=100, V=100, x=0x10000, k=5, ids=0x20000, values=0x30000, temperature=1.0, kept=0x40000,
-        loss=0x50000, total=0x60000, d_loss=0x70000, dx=0x80000))
+        loss=0x50000, total=0x60000, parts=0x90000, d_loss=0x70000, dx=0x80000))
     for grad in (0, 1):
         assert call(grad, dtype=3) == call(grad, V=0) == call(grad, rows=-1) == call(grad, inner=0) == call(grad, k=0) == VALUE
         assert call(grad, temperature=0.0) == call(grad, temperature=NAN) == call(grad, temperature=INF) == VALUE
@@ -78,6 +78,7 @@ def test_distill_validates_before_launch():
         assert call(grad, k=_native.DISTILL_MAX_K + 1) == call(grad, V=(1 << 28) + 1) == UNSUPPORTED
         assert call(grad, tail=1, V=_native.DISTILL_MAX_TAIL_V + 1) == UNSUPPORTED
         assert call(grad, x=0x10001) == call(grad, ids=0x20004) == call(grad, values=0x30002) == ALIGN
+    assert call(0, parts=0x90004) == ALIGN and call(0, parts=None) == VALUE
     assert call(0, loss=None) == call(1, d_loss=None) == call(1, dx=None) == call(0, kept=None) == VALUE
     assert call(1, rows=0) == _native.CYFA_OK
     assert _native.load_library().cyfa_distill_loss(None, 0, 0, None) == VALUE
