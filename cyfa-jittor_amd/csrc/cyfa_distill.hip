@@ -152,29 +152,21 @@ __global__ __launch_bounds__(NT * rows_of(NT)) void distill_sums_kernel(DistillP
 
 // The rows' losses and what the gradient needs, from those sums and the entries: a
 // wave to a row, rows beyond the grid in turn, and the workgroup's part of the mean.
-template <class E, bool TAIL>
+template <class E, bool TAIL, int Q>  // Q: most entries of a lane
 __global__ __launch_bounds__(256) void distill_rows_kernel(DistillParams p) {
-    constexpr int Q = DISTILL_MAX_K / 64;  // entries of a lane
     __shared__ double part_s[2][4];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const float c = kLog2e / p.temperature;
     const double T = p.temperature;
     double part = 0., parts = 0.;
     for (long long r = (long long)blockIdx.x * 4 + wv; r < p.rows; r += (long long)gridDim.x * 4) {
-        const float weight = row_weight(p, r);
-        DistillRow* keep = reinterpret_cast<DistillRow*>(p.kept) + r;
-        if (weight == 0.f) {
-            if (lane == 0) {
-                keep->weight = 0.f;
-                keep->loss = 0.f;
-            }
-            continue;
-        }
         const E* x = static_cast<const E*>(row_at(p, r, sizeof(E)));
-        const Sum a = {keep->rm, keep->rls};
+        DistillRow* keep = reinterpret_cast<DistillRow*>(p.kept) + r;
+        const Sum a = {keep->rm, keep->rls};  // (nothing yet in rows that do not count)
         int id[Q];  // -1: none
         float t[Q], e[Q];
         float tmax = -INFINITY;
+        bool any = false;
 #pragma unroll
         for (int q = 0; q < Q; q++) {
             const int i = q * 64 + lane;
@@ -187,8 +179,17 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillParams p) {
                     id[q] = (int)at;
                     e[q] = wide(x[at]);
                     tmax = fmaxf(tmax, t[q]);
+                    any = true;
                 }
             }
+        }
+        const float weight = __any(any) ? (p.weights ? p.weights[r] : 1.f) : 0.f;
+        if (weight == 0.f) {
+            if (lane == 0) {
+                keep->weight = 0.f;
+                keep->loss = 0.f;
+            }
+            continue;
         }
         Sum all = a;
         if (TAIL) {  // the entries' columns, each once
@@ -214,14 +215,15 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillParams p) {
         }
         const float ls = log2f(all.s), rls = log2f(a.s);
         tmax = wave_max(tmax);
+        // masses (TAIL: in double, since 1 - their sum cancels) over their norm
         double p_[Q], mass = 0.;
 #pragma unroll
         for (int q = 0; q < Q; q++) {
-            p_[q] = id[q] >= 0 ? exp(TAIL ? (double)t[q] : ((double)t[q] - tmax) / T) : 0.;
+            p_[q] = id[q] < 0 ? 0. : TAIL ? exp((double)t[q]) : (double)fast_exp2((t[q] - tmax) * c);
             mass += p_[q];
         }
         mass = wave_sum(mass);
-        const double lognorm = TAIL ? 0. : (double)tmax / T + log(mass), scale = TAIL ? 1. : 1. / mass;
+        const double lognorm = TAIL ? 0. : (double)tmax / T + (double)logf((float)mass), scale = TAIL ? 1. : 1. / mass;
         double loss = 0.;
 #pragma unroll
         for (int q = 0; q < Q; q++)
@@ -264,18 +266,27 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillParams p) {
 }
 
 // The weighted mean over the rows from the workgroups' parts, in a fixed order.
-__global__ __launch_bounds__(DISTILL_PARTS) void distill_mean_kernel(DistillParams p, int parts) {
-    __shared__ double sums[2][DISTILL_PARTS / 64];
-    const bool is = (int)threadIdx.x < parts;
-    const double s = wave_sum(is ? p.parts[2 * threadIdx.x] : 0.), n = wave_sum(is ? p.parts[2 * threadIdx.x + 1] : 0.);
+__global__ __launch_bounds__(1024) void distill_mean_kernel(DistillParams p, int parts) {
+    __shared__ double sums[2][16];
+    double s = 0., n = 0.;
+#pragma unroll
+    for (int i = 0; i < DISTILL_PARTS / 1024; i++) {
+        const int at = i * 1024 + threadIdx.x;
+        if (at < parts) {
+            s += p.parts[2 * at];
+            n += p.parts[2 * at + 1];
+        }
+    }
+    s = wave_sum(s);
+    n = wave_sum(n);
     if ((threadIdx.x & 63) == 0) {
         sums[0][threadIdx.x >> 6] = s;
         sums[1][threadIdx.x >> 6] = n;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-        double s = 0., n = 0.;
-        for (int w = 0; w < DISTILL_PARTS / 64; w++) {
+        s = n = 0.;
+        for (int w = 0; w < 16; w++) {
             s += sums[0][w];
             n += sums[1][w];
         }
@@ -286,23 +297,27 @@ __global__ __launch_bounds__(DISTILL_PARTS) void distill_mean_kernel(DistillPara
 
 // The gradient of the columns [c0, c1) of a row by NT threads: blockIdx.y's
 // share of the row, whole vectors. The entries' columns are stored a second
-// time, by one thread each. The rows are taken from the last to the first: those
-// that the forward read last are in the caches still; a large gradient in whole
-// lines goes past them (STREAM).
+// time, by one thread each. (Vectors that look for the entries among theirs
+// instead took 345 us for 347 with 20 of them, and 65 for 34 with 64.) The rows
+// are taken from the last to the first: those that the forward read last are in
+// the caches still; a large gradient in whole lines goes past them (STREAM).
 template <class E, int NT, bool STREAM>
 __global__ __launch_bounds__(256) void distill_grad_kernel(DistillParams p, int share) {
     constexpr int N = RowVec<E>::N, RW = 256 / NT;
-    const int tid = threadIdx.x % NT;
+    __shared__ int id_s[RW][DISTILL_MAX_K];  // column in the share; -1: none
+    __shared__ float mass_s[RW][DISTILL_MAX_K];
+    const int tid = threadIdx.x % NT, sub = threadIdx.x / NT;
+    int* const id = id_s[sub];
+    float* const mass = mass_s[sub];
     const int c0 = blockIdx.y * share, c1 = min(c0 + share, p.V);
     const int nvec = (c1 - c0) / N, tail = c1 - c0 - nvec * N;
     const float c = kLog2e / p.temperature;
-    for (long long i = (long long)blockIdx.x * RW + threadIdx.x / NT; i < p.rows; i += (long long)gridDim.x * RW) {
+    for (long long i = (long long)blockIdx.x * RW + sub; i < p.rows; i += (long long)gridDim.x * RW) {
         const long long r = p.rows - 1 - i;
         const E* x = static_cast<const E*>(row_at(p, r, sizeof(E))) + c0;
         E* dx = static_cast<E*>(p.dx) + r * p.V + c0;
-        const DistillRow* keep = reinterpret_cast<const DistillRow*>(p.kept) + r;
-        const float weight = keep->weight;
-        const float g = weight == 0.f ? 0.f : *p.d_loss * weight / *p.total / p.temperature;
+        const DistillRow row = reinterpret_cast<const DistillRow*>(p.kept)[r];
+        const float g = row.weight == 0.f ? 0.f : *p.d_loss * row.weight / *p.total / p.temperature;
         typename RowVec<E>::type o;
         if (g == 0.f) {
 #pragma unroll
@@ -311,7 +326,12 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillParams p, int 
             if (tid < tail) dx[nvec * N + tid] = (E)0.f;
             continue;
         }
-        const DistillRow row = *keep;
+        for (int j = tid; j < p.k; j += NT) {
+            const long long at = p.ids[r * p.k + j];
+            const float t = p.values[r * p.k + j];
+            id[j] = at >= c0 && at < c1 && t != -INFINITY ? (int)at - c0 : -1;
+            mass[j] = fast_exp2(t * c - row.norm);
+        }
         const float a = g * row.rest;
         const auto grad = [&](float e) { return a * fast_exp2((e - row.rm) * c - row.rls); };
         for (int i0 = 0; i0 < nvec; i0 += NT * DS_NV) {
@@ -329,23 +349,18 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillParams p, int 
             }
         }
         if (tid < tail) dx[nvec * N + tid] = (E)grad(wide(x[nvec * N + tid]));
-        row_sync<NT>();  // the entries' columns are written again
-        const long long* ids = p.ids + r * p.k;
-        const float* t = p.values + r * p.k;
+        row_sync<NT>();  // the entries' columns are written again, by the first entry of each
         for (int j = tid; j < p.k; j += NT) {
-            const long long id = ids[j];
-            bool first = id >= c0 && id < c1 && t[j] != -INFINITY;
+            const int at = id[j];
+            if (at < 0) continue;
+            bool first = true;
             float sum = 0.f;
-            if (first)
-                for (int l = 0; l < p.k; l++)
-                    if (ids[l] == id && t[l] != -INFINITY) {
-                        if (l < j) first = false;
-                        sum += fast_exp2(t[l] * c - row.norm);
-                    }
-            if (first) {
-                const float q = fast_exp2((wide(x[id - c0]) - row.m) * c - row.ls);
-                dx[id - c0] = (E)(g * (q * row.entry - sum));
-            }
+            for (int l = 0; l < p.k; l++)
+                if (id[l] == at) {
+                    if (l < j) first = false;
+                    sum += mass[l];
+                }
+            if (first) dx[at] = (E)(g * (fast_exp2((wide(x[at]) - row.m) * c - row.ls) * row.entry - sum));
         }
         row_sync<NT>();
     }
@@ -398,10 +413,11 @@ void launch(const DistillParams& p, bool grad, hipStream_t stream) {
     }
     narrow ? launch_sums<E, 64>(p, stream) : launch_sums<E, 256>(p, stream);
     const dim3 grid((unsigned)parts_of(p.rows));
-    if (p.tail)
-        hipLaunchKernelGGL((distill_rows_kernel<E, true>), grid, dim3(256), 0, stream, p);
+    const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, p); };
+    if (p.k <= 64)
+        p.tail ? run(distill_rows_kernel<E, true, 1>) : run(distill_rows_kernel<E, false, 1>);
     else
-        hipLaunchKernelGGL((distill_rows_kernel<E, false>), grid, dim3(256), 0, stream, p);
+        p.tail ? run(distill_rows_kernel<E, true, DISTILL_MAX_K / 64>) : run(distill_rows_kernel<E, false, DISTILL_MAX_K / 64>);
 }
 
 }  // namespace
@@ -415,7 +431,7 @@ void launch_distill(const DistillParams& p, int dtype, bool grad, hipStream_t st
         else
             launch<f16_t>(p, grad, stream);
     }
-    if (!grad) hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(DISTILL_PARTS), 0, stream, p, parts_of(p.rows));
+    if (!grad) hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, stream, p, parts_of(p.rows));
 }
 
 }  // namespace cyfa

@@ -692,7 +692,7 @@ struct DistillParams {
     int words;                   // set by the launcher
     long long first;             // row of a launch's first workgroup, set by the launcher
 };
-constexpr int DISTILL_PARTS = 1024;
+constexpr int DISTILL_PARTS = 4096;
 constexpr int DISTILL_ROW_FLOATS = 10, DISTILL_MAX_K = 256;
 constexpr int DISTILL_MAX_TAIL_V = 1 << 19;  // a bit a column in 64 KiB of LDS
 void launch_distill(const DistillParams& p, int dtype, bool grad, hipStream_t stream);

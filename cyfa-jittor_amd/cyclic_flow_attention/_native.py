@@ -1168,7 +1168,7 @@ def residual_norm_grad(x, y, weight, post, gate, scale, eps, stats, d_s, d_h, ne
 # CYFA_DISTILL_MAX_K): token biases of a row; tokens of a teacher; the vocabulary
 # beside a teacher's tail. Floats a row that distill_loss keeps for its gradient;
 # parts of its mean.
-ADJUST_MAX_TOKENS, DISTILL_MAX_K, DISTILL_MAX_TAIL_V, DISTILL_ROW_FLOATS, DISTILL_PARTS = 1024, 256, 1 << 19, 10, 1024
+ADJUST_MAX_TOKENS, DISTILL_MAX_K, DISTILL_MAX_TAIL_V, DISTILL_ROW_FLOATS, DISTILL_PARTS = 1024, 256, 1 << 19, 10, 4096
 
 
 def leading_strides(t):

@@ -774,7 +774,7 @@ typedef struct CyfaDistillArgs {
 
 #define CYFA_DISTILL_MAX_K 256
 #define CYFA_DISTILL_ROW_FLOATS 10
-#define CYFA_DISTILL_PARTS 1024
+#define CYFA_DISTILL_PARTS 4096
 int cyfa_distill_loss(const CyfaDistillArgs *args, int dtype, int grad, void *hip_stream);
 
 /* Thread-local message of the last failing call (never NULL). No reference
