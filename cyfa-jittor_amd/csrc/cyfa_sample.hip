@@ -39,6 +39,7 @@ typedef unsigned long long u64;
 
 constexpr double kLog2eD = 1.4426950408889634;
 constexpr int SM_FEW = 512;   // elements ranked each against each, by eight threads each
+constexpr int SM_PIECE = 4;  // elements of a row's piece
 constexpr int SM_TOP = 128;   // largest top_k that one wave handles
 
 __device__ __forceinline__ uint32_t value_key(float x) {
@@ -251,7 +252,7 @@ __device__ __forceinline__ PartStats join_parts(const SampleParams& p, long long
 // The counts and masses of a part's bins.
 template <class E>
 __global__ __launch_bounds__(256) void sample_bins_kernel(SampleParams p) {
-    constexpr int N = RowVec<E>::N, P = N / 2;
+    constexpr int P = SM_PIECE;
     typedef E Piece __attribute__((ext_vector_type(P)));
     __shared__ u64 mass_s[SM_BINS];
     __shared__ unsigned count_s[SM_BINS];
@@ -277,7 +278,7 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(SampleParams p) {
 #pragma unroll 1
     for (int i = tid; i < npiece; i += 256) {
         Piece v;
-        __builtin_memcpy(&v, x + (size_t)i * P, 8);
+        __builtin_memcpy(&v, x + (size_t)i * P, sizeof v);
 #pragma unroll
         for (int c = 0; c < P; c++) add(v[c]);
     }
@@ -292,12 +293,12 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(SampleParams p) {
 
 // The rows of a launch, a workgroup each. PARTS: with what the two launches before
 // found of the row's p.parts parts.
-// Passes that form weights take the row in pieces of 8 bytes: of whole vectors the
-// compiler holds eight exponentials' operands at a time, and spills them.
+// Passes that form weights take the row in pieces of four elements: of eight the
+// compiler holds all exponentials' operands at a time, and spills them.
 template <class E, int NT, bool PARTS>
 __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     typedef typename RowVec<E>::type Vec;
-    constexpr int N = RowVec<E>::N, P = N / 2, W = NT / 64, BINS = NT > SM_BINS ? SM_BINS : NT;
+    constexpr int N = RowVec<E>::N, P = SM_PIECE, W = NT / 64, BINS = NT > SM_BINS ? SM_BINS : NT;
     constexpr int RUNS = W > 8 ? 8 : W;
     typedef E Piece __attribute__((ext_vector_type(P)));
     __shared__ u64 run_s[PARTS ? 1 : RUNS][BINS];  // masses of the runs' bins
@@ -337,7 +338,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     const auto piece = [&](int i) {
         Piece v;
         if ((i + 1) * P <= p.V) {
-            __builtin_memcpy(&v, x + (size_t)i * P, 8);
+            __builtin_memcpy(&v, x + (size_t)i * P, sizeof v);
         } else {
 #pragma unroll
             for (int c = 0; c < P; c++) v[c] = i * P + c < p.V ? x[(size_t)i * P + c] : (E)-INFINITY;

@@ -1175,15 +1175,19 @@ def leading_strides(t):
     """(outer, row) strides of t [rows..., n], its rows contiguous: row r of the
     flattened leading dimensions at (r / inner) outer + (r % inner) row, inner
     the last of them; and the tensor they describe: t, or a copy."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    strides = t.stride()
+    if strides[-1] != 1 and t.shape[-1] > 1:
         t = t.contiguous()
-    if t.dim() == 1:
-        return (0, 0), t
-    if t.dim() == 2:
-        return (0, t.stride(0)), t
-    if t.dim() > 3:
+        strides = t.stride()
+    n = len(strides)
+    if n == 2:
+        return 0, strides[0], t
+    if n == 1:
+        return 0, 0, t
+    if n > 3:
         t = t.reshape(-1, *t.shape[-2:])
-    return (t.stride(0), t.stride(1)), t
+        strides = t.stride()
+    return strides[0], strides[1], t
 
 
 def adjust(logits, out, history, lengths, prompts, penalties, bias, tokens, allowed, dy=None):
@@ -1194,41 +1198,48 @@ def adjust(logits, out, history, lengths, prompts, penalties, bias, tokens, allo
     [..., V] bool or [..., words] int32 have the logits' leading shape (expanded
     views are read in place), lengths and prompts are int64 contiguous, each of
     the three penalties a number or fp32 contiguous; all of them may be None."""
-    dev = logits.device
-    V = logits.shape[-1]
-    (xo, xr), x = leading_strides(logits)
-    (yo, yr), y = ((xo, xr), x) if out is logits else leading_strides(out)
-    args = CyfaAdjustArgs(logits.numel() // V, logits.shape[-2] if logits.dim() > 1 else 1, V, x.data_ptr(), xo, xr)
-    args.inner = max(args.inner, 1)
-    args.y, args.y_outer, args.y_row = y.data_ptr(), yo, yr
-    kept = [x, y]  # alive until the launch
+    shape = logits.shape
+    V = shape[-1]
+    xo, xr, x = leading_strides(logits)
+    yo, yr, y = (xo, xr, x) if out is logits else leading_strides(out)
+    # (unset fields stay NULL and 0; what a copy was made of lives until the launch)
+    args = CyfaAdjustArgs(logits.numel() // V, shape[-2] if len(shape) > 1 else 1, V, x.data_ptr(), xo, xr, y=y.data_ptr(),
+                          y_outer=yo, y_row=yr)
     if history is not None and history.shape[-1] > 0:
-        (args.h_outer, args.h_row), history = leading_strides(history)
+        args.h_outer, args.h_row, history = leading_strides(history)
         args.history, args.L, args.wide = history.data_ptr(), history.shape[-1], history.dtype is torch.int64
-        args.lengths, args.prompts = ptr(lengths), ptr(prompts)
-        kept.append(history)
-    for name, v in zip(("repetition", "presence", "frequency"), penalties):
-        if isinstance(v, torch.Tensor):
-            setattr(args, name[:-1] + "ies" if name == "frequency" else name + "s", v.data_ptr())
-        else:
-            setattr(args, name, v)
+        if lengths is not None:
+            args.lengths = lengths.data_ptr()
+        if prompts is not None:
+            args.prompts = prompts.data_ptr()
+    repetition, presence, frequency = penalties
+    if isinstance(repetition, torch.Tensor):
+        args.repetitions = repetition.data_ptr()
+    else:
+        args.repetition = repetition
+    if isinstance(presence, torch.Tensor):
+        args.presences = presence.data_ptr()
+    else:
+        args.presence = presence
+    if isinstance(frequency, torch.Tensor):
+        args.frequencies = frequency.data_ptr()
+    else:
+        args.frequency = frequency
     if bias is not None:
-        (args.b_outer, args.b_row), bias = leading_strides(bias)
+        args.b_outer, args.b_row, bias = leading_strides(bias)
         args.bias = bias.data_ptr()
-        kept.append(bias)
     if tokens is not None and tokens[0].shape[-1] > 0:
-        (args.ti_outer, args.ti_row), ids = leading_strides(tokens[0])
-        (args.tv_outer, args.tv_row), values = leading_strides(tokens[1])
+        args.ti_outer, args.ti_row, ids = leading_strides(tokens[0])
+        args.tv_outer, args.tv_row, values = leading_strides(tokens[1])
         args.token_ids, args.token_values, args.n_tokens = ids.data_ptr(), values.data_ptr(), ids.shape[-1]
-        kept += [ids, values]
     if allowed is not None:
-        (ao, ar), allowed = leading_strides(allowed)
-        args.packed = allowed.dtype is torch.int32
-        size = 4 if args.packed else 1
-        args.allowed, args.a_outer, args.a_row = allowed.data_ptr(), ao * size, ar * size
-        kept.append(allowed)
-    args.dy = ptr(dy)
-    _lm_call("cyfa_adjust_logits", args, logits.dtype, 0 if dy is None else 1, dev)
+        ao, ar, allowed = leading_strides(allowed)
+        if allowed.dtype is torch.int32:  # (strides in bytes)
+            args.packed, ao, ar = 1, 4 * ao, 4 * ar
+        args.allowed, args.a_outer, args.a_row = allowed.data_ptr(), ao, ar
+    if dy is not None:
+        args.dy = dy.data_ptr()
+    _lm_call("cyfa_adjust_logits", args, logits.dtype, 0 if dy is None else 1, logits.device)
 
 
 @functools.lru_cache(64)

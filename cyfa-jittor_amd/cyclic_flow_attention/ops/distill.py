@@ -59,15 +59,21 @@ def distill_loss(logits, top_ids, top_logprobs, temperature=1.0, tail=False, wei
         if t is not None and torch.is_grad_enabled() and t.requires_grad:
             raise NotImplementedError(f"{what}: {name} gets no gradient here; give it detached")
     ids = top_ids.contiguous() if top_ids.dtype is torch.int64 else top_ids.long().contiguous()
-    values = top_logprobs.detach().float().contiguous()
+    values = _float32(top_logprobs)
     if weights is not None:
-        weights = weights.detach().float().contiguous()
+        weights = _float32(weights)
     _native.require_device(logits, ids, values, weights)
     if not kernel_ok(logits, ids, values, weights):
         return _plain(logits, ids, values, weights, temperature, tail)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillLoss.apply(logits, ids, values, weights, temperature, tail)
     return _native.distill_loss(logits, ids, values, weights, temperature, tail)[0]
+
+
+def _float32(t):
+    if t.requires_grad:
+        t = t.detach()
+    return (t if t.dtype is torch.float32 else t.float()).contiguous()
 
 
 def _plain(logits, ids, values, weights, temperature, tail):

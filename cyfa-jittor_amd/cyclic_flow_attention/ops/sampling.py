@@ -34,7 +34,9 @@ def _check_logits(what, logits):
 
 
 def _constant(what, name, t):
-    if torch.is_grad_enabled() and t.requires_grad:
+    if not t.requires_grad:
+        return t
+    if torch.is_grad_enabled():
         raise NotImplementedError(f"{what}: {name} gets no gradient here; give it detached")
     return t.detach()
 
@@ -53,6 +55,8 @@ def _per_row(what, name, v, lead, dtype=torch.float32):
     """An option: a number, or a contiguous tensor of dtype for the rows ``lead``."""
     if not isinstance(v, torch.Tensor):
         return float(v) if dtype is torch.float32 else int(v)
+    if v.dtype is dtype and v.shape == lead and not v.requires_grad and v.is_contiguous():
+        return v
     if dtype is torch.float32 and not v.dtype.is_floating_point or dtype is torch.int64 and v.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"{what}: {name} must be {'a float' if dtype is torch.float32 else 'an int64 or int32'} tensor, got {v.dtype}")
     v = _constant(what, name, v)
@@ -62,6 +66,8 @@ def _per_row(what, name, v, lead, dtype=torch.float32):
 
 
 def _integers(what, name, t, lead):
+    if t.dtype is torch.int64 and t.shape == lead and t.is_contiguous():
+        return t
     if t.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"{what}: {name} must be int64 or int32, got {t.dtype}")
     if t.dtype is torch.int32:
@@ -115,8 +121,9 @@ def adjust_logits(logits, history=None, lengths=None, prompt_lengths=None, repet
             lengths = _integers(what, "lengths", lengths, lead)
         if prompt_lengths is not None:
             prompt_lengths = _integers(what, "prompt_lengths", prompt_lengths, lead)
-    repetition, presence, frequency = (_per_row(what, n, v, lead) for n, v in (
-        ("repetition", repetition), ("presence", presence), ("frequency", frequency)))
+    repetition = _per_row(what, "repetition", repetition, lead)
+    presence = _per_row(what, "presence", presence, lead)
+    frequency = _per_row(what, "frequency", frequency, lead)
     if not isinstance(repetition, torch.Tensor) and not repetition > 0:
         raise ValueError(f"{what}: repetition must be positive, got {repetition}")
     if bias is not None:
@@ -139,7 +146,8 @@ def adjust_logits(logits, history=None, lengths=None, prompt_lengths=None, repet
         if allowed.dim() == 0 or allowed.shape[-1] != columns:
             raise ValueError(f"{what}: allowed must be [..., {columns}] in {allowed.dtype}, got {tuple(allowed.shape)}")
         allowed = _expanded(what, "allowed", allowed, lead + (columns,))
-    args = (history, lengths, prompt_lengths, (repetition, presence, frequency), bias, token_bias, allowed)
+    penalties = (repetition, presence, frequency)
+    args = (history, lengths, prompt_lengths, penalties, bias, token_bias, allowed)
     recorded = torch.is_grad_enabled() and logits.requires_grad
     if out is not None:
         if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
@@ -154,13 +162,12 @@ def adjust_logits(logits, history=None, lengths=None, prompt_lengths=None, repet
         if (out.numel() and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr()
                 and (out.data_ptr(), out.stride()) != (logits.data_ptr(), logits.stride())):
             raise ValueError(f"{what}: out has to be the logits themselves or apart from them")
-    tensors = [logits, history, lengths, prompt_lengths, bias, allowed, *(token_bias or ()),
-               *(v for v in args[3] if isinstance(v, torch.Tensor))]
-    if not kernel_ok(out, *tensors):
-        _native.require_device(*tensors)
+    tensors = [t for t in (logits, out, history, lengths, prompt_lengths, bias, allowed, *(token_bias or ()), *penalties)
+               if isinstance(t, torch.Tensor)]
+    _native.require_device(*tensors)
+    if not kernel_ok(*tensors):
         y = _plain_adjust(logits, *args)
         return y if out is None else out.copy_(y)
-    _native.require_device(out, *tensors)
     if recorded:
         return _AdjustLogits.apply(logits, args)
     if out is None:
@@ -287,11 +294,10 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
         raise ValueError(f"{what}: top_p must be in (0, 1], got {top_p}")
     if not isinstance(min_p, torch.Tensor) and not 0 <= min_p <= 1:
         raise ValueError(f"{what}: min_p must be in [0, 1], got {min_p}")
-    tensors = [logits, uniform, *(v for v in (temperature, top_k, top_p, min_p) if isinstance(v, torch.Tensor))]
-    if not kernel_ok(*tensors):
-        _native.require_device(*tensors)
-        return _plain_sample(logits.detach(), uniform.detach(), temperature, top_k, top_p, min_p)
+    tensors = [t for t in (logits, uniform, temperature, top_k, top_p, min_p) if isinstance(t, torch.Tensor)]
     _native.require_device(*tensors)
+    if not kernel_ok(*tensors):
+        return _plain_sample(logits.detach(), uniform.detach(), temperature, top_k, top_p, min_p)
     return SampledTokens(*_native.sample(logits, uniform.contiguous(), temperature, top_k, top_p, min_p))
 
 
