@@ -506,6 +506,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         }
         from = thr;  // many equal elements: the bins tell
         base = order_key(thr, 0x7fffffff);
+        if (PARTS) least = join_parts(p, r, p.parts).least;  // (without the -inf past the row's end: the parts' bins)
         __syncthreads();
     }
     const Bins bins(best, least, T, BINS);

@@ -257,6 +257,31 @@ def test_sample_with_settings_of_each_row(dtype):
     _check_choice(x, u, got, T, k, p, least)
 
 
+@pytest.mark.parametrize("V,dtype", [(50001, BF), (50001, F32), (40000, F16), (131073, BF)])
+def test_sample_of_few_wide_rows_with_settings_of_each(V, dtype):
+    """Rows that are shared out, of which some have a top_k that one wave handles:
+    thousands of equal elements behind a few larger ones, rows of one value, rows
+    without probabilities, a vocabulary that ends inside a vector."""
+    rows = 12
+    x = (_randn(V, rows, V) * 2).clamp(max=9.0).to(dtype)
+    x[0:6] = torch.where(torch.arange(V) % 3 == 0, 1.0, -2.0 - torch.arange(V) % 2).to(dtype)
+    x[0:6, 17:20] = torch.tensor([3.0, 2.0, 2.5]).to(dtype)
+    x[6, V // 2:] = -INF
+    x[7] = 0.5
+    x[8, 4000] = NAN
+    x[9] = -INF
+    x[10, 39999], x[10, 4] = INF, INF
+    u = _rand(V + 1, rows)
+    k = torch.tensor([50, 128, 129, 0, 1, 20000, 64, 100, 5, 5, 5, 0])
+    p = torch.tensor([1.0, 0.9, 0.8, 0.5, 1.0, 0.99, 1.0, 0.7, 0.9, 0.9, 0.9, 0.9])
+    least = torch.tensor([0.0, 0.0, 0.05, 0.2, 0.0, 0.0, 0.1, 0.0, 0.0, 0.0, 0.0, 0.0])
+    T = torch.tensor([1.0, 2.0, 0.7, 1.0, 1.0, 1.5, 1.0, 1.0, 1.0, 1.0, 1.0, 0.8])
+    got = _ops().sample_tokens(x.cuda(), u.cuda(), temperature=T.cuda(), top_k=k.cuda(), top_p=p.cuda(), min_p=least.cuda())
+    fine = torch.tensor([0, 1, 2, 3, 4, 5, 6, 7, 11])
+    _check_choice(x[fine], u[fine], type(got)(got.ids.cpu()[fine], got.logprob.cpu()[fine]), T[fine], k[fine], p[fine], least[fine])
+    assert got.ids[8:11].tolist() == [4000, 0, 4] and got.logprob[8:11].isnan().all()
+
+
 def test_sample_at_the_borders():
     """Weights whose sums are exact: which token a number on a border takes, ties
     by the lower id, the first kept and the last number below one."""
