@@ -30,9 +30,9 @@ struct DistillRow {
     float m, ls;        // of all columns: the maximum, log2 of the sum of 2^((x - m) c)
     float rm, rls;      // of the columns of no entry (with the tail; else of all)
     float rest, entry;  // what multiplies the softmax of the columns of no entry, of the entries
-    float norm;         // p_i = 2^(t_i c - norm)
+    float top, norm;    // p_i = 2^((t_i - top) c - norm)
     float weight;       // of the row in the mean, 0 without entries
-    float loss, pad;
+    float loss;
 };
 static_assert(sizeof(DistillRow) == DISTILL_ROW_FLOATS * 4, "DISTILL_ROW_FLOATS");
 
@@ -223,13 +223,13 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillParams p) {
             mass += p_[q];
         }
         mass = wave_sum(mass);
-        const double lognorm = TAIL ? 0. : (double)tmax / T + (double)logf((float)mass), scale = TAIL ? 1. : 1. / mass;
+        const double top = TAIL ? 0. : (double)tmax, lognorm = TAIL ? 0. : (double)logf((float)mass), scale = TAIL ? 1. : 1. / mass;
         double loss = 0.;
 #pragma unroll
         for (int q = 0; q < Q; q++)
             if (id[q] >= 0 && p_[q] != 0.) {
                 const float lq = (e[q] - all.m) / p.temperature - kLn2 * ls;
-                loss += p_[q] * scale * (((double)t[q] / T - lognorm) - (double)lq);
+                loss += p_[q] * scale * ((((double)t[q] - top) / T - lognorm) - (double)lq);
             }
         loss = wave_sum(loss);
         DistillRow row;
@@ -238,9 +238,9 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillParams p) {
         row.rm = a.s == 0.f ? 0.f : a.m;  // (no column of no entry but -inf: a softmax of zeros)
         row.rls = a.s == 0.f ? 0.f : rls;
         row.rest = row.entry = 1.f;
+        row.top = (float)top;
         row.norm = (float)(lognorm * 1.4426950408889634);
         row.weight = weight;
-        row.pad = 0.f;
         if (TAIL) {
             // the rest, where the student has any
             const double pr = a.s > 0.f ? fmax(0., 1. - mass) : 0.;
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(256) void distill_grad_kernel(DistillParams p, int 
             const long long at = p.ids[r * p.k + j];
             const float t = p.values[r * p.k + j];
             id[j] = at >= c0 && at < c1 && t != -INFINITY ? (int)at - c0 : -1;
-            mass[j] = fast_exp2(t * c - row.norm);
+            mass[j] = fast_exp2((t - row.top) * c - row.norm);
         }
         const float a = g * row.rest;
         const auto grad = [&](float e) { return a * fast_exp2((e - row.rm) * c - row.rls); };

@@ -450,6 +450,24 @@ def test_distill_of_special_rows(V, tail, T):
     _check_distill(x, ids, values, T, tail, None)
 
 
+@pytest.mark.parametrize("T", [0.25, 1.0, 3.0])
+def test_distill_of_a_teachers_logits_of_any_size(T):
+    """The loss and the gradient know the teacher's logits by their differences:
+    a row of the type's lowest value is one of zeros, and large logits cost no digits."""
+    x = _randn(1, 5, 90).cuda().requires_grad_(True)
+    ids, near = _randint(2, 90, 5, 7).cuda(), (_randint(3, 64, 5, 7) / 8.0).cuda()
+    near[0] = near[1] = 0.0
+    far = near + 2.0**16  # exact: 19 bits
+    far[0], far[1] = torch.finfo(F32).min, torch.finfo(F32).max
+    results = []
+    for values in (near, far):
+        loss = _ops().distill_loss(x, ids, values, temperature=T)
+        results.append((loss, *torch.autograd.grad(loss, [x])))
+    (a, da), (b, db) = results
+    # the same numbers are formed of the same differences
+    assert torch.equal(a, b) and torch.equal(da, db)
+
+
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_of_rows_without_probabilities(tail):
     x = _randn(3, 5, 200)
