@@ -90,7 +90,8 @@ def _plain(logits, ids, values, weights, temperature, tail):
     if tail:
         log_p = t
     else:
-        t = (t / temperature).masked_fill(~valid, float("-inf"))
+        t = t.masked_fill(~valid, float("-inf"))
+        t = (t - torch.where(live[..., None], t.amax(-1, keepdim=True), 0.0)) / temperature
         log_p = t - t.masked_fill(~live[..., None], 0.0).logsumexp(-1, keepdim=True)
     p = torch.where(valid & live[..., None], log_p.exp(), 0.0)
     given = p > 0

@@ -354,6 +354,19 @@ def test_recorded_backward_passes(no_launch):
     assert words[0].nonzero()[:, 0].tolist() == [0, 2, 35] and words[1].nonzero()[:, 0].tolist() == list(range(33))
 
 
+@pytest.mark.parametrize("T", [0.25, 1.0])
+def test_a_teachers_logits_of_any_size(no_launch, T):
+    from cyclic_flow_attention.ops import distill
+
+    x, ids = _randn(1, 3, 20), torch.arange(12).view(3, 4)
+    values = torch.zeros(3, 4)
+    values[2] = torch.arange(4.0)
+    far = values + 2.0**16
+    far[0], far[1] = torch.finfo(torch.float32).min, torch.finfo(torch.float32).max
+    near, much = (distill._plain(x, ids, v, None, T, False) for v in (values, far))
+    assert torch.equal(near, much) and near.isfinite()
+
+
 @pytest.mark.parametrize("tail,T", [(False, 1.0), (False, 3.0), (True, 1.0)])
 def test_distillation_without_a_rest_or_rows(no_launch, tail, T):
     """Teachers that know every token, rows that do not count, values of -inf."""
