@@ -235,8 +235,8 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillParams p) {
         DistillRow row;
         row.m = all.m;
         row.ls = ls;
-        row.rm = a.s == 0.f ? 0.f : a.m;  // (no column of no entry but -inf: a softmax of zeros)
-        row.rls = a.s == 0.f ? 0.f : rls;
+        row.rm = TAIL && a.s == 0.f ? 0.f : a.m;  // (no column of no entry but -inf: a softmax of zeros)
+        row.rls = TAIL && a.s == 0.f ? 0.f : rls;
         row.rest = row.entry = 1.f;
         row.top = (float)top;
         row.norm = (float)(lognorm * 1.4426950408889634);
