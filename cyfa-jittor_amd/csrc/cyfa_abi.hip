@@ -154,6 +154,7 @@ int cyfa_adjust_logits(const CyfaAdjustArgs* a, int dtype, int grad, void* hip_s
     if (a->rows == 0) return CYFA_OK;
     if (!a->x || !a->y || (grad && !a->dy) || (a->L > 0 && !a->history) || (a->n_tokens > 0 && (!a->token_ids || !a->token_values)))
         return fail(CYFA_ERR_VALUE, "%s: null required pointer", what);
+    if (grad && (a->y == a->x || a->y == a->dy)) return fail(CYFA_ERR_VALUE, "%s: a gradient is not formed in place", what);
     cyfa::AdjustParams p{};
     p.rows = a->rows;
     p.inner = a->inner;

@@ -82,6 +82,15 @@ def _float32(what, name, t):
     return t if t.dtype is torch.float32 else t.float()
 
 
+def _share(a, b):
+    """Whether the memory between a's first and last element meets b's."""
+    if not isinstance(b, torch.Tensor) or not a.numel() or not b.numel() or a.device != b.device:
+        return False
+    first, end = zip(*((t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size())
+                       for t in (a, b)))
+    return max(first) < min(end)
+
+
 def adjust_logits(logits, history=None, lengths=None, prompt_lengths=None, repetition=1.0, presence=0.0, frequency=0.0,
                   bias=None, token_bias=None, allowed=None, out=None):
     """``logits`` [..., V] with penalties for the tokens a sequence holds already,
@@ -159,9 +168,10 @@ def adjust_logits(logits, history=None, lengths=None, prompt_lengths=None, repet
             raise ValueError(f"{what}: out needs contiguous rows and at most three dimensions")
         if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
             raise ValueError(f"{what}: out has to be one element of memory for each of its own")
-        if (out.numel() and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr()
-                and (out.data_ptr(), out.stride()) != (logits.data_ptr(), logits.stride())):
+        if _share(out, logits) and (out.data_ptr(), out.stride()) != (logits.data_ptr(), logits.stride()):
             raise ValueError(f"{what}: out has to be the logits themselves or apart from them")
+        if any(_share(out, t) for t in (*args[:3], *penalties, bias, *(token_bias or ()), allowed)):
+            raise ValueError(f"{what}: out has to be apart from what is read with the logits")
     tensors = [t for t in (logits, out, history, lengths, prompt_lengths, bias, allowed, *(token_bias or ()), *penalties)
                if isinstance(t, torch.Tensor)]
     _native.require_device(*tensors)

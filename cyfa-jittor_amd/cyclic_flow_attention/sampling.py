@@ -51,6 +51,8 @@ class Sampler:
         self.history[:, :T] = prompts
         if lengths is None:
             lengths = torch.full((B,), T, dtype=torch.int64, device=dev)
+        elif lengths.shape != (B,) or lengths.dtype not in (torch.int64, torch.int32) or bool(((lengths < 0) | (lengths > T)).any()):
+            raise ValueError(f"a Sampler's lengths must be {B} integers from 0 to {T}")
         self.prompt_lengths = lengths.to(device=dev, dtype=torch.int64).clone()
         self.lengths = self.prompt_lengths.clone()
         self.generator = torch.Generator(device=dev).manual_seed(sampling.seed)

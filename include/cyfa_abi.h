@@ -677,7 +677,7 @@ int cyfa_residual_norm(const CyfaResidualArgs *args, int dtype, int grad, void *
  *   y = -inf                                      where j is not allowed
  *   dx = dy (n > 0 ? (x > 0 ? 1 / repetition : repetition) : 1), 0 where j is not allowed
  * in f32, rounded once. Lengths are clamped to [0, L]; tokens outside [0, V) are
- * passed over. y may be x, with the same strides. No counterpart in the
+ * passed over. y may be x, with the same strides (not of grad 1). No counterpart in the
  * reference, whose generation samples the logits as they are (generation.py:23-62). */
 typedef struct CyfaAdjustArgs {
     long long rows, inner;        /* inner > 0 */

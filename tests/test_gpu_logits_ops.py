@@ -481,6 +481,7 @@ def test_distill_of_rows_without_probabilities(tail):
         loss = _ops().distill_loss(xg, ids[r:r + 1].cuda(), values[r:r + 1].cuda(), tail=tail)
         (dx,) = torch.autograd.grad(loss, [xg])
         assert loss.isnan() and dx.isnan().any()
+        assert tail or dx.isnan().all()
     none = _ops().distill_loss(x.cuda(), torch.full_like(ids, -100).cuda(), values.cuda(), tail=tail)
     assert none.isnan()
     assert _ops().distill_loss(x[:0].cuda(), ids[:0].cuda(), values[:0].cuda(), tail=tail).isnan()
@@ -649,6 +650,51 @@ def test_offsets_past_32_bits():
     lastg = last.clone().requires_grad_(True)
     want = ops.distill_loss(lastg, ids[-3:], values[-3:], tail=True)
     assert torch.equal(loss, want) and torch.equal(dx[-3:], torch.autograd.grad(want, [lastg])[0]) and not dx[:-3].any()
+
+
+def test_more_rows_than_a_launch_takes():
+    """2^20 and more workgroups: the last rows as in calls of their own."""
+    ops, rows = _ops(), (1 << 22) + 9
+    x = (_randn(1, rows, 5) * 2).to(BF).cuda()
+    history = _randint(2, 5, rows, 3).cuda()
+    y = ops.adjust_logits(x, history, repetition=1.5, frequency=0.25)
+    allowed = torch.ones(5, dtype=torch.bool, device="cuda")
+    plain = x.float()
+    n = torch.zeros(rows, 5, device="cuda").scatter_add_(1, history, torch.ones(rows, 3, device="cuda"))
+    plain = torch.where(n > 0, torch.where(plain > 0, plain / 1.5, plain * 1.5) - 0.25 * n, plain).to(BF)
+    assert torch.equal(y, plain) and torch.equal(ops.adjust_logits(x, history, repetition=1.5, frequency=0.25, allowed=allowed), plain)
+    u = _rand(3, rows).cuda()
+    got = ops.sample_tokens(x, u, top_k=3, top_p=0.9)
+    ids, values = _randint(4, 6, rows, 2).cuda(), -_rand(5, rows, 2).cuda() - 1
+    weights = torch.zeros(rows, device="cuda")
+    weights[-9:] = 1.0
+    xg = x.clone().requires_grad_(True)
+    loss = ops.distill_loss(xg, ids, values, tail=True, weights=weights)
+    (dx,) = torch.autograd.grad(loss, [xg])
+    assert not dx[:-9].any()
+    for part in (slice(0, 7), slice((1 << 20) - 3, (1 << 20) + 3), slice((1 << 22) - 3, rows)):
+        own = ops.sample_tokens(x[part], u[part], top_k=3, top_p=0.9)
+        assert torch.equal(got.ids[part], own.ids) and torch.equal(got.logprob[part], own.logprob)
+    xg = x[-9:].clone().requires_grad_(True)
+    last = ops.distill_loss(xg, ids[-9:], values[-9:], tail=True)
+    assert torch.equal(last, loss) and torch.equal(torch.autograd.grad(last, [xg])[0], dx[-9:])
+
+
+def test_the_most_shared_memory():
+    """The largest slices, histories and token biases, and the largest vocabulary beside a tail, of one workgroup."""
+    rows, V, L = 136, 65536, 16383
+    x, kw, allowed = _adjust_case(5, 3, V, L, BF, False, False, 1024, "bits")
+    kw["lengths"][:] = L
+    args = {n: _cuda(t) for n, t in kw.items()}
+    args["token_bias"] = tuple(t.repeat(46, 1)[:rows] for t in args["token_bias"])
+    y = _ops().adjust_logits(x.cuda().repeat(46, 1)[:rows], **{n: t if isinstance(t, tuple) else t.repeat(46, *[1] * (t.dim() - 1))[:rows]
+                                                              for n, t in args.items()})
+    lm.assert_within(y[:3], *_adjust_ref(x, kw, allowed), "y")
+    assert all(torch.equal(y[r].view(torch.uint8), y[r % 3].view(torch.uint8)) for r in (3, 70, 135))
+    V = 1 << 19
+    x = (_randn(6, 2, V) * 3).to(BF)
+    ids, values = _teacher(7, x, 256)
+    _check_distill(x, ids, values, 1.0, True, None)
 
 
 def test_inference_tensors():

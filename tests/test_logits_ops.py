@@ -52,7 +52,7 @@ def test_adjust_validates_before_launch():
         assert call(grad, x=0x10001) == call(grad, dtype=1, y=0x20002) == call(grad, lengths=0x40004) == ALIGN
         assert call(grad, history=0x40004, wide=1) == call(grad, history=0x40002) == call(grad, bias=0x40002) == ALIGN
         assert call(grad, rows=0) == _native.CYFA_OK
-    assert call(1, dy=None) == VALUE
+    assert call(1, dy=None) == call(1, y=0x10000) == call(1, y=0x30000) == VALUE
     assert _native.load_library().cyfa_adjust_logits(None, 0, 0, None) == VALUE
 
 
@@ -65,6 +65,11 @@ def test_sample_validates_before_launch():
     assert call(0, x=0x10001) == call(0, uniform64=0x20004) == call(0, top_ks=0x20004) == call(0, top_ps=0x20002) == ALIGN
     assert call(0, rows=0) == _native.CYFA_OK
     assert _native.load_library().cyfa_sample_tokens(None, 0, 0, None) == VALUE
+    size = _native._sample_bytes(4, 50000)  # few rows of many columns are shared out
+    assert size > 0 and _native._sample_bytes(4, 100) == _native._sample_bytes(4096, 50000) == _native._sample_bytes(0, 50000) == 0
+    wide = dict(V=50000, row_stride=50000)
+    assert call(0, **wide) == call(0, workspace=0x50000, workspace_bytes=size - 1, **wide) == _native.CYFA_ERR_WORKSPACE
+    assert call(0, workspace=0x50008, workspace_bytes=size, **wide) == ALIGN
 
 
 def test_distill_validates_before_launch():
@@ -172,6 +177,23 @@ def test_sampler_refuses():
     sampler.take()
     with pytest.raises(ValueError, match="room"):
         sampler.next(torch.zeros(3, 9))
+
+
+    for lengths in (torch.tensor([1, 2]), torch.tensor([1, 2, 3]), torch.tensor([0, -1, 2]), torch.tensor([1.0, 1.0, 1.0])):
+        with pytest.raises(ValueError, match="lengths"):
+            Sampler(Sampling(), torch.zeros(3, 2, dtype=torch.int64), 1, lengths)
+
+
+def test_out_apart_from_what_is_read():
+    """out may lie beside the logits and the options in one allocation, not among them."""
+    whole = torch.zeros(4, 3, 8)
+    with pytest.raises(ValueError, match="GPU device"):  # (no other objection)
+        ops.adjust_logits(whole[0], bias=whole[1], out=whole[2])
+    for out, kw in ((whole.view(-1)[4:28].view(3, 8), {}), (whole[:, 0, :][:3], {}), (whole[2], dict(bias=whole[2, 1])),
+                    (whole[0], dict(bias=whole[0])), (whole[3], dict(presence=whole[3, 0, 4:7])),
+                    (whole[1], dict(token_bias=(torch.zeros(2, dtype=torch.int64), whole[1, 2, 3:5])))):
+        with pytest.raises(ValueError, match="apart"):
+            ops.adjust_logits(whole[0], out=out, **kw)
 
 
 def test_generate_refuses_two_settings():
