@@ -666,8 +666,8 @@ struct SampleParams {
     long long first;             // row of a launch's first workgroup
 };
 constexpr int SAMPLE_PARTS = 32;         // most parts of a row
-constexpr int SAMPLE_PART_COLS = 8192;   // fewest columns of a part
-constexpr int SAMPLE_MIN_V = 40000, SAMPLE_MAX_ROWS = 32;  // rows that are shared out
+constexpr int SAMPLE_PART_COLS = 4096;   // fewest columns of a part
+constexpr int SAMPLE_MIN_V = 40000, SAMPLE_MAX_ROWS = 64;  // rows that are shared out
 size_t sample_workspace_bytes(long long rows, int V);
 void launch_sample(SampleParams p, int dtype, hipStream_t stream);
 

@@ -919,10 +919,11 @@ void launch_rows(SampleParams p, hipStream_t stream) {
 
 // Parts of a row, 1 where it is not shared out: few wide rows, but for a top_k that
 // one wave handles (of which a call with a top_k for each row may hold some). us
-// on MI355X, bf16, one workgroup a row against parts: top_p 0.9, 16 rows of 32000
-// 21 / 22, of 50001 37 / 32, of 131072 62 / 40; 64 rows of 131072 62 / 59; 128 68 /
-// 94; whole distributions, 16 rows of 32000 16 / 15, of 50001 22 / 18; top_k 50, 16
-// rows of 131072 19 / 28.
+// on MI355X, bf16, one workgroup a row against parts of 4096 columns and more:
+//   top_p 0.9: 16 rows of 32000 22 / 23, of 50001 34 / 25, of 131072 58 / 35; 64 rows 22 / 26, 34 / 29, 59 / 47; 128 23 / 28, 34 / 33, 60 / 62
+//   whole distributions: 16 rows 16 / 16, 22 / 16, 41 / 18; 64 rows 17 / 18, 23 / 19, 41 / 30; 128 17 / 21, 23 / 24, 43 / 42
+//   top_k 1000: 64 rows 27 / 25, 37 / 27, 66 / 39; top_k 50: 16 rows 12 / 19, 15 / 22, 18 / 27
+// Parts of 8192 columns: top_p 0.95, 4 rows of 50001 30 for 27, as long at 131072.
 int row_parts(const SampleParams& p) {
     if (p.V < SAMPLE_MIN_V || p.rows > SAMPLE_MAX_ROWS || p.rows <= 0 || (!p.top_ks && p.top_k > 0 && p.top_k <= SM_TOP)) return 1;
     return min(p.V / SAMPLE_PART_COLS, SAMPLE_PARTS);
