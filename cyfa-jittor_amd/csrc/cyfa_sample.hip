@@ -12,20 +12,27 @@
 // past 2^16 columns, so that a row's sum fits 64), and integers add up the same
 // in any order. Weights below half of that step count nothing.
 //
-// A workgroup to a row, whose passes find it in the L2 (rows held in LDS took as
-// long: 13.6 us against 14.0 for 256 rows of 32000 bf16). A prefix is found by
-// counting: the elements, or their mass, by bins of their distance to the
-// maximum; the bin in which the prefix ends gives its elements to a list, whose
+// Whole distributions (and what min_p leaves of them) take two passes over a row,
+// the maximum and the weights (sample_draw_kernel). Where top_k or top_p cut them
+// (sample_kernel), a workgroup to a row, whose passes find it in the L2 (rows held
+// in LDS took as long: 13.6 us against 14.0 for 256 rows of 32000 bf16). A prefix
+// is found by counting: the elements, or their mass, by bins of their distance to
+// the maximum; the bin in which the prefix ends gives its elements to a list, whose
 // keys are binned again until few enough are left to rank each against each.
 // Masses are counted for runs of the row apart, so that the run that holds the
 // token is known from the bins and its weights alone are formed again. A top_k of
-// at most 64, the usual one, needs no bins: a value that at least k elements reach
-// and seldom many more is the k-th largest of the largest elements of 64 sets of
-// threads, and the few that reach it are ranked, cut and drawn from by one wave.
+// at most 128, the usual one, needs no bins: a value that at least k elements reach
+// and seldom many more is the k-th largest of the largest elements of 64 (128) sets
+// of threads, and the few that reach it are ranked, cut and drawn from by one wave.
 //
-// Few rows are shared out: a workgroup to each part of a row finds its maximum, a
-// second launch counts the parts' bins, and a third, a workgroup to a row, goes on
-// from there with the parts as runs.
+// Few wide rows are shared out: a workgroup to each part of a row finds its
+// maximum, a second launch counts the parts' bins, and a third, a workgroup to a
+// row, goes on from there with the parts as runs.
+//
+// Bound by the VALU: an element's weight costs 17 operations in double, of 4.3 to 5
+// cycles of a SIMD each, and 6 others: 0.11 ns on 256 compute units, where its two
+// bytes take 0.04 from memory. Rows of a single compute unit each wait besides at
+// their dozen barriers.
 #include <type_traits>
 
 #include "cyfa_internal.h"
@@ -178,11 +185,15 @@ __device__ __forceinline__ const E* row_of(const SampleParams& p, long long r) {
     return static_cast<const E*>(p.x) + (r / p.inner) * p.outer_stride + (r % p.inner) * p.row_stride;
 }
 
-__device__ __forceinline__ Choice choice_of(const SampleParams& p, float m, double T) {
-    Choice ch;
+__device__ __forceinline__ void set_choice(Choice& ch, float m, double T) {
     ch.m = m;
     ch.c = fmax(fmin(kLog2eD / T, 1e300), 1e-300);  // (0 times it stays 0, -inf times it -inf)
     ch.least = -60. / ch.c;
+}
+
+__device__ __forceinline__ Choice choice_of(const SampleParams& p, float m, double T) {
+    Choice ch;
+    set_choice(ch, m, T);
     ch.unit = p.unit;
 #pragma unroll
     for (int i = 0; i < SM_DEGREE; i++) {
@@ -190,6 +201,44 @@ __device__ __forceinline__ Choice choice_of(const SampleParams& p, float m, doub
         asm("" : "+s"(ch.k[i]));  // (as literals each would be moved to the sum's registers before its product)
     }
     return ch;
+}
+
+// The least fp32 value that min_p keeps of a row; the largest is always kept.
+__device__ __forceinline__ float lowest_of(double min_p, double m, double T) {
+    float lowest = -INFINITY;
+    if (min_p > 0.) {
+        const double border = fmin(m, m + T * log(min_p));
+        lowest = (float)border;
+        if ((double)lowest < border) lowest = nextafterf(lowest, INFINITY);
+    }
+    return lowest;
+}
+
+// What the running mass has to pass.
+__device__ __forceinline__ u64 mass_at(double u, u64 total) {
+    const u64 target = u > 0. ? (u64)fmin(u * (double)total, 0x1p63) : 0;
+    return target >= total ? total - 1 : target;
+}
+
+// f(piece, its index) of the whole pieces begin, begin + STEP, ... below end of a
+// row, each on its way while the one before is worked on.
+template <int STEP, class E, class F>
+__device__ __forceinline__ void each_piece(const E* x, int begin, int end, F&& f) {
+    typedef E Piece __attribute__((ext_vector_type(SM_PIECE)));
+    if (begin >= end) return;
+    const auto load = [&](int i) {
+        Piece v;
+        __builtin_memcpy(&v, x + (size_t)i * SM_PIECE, sizeof v);
+        return v;
+    };
+    Piece next = load(begin);
+    asm volatile("" : "+v"(next));  // (else the compiler takes this load for the loop's, and waits for each where it is used)
+#pragma unroll 1
+    for (int i = begin; i < end; i += STEP) {
+        const Piece v = next;
+        next = load(min(i + STEP, end - 1));
+        f(v, i);
+    }
 }
 
 // This part of a row: maximum, least element, NaN. Parts are whole vectors.
@@ -249,11 +298,11 @@ __device__ __forceinline__ PartStats join_parts(const SampleParams& p, long long
     return a;
 }
 
-// The counts and masses of a part's bins.
+// The counts and masses of a part's bins (16 rows of 131072 bf16, a part of 4096 to
+// a workgroup: the statistics 3.5 us, the bins 7, the rows themselves 26).
 template <class E>
 __global__ __launch_bounds__(256) void sample_bins_kernel(SampleParams p) {
     constexpr int P = SM_PIECE;
-    typedef E Piece __attribute__((ext_vector_type(P)));
     __shared__ u64 mass_s[SM_BINS];
     __shared__ unsigned count_s[SM_BINS];
     const int tid = threadIdx.x;
@@ -275,13 +324,10 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(SampleParams p) {
         atomicAdd(&count_s[b], 1u);
         atomicAdd(&mass_s[b], weight(ch, wide(v)));
     };
-#pragma unroll 1
-    for (int i = tid; i < npiece; i += 256) {
-        Piece v;
-        __builtin_memcpy(&v, x + (size_t)i * P, sizeof v);
+    each_piece<256>(x, tid, npiece, [&](const auto& v, int) {
 #pragma unroll
         for (int c = 0; c < P; c++) add(v[c]);
-    }
+    });
     if (tid < tail) add(x[npiece * P + tid]);
     __syncthreads();
     const long long at = (r * gridDim.y + blockIdx.y) * SM_BINS;
@@ -425,16 +471,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         return;
     }
     const Choice ch = choice_of(p, best, T);
-    float lowest = -INFINITY;  // the least fp32 value that min_p keeps; the largest is always kept
-    if (min_p > 0.) {
-        const double border = fmin(ch.m, ch.m + T * log(min_p));
-        lowest = (float)border;
-        if ((double)lowest < border) lowest = nextafterf(lowest, INFINITY);
-    }
-    const auto mass_at = [&](u64 total) {  // what the running mass has to pass
-        u64 target = u > 0. ? (u64)fmin(u * (double)total, 0x1p63) : 0;
-        return target >= total ? total - 1 : target;
-    };
+    const float lowest = lowest_of(min_p, ch.m, T);
     const auto put = [&](int i, u64 w, u64 total) {
         p.ids[r] = i;
         p.logprob[r] = (float)log((double)w / (double)total);
@@ -490,7 +527,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
                 for (int h = 0; h < 2; h++)
                     kept += __popcll(__ballot((lane == 0 && h == 0) || (lane + 64 * h < k && e[h] >= lowest &&
                                                                         !(cut_p && (double)(sum[h] - w[h]) >= top_p * (double)before))));
-                const u64 total = kept > 64 ? lane_u64(sum[1], kept - 65) : lane_u64(sum[0], kept - 1), target = mass_at(total);
+                const u64 total = kept > 64 ? lane_u64(sum[1], kept - 65) : lane_u64(sum[0], kept - 1), target = mass_at(u, total);
                 u64 upto[2] = {0, 0};  // the mass of the kept up to these by index
                 const auto pass = [&](u64 other, u64 ow) {
 #pragma unroll
@@ -602,25 +639,25 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
             }
         } else if (MASS) {  // (the count of the bin that matters is that of the list)
             counted = true;
-            const int run = wv * RUNS / W, begin = run * run_len, end = min(begin + run_len, npiece);
             constexpr int STEP = NT / RUNS;
+            const int run = wv * RUNS / W, begin = run * run_len, end = min(begin + run_len, p.V / P);
+            const auto add = [&](float e, int i, int run) {
+                if (base == 0 || (e >= from && order_key(e, i) >= base)) atomicAdd(&run_s[PARTS ? 0 : run][bins.of(e)], weight(ch, e));
+            };
             if (base == 0) {
-#pragma unroll 1
-                for (int i = begin + tid % STEP; i < end; i += STEP) {
-                    const Piece v = piece(i);
+                each_piece<STEP>(x, begin + tid % STEP, end, [&](const auto& v, int) {
 #pragma unroll
                     for (int c = 0; c < P; c++) atomicAdd(&run_s[PARTS ? 0 : run][bins.of(wide(v[c]))], weight(ch, wide(v[c])));
-                }
+                });
             } else {
-#pragma unroll 1
-                for (int i = begin + tid % STEP; i < end; i += STEP) {
-                    const Piece v = piece(i);
+                each_piece<STEP>(x, begin + tid % STEP, end, [&](const auto& v, int i) {
 #pragma unroll
-                    for (int c = 0; c < P; c++) {
-                        const float e = wide(v[c]);
-                        if (e >= from && order_key(e, i * P + c) >= base) atomicAdd(&run_s[PARTS ? 0 : run][bins.of(e)], weight(ch, e));
-                    }
-                }
+                    for (int c = 0; c < P; c++) add(wide(v[c]), i * P + c, run);
+                });
+            }
+            if (tid < p.V % P) {  // (columns behind the last whole piece)
+                const int i = p.V / P * P + tid;
+                add(wide(x[i]), i, i / P / run_len);
             }
             __syncthreads();
             c = 0;
@@ -870,7 +907,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     }
     total = 0;
     for (int i = 0; i < runs; i++) total += runs_s[i];
-    const u64 target = mass_at(total);
+    const u64 target = mass_at(u, total);
     u64 passed = 0;
     int run = 0;
     while (run < runs - 1 && passed + runs_s[run] <= target) passed += runs_s[run++];
@@ -909,6 +946,222 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     }
 }
 
+// Rows whose whole distribution is drawn from, or (KEEP) what min_p leaves of it.
+// A workgroup takes rows in turn: while it forms a row's weights it finds the next
+// row's maximum, so that one row is on its way from memory while the exponentials
+// of the one before, which come from the caches a second time, keep the VALU busy.
+// A wave to each run of the row; the run that holds the token is formed again.
+// us on MI355X, by sample_kernel / by this one: 1021 x 50001 fp32 88 / 80 (2.6 TB/s
+// of one read; 58 with every row in the L2, for the VALU's 45), with min_p 0.05 76 /
+// 67; bf16, 4096 x 32000 156 / 149, with min_p 119 / 112; 256 x 32000 27 / 13; 1 x
+// 32000 16 / 12; 1024 x 4096 13 / 10.5; 16384 x 1000 81 / 79. Threads of a row, 256 /
+// 512 / 1024: 1021 x 50001 fp32 90 / 79 / 82, 4096 x 32000 154 / 148 / 170, 1024 x 4096
+// 10.4 / 14 / 25.
+template <class E, int NT, bool KEEP>
+__global__ __launch_bounds__(NT) void sample_draw_kernel(SampleParams p) {
+    constexpr int P = SM_PIECE, W = NT / 64;
+    constexpr int U = NT > 256 && sizeof(E) == 2 ? 2 : 1;  // pieces of a row that a thread forms at a time
+    typedef E Piece __attribute__((ext_vector_type(P)));
+    __shared__ u64 sums_s[2][W];
+    __shared__ float best_s[W];
+    __shared__ unsigned first_s[W];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int full = p.V / P, npiece = (p.V + P - 1) / P, len = (npiece + W - 1) / W;
+    const int begin = min(wv * len, npiece), end = min(begin + len, npiece), whole = min(end, full);
+    const int rest = end > full && begin <= full ? p.V - full * P : 0;  // columns behind the last whole piece, if they are this wave's
+    const auto load = [](const E* x, int i) {
+        Piece v;
+        __builtin_memcpy(&v, x + (size_t)i * P, sizeof v);
+        return v;
+    };
+    const auto top = [](float best, const Piece& v) {
+#pragma unroll
+        for (int c = 0; c < P; c++) best = __builtin_elementwise_maximum(best, wide(v[c]));  // (a NaN stays)
+        return best;
+    };
+    // The maximum of a wave's runs to that of the row, a NaN where there is one.
+    const auto put_best = [&](float best) {
+        const bool bad = __any(best != best);
+        best = wave_max(best);
+        if (lane == 0) best_s[wv] = bad ? __builtin_nanf("") : best;
+    };
+    const auto get_best = [&]() {
+        float best = best_s[0];
+#pragma unroll
+        for (int w = 1; w < W; w++) best = __builtin_elementwise_maximum(best, best_s[w]);
+        return best;
+    };
+    const auto find_best = [&](const E* x) {  // of this wave's run
+        float best = lane < rest ? wide(x[full * P + lane]) : -INFINITY;
+        for (int i0 = begin + lane; i0 < whole; i0 += 64 * 4) {
+            Piece v[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = load(x, min(i0 + j * 64, whole - 1));
+#pragma unroll
+            for (int j = 0; j < 4; j++) best = top(best, v[j]);
+        }
+        return best;
+    };
+    long long r = blockIdx.x;
+    const E* x = row_of<E>(p, r);
+    put_best(find_best(x));
+    __syncthreads();
+    float best = get_best();
+    Choice ch = choice_of(p, best, 1.);
+    for (;;) {
+        const long long next = r + gridDim.x;
+        const bool more = next < p.rows;
+        const E* xn = more ? row_of<E>(p, next) : x;
+        const double T = p.temperatures ? (double)p.temperatures[r] : p.temperature;
+        const double u = p.uniform64 ? p.uniform64[r] : (double)p.uniform[r];
+        const bool none = !(fabsf(best) < INFINITY);
+        __syncthreads();  // (all have read best_s)
+        if (none || !(T > 0.)) {  // the first of the largest, a NaN before all
+            unsigned at = 0xffffffffu;
+            for (int c = tid; c < p.V; c += NT) {
+                const float e = wide(x[c]);
+                if (best != best ? e != e : e == best) at = min(at, (unsigned)c);
+            }
+            for (int d = 32; d > 0; d >>= 1) at = min(at, (unsigned)__shfl_xor((int)at, d));
+            if (lane == 0) first_s[wv] = at;
+            if (more) put_best(find_best(xn));
+            __syncthreads();
+            if (tid == 0) {
+                for (int w = 1; w < W; w++) at = min(at, first_s[w]);
+                p.ids[r] = at;
+                p.logprob[r] = none ? __builtin_nanf("") : 0.f;
+            }
+        } else {
+            set_choice(ch, best, T);
+            float lowest = -INFINITY;
+            if (KEEP) lowest = lowest_of(p.min_ps ? (double)p.min_ps[r] : p.min_p, ch.m, T);
+            const auto weight_of = [&](float e) { return weight(ch, KEEP && e < lowest ? -INFINITY : e); };
+            const auto sum_of = [&](const Piece& v) {
+                u64 s = 0;
+                if (!KEEP || top(-INFINITY, v) >= lowest)
+#pragma unroll
+                    for (int c = 0; c < P; c++) s += weight_of(wide(v[c]));
+                return s;
+            };
+            u64 sum = lane < rest ? weight_of(wide(x[full * P + lane])) : 0;
+            float nbest = more && lane < rest ? wide(xn[full * P + lane]) : -INFINITY;
+            const auto pass = [&](auto with_next) {
+                constexpr bool NEXT = decltype(with_next)::value;
+                if (begin >= whole) return;
+                Piece a[U], b[NEXT ? U : 1];
+                const auto fetch = [&](int i0) {
+#pragma unroll
+                    for (int j = 0; j < U; j++) {
+                        const int i = min(i0 + j * 64, whole - 1);
+                        a[j] = load(x, i);
+                        if (NEXT) b[j] = load(xn, i);
+                    }
+                };
+                fetch(begin + lane);
+#pragma unroll
+                for (int j = 0; j < U; j++) {  // (else the compiler takes these loads for the loop's, and waits for each where it is used)
+                    asm volatile("" : "+v"(a[j]));
+                    if (NEXT) asm volatile("" : "+v"(b[j]));
+                }
+#pragma unroll 1
+                for (int i0 = begin + lane; i0 - lane < whole; i0 += 64 * U) {
+                    Piece now[U];
+#pragma unroll
+                    for (int j = 0; j < U; j++) {
+                        now[j] = a[j];
+                        if (NEXT) nbest = top(nbest, b[j]);
+                    }
+                    fetch(i0 + 64 * U);
+#pragma unroll
+                    for (int j = 0; j < U; j++) {
+                        const u64 s = sum_of(now[j]);
+                        sum += i0 + j * 64 < whole ? s : 0;
+                    }
+                }
+            };
+            more ? pass(std::true_type{}) : pass(std::false_type{});
+            sum = wave_add(sum);
+            if (lane == 0) sums_s[0][wv] = sum;
+            if (more) put_best(nbest);
+            __syncthreads();
+            // of W sums the one that holds the target, and the mass before it (in every lane)
+            u64 total, passed = 0, target = 0;
+            const auto find = [&](const u64* sums) {
+                const u64 mine = lane < W ? sums[lane] : 0, upto = wave_scan(mine);
+                total = lane_u64(upto, 63);
+                return upto;
+            };
+            const u64 runs = find(sums_s[0]), mass = total;
+            target = mass_at(u, mass);
+            const int run = min(__popcll(__ballot(runs <= target)), W - 1);
+            if (run > 0) passed = lane_u64(runs, run - 1);
+            // the run again, a wave to each part of it
+            const auto piece_of = [&](int i) {
+                Piece v;
+                if (i < full)
+                    v = load(x, i);
+                else
+#pragma unroll
+                    for (int c = 0; c < P; c++) v[c] = i * P + c < p.V ? x[(size_t)i * P + c] : (E)-INFINITY;
+                return v;
+            };
+            int from = min(run * len, npiece), to = min(from + len, npiece);
+            const int share = (to - from + W - 1) / W;
+            from = min(from + wv * share, to);
+            to = min(from + share, to);
+            u64 part = 0;
+            Piece last;  // this lane's last piece, and its mass
+            u64 last_mass = 0;
+#pragma unroll 1
+            for (int i = from + lane; i < to; i += 64) {
+                last = piece_of(i);
+                last_mass = sum_of(last);
+                part += last_mass;
+            }
+            part = wave_add(part);
+            if (lane == 0) sums_s[1][wv] = part;
+            __syncthreads();
+            const u64 parts = find(sums_s[1]);
+            if (wv > 0) passed += lane_u64(parts, wv - 1);
+            if (passed <= target && target < passed + part) {  // (one wave)
+#pragma unroll 1
+                for (int i0 = from; i0 < to; i0 += 64) {
+                    const int i = i0 + lane;
+                    if (share > 64) {
+                        if (i < to) last = piece_of(i);
+                        last_mass = i < to ? sum_of(last) : 0;
+                    }
+                    const u64 upto = wave_scan(last_mass), all = lane_u64(upto, 63);
+                    if (passed + all > target) {
+                        u64 before = passed + upto - last_mass;
+                        if (before <= target && target < before + last_mass) {  // (one lane)
+                            int at = -1;
+                            u64 taken = 0;
+#pragma unroll
+                            for (int c = 0; c < P; c++) {
+                                const u64 w = weight_of(wide(last[c]));
+                                before += w;
+                                if (at < 0 && before > target) {
+                                    at = i * P + c;
+                                    taken = w;
+                                }
+                            }
+                            p.ids[r] = at;
+                            p.logprob[r] = (float)log((double)taken / (double)mass);
+                        }
+                        break;
+                    }
+                    passed += all;
+                }
+            }
+        }
+        if (!more) return;
+        best = get_best();
+        r = next;
+        x = xn;
+    }
+}
+
 template <class E, int NT>
 void launch_rows(SampleParams p, hipStream_t stream) {
     for (p.first = 0; p.first < p.rows; p.first += LOGPROBS_MAX_GRID) {
@@ -917,15 +1170,32 @@ void launch_rows(SampleParams p, hipStream_t stream) {
     }
 }
 
+// Workgroups of a compute unit that the rows of sample_draw_kernel are shared out to.
+template <class E, int NT, bool KEEP>
+void launch_draw(const SampleParams& p, int per_unit, hipStream_t stream) {
+    const long long slots = 256ll * per_unit, turns = (p.rows + slots - 1) / slots;
+    const dim3 grid((unsigned)((p.rows + turns - 1) / turns));
+    hipLaunchKernelGGL((sample_draw_kernel<E, NT, KEEP>), grid, dim3(NT), 0, stream, p);
+}
+
+template <class E, int NT>
+void launch_draws(const SampleParams& p, int per_unit, hipStream_t stream) {
+    p.min_ps || p.min_p > 0. ? launch_draw<E, NT, true>(p, per_unit, stream) : launch_draw<E, NT, false>(p, per_unit, stream);
+}
+
+// Whether nothing but min_p cuts the rows.
+bool draws(const SampleParams& p) { return !p.top_ks && !p.top_ps && (p.top_k <= 0 || p.top_k >= p.V) && !(p.top_p < 1.); }
+
 // Parts of a row, 1 where it is not shared out: few wide rows, but for a top_k that
 // one wave handles (of which a call with a top_k for each row may hold some). us
 // on MI355X, bf16, one workgroup a row against parts of 4096 columns and more:
-//   top_p 0.9: 16 rows of 32000 22 / 23, of 50001 34 / 25, of 131072 58 / 35; 64 rows 22 / 26, 34 / 29, 59 / 47; 128 23 / 28, 34 / 33, 60 / 62
-//   whole distributions: 16 rows 16 / 16, 22 / 16, 41 / 18; 64 rows 17 / 18, 23 / 19, 41 / 30; 128 17 / 21, 23 / 24, 43 / 42
-//   top_k 1000: 64 rows 27 / 25, 37 / 27, 66 / 39; top_k 50: 16 rows 12 / 19, 15 / 22, 18 / 27
+//   top_p 0.9: 16 rows of 32000 22 / 23, of 50001 33 / 25, of 131072 57 / 37; 64 rows 22 / 26, 33 / 28, 58 / 47; 128 23 / 28, 34 / 33, 60 / 62
+//   whole distributions: 16 rows of 50001 19 / 16, of 131072 36 / 18; 64 rows 20 / 20, 36 / 30; 128 20 / 24, 37 / 42
+//   the same with min_p 0.05: 16 rows 15 / 18, 24 / 23; 64 rows 18 / 22, 26 / 34
+//   top_k 1000: 64 rows of 32000 27 / 25, of 50001 37 / 27, of 131072 66 / 39; top_k 50: 16 rows 12 / 19, 15 / 22, 18 / 27
 // Parts of 8192 columns: top_p 0.95, 4 rows of 50001 30 for 27, as long at 131072.
 int row_parts(const SampleParams& p) {
-    if (p.V < SAMPLE_MIN_V || p.rows > SAMPLE_MAX_ROWS || p.rows <= 0 || (!p.top_ks && p.top_k > 0 && p.top_k <= SM_TOP)) return 1;
+    if (p.V < (draws(p) ? 2 * SAMPLE_MIN_V : SAMPLE_MIN_V) || p.rows > SAMPLE_MAX_ROWS || p.rows <= 0 || (!p.top_ks && p.top_k > 0 && p.top_k <= SM_TOP)) return 1;
     return min(p.V / SAMPLE_PART_COLS, SAMPLE_PARTS);
 }
 
@@ -944,6 +1214,8 @@ void launch(SampleParams p, hipStream_t stream) {
         hipLaunchKernelGGL(sample_stats_kernel<E>, grid, dim3(256), 0, stream, p);
         hipLaunchKernelGGL(sample_bins_kernel<E>, grid, dim3(256), 0, stream, p);
         hipLaunchKernelGGL((sample_kernel<E, 1024, true>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
+    } else if (p.rows > 0 && draws(p)) {
+        p.V <= 8192 ? launch_draws<E, 256>(p, 8, stream) : launch_draws<E, 512>(p, 4, stream);
     } else if (p.V <= 8192) {
         launch_rows<E, 256>(p, stream);
     } else if (p.rows <= 256) {
@@ -952,10 +1224,10 @@ void launch(SampleParams p, hipStream_t stream) {
         launch_rows<E, 512>(p, stream);
     }
     // Threads of a row by us on MI355X, bf16, 256 / 512 / 1024 threads:
-    //   4096 columns, 1024 rows: whole 14 / 18 / 33, top_k 50 15 / 20 / 34, top_p 0.9 20 / 29 / 52; 1 row: 7 / 7 / 8, 11 / 9 / 9, 12 / 12 / 13
+    //   4096 columns, 1024 rows: top_k 50 15 / 20 / 34, top_p 0.9 20 / 29 / 52; 1 row: 11 / 9 / 9, 12 / 12 / 13
     //   16384, 1024 rows: top_k 21 / 25 / 40, top_p 46 / 46 / 70; 1 row: 15 / 11 / 10, 27 / 17 / 17
-    //   32000, 1024 rows: whole 62 / 54 / 66, top_k 33 / 35 / 48, top_p 0.95 79 / 74 / 95; 64 rows: top_p 41 / 27 / 24
-    //   50001 fp32, 1021 rows: whole 116 / 100 / 112, top_k 65 / 67 / 80, top_p 336 / 140 / 173
+    //   32000, 1024 rows: top_k 33 / 35 / 48, top_p 0.95 79 / 74 / 95; 64 rows: top_p 41 / 27 / 24
+    //   50001 fp32, 1021 rows: top_k 65 / 67 / 80, top_p 336 / 140 / 173
 }
 
 }  // namespace
