@@ -282,6 +282,31 @@ def test_sample_of_few_wide_rows_with_settings_of_each(V, dtype):
     assert got.ids[8:11].tolist() == [4000, 0, 4] and got.logprob[8:11].isnan().all()
 
 
+@pytest.mark.parametrize("rows,V,dtype", [(2100, 3, F32), (4111, 37, BF), (2309, 1022, F16), (1031, 8205, BF), (1030, 8194, F32), (5, 8191, BF)])
+def test_sample_of_whole_rows_in_turn(rows, V, dtype):
+    """More rows than workgroups, which take them one after another: ordinary rows
+    beside those without probabilities, greedy ones, rows of one value."""
+    x = (_randn(V, rows, V) * 3).to(dtype)
+    kind = _randint(rows, 8, rows)
+    kind[-3:] = torch.tensor([0, 1, 7])
+    x[kind == 0, V // 2] = NAN
+    x[kind == 1] = -INF
+    x[kind == 2, V - 1] = INF
+    x[kind == 3] = 0.25
+    x[kind == 4, : V - 1] = -INF
+    u, T = _rand(1, rows), 0.2 + 2 * _rand(2, rows)
+    T[kind == 5] = 0.0
+    for least in (0.0, 0.3 * _rand(3, rows) - 0.05):
+        got = _ops().sample_tokens(x.cuda(), u.cuda(), temperature=T.cuda(), min_p=least.cuda() if isinstance(least, torch.Tensor) else least)
+        fine = (kind > 2).nonzero()[:, 0]
+        own = least[fine] if isinstance(least, torch.Tensor) else least
+        _check_choice(x[fine], u[fine], type(got)(got.ids.cpu()[fine], got.logprob.cpu()[fine]), T[fine], 0, 1.0, own, (rows, V))
+        for k, at in ((0, V // 2), (1, 0), (2, V - 1)):
+            assert (got.ids.cpu()[kind == k] == at).all() and got.logprob.cpu()[kind == k].isnan().all()
+    again = _ops().sample_tokens(x[7:].cuda(), u[7:].cuda(), temperature=T[7:].cuda(), min_p=least[7:].cuda())  # others' turns
+    assert torch.equal(again.ids, got.ids[7:]) and torch.equal(again.logprob.nan_to_num(9.0), got.logprob[7:].nan_to_num(9.0))
+
+
 def test_sample_at_the_borders():
     """Weights whose sums are exact: which token a number on a border takes, ties
     by the lower id, the first kept and the last number below one."""
