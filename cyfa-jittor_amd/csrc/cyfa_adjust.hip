@@ -17,6 +17,17 @@
 // and the listed columns are formed and stored a second time. So the pass reads no
 // counts, and runs at the memory's rate. (In place it has to read them: a listed
 // column's logit is gone after the pass.)
+//
+// Bound by memory where rows are many. On MI355X 4096 x 32000 bf16 with histories of
+// 1280 take 116 us (0.52 GB of logits and 42 MB of tokens: 4.9 TB/s, where a copy
+// of 1 GiB moves 5.0) and their gradient 142, which reads the listed columns' logits
+// besides, a cache line for each; 256 x 50001 fp16 with a bias, a mask of bytes and
+// 8191 tokens a row 36 (81 MB, 2.2 TB/s: two slices of a row each read its tokens
+// and mark them one by one before the listed columns can be stored). Few rows are bound
+// by the steps of a workgroup, the tokens' load, the marks, the list and a second
+// load and store: 64 x 32000 with 2048 tokens, 16 token biases and a bit mask 9 us,
+// one row 5. When every vector read its columns' counts, the 4096 rows took 502 with
+// their gradient for 349 by the list (and 262 by larger slices).
 #include "cyfa_internal.h"
 #include "cyfa_rows.h"
 

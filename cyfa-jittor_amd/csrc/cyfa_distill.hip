@@ -14,6 +14,12 @@
 // its own: at the end of the row's pass three waves of four would wait for it. The
 // columns of no entry keep a maximum and a sum of their own with the tail: taken
 // as the difference of the row's sum and the entries', a small rest would be lost.
+//
+// Bound by memory. On MI355X 16384 x 32000 bf16 rows with 20 entries (1.05 GB) take
+// 139 us for the sums (7.5 TB/s), 11 for the entries, 5 for the mean and 344 for the
+// gradient (6.1 TB/s both ways; a copy of 1 GiB moves 5.0); 1021 x 50001 fp16 rows
+// with a tail and 64 entries 22, 7, 3 and 34 (4.7 and 6.0 TB/s). A few rows of 256
+// columns take 4, 4, 2 and 5, the latency of each launch's loads.
 #include "cyfa_internal.h"
 #include "cyfa_rows.h"
 
