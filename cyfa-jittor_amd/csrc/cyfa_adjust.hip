@@ -19,9 +19,10 @@
 // column's logit is gone after the pass.)
 //
 // Bound by memory where rows are many. On MI355X 4096 x 32000 bf16 with histories of
-// 1280 take 116 us (0.52 GB of logits and 42 MB of tokens: 4.9 TB/s, where a copy
-// of 1 GiB moves 5.0) and their gradient 142, which reads the listed columns' logits
-// besides, a cache line for each; 256 x 50001 fp16 with a bias, a mask of bytes and
+// up to 1280 tokens, each shared by 1024 rows, take 116 us (0.52 GB: 4.5 TB/s, where
+// a copy of 1 GiB moves 5.0 to 5.2; the columns' second stores write 45 MB more) and
+// their gradient 142, which reads the listed columns' logits besides, a cache line
+// for each (0.13 GB more); 256 x 50001 fp16 with a bias, a mask of bytes and
 // 8191 tokens a row 36 (81 MB, 2.2 TB/s: two slices of a row each read its tokens
 // and mark them one by one before the listed columns can be stored). Few rows are bound
 // by the steps of a workgroup, the tokens' load, the marks, the list and a second

@@ -15,11 +15,12 @@
 // columns of no entry keep a maximum and a sum of their own with the tail: taken
 // as the difference of the row's sum and the entries', a small rest would be lost.
 //
-// Bound by memory. On MI355X 16384 x 32000 bf16 rows with 20 entries (1.05 GB) take
-// 139 us for the sums (7.5 TB/s), 11 for the entries, 5 for the mean and 344 for the
-// gradient (6.1 TB/s both ways; a copy of 1 GiB moves 5.0); 1021 x 50001 fp16 rows
-// with a tail and 64 entries 22, 7, 3 and 34 (4.7 and 6.0 TB/s). A few rows of 256
-// columns take 4, 4, 2 and 5, the latency of each launch's loads.
+// Bound by memory. On MI355X 16384 x 32000 bf16 rows with 20 entries, of which 78 %
+// count (0.82 GB of logits read, 1.05 of gradient written), take 139 us for the sums
+// (5.9 TB/s), 11 for the entries, 5 for the mean and 344 for the gradient (5.4 TB/s
+// both ways; a copy of 1 GiB moves 5.0 to 5.2); 1021 x 50001 fp16 rows with a tail and
+// 64 entries, 65 % of them counting, 22, 7, 3 and 34. A few rows of 256 columns take 4,
+// 4, 2 and 5, the latency of each launch's loads.
 #include "cyfa_internal.h"
 #include "cyfa_rows.h"
 
