@@ -90,6 +90,8 @@ class Sampler:
     def choose(self, logits, allowed=None):
         """The next tokens [B] for logits [B, V], kept as the sequences' last; the
         caller has counted them (``take``). ``allowed`` in place of the Sampling's."""
+        if logits.dim() != 2 or logits.shape[0] != self.history.shape[0]:
+            raise ValueError(f"a Sampler of {self.history.shape[0]} sequences needs their logits [B, V], got {tuple(logits.shape)}")
         if allowed is None:
             allowed = self._allowed if isinstance(self._allowed, torch.Tensor) else None
         else:

@@ -179,6 +179,10 @@ def test_sampler_refuses():
         sampler.next(torch.zeros(3, 9))
 
 
+    sampler = Sampler(Sampling(), torch.zeros(1, 2, dtype=torch.int64), 4)
+    for shape in ((3, 9), (9,), (1, 1, 9)):
+        with pytest.raises(ValueError, match="sequences"):
+            sampler.next(torch.zeros(shape))
     for lengths in (torch.tensor([1, 2]), torch.tensor([1, 2, 3]), torch.tensor([0, -1, 2]), torch.tensor([1.0, 1.0, 1.0])):
         with pytest.raises(ValueError, match="lengths"):
             Sampler(Sampling(), torch.zeros(3, 2, dtype=torch.int64), 1, lengths)
