@@ -91,6 +91,19 @@ __device__ __forceinline__ u64 lane_u64(u64 x, int lane) {
 // The sum over the lanes, in every lane.
 __device__ __forceinline__ u64 wave_add(u64 x) { return lane_u64(wave_scan(x), 63); }
 
+// The sum over eight lanes (8 i .. 8 i + 7), in each of them.
+__device__ __forceinline__ unsigned eight_add(unsigned x) {
+    x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, false);
+    x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, false);
+    return x + (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xF, 0xF, false);
+}
+
+__device__ __forceinline__ u64 eight_add(u64 x) {
+    x += dpp_or_zero<0xB1>(x);
+    x += dpp_or_zero<0x4E>(x);
+    return x + dpp_or_zero<0x141>(x);
+}
+
 // The largest of the lanes, in every lane: as wave_max.
 __device__ __forceinline__ u64 wave_most(u64 x) {
     const auto most = [](u64 a, u64 b) { return a > b ? a : b; };
@@ -511,11 +524,12 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
                 if ((tid & 7) == 0 && rank < k) all_s[rank] = key;
             }
             __syncthreads();
-            if (wv == 0) {  // a lane to each of the first 64 and to each of the second
-                u64 keys[2], w[2], sum[2], before = 0;
-                float e[2];
+            const auto draw = [&](auto halves) {  // a lane to each of the first 64 and (2) to each of the second
+                constexpr int H = decltype(halves)::value;
+                u64 keys[H], w[H], sum[H], before = 0;
+                float e[H];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int h = 0; h < H; h++) {
                     keys[h] = lane + 64 * h < k ? all_s[lane + 64 * h] : 0;
                     e[h] = key_value(keys[h]);
                     w[h] = lane + 64 * h < k ? weight(ch, e[h]) : 0;
@@ -524,21 +538,23 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
                 }
                 int kept = 0;
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int h = 0; h < H; h++)
                     kept += __popcll(__ballot((lane == 0 && h == 0) || (lane + 64 * h < k && e[h] >= lowest &&
                                                                         !(cut_p && (double)(sum[h] - w[h]) >= top_p * (double)before))));
-                const u64 total = kept > 64 ? lane_u64(sum[1], kept - 65) : lane_u64(sum[0], kept - 1), target = mass_at(u, total);
-                u64 upto[2] = {0, 0};  // the mass of the kept up to these by index
+                const u64 total = H > 1 && kept > 64 ? lane_u64(sum[H - 1], kept - 65) : lane_u64(sum[0], kept - 1), target = mass_at(u, total);
+                u64 upto[H] = {};  // the mass of the kept up to these by index
                 const auto pass = [&](u64 other, u64 ow) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++) upto[h] += (uint32_t)other >= (uint32_t)keys[h] ? ow : 0;
+                    for (int h = 0; h < H; h++) upto[h] += (uint32_t)other >= (uint32_t)keys[h] ? ow : 0;
                 };
                 for (int i = 0; i < min(kept, 64); i++) pass(lane_u64(keys[0], i), lane_u64(w[0], i));
-                for (int i = 64; i < kept; i++) pass(lane_u64(keys[1], i - 64), lane_u64(w[1], i - 64));
+                if (H > 1)
+                    for (int i = 64; i < kept; i++) pass(lane_u64(keys[H - 1], i - 64), lane_u64(w[H - 1], i - 64));
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int h = 0; h < H; h++)
                     if (lane + 64 * h < kept && upto[h] > target && upto[h] - w[h] <= target) put(key_index(keys[h]), w[h], total);
-            }
+            };
+            if (wv == 0) k <= 64 ? draw(std::integral_constant<int, 1>{}) : draw(std::integral_constant<int, 2>{});
             return;
         }
         from = thr;  // many equal elements: the bins tell
@@ -816,7 +832,9 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
         if (BOTH && tid < (int)n) list_w[tid] = weight(ch, key_value(list_s[tid]));
         __syncthreads();
         // each against each, eight threads to one
-        for (int at = tid / 8; at < (int)n; at += NT / 8) {
+        u64 lowest_key = ~0ull, kept_mass = 0;
+        for (int at0 = 0; at0 < (int)n; at0 += NT / 8) {
+            const int at = min(at0 + tid / 8, (int)n - 1);
             const u64 key = list_s[at];
             unsigned before = 0;
             u64 mass = 0;
@@ -826,15 +844,18 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
                 before += first;
                 if (BOTH) mass += first ? list_w[i] : 0;
             }
-#pragma unroll
-            for (int d = 4; d > 0; d >>= 1) {
-                before += __shfl_xor(before, d);
-                if (BOTH) mass += __shfl_xor(mass, d);
+            before = eight_add(before);
+            if (BOTH) mass = eight_add(mass);
+            if ((tid & 7) == 0 && at0 + tid / 8 < (int)n && !dropped(ca + before, wa + mass, total)) {
+                lowest_key = key < lowest_key ? key : lowest_key;
+                if (BOTH) kept_mass += list_w[at];
             }
-            if ((tid & 7) == 0 && !dropped(ca + before, wa + mass, total)) {
-                atomicMin(&found_key, key);
-                if (BOTH) atomicAdd(&found_kept, list_w[at]);
-            }
+        }
+        lowest_key = ~wave_most(~lowest_key);
+        if (BOTH) kept_mass = wave_add(kept_mass);
+        if (lane == 0) {
+            atomicMin(&found_key, lowest_key);
+            if (BOTH) atomicAdd(&found_kept, kept_mass);
         }
         __syncthreads();
         base = found_key;
@@ -855,8 +876,7 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     // ---- the draw: the runs' masses, those of a wave each of the run of the token, that wave
     const bool every = base == 0;
     const auto kept = [&](float e, int i) { return every || e > from || (e == from && order_key(e, i) >= base); };
-    const auto piece_weight = [&](int i) {
-        const Piece v = piece(i);
+    const auto mass_of = [&](const Piece& v, int i) {
         float top = wide(v[0]);
 #pragma unroll
         for (int c = 1; c < P; c++) top = fmaxf(top, wide(v[c]));
@@ -868,12 +888,6 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
                 s += kept(wide(v[c]), i * P + c) ? w : 0;
             }
         return s;
-    };
-    const auto wave_mass = [&](int begin, int end) {
-        u64 s = 0;
-#pragma unroll 1
-        for (int i = begin + lane; i < end; i += 64) s += piece_weight(i);
-        return wave_add(s);
     };
     if (counted) {  // by bins
         const int border = every ? BINS : bins.of(from);
@@ -900,44 +914,61 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
     } else {
         runs = W;
         run_len = (npiece + W - 1) / W;
-        const int begin = min(wv * run_len, npiece);
-        const u64 s = wave_mass(begin, min(begin + run_len, npiece));
+        const int begin = min(wv * run_len, npiece), end = min(begin + run_len, npiece);
+        u64 s = 0;
+#pragma unroll 1
+        for (int i = begin + lane; i < end; i += 64) s += mass_of(piece(i), i);
+        s = wave_add(s);
         if (lane == 0) runs_s[wv] = s;
         __syncthreads();
     }
-    total = 0;
-    for (int i = 0; i < runs; i++) total += runs_s[i];
+    const u64 upto_run = wave_scan(lane < runs ? runs_s[lane] : 0);
+    total = lane_u64(upto_run, 63);
     const u64 target = mass_at(u, total);
-    u64 passed = 0;
-    int run = 0;
-    while (run < runs - 1 && passed + runs_s[run] <= target) passed += runs_s[run++];
+    const int run = min(__popcll(__ballot(upto_run <= target)), runs - 1);
+    u64 passed = run > 0 ? lane_u64(upto_run, run - 1) : 0;
     int begin = min(run * run_len, npiece), end = min(begin + run_len, npiece);
     const int len = (end - begin + W - 1) / W;
     begin = min(begin + wv * len, end);
     end = min(begin + len, end);
-    const u64 sum = wave_mass(begin, end);
+    u64 sum = 0, last_mass = 0;
+    Piece last;  // this lane's last piece, and its mass
+#pragma unroll 1
+    for (int i = begin + lane; i < end; i += 64) {
+        last = piece(i);
+        last_mass = mass_of(last, i);
+        sum += last_mass;
+    }
+    sum = wave_add(sum);
     if (lane == 0) red_s[0][wv] = sum;
     __syncthreads();
-    for (int w = 0; w < wv; w++) passed += red_s[0][w];
+    const u64 upto_part = wave_scan(lane < W ? red_s[0][lane] : 0);
+    if (wv > 0) passed += lane_u64(upto_part, wv - 1);
     if (passed <= target && target < passed + sum) {  // (one wave)
 #pragma unroll 1
         for (int i0 = begin; i0 < end; i0 += 64) {
             const int i = i0 + lane;
-            const u64 s = i < end ? piece_weight(i) : 0;
-            const u64 upto = wave_scan(s), all = lane_u64(upto, 63);
+            if (len > 64) {
+                if (i < end) last = piece(i);
+                last_mass = i < end ? mass_of(last, i) : 0;
+            }
+            const u64 upto = wave_scan(last_mass), all = lane_u64(upto, 63);
             if (passed + all > target) {
-                u64 mass = passed + upto - s;
-                if (mass <= target && target < mass + s) {  // (one lane)
-#pragma unroll 1
+                u64 mass = passed + upto - last_mass;
+                if (mass <= target && target < mass + last_mass) {  // (one lane)
+                    int at = -1;
+                    u64 taken = 0;
+#pragma unroll
                     for (int c = 0; c < P; c++) {
-                        const float e = wide(x[(size_t)i * P + c]);
+                        const float e = wide(last[c]);
                         const u64 w = kept(e, i * P + c) ? weight(ch, e) : 0;
                         mass += w;
-                        if (mass > target) {
-                            put(i * P + c, w, total);
-                            break;
+                        if (at < 0 && mass > target) {
+                            at = i * P + c;
+                            taken = w;
                         }
                     }
+                    put(at, taken, total);
                 }
                 break;
             }
