@@ -312,7 +312,7 @@ __device__ __forceinline__ PartStats join_parts(const SampleParams& p, long long
 }
 
 // The counts and masses of a part's bins (16 rows of 131072 bf16, a part of 4096 to
-// a workgroup: the statistics 3.5 us, the bins 7, the rows themselves 26).
+// a workgroup: the statistics 3 us, the bins 6, the rows themselves 25).
 template <class E>
 __global__ __launch_bounds__(256) void sample_bins_kernel(SampleParams p) {
     constexpr int P = SM_PIECE;
@@ -1220,10 +1220,10 @@ bool draws(const SampleParams& p) { return !p.top_ks && !p.top_ps && (p.top_k <=
 // Parts of a row, 1 where it is not shared out: few wide rows, but for a top_k that
 // one wave handles (of which a call with a top_k for each row may hold some). us
 // on MI355X, bf16, one workgroup a row against parts of 4096 columns and more:
-//   top_p 0.9: 16 rows of 32000 22 / 23, of 50001 33 / 25, of 131072 57 / 37; 64 rows 22 / 26, 33 / 28, 58 / 47; 128 23 / 28, 34 / 33, 60 / 62
-//   whole distributions: 16 rows of 50001 19 / 16, of 131072 36 / 18; 64 rows 20 / 20, 36 / 30; 128 20 / 24, 37 / 42
-//   the same with min_p 0.05: 16 rows 15 / 18, 24 / 23; 64 rows 18 / 22, 26 / 34
-//   top_k 1000: 64 rows of 32000 27 / 25, of 50001 37 / 27, of 131072 66 / 39; top_k 50: 16 rows 12 / 19, 15 / 22, 18 / 27
+//   top_p 0.9: 16 rows of 32000 21 / 22, of 50001 32 / 24, of 131072 54 / 33; 64 rows 21 / 24, 32 / 27, 55 / 45; 128 22 / 27, 32 / 32, 57 / 57
+//   whole distributions: 16 rows of 50001 19 / 16, of 131072 36 / 16; 64 rows 19 / 18, 37 / 28; 128 20 / 23, 37 / 38
+//   the same with min_p 0.05: 16 rows 16 / 17, 22 / 21; 64 rows 17 / 21, 26 / 30
+//   top_k 1000: 64 rows of 32000 25 / 24, of 50001 36 / 26, of 131072 66 / 36; top_k 50: 16 rows 11 / 18, 14 / 21, 18 / 25
 // Parts of 8192 columns: top_p 0.95, 4 rows of 50001 30 for 27, as long at 131072.
 int row_parts(const SampleParams& p) {
     if (p.V < (draws(p) ? 2 * SAMPLE_MIN_V : SAMPLE_MIN_V) || p.rows > SAMPLE_MAX_ROWS || p.rows <= 0 || (!p.top_ks && p.top_k > 0 && p.top_k <= SM_TOP)) return 1;
@@ -1255,10 +1255,10 @@ void launch(SampleParams p, hipStream_t stream) {
         launch_rows<E, 512>(p, stream);
     }
     // Threads of a row by us on MI355X, bf16, 256 / 512 / 1024 threads:
-    //   4096 columns, 1024 rows: top_k 50 15 / 20 / 34, top_p 0.9 20 / 29 / 52; 1 row: 11 / 9 / 9, 12 / 12 / 13
-    //   16384, 1024 rows: top_k 21 / 25 / 40, top_p 46 / 46 / 70; 1 row: 15 / 11 / 10, 27 / 17 / 17
-    //   32000, 1024 rows: top_k 33 / 35 / 48, top_p 0.95 79 / 74 / 95; 64 rows: top_p 41 / 27 / 24
-    //   50001 fp32, 1021 rows: top_k 65 / 67 / 80, top_p 336 / 140 / 173
+    //   4096 columns, 1024 rows: top_k 50 15 / 18 / 32, top_p 0.9 18 / 24 / 47; 1 row: 11 / 9 / 9, 11 / 11 / 12
+    //   16384, 1024 rows: 20 / 23 / 37, 40 / 36 / 62; 1 row: 14 / 11 / 10, 18 / 15 / 16
+    //   32000, 1024 rows: 32 / 34 / 45, 72 / 60 / 82; 64 rows: 20 / 14 / 12, 37 / 23 / 21
+    //   50001 fp32, 1021 rows: 65 / 69 / 71, 248 / 114 / 135
 }
 
 }  // namespace
