@@ -15,20 +15,23 @@
 // behind the prompt; integers, so that their order does not matter) and lists the
 // columns that it meets; the slice is passed over as where nothing is repeated,
 // and the listed columns are formed and stored a second time. So the pass reads no
-// counts, and runs at the memory's rate. (In place it has to read them: a listed
-// column's logit is gone after the pass.)
+// counts and does not wait for them. Where many columns are met, or many workgroups
+// take turns anyway, it does read them, and nothing is stored twice. (In place a
+// listed column's logit is gone after the pass, which is made for what it has met.)
 //
 // Bound by memory where rows are many. On MI355X 4096 x 32000 bf16 with histories of
-// up to 1280 tokens, each shared by 1024 rows, take 116 us (0.52 GB: 4.5 TB/s, where
-// a copy of 1 GiB moves 5.0 to 5.2; the columns' second stores write 45 MB more) and
-// their gradient 142, which reads the listed columns' logits besides, a cache line
-// for each (0.13 GB more); 256 x 50001 fp16 with a bias, a mask of bytes and
-// 8191 tokens a row 36 (81 MB, 2.2 TB/s: two slices of a row each read its tokens
-// and mark them one by one before the listed columns can be stored). Few rows are bound
+// up to 1280 tokens, each shared by 1024 rows, take 113 us (0.52 GB: 4.6 TB/s, where
+// a copy of 1 GiB moves 5.0 to 5.2) and their gradient 142, which reads the listed
+// columns' logits besides, a cache line for each, and stores them a second time (0.13
+// GB more); 256 x 50001 fp16 with a bias, a mask of bytes and 8191 tokens a row 29
+// (81 MB, 2.8 TB/s: two slices of a row each read its tokens and mark them one by
+// one before their pass). Few rows are bound
 // by the steps of a workgroup, the tokens' load, the marks, the list and a second
 // load and store: 64 x 32000 with 2048 tokens, 16 token biases and a bit mask 9 us,
 // one row 5. When every vector read its columns' counts, the 4096 rows took 502 with
 // their gradient for 349 by the list (and 262 by larger slices).
+#include <type_traits>
+
 #include "cyfa_internal.h"
 #include "cyfa_rows.h"
 
@@ -105,24 +108,28 @@ __global__ __launch_bounds__(NT) void adjust_kernel(AdjustParams p) {
     const float repetition = p.repetitions ? p.repetitions[r] : p.repetition;
     const float presence = p.presences ? p.presences[r] : p.presence;
     const float frequency = p.frequencies ? p.frequencies[r] : p.frequency;
-    const auto result = [&](int c, uint32_t w, float xc, float value) {
+    const auto penalised = [&](uint32_t w, float e) {
         const uint32_t made = w & C::MADE;
+        if (w & (C::SEEN | C::MADE)) e = e > 0.f ? e / repetition : e * repetition;
+        if (made) e = e - ((float)made * frequency + presence);
+        return e;
+    };
+    const auto result = [&](int c, uint32_t w, float xc, float value) {
         if (GRAD) {
             float e = (float)from[c];
             if (e != 0.f) e *= xc > 0.f ? 1.f / repetition : repetition;
             return kept(c) ? e : 0.f;
         }
-        float e = xc;
-        if (w & (C::SEEN | C::MADE)) e = e > 0.f ? e / repetition : e * repetition;
-        if (made) e = e - ((float)made * frequency + presence);
+        float e = penalised(w, xc);
         if (bias) e = e + bias[c];
         if (w & C::BIASED) e = e + value;
         return kept(c) ? e : -INFINITY;
     };
-    const bool apart = GRAD || y != x;
-    // ---- the slice as where nothing is repeated
+    const bool apart = GRAD || y != x, dense = !GRAD && apart && p.dense;  // (the pass reads the counts)
+    // ---- the slice as where nothing is repeated, or (COUNTED) with what its columns have met
     const float out = GRAD ? 0.f : -INFINITY;
-    const auto pass = [&]() {
+    const auto pass = [&](auto with_counts) {
+        constexpr bool COUNTED = decltype(with_counts)::value;
         const int nvec = cols / N, tail = cols - nvec * N;
         for (int i0 = 0; i0 < nvec; i0 += NT * AJ_NV) {
             Vec v[AJ_NV];
@@ -142,7 +149,29 @@ __global__ __launch_bounds__(NT) void adjust_kernel(AdjustParams p) {
             for (int j = 0; j < AJ_NV; j++) {
                 const int i = i0 + j * NT + tid;
                 if (i >= nvec) continue;
-                if (bias) {
+                if (COUNTED) {
+                    constexpr int M = N * BITS / 32;
+                    uint32_t met[M], any = 0;
+                    __builtin_memcpy(met, lds + (size_t)i * M, sizeof met);
+#pragma unroll
+                    for (int c = 0; c < M; c++) any |= met[c];
+                    if (any || bias) {
+                        float e[N];
+#pragma unroll
+                        for (int c = 0; c < N; c++) e[c] = (float)v[j][c];
+                        if (any)
+#pragma unroll
+                            for (int c = 0; c < N; c++) e[c] = penalised(C::of(met[c * BITS / 32], c), e[c]);
+                        if (bias) {
+                            float b[N];
+                            __builtin_memcpy(b, bias + (size_t)i * N, sizeof b);
+#pragma unroll
+                            for (int c = 0; c < N; c++) e[c] = e[c] + b[c];
+                        }
+#pragma unroll
+                        for (int c = 0; c < N; c++) v[j][c] = (E)e[c];
+                    }
+                } else if (bias) {
                     float b[N];
                     __builtin_memcpy(b, bias + (size_t)i * N, sizeof b);
 #pragma unroll
@@ -161,12 +190,13 @@ __global__ __launch_bounds__(NT) void adjust_kernel(AdjustParams p) {
         if (tid < tail) {
             const int c = nvec * N + tid;
             float e = (float)from[c];
+            if (COUNTED) e = penalised(counts[c], e);
             if (bias) e = e + bias[c];
             y[c] = (E)(kept(c) ? e : out);
         }
     };
     if (!touches) {
-        pass();
+        pass(std::false_type{});
         return;
     }
     // The first store of an output that is apart is on its way while the row's tokens are counted.
@@ -182,7 +212,7 @@ __global__ __launch_bounds__(NT) void adjust_kernel(AdjustParams p) {
             values_s[i] = v[i];
         }
     }
-    if (apart) pass();
+    if (apart && !dense) pass(std::false_type{});
     __syncthreads();
     for (long long i0 = 0; i0 < n; i0 += NT * U) {
         if (i0 > 0) load_tokens(i0);
@@ -191,7 +221,7 @@ __global__ __launch_bounds__(NT) void adjust_kernel(AdjustParams p) {
             const long long i = i0 + u * NT + tid, c = t[u] - c0;
             if (i < n && c >= 0 && c < cols) {
                 const uint32_t before = i < prompt ? counts.mark((int)c, C::SEEN) : counts.count((int)c);
-                if (before == 0) list[atomicAdd(&listed_s, 1)] = (uint16_t)c;
+                if (before == 0 && !dense) list[atomicAdd(&listed_s, 1)] = (uint16_t)c;
             }
         }
     }
@@ -222,6 +252,10 @@ __global__ __launch_bounds__(NT) void adjust_kernel(AdjustParams p) {
     }
     // ---- the touched columns
     if (apart) {
+        if (!GRAD && dense) {
+            pass(std::true_type{});
+            __syncthreads();
+        }
         for (int i = tid; i < listed_s; i += NT) {
             const int c = list[i];
             const uint32_t w = counts[c];
@@ -274,8 +308,20 @@ void launch_slices(AdjustParams p, long long cols, hipStream_t stream) {
     }
 }
 
+// Whether the pass over the logits reads the counts, after them, for a list of the
+// touched columns and a second store of each, beside which the pass is on its way
+// while the counting goes on. us on MI355X, list / counts, bf16:
+//   4096 x 32000, 64 tokens 105 / 101, 500 131 / 110, 1000 141 / 114, 4000 262 / 141; 1024 rows, 200 27 / 29, 500 30.5 / 30, 2000 44 / 35
+//   512 x 32000, 500 17 / 19, 1000 20 / 20, 2000 25 / 21; 64 rows, 1000 7.0 / 7.6, 2000 7.6 / 7.9, 4000 9.7 / 8.8, 16000 19 / 13
+//   256 x 50001 fp16, 1000 18 / 19, 2000 22 / 21, 4000 28 / 23, 8000 33 / 26, with a bias 39 / 28
+//   16384 x 4096, 200 69 / 71, 500 85 / 75; 1024 rows, 500 9.1 / 9.9, 1000 10.4 / 10.1, 4000 20 / 14; 4096 x 1000 fp32, 200 15.7 / 15.5, 1000 20 / 17
+bool reads_counts(const AdjustParams& p) {
+    return (p.L >= 500 && p.rows * p.V >= 1ll << 24) || (p.L * 4 >= min(p.V, 4096) && p.L * 14 >= p.V);
+}
+
 template <class E, bool GRAD>
-void launch(const AdjustParams& p, hipStream_t stream) {
+void launch(AdjustParams p, hipStream_t stream) {
+    p.dense = !GRAD && reads_counts(p);
     // Columns of a slice and threads that take it, by us on MI355X (forward / gradient
     // of bf16). Each slice reads the history; few large ones leave compute units idle:
     //   4096 x 32000, 768 tokens: 256 threads, 4096 columns 130 / 147, 8192 123 / 160; 512, 8192 136 / 148,

@@ -637,7 +637,7 @@ struct AdjustParams {
     const void* dy;              // gradient: [rows, V]
     void* y;                     // may be x, with its strides; gradient: dx
     long long y_outer, y_row;
-    int cols;                    // of a slice, set by the launcher
+    int cols, dense;             // of a slice; whether its pass reads the counts; set by the launcher
     long long first;             // a launch's first slice, set by the launcher
 };
 constexpr int ADJUST_MAX_TOKENS = 1024;
