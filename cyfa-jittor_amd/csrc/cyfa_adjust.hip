@@ -114,10 +114,13 @@ __global__ __launch_bounds__(NT) void adjust_kernel(AdjustParams p) {
         if (made) e = e - ((float)made * frequency + presence);
         return e;
     };
+    const auto sloped = [&](float e, float xc) {
+        if (e != 0.f) e *= xc > 0.f ? 1.f / repetition : repetition;
+        return e;
+    };
     const auto result = [&](int c, uint32_t w, float xc, float value) {
         if (GRAD) {
-            float e = (float)from[c];
-            if (e != 0.f) e *= xc > 0.f ? 1.f / repetition : repetition;
+            const float e = sloped((float)from[c], xc);
             return kept(c) ? e : 0.f;
         }
         float e = penalised(w, xc);
@@ -125,7 +128,7 @@ __global__ __launch_bounds__(NT) void adjust_kernel(AdjustParams p) {
         if (w & C::BIASED) e = e + value;
         return kept(c) ? e : -INFINITY;
     };
-    const bool apart = GRAD || y != x, dense = !GRAD && apart && p.dense;  // (the pass reads the counts)
+    const bool apart = GRAD || y != x, dense = apart && p.dense;  // (the pass reads the counts)
     // ---- the slice as where nothing is repeated, or (COUNTED) with what its columns have met
     const float out = GRAD ? 0.f : -INFINITY;
     const auto pass = [&](auto with_counts) {
@@ -145,23 +148,36 @@ __global__ __launch_bounds__(NT) void adjust_kernel(AdjustParams p) {
                     else
                         __builtin_memcpy(keep[j], allowed + c, N);
                 }
+            constexpr int M = N * BITS / 32;
+            uint32_t met[COUNTED ? AJ_NV : 1][M], any[COUNTED ? AJ_NV : 1];
+            Vec own[COUNTED && GRAD ? AJ_NV : 1];  // the logits of vectors with a column that was met
+            if (COUNTED)
+#pragma unroll
+                for (int j = 0; j < AJ_NV; j++) {
+                    const int i = min(i0 + j * NT + tid, nvec - 1);
+                    __builtin_memcpy(met[j], lds + (size_t)i * M, sizeof met[j]);
+                    any[j] = 0;
+#pragma unroll
+                    for (int c = 0; c < M; c++) any[j] |= met[j][c];
+                    if (GRAD && any[j]) own[j] = load_row(x + (size_t)i * N);
+                }
 #pragma unroll
             for (int j = 0; j < AJ_NV; j++) {
                 const int i = i0 + j * NT + tid;
                 if (i >= nvec) continue;
-                if (COUNTED) {
-                    constexpr int M = N * BITS / 32;
-                    uint32_t met[M], any = 0;
-                    __builtin_memcpy(met, lds + (size_t)i * M, sizeof met);
+                if (COUNTED && GRAD) {
+                    if (any[j])
 #pragma unroll
-                    for (int c = 0; c < M; c++) any |= met[c];
-                    if (any || bias) {
+                        for (int c = 0; c < N; c++)
+                            if (C::of(met[j][c * BITS / 32], c)) v[j][c] = (E)sloped((float)v[j][c], (float)own[j][c]);
+                } else if (COUNTED) {
+                    if (any[j] || bias) {
                         float e[N];
 #pragma unroll
                         for (int c = 0; c < N; c++) e[c] = (float)v[j][c];
-                        if (any)
+                        if (any[j])
 #pragma unroll
-                            for (int c = 0; c < N; c++) e[c] = penalised(C::of(met[c * BITS / 32], c), e[c]);
+                            for (int c = 0; c < N; c++) e[c] = penalised(C::of(met[j][c * BITS / 32], c), e[c]);
                         if (bias) {
                             float b[N];
                             __builtin_memcpy(b, bias + (size_t)i * N, sizeof b);
@@ -190,7 +206,8 @@ __global__ __launch_bounds__(NT) void adjust_kernel(AdjustParams p) {
         if (tid < tail) {
             const int c = nvec * N + tid;
             float e = (float)from[c];
-            if (COUNTED) e = penalised(counts[c], e);
+            if (COUNTED && !GRAD) e = penalised(counts[c], e);
+            if (COUNTED && GRAD && counts[c]) e = sloped(e, (float)x[c]);
             if (bias) e = e + bias[c];
             y[c] = (E)(kept(c) ? e : out);
         }
@@ -252,7 +269,7 @@ __global__ __launch_bounds__(NT) void adjust_kernel(AdjustParams p) {
     }
     // ---- the touched columns
     if (apart) {
-        if (!GRAD && dense) {
+        if (dense) {
             pass(std::true_type{});
             __syncthreads();
         }
@@ -321,7 +338,7 @@ bool reads_counts(const AdjustParams& p) {
 
 template <class E, bool GRAD>
 void launch(AdjustParams p, hipStream_t stream) {
-    p.dense = !GRAD && reads_counts(p);
+    p.dense = reads_counts(p);
     // Columns of a slice and threads that take it, by us on MI355X (forward / gradient
     // of bf16). Each slice reads the history; few large ones leave compute units idle:
     //   4096 x 32000, 768 tokens: 256 threads, 4096 columns 130 / 147, 8192 123 / 160; 512, 8192 136 / 148,
