@@ -20,16 +20,17 @@
 // listed column's logit is gone after the pass, which is made for what it has met.)
 //
 // Bound by memory where rows are many. On MI355X 4096 x 32000 bf16 with histories of
-// up to 1280 tokens, each shared by 1024 rows, take 113 us (0.52 GB: 4.6 TB/s, where
-// a copy of 1 GiB moves 5.0 to 5.2) and their gradient 142, which reads the listed
-// columns' logits besides, a cache line for each, and stores them a second time (0.13
-// GB more); 256 x 50001 fp16 with a bias, a mask of bytes and 8191 tokens a row 29
-// (81 MB, 2.8 TB/s: two slices of a row each read its tokens and mark them one by
-// one before their pass). Few rows are bound
-// by the steps of a workgroup, the tokens' load, the marks, the list and a second
-// load and store: 64 x 32000 with 2048 tokens, 16 token biases and a bit mask 9 us,
-// one row 5. When every vector read its columns' counts, the 4096 rows took 502 with
-// their gradient for 349 by the list (and 262 by larger slices).
+// up to 1280 tokens, each shared by 1024 rows, take 110 us (0.52 GB: 4.8 TB/s, where
+// a copy of 1 GiB moves 5.0 to 5.2) and their gradient 125, which reads the logits of
+// the vectors with a column that was met besides (0.09 GB more); 256 x 50001 fp16
+// with a bias, a mask of bytes and 8191 tokens a row 29 to 31 (81 MB, 2.7 TB/s: two slices
+// of a row each read its tokens and mark them one by one before their pass). Few rows
+// are bound by the steps of a workgroup, the tokens' load, the marks, the list and a
+// second load and store: 64 x 32000 with 2048 tokens, 16 token biases and a bit mask
+// 9 us, one row 5. The 4096 rows and their gradient took 502 when every vector of
+// 8192-column slices read 32-bit counts, 262 with 16 bits, larger slices and the list
+// in both, 235 where their pass reads 16-bit counts.
+
 #include <type_traits>
 
 #include "cyfa_internal.h"
@@ -332,6 +333,9 @@ void launch_slices(AdjustParams p, long long cols, hipStream_t stream) {
 //   512 x 32000, 500 17 / 19, 1000 20 / 20, 2000 25 / 21; 64 rows, 1000 7.0 / 7.6, 2000 7.6 / 7.9, 4000 9.7 / 8.8, 16000 19 / 13
 //   256 x 50001 fp16, 1000 18 / 19, 2000 22 / 21, 4000 28 / 23, 8000 33 / 26, with a bias 39 / 28
 //   16384 x 4096, 200 69 / 71, 500 85 / 75; 1024 rows, 500 9.1 / 9.9, 1000 10.4 / 10.1, 4000 20 / 14; 4096 x 1000 fp32, 200 15.7 / 15.5, 1000 20 / 17
+// The gradient, which reads the logits of the vectors with counts: 4096 x 32000, 200
+// tokens 129 / 120, 1000 182 / 142, 4000 403 / 170; 1024 rows, 500 35 / 31; 256 x 50001, 500 17.9 / 18.5, 2000 25 / 21; 64 x 32000, 1000
+// 7.0 / 7.1, 4000 9.7 / 8.2; 16384 x 4096, 200 82 / 77, 2000 308 / 127; 1024 x 4096, 500 9.0 / 9.0, 4000 23 / 14.
 bool reads_counts(const AdjustParams& p) {
     return (p.L >= 500 && p.rows * p.V >= 1ll << 24) || (p.L * 4 >= min(p.V, 4096) && p.L * 14 >= p.V);
 }
@@ -339,12 +343,10 @@ bool reads_counts(const AdjustParams& p) {
 template <class E, bool GRAD>
 void launch(AdjustParams p, hipStream_t stream) {
     p.dense = reads_counts(p);
-    // Columns of a slice and threads that take it, by us on MI355X (forward / gradient
-    // of bf16). Each slice reads the history; few large ones leave compute units idle:
-    //   4096 x 32000, 768 tokens: 256 threads, 4096 columns 130 / 147, 8192 123 / 160; 512, 8192 136 / 148,
-    //     16384 116 / 142 (stored past the caches 107 / 138 here, and no faster where a loss reads the results);
-    //     1024, 32000 120 / 140
-    //   256 x 50001 fp16 with a mask, 6100 tokens: 512, 8192 40, 16384 46; 1024, 16704 40, 25024 36
+    // Columns of a slice and threads that take it, by us on MI355X. Each slice reads
+    // the history; few large ones leave compute units idle:
+    //   4096 x 32000 bf16, 1000 tokens: 512 threads, 8192 columns 153, 16384 114; 1024, 32000 158
+    //   256 x 50001 fp16: 512, 16384: 2000 tokens 20, 8000 26, 16000 36; 1024, 25024 22, 26, 30
     //   64 x 32000 with a mask, 1500 tokens: 512, 8192 8.7, 16384 9.2; 1024, 25024 10.2
     //   1024 x 4096, 380 tokens: 256, 4096 7.3; 512 9.4
     const long long whole = (p.V + 31ll) / 32 * 32, slices = (whole + 32767) / 32768;
