@@ -634,6 +634,37 @@ def test_together_captured_and_replayed():
                 inputs[0].mul_(1.01)
 
 
+def test_wide_and_whole_rows_captured_and_replayed():
+    """The paths of few wide rows, of whole rows in turn and of long histories in two graphs, replayed in turn."""
+    ops, graphs = _ops(), []
+    for seed in (3, 4):
+        wide, many = (_randn(seed, 5, 50001) * 3).to(BF).cuda(), (_randn(seed + 1, 2500, 300) * 3).cuda()
+        history, u, v = _randint(seed, 300, 2500, 600).cuda(), _rand(seed, 5).cuda(), _rand(seed, 2500).cuda()
+
+        def run(wide=wide, many=many, history=history, u=u, v=v):
+            y = ops.adjust_logits(many, history, repetition=1.2, frequency=0.1)
+            return (*ops.sample_tokens(wide, u, top_p=0.9), *ops.sample_tokens(wide, u, temperature=2.0), y, *ops.sample_tokens(y, v, min_p=0.01))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = run()
+        graphs.append((g, run, out, (u, v, history)))
+    for n in range(4):
+        for g, _, _, (u, v, history) in graphs:
+            u.copy_(_rand(n, 5))
+            v.copy_(_rand(n + 9, 2500))
+            history.copy_(_randint(n, 300, 2500, 600))
+            g.replay()
+        torch.cuda.synchronize()
+        for _, run, out, _ in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, run()))
+
+
 def test_together_on_other_streams_and_threads():
     from concurrent.futures import ThreadPoolExecutor
 
