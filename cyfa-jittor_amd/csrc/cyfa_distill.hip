@@ -9,6 +9,8 @@
 //   loss = sum p_i (log p_i - log q_id) + p_r (log p_r - log q_r)
 //   dx_j = q_j P - sum of p_i over id_i = j, P = sum p_i + p_r,  at the entries' columns
 //   dx_j = (q_j / q_r) (q_r P - p_r)                             elsewhere
+// The loss is over the entries: where an id is there several times it is less than
+// with one entry of their whole mass, by a constant; the gradient is the same.
 // One pass over the row each way, sums in fp32; what the teacher's few entries
 // give is formed in double (1 - sum p_i cancels), by a wave a row in a launch of
 // its own: at the end of the row's pass three waves of four would wait for it. The

@@ -19,7 +19,13 @@ def distill_loss(logits, top_ids, top_logprobs, temperature=1.0, tail=False, wei
     p is exp(top_logprobs) itself and the rest of either distribution, the mass of
     all other tokens, one more outcome (temperature 1; V at most 2^19; nothing
     where the student's other logits are all -inf). Entries with an id outside
-    [0, V) or a log probability of -inf are left out; equal ids add up.
+    [0, V) or a log probability of -inf are left out.
+
+    The sum is over the entries, each with its own p and the q of its id, not over
+    the tokens. Teachers as score(top_k) gives them name a token once, and the two
+    are the same. Of a token that a row names several times, with p_1, p_2, ...
+    that add up to P, the gradient is that of one entry of P, and the loss is less
+    than the divergence by the constant sum p_i log(P / p_i): it may be negative.
 
     ``weights`` [...], float: each row's in the mean, 1 without. A row without
     entries or with weight 0 does not count, gets a gradient of zeros and is not

@@ -752,7 +752,9 @@ int cyfa_sample_tokens(const CyfaSampleArgs *args, int dtype, int grad, void *hi
  *     (nothing where those are all -inf)
  *   loss = sum of weights l / sum of weights, over the rows with an entry and a weight other than 0
  * and the logits' gradient (grad 1), contiguous, from kept and total as grad 0
- * left them; rows that do not count get zeros. Equal ids add up. No counterpart in the reference. */
+ * left them; rows that do not count get zeros. The sums of p are over the entries, each with a p of its
+ * own: of ids that are equal the gradient is that of one entry of their whole P, and l is that entry's less
+ * sum p_i log(P / p_i), a constant. No counterpart in the reference. */
 typedef struct CyfaDistillArgs {
     long long rows, inner;        /* inner > 0 */
     long long outer_stride, row_stride;

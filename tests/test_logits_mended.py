@@ -1,0 +1,40 @@
+"""The torch operations behind the operators on a model's logits where ids
+repeat and options leave their range (no GPU compute)."""
+
+import math
+
+import pytest
+import torch
+
+from cyclic_flow_attention import _native, ops
+from cyclic_flow_attention.ops import distill, sampling
+
+NAN = float("nan")
+
+
+@pytest.fixture(autouse=True)
+def in_torch(monkeypatch):
+    monkeypatch.setattr(_native, "require_device", lambda *tensors: tensors[0].device)
+    for module in (distill, sampling):
+        monkeypatch.setattr(module, "kernel_ok", lambda *tensors: False)
+
+
+def _randn(seed, *shape):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed))
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_a_token_named_several_times(tail):
+    """Entries of 0.1, 0.2 and 0.3 for one token against one of 0.6: the loss by
+    entries is less by the constant sum p_i log(P / p_i), the gradient the same."""
+    x = _randn(1, 1, 9).requires_grad_(True)
+    split, whole = torch.tensor([[0.1, 0.2, 0.3, 0.25]]), torch.tensor([[0.6, 0.25]])
+    losses, grads = [], []
+    for ids, p in ((torch.tensor([[5, 5, 5, 2]]), split), (torch.tensor([[5, 2]]), whole)):
+        losses.append(ops.distill_loss(x, ids, p.log(), tail=tail))
+        grads.append(torch.autograd.grad(losses[-1], [x])[0])
+    scale = 1.0 if tail else 1 / 0.85
+    less = scale * sum(p * math.log(0.6 / p) for p in (0.1, 0.2, 0.3))
+    # fp32 values of order one through sums of nine terms
+    assert abs(losses[1].item() - losses[0].item() - less) < 2.0**-19
+    assert (grads[0] - grads[1]).abs().max() < 2.0**-20
