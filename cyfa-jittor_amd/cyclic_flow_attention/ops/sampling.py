@@ -338,7 +338,7 @@ def _plain_sample(logits, uniform, temperature, top_k, top_p, min_p):
     kept = w * torch.zeros_like(w).scatter(-1, order, keep.to(w.dtype))
     mass = kept.cumsum(-1)
     total = mass[..., -1:]
-    passed = (mass <= uniform.double().clamp(0, 1 - 2.0**-53)[..., None] * total).sum(-1)
+    passed = (mass <= uniform.double().nan_to_num(0.0).clamp(0, 1 - 2.0**-53)[..., None] * total).sum(-1)
     last = torch.where(kept > 0, rank, 0).amax(-1)
     ids = torch.minimum(passed, last)
     logprob = (kept.gather(-1, ids[..., None]) / total).log()[..., 0]

@@ -38,3 +38,10 @@ def test_a_token_named_several_times(tail):
     # fp32 values of order one through sums of nine terms
     assert abs(losses[1].item() - losses[0].item() - less) < 2.0**-19
     assert (grads[0] - grads[1]).abs().max() < 2.0**-20
+
+
+def test_a_number_that_is_none_takes_the_first_kept_token():
+    x = torch.tensor([[1.0, 3, 3, 0, 2, 5], [-math.inf, 1, 0, 2, 2, 2], [0, 0, 0, 0, 0, 0]])
+    got = ops.sample_tokens(x, torch.full((3,), NAN), top_k=torch.tensor([1, 5, 0]), top_p=torch.tensor([1.0, 0.9, 1.0]))
+    zero = ops.sample_tokens(x, torch.zeros(3), top_k=torch.tensor([1, 5, 0]), top_p=torch.tensor([1.0, 0.9, 1.0]))
+    assert got.ids.tolist() == zero.ids.tolist() == [5, 1, 0] and torch.equal(got.logprob, zero.logprob)
