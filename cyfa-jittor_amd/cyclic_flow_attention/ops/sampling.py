@@ -282,7 +282,7 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
 
     Each option is a number or a tensor [...] (top_k int64 or int32, the others
     float, read in fp32). Temperature 0, or below in a tensor: the first largest
-    logit, logprob 0. A row that holds a NaN or +inf, or nothing but -inf, has no
+    logit, logprob 0. A min_p above 1 in a tensor counts as 1. A row that holds a NaN or +inf, or nothing but -inf, has no
     probabilities: its first largest logit (a NaN before all others), logprob NaN.
     A choice has no gradient: logits that require one are read as they are."""
     what = "sample_tokens"
@@ -334,7 +334,7 @@ def _plain_sample(logits, uniform, temperature, top_k, top_p, min_p):
     mass_of = torch.where((k <= 0) | (rank < k), sorted_w, 0.0)
     before = mass_of.cumsum(-1) - mass_of
     keep = (mass_of > 0) & ((rank == 0) | ~(p < 1) | (before < p * mass_of.sum(-1, keepdim=True)))
-    keep = keep & ((rank == 0) | ~(sorted_w < column(min_p)))
+    keep = keep & ((rank == 0) | ~(sorted_w < column(min_p).clamp(max=1.0)))
     kept = w * torch.zeros_like(w).scatter(-1, order, keep.to(w.dtype))
     mass = kept.cumsum(-1)
     total = mass[..., -1:]

@@ -714,7 +714,7 @@ int cyfa_adjust_logits(const CyfaAdjustArgs *args, int dtype, int grad, void *hi
  * them) with a number u in [0, 1) for each. With w_j = e^((x_j - max) / T), in the
  * order of falling x, the lower index first, kept are the first top_k (0 or V and
  * more: all), of those the ones before which less than top_p of their mass lies
- * (1 and more: all; the first is always kept), of those the ones with w >= min_p.
+ * (1 and more: all; the first is always kept), of those the ones with w >= min_p (above 1: as 1).
  * ids[r] is the first kept column, in the order of the columns, at which the
  * running mass of the kept passes u times their mass; logprob[r] the logarithm of
  * its share of that mass. T = 0: the first largest, logprob 0. A row that holds a

@@ -45,3 +45,13 @@ def test_a_number_that_is_none_takes_the_first_kept_token():
     got = ops.sample_tokens(x, torch.full((3,), NAN), top_k=torch.tensor([1, 5, 0]), top_p=torch.tensor([1.0, 0.9, 1.0]))
     zero = ops.sample_tokens(x, torch.zeros(3), top_k=torch.tensor([1, 5, 0]), top_p=torch.tensor([1.0, 0.9, 1.0]))
     assert got.ids.tolist() == zero.ids.tolist() == [5, 1, 0] and torch.equal(got.logprob, zero.logprob)
+
+
+def test_a_min_p_above_one_is_one():
+    """The tokens as large as the largest are kept, all of them."""
+    x = torch.tensor([[3.0, 0, 3, 3]]).expand(4, 4)
+    u, least = torch.tensor([0.1, 0.5, 0.9, 0.9]), torch.tensor([2.0, math.inf, 1.0, 1.5])
+    got = ops.sample_tokens(x, u, min_p=least)
+    assert got.ids.tolist() == [0, 2, 3, 3] and (got.logprob + math.log(3)).abs().max() < 1e-6
+    got = ops.sample_tokens(x, u, min_p=least, top_k=torch.tensor([2, 2, 1, 0]))
+    assert got.ids.tolist() == [0, 2, 0, 3]
