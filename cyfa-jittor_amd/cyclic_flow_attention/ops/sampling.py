@@ -282,8 +282,9 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
 
     Each option is a number or a tensor [...] (top_k int64 or int32, the others
     float, read in fp32). Temperature 0, or below in a tensor: the first largest
-    logit, logprob 0. A min_p above 1 in a tensor counts as 1. A row that holds a NaN or +inf, or nothing but -inf, has no
-    probabilities: its first largest logit (a NaN before all others), logprob NaN.
+    logit, logprob 0. A min_p above 1 in a tensor counts as 1. A row that holds
+    a NaN or +inf, or nothing but -inf, has no probabilities: its first largest
+    logit (a NaN before all others), logprob NaN.
     A choice has no gradient: logits that require one are read as they are."""
     what = "sample_tokens"
     _check_logits(what, logits)
@@ -327,7 +328,7 @@ def _plain_sample(logits, uniform, temperature, top_k, top_p, min_p):
     first = torch.where(nan.any(-1, keepdim=True), nan, x == top).int().argmax(-1)
     x = torch.where(none, 0.0, x)
     top = torch.where(none, 0.0, top)
-    w = torch.where(x == top, 1.0, torch.exp((x - top) / torch.where(greedy, 1.0, T)))
+    w = torch.where(x == top, 1.0, torch.exp((x - top) / torch.where(greedy, 1.0, T))).masked_fill(x == float("-inf"), 0.0)
     order = torch.sort(x, dim=-1, descending=True, stable=True).indices
     sorted_w = w.gather(-1, order)
     rank = torch.arange(V, device=x.device)

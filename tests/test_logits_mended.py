@@ -55,3 +55,13 @@ def test_a_min_p_above_one_is_one():
     assert got.ids.tolist() == [0, 2, 3, 3] and (got.logprob + math.log(3)).abs().max() < 1e-6
     got = ops.sample_tokens(x, u, min_p=least, top_k=torch.tensor([2, 2, 1, 0]))
     assert got.ids.tolist() == [0, 2, 0, 3]
+
+
+@pytest.mark.parametrize("least", [0.0, 0.5, 1.0])
+def test_an_infinite_temperature_weighs_the_finite_alike(least):
+    x = torch.tensor([[1.0, -math.inf, 3, -math.inf, 2, -1e30]]).expand(4, 6)
+    u = torch.tensor([0.0, 0.3, 0.5, 0.9])
+    got = ops.sample_tokens(x, u, temperature=math.inf, min_p=least)
+    assert got.ids.tolist() == [0, 2, 4, 5] and (got.logprob + math.log(4)).abs().max() < 1e-6
+    got = ops.sample_tokens(x, u, temperature=math.inf, top_k=3)
+    assert got.ids.tolist() == [0, 0, 2, 4] and (got.logprob + math.log(3)).abs().max() < 1e-6
