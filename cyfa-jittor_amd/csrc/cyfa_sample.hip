@@ -216,10 +216,11 @@ __device__ __forceinline__ Choice choice_of(const SampleParams& p, float m, doub
     return ch;
 }
 
-// The least fp32 value that min_p keeps of a row; the largest is always kept.
+// The least fp32 value that min_p keeps of a row; the largest is always kept. (An
+// infinite temperature gives all finite ones the weight 1.)
 __device__ __forceinline__ float lowest_of(double min_p, double m, double T) {
     float lowest = -INFINITY;
-    if (min_p > 0.) {
+    if (min_p > 0. && T < INFINITY) {
         const double border = fmin(m, m + T * log(min_p));
         lowest = (float)border;
         if ((double)lowest < border) lowest = nextafterf(lowest, INFINITY);
