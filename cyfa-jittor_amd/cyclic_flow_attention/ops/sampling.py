@@ -106,10 +106,11 @@ def adjust_logits(logits, history=None, lengths=None, prompt_lengths=None, repet
     ``prompt_lengths`` [...] (none without) are the prompt's. Tokens outside
     [0, V) are passed over. ``repetition``, ``presence``, ``frequency``: numbers or
     float tensors [...]. ``bias``: float [..., V]. ``token_bias``: (ids [..., n],
-    values [..., n]), n at most 1024; equal ids add up, ids outside [0, V) are
-    passed over. ``allowed``: bool [..., V], or int32 [..., ceil(V / 32)] with token
-    j at bit j % 32 of word j // 32. Each of them may have any shape that
-    broadcasts to the logits' leading one, and is read in place where it does.
+    values [..., n]), n at most 1024; the values of equal ids are added up, in
+    their order, before the logit, ids outside [0, V) are passed over.
+    ``allowed``: bool [..., V], or int32 [..., ceil(V / 32)] with token j at bit
+    j % 32 of word j // 32. Each of them may have any shape that broadcasts to the
+    logits' leading one, and is read in place where it does.
     ``out``: a tensor of the logits' shape and dtype, or the logits themselves.
 
     Differentiable in the logits (not with ``out``): a row without allowed tokens is
@@ -224,8 +225,10 @@ def _plain_adjust(logits, history, lengths, prompts, penalties, bias, tokens, al
         y = y + bias
     if tokens is not None:
         ids, values = tokens
-        inside = (ids >= 0) & (ids < logits.shape[-1])
-        y = y.scatter_add(-1, ids.clamp(0, logits.shape[-1] - 1), torch.where(inside, values, 0.0))
+        inside, at = (ids >= 0) & (ids < logits.shape[-1]), ids.clamp(0, logits.shape[-1] - 1)
+        named = torch.zeros(y.shape, dtype=torch.int32, device=y.device).scatter_add(-1, at, inside.int()) > 0
+        sums = torch.zeros(y.shape, dtype=y.dtype, device=y.device).scatter_add(-1, at, torch.where(inside, values, 0.0))
+        y = torch.where(named, y + sums, y)
     if allowed is not None:
         y = torch.where(allowed, y, float("-inf"))
     return y.to(logits.dtype)

@@ -39,3 +39,15 @@ def test_an_infinite_temperature_weighs_the_finite_alike(rows, V, dtype):
             assert (got.ids == at[1]).all() and (got.logprob + math.log(3)).abs().max() < 1e-6, least
             got = ops.sample_tokens(x, u, temperature=T, min_p=least, top_p=0.5)
             assert (got.ids == at[3]).all() and (got.logprob + math.log(2)).abs().max() < 1e-6, least
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("V", [9, 8200, 50001])
+def test_equal_token_biases_are_added_up_before_the_logit(V, inplace):
+    """1 + (2^-24 + 2^-24) is one step above 1 in fp32, (1 + 2^-24) + 2^-24 is 1."""
+    step, x = 2.0**-24, torch.ones(3, V).cuda()
+    ids, values = torch.tensor([V - 1, 2, V - 1, V, 0]).cuda(), torch.tensor([step, 1.0, step, 5.0, step]).cuda()
+    want = x.clone()
+    want[:, V - 1], want[:, 2] = 1 + 2 * step, 2.0
+    y = ops.adjust_logits(x, token_bias=(ids, values), out=x if inplace else None)
+    assert torch.equal(y, want)

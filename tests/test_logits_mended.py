@@ -9,7 +9,7 @@ import torch
 from cyclic_flow_attention import _native, ops
 from cyclic_flow_attention.ops import distill, sampling
 
-NAN = float("nan")
+INF, NAN = float("inf"), float("nan")
 
 
 @pytest.fixture(autouse=True)
@@ -65,3 +65,13 @@ def test_an_infinite_temperature_weighs_the_finite_alike(least):
     assert got.ids.tolist() == [0, 2, 4, 5] and (got.logprob + math.log(4)).abs().max() < 1e-6
     got = ops.sample_tokens(x, u, temperature=math.inf, top_k=3)
     assert got.ids.tolist() == [0, 0, 2, 4] and (got.logprob + math.log(3)).abs().max() < 1e-6
+
+
+def test_equal_token_biases_are_added_up_before_the_logit():
+    """As the kernel does it: 1 + (2^-24 + 2^-24) is one step above 1 in fp32, (1 + 2^-24) + 2^-24 is 1."""
+    step = 2.0**-24
+    x = torch.tensor([[1.0, -0.0, 1.0, 0.5], [1.0, 1.0, 1.0, -INF]]).requires_grad_(True)
+    y = ops.adjust_logits(x, token_bias=(torch.tensor([[0, 2, 0, 9], [3, 1, 3, 1]]), torch.tensor([[step, 1.0, step, 5.0], [1.0, step, 1.0, step]])))
+    assert y.tolist() == [[1 + 2 * step, -0.0, 2.0, 0.5], [1.0, 1 + 2 * step, 1.0, -INF]] and y[0, 1].signbit()
+    (dx,) = torch.autograd.grad(y, [x], torch.ones(2, 4))
+    assert dx.tolist() == [[1.0] * 4] * 2
