@@ -99,7 +99,10 @@ class Sampler:
         if self._penalised or self._bias is not None or self._token_bias is not None or allowed is not None:
             given = (self.history, self.lengths, self.prompt_lengths) if self._penalised else (None, None, None)
             logits = adjust_logits(logits, *given, **self._penalties, bias=self._bias, token_bias=self._token_bias, allowed=allowed)
-        uniform = torch.rand(logits.shape[0], device=logits.device, generator=self.generator)
+        # A number in [0, 1) and one of 2^-24 of that beside it: the first alone is 0, which takes the first kept token
+        # however unlikely that is, once in 2^24 or 2^25 draws, and near 1 passes over shares below 2^-24.
+        high, low = torch.rand(2, logits.shape[0], device=logits.device, generator=self.generator)
+        uniform = high.double().add_(low, alpha=2.0**-24)
         ids = sample_tokens(logits, uniform, **self._choice).ids
         at = self.lengths.clamp(max=self.history.shape[1] - 1)[:, None]
         self.history.scatter_(1, at, ids[:, None])
