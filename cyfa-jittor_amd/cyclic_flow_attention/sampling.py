@@ -46,7 +46,10 @@ class Sampler:
         if prompts.dim() != 2 or prompts.dtype not in (torch.int64, torch.int32) or room < 0:
             raise ValueError("a Sampler needs prompts [B, T] of int64 or int32 tokens and room for no fewer than 0 more")
         dev, (B, T) = prompts.device, prompts.shape
+        if not (sampling.allowed is None or callable(sampling.allowed) or isinstance(sampling.allowed, torch.Tensor)):
+            raise ValueError(f"a Sampling's mask (allowed) must be a tensor or a function that returns one, got {type(sampling.allowed).__name__}")
         self.sampling, self.room = sampling, room
+        self._follows = sampling.allowed is not None and not isinstance(sampling.allowed, torch.Tensor)  # the tokens
         self.history = torch.full((B, T + room), -1, dtype=torch.int64, device=dev)
         self.history[:, :T] = prompts
         if lengths is None:
@@ -86,15 +89,20 @@ class Sampler:
             raise ValueError("the Sampler has no room for more tokens")
         self.room -= 1
 
-    @torch.no_grad()
     def choose(self, logits, allowed=None):
         """The next tokens [B] for logits [B, V], kept as the sequences' last; the
         caller has counted them (``take``). ``allowed`` in place of the Sampling's."""
+        if allowed is None:
+            if self._follows:
+                raise ValueError("the Sampling's mask follows the tokens: next takes them, or choose the mask")
+            allowed = self._allowed
+        return self._choose(logits, allowed)
+
+    @torch.no_grad()
+    def _choose(self, logits, allowed):
         if logits.dim() != 2 or logits.shape[0] != self.history.shape[0]:
             raise ValueError(f"a Sampler of {self.history.shape[0]} sequences needs their logits [B, V], got {tuple(logits.shape)}")
-        if allowed is None:
-            allowed = self._allowed if isinstance(self._allowed, torch.Tensor) else None
-        else:
+        if allowed is not None:
             allowed = allowed.to(logits.device)
         if self._penalised or self._bias is not None or self._token_bias is not None or allowed is not None:
             given = (self.history, self.lengths, self.prompt_lengths) if self._penalised else (None, None, None)
@@ -111,6 +119,7 @@ class Sampler:
 
     def next(self, logits, generated=None):
         """take and choose, with a mask from the Sampling's function of ``generated``."""
+        if self._follows and generated is None:
+            raise ValueError("the Sampling's mask follows the tokens: next needs the sequences' new ones")
         self.take()
-        allowed = self.sampling.allowed
-        return self.choose(logits, allowed(generated) if callable(allowed) and not isinstance(allowed, torch.Tensor) else None)
+        return self._choose(logits, self.sampling.allowed(generated)) if self._follows else self.choose(logits)

@@ -6,6 +6,7 @@ import torch
 
 import cyclic_flow_attention.sampling as module
 from cyclic_flow_attention import Sampler, Sampling, _native
+from cyclic_flow_attention.generation import generate, generate_batch
 from cyclic_flow_attention.ops import sampling
 
 
@@ -42,3 +43,42 @@ def test_a_first_token_next_to_impossible_is_not_taken(monkeypatch):
                         else torch.zeros(*shape))
     logits = torch.tensor([[0.0, 25.0, 25.0]]).expand(50, 3)
     assert (_sampler(rows=50).next(logits) == 1).all()
+
+
+class _Model(torch.nn.Module):
+    """Answers with the logits 0, 1, ..., 8, or ``logits``, whatever it is asked."""
+
+    def __init__(self, logits=None):
+        super().__init__()
+        self.embedding = torch.nn.Parameter(torch.zeros(1))
+        self.logits = torch.arange(9.0) if logits is None else logits
+        self.lm_head = lambda hidden: self._of(hidden.shape[:-1])
+        self.model = lambda ids, **kw: (torch.zeros(*ids.shape, 1), None)
+
+    def _of(self, shape):
+        return self.logits.expand(*shape, 9).clone()
+
+    def forward(self, ids, cache=None, use_cache=True):
+        return dict(logits=self._of(ids.shape), cache=None)
+
+
+@pytest.mark.parametrize("mask", [[False] * 8 + [True], (True,) * 9, torch.ones(9, dtype=torch.bool).numpy(), 5])
+def test_masks_that_are_no_masks_are_refused(mask):
+    """They were passed over."""
+    with pytest.raises(ValueError, match="mask"):
+        _sampler(allowed=mask)
+
+
+def test_masks_that_follow_the_tokens_need_them():
+    """choose, and next without the tokens, passed over the function."""
+    sampler = _sampler(allowed=lambda rows: torch.arange(9) == len(rows[0]) + 3)
+    with pytest.raises(ValueError, match="follows the tokens"):
+        sampler.choose(torch.zeros(3, 9))
+    with pytest.raises(ValueError, match="follows the tokens"):
+        sampler.next(torch.zeros(3, 9))
+    assert sampler.room == 4 and (sampler.lengths == 2).all()
+    assert sampler.next(torch.zeros(3, 9), [[], [], []]).tolist() == [3] * 3
+    assert sampler.choose(torch.zeros(3, 9), torch.arange(9) == 7).tolist() == [7] * 3
+    free = _sampler(allowed=lambda rows: None)
+    assert free.next(torch.arange(9.0).mul(99).expand(3, 9), [[], [], []]).tolist() == [8] * 3
+    assert generate(_Model(), [1], 3, sampling=Sampling(allowed=lambda rows: torch.arange(9) == len(rows[0]) + 3)) == [3, 4, 5]
