@@ -42,7 +42,8 @@ def generate(model, ids, max_new_tokens=64, eos_token_id=None, temperature=0.0, 
     max_new_tokens, on eos_token_id (which is kept), or when
     on_token(generated) returns true. ValueError for an empty prompt, a
     negative length or temperature, or top_p outside (0, 1]. ``sampling`` (a
-    Sampling) in place of temperature, top_p and seed."""
+    Sampling) in place of temperature, top_p and seed; ValueError where its mask or
+    the logits leave no next token."""
     if not ids or max_new_tokens < 0 or temperature < 0 or not 0 < top_p <= 1:
         raise ValueError("Invalid prompt or sampling options")
     if sampling is not None and (temperature, top_p, seed) != (0.0, 1.0, 42):
@@ -57,7 +58,7 @@ def generate(model, ids, max_new_tokens=64, eos_token_id=None, temperature=0.0, 
         cache = result["cache"]
         last = result["logits"][0, -1]
         if sampler is not None:
-            token = int(sampler.next(last[None], [generated]))
+            (token,) = sampler.to_list(sampler.next(last[None], [generated]))
         elif temperature == 0:
             # greedy: the first largest logit, found on the device (one index
             # crosses to the host, not the row); NaN counts as largest, as in
@@ -77,7 +78,8 @@ def generate(model, ids, max_new_tokens=64, eos_token_id=None, temperature=0.0, 
 @torch.no_grad()
 def generate_batch(model, prompts, max_new_tokens=48, eos_token_id=None, on_token=None, sampling=None):
     """Continuations of several prompts at once, greedy or with ``sampling`` (a
-    Sampling). The prompts are
+    Sampling; ValueError where its mask or the logits leave a row that has not
+    stopped no next token). The prompts are
     right-padded to a multiple of 64 tokens and run through one prefill with
     an attention mask (pads leave the state and the conv cache unchanged);
     each row's first token comes from the logits at its last prompt token.
@@ -102,7 +104,7 @@ def generate_batch(model, prompts, max_new_tokens=48, eos_token_id=None, on_toke
     sampler = None if sampling is None else Sampler(sampling, ids.to(dev), max_new_tokens, lengths)
     for step in range(max_new_tokens):
         tokens = logits.argmax(-1) if sampler is None else sampler.next(logits, generated)
-        for row, token in enumerate(tokens.tolist()):
+        for row, token in enumerate(tokens.tolist() if sampler is None else sampler.to_list(tokens, finished)):
             if finished[row]:
                 continue
             generated[row].append(int(token))

@@ -355,7 +355,9 @@ class CyclicFlowAttentionForCausalLM(nn.Module):
     @torch.no_grad()
     def generate(self, input_ids, max_new_tokens=32, eos_token_id=None, sampling=None):
         """Decoding with the constant-size state (modeling_cyfa.py:142-158), greedy
-        or with ``sampling`` (a sampling.Sampling without a function of the tokens).
+        or with ``sampling`` (a sampling.Sampling without a function of the tokens;
+        ValueError at the end where its mask or the logits left a sequence, before
+        its eos_token_id, no next token).
 
         The choice stays on the device; tokens are copied to the host once at
         the end (the reference synchronises every step)."""
@@ -363,6 +365,7 @@ class CyclicFlowAttentionForCausalLM(nn.Module):
         sampler = None if sampling is None else Sampler(sampling, input_ids, max_new_tokens)
         if sampler is not None and callable(sampling.allowed):
             raise ValueError("generate: masks that follow the tokens are generation.generate_batch's")
+        ended = stuck = None if sampler is None else sampler.stuck  # (none yet)
         tokens = [input_ids]
         cache = None
         current = input_ids
@@ -372,8 +375,14 @@ class CyclicFlowAttentionForCausalLM(nn.Module):
             last = result["logits"][:, -1:]
             current = last.argmax(-1) if sampler is None else sampler.next(last[:, 0])[:, None]
             tokens.append(current)
+            if sampler is not None:
+                stuck = stuck | (sampler.stuck & ~ended)
+                if eos_token_id is not None:
+                    ended = ended | (current[:, 0] == eos_token_id)
             if eos_token_id is not None and bool((current == eos_token_id).all()):
                 break
+        if sampler is not None:
+            sampler.check(stuck.tolist())
         return torch.cat(tokens, dim=1)
 
 

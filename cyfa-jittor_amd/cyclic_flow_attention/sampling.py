@@ -40,7 +40,9 @@ class Sampler:
     tokens: ``prompts`` [B, T], of which the first ``lengths`` [B] (all without)
     count, and up to ``room`` tokens more. Its calls can be captured into a HIP
     graph (GraphedDecodeStep does), where ``generator`` has to be registered and
-    the caller counts the replays with ``take``."""
+    the caller counts the replays with ``take``. A sequence that had no next token
+    at a choice, because the mask left none or the logits held a NaN, is ``stuck``
+    from then on: the token answered there is none that could follow."""
 
     def __init__(self, sampling, prompts, room, lengths=None):
         if prompts.dim() != 2 or prompts.dtype not in (torch.int64, torch.int32) or room < 0:
@@ -58,6 +60,7 @@ class Sampler:
             raise ValueError(f"a Sampler's lengths must be {B} integers from 0 to {T}")
         self.prompt_lengths = lengths.to(device=dev, dtype=torch.int64).clone()
         self.lengths = self.prompt_lengths.clone()
+        self._least = torch.full((B, 1), float("inf"), device=dev)  # of the chosen tokens' logits: -inf or NaN where none could follow
         self.generator = torch.Generator(device=dev).manual_seed(sampling.seed)
 
         def here(v):
@@ -78,7 +81,7 @@ class Sampler:
     def __deepcopy__(self, memo):
         """A Sampler of its own state (the random numbers' among it), for a trial run."""
         other = copy.copy(self)
-        other.history, other.lengths = self.history.clone(), self.lengths.clone()
+        other.history, other.lengths, other._least = self.history.clone(), self.lengths.clone(), self._least.clone()
         other.generator = torch.Generator(device=self.generator.device)
         other.generator.set_state(self.generator.get_state())
         return other
@@ -112,8 +115,10 @@ class Sampler:
         high, low = torch.rand(2, logits.shape[0], device=logits.device, generator=self.generator)
         uniform = high.double().add_(low, alpha=2.0**-24)
         ids = sample_tokens(logits, uniform, **self._choice).ids
+        chosen = ids[:, None]
+        torch.minimum(self._least, logits.gather(1, chosen).float(), out=self._least)  # (a NaN stays)
         at = self.lengths.clamp(max=self.history.shape[1] - 1)[:, None]
-        self.history.scatter_(1, at, ids[:, None])
+        self.history.scatter_(1, at, chosen)
         self.lengths.add_(1)
         return ids
 
@@ -123,3 +128,22 @@ class Sampler:
             raise ValueError("the Sampling's mask follows the tokens: next needs the sequences' new ones")
         self.take()
         return self._choose(logits, self.sampling.allowed(generated)) if self._follows else self.choose(logits)
+
+    @property
+    def stuck(self):
+        """bool [B]: the sequences that had no next token at a choice so far."""
+        return ~(self._least[:, 0] > float("-inf"))  # (a logit of +inf, as of a bias that forces a token, is taken)
+
+    def to_list(self, tokens, ended=None):
+        """Tokens [B] that choose or next gave, on the host; ValueError where a
+        sequence is stuck that has not ``ended`` (a truth value each), -1 where it has."""
+        tokens = torch.where(self.stuck, -1, tokens).tolist()
+        self.check([t < 0 and not (ended and ended[n]) for n, t in enumerate(tokens)])
+        return tokens
+
+    @staticmethod
+    def check(stuck):
+        """ValueError with the first of the sequences that are ``stuck`` (truth values)."""
+        for n, s in enumerate(stuck):
+            if s:
+                raise ValueError(f"sequence {n} has no next token: its mask leaves none, or its logits hold a NaN or nothing but -inf")

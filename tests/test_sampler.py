@@ -1,6 +1,8 @@
 """A Sampler's random numbers, masks and sequences without a next token, and the
 generation calls that meet them, through the torch operations (no GPU compute)."""
 
+import copy
+
 import pytest
 import torch
 
@@ -82,3 +84,66 @@ def test_masks_that_follow_the_tokens_need_them():
     free = _sampler(allowed=lambda rows: None)
     assert free.next(torch.arange(9.0).mul(99).expand(3, 9), [[], [], []]).tolist() == [8] * 3
     assert generate(_Model(), [1], 3, sampling=Sampling(allowed=lambda rows: torch.arange(9) == len(rows[0]) + 3)) == [3, 4, 5]
+
+
+NONE, NAN_ROW = torch.full((9,), -float("inf")), torch.tensor([0.0] * 8 + [float("nan")])
+
+
+def test_sequences_without_a_next_token_are_told():
+    """A mask that leaves nothing, logits of NaN or nothing but -inf; told from then
+    on. (A logit of +inf, as of a bias that forces a token, is taken.)"""
+    sampler = _sampler(rows=5, room=3, temperature=torch.tensor([1.0, 1, 1, 1, 0]), top_k=3)
+    assert sampler.stuck.dtype is torch.bool and not sampler.stuck.any()
+    fine, inf = torch.arange(9.0), torch.tensor([float("inf")] + [0.0] * 8)
+    trial = copy.deepcopy(sampler)
+    trial.choose(torch.stack([fine, NAN_ROW, inf, NONE, fine]))
+    assert trial.stuck.tolist() == [False, True, False, True, False] and not sampler.stuck.any()
+    allowed = torch.ones(5, 9, dtype=torch.bool)
+    allowed[4] = False
+    ids = sampler.choose(torch.stack([99 * fine, 99 * fine, 99 * fine, NAN_ROW, fine]), allowed)
+    assert sampler.stuck.tolist() == [False, False, False, True, True]
+    assert sampler.to_list(ids, [False, False, False, True, True]) == [8, 8, 8, -1, -1]
+    with pytest.raises(ValueError, match="sequence 3 has no next token"):
+        sampler.to_list(ids)
+    with pytest.raises(ValueError, match="sequence 4 has no next token"):
+        sampler.to_list(ids, [False, False, False, True, False])
+    sampler.choose(torch.stack([fine] * 5))
+    assert sampler.stuck.tolist() == [False, False, False, True, True]
+
+
+def _ends_after(n):
+    def allowed(rows):
+        return torch.tensor([[len(tokens) < n] * 9 for tokens in rows])
+    return allowed
+
+
+def test_generate_raises_where_a_sequence_has_no_next_token():
+    """It answered token 0, which the mask forbids."""
+    s = Sampling(allowed=_ends_after(2), top_k=1)
+    assert generate(_Model(), [1, 2], 2, sampling=s) == [8, 8]
+    with pytest.raises(ValueError, match="no next token"):
+        generate(_Model(), [1, 2], 3, sampling=s)
+    for logits in (NONE, NAN_ROW):
+        with pytest.raises(ValueError, match="no next token"):
+            generate(_Model(logits), [1, 2], 3, sampling=Sampling())
+    assert generate(_Model(), [1, 2], 5, sampling=s, on_token=lambda tokens: len(tokens) == 2) == [8, 8]
+
+
+def test_generate_batch_raises_where_a_row_that_goes_on_has_no_next_token():
+    def allowed(rows):  # the first row ends after one token, the second by its mask after two
+        return torch.tensor([[len(tokens) < n] * 9 for tokens, n in zip(rows, (1, 2))])
+
+    prompts = [[1, 2], [3]]
+    with pytest.raises(ValueError, match="sequence 0 has no next token"):
+        generate_batch(_Model(), prompts, 2, sampling=Sampling(allowed=allowed, top_k=1))
+    assert generate_batch(_Model(), prompts, 1, sampling=Sampling(allowed=allowed, top_k=1)) == [[8], [8]]
+    # rows that have stopped have no mask to keep to
+    first = Sampling(allowed=lambda rows: torch.tensor([[c == 8 and not rows[0] for c in range(9)], [c < 8 for c in range(9)]]), top_k=1)
+    assert generate_batch(_Model(), prompts, 3, sampling=first, eos_token_id=8) == [[8], [7, 7, 7]]
+
+
+def test_a_forced_token_goes_on():
+    for temperature in (0.0, 1.0):
+        s = Sampling(temperature=temperature, token_bias={5: float("inf")})
+        assert generate(_Model(), [1], 3, sampling=s) == [5, 5, 5]
+        assert generate_batch(_Model(), [[1], [2, 3]], 2, sampling=s) == [[5, 5], [5, 5]]
