@@ -51,3 +51,46 @@ def test_equal_token_biases_are_added_up_before_the_logit(V, inplace):
     want[:, V - 1], want[:, 2] = 1 + 2 * step, 2.0
     y = ops.adjust_logits(x, token_bias=(ids, values), out=x if inplace else None)
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("V", [1000, 9000, 50000])
+def test_numbers_on_the_borders_of_equal_shares(V):
+    """500 tokens of one weight: number u takes token floor(500 u), for every u by itself."""
+    x = torch.full((8, V), -INF)
+    x[:, :500] = 0.0
+    u = torch.tensor([0.0, 0.25, 0.5, 0.998, 1 - 2.0**-24, 0.002, 0.75, 0.001])
+    want = (u.double() * 500).floor().long()  # (the weights and their sum are exact)
+    assert want.tolist() == [0, 125, 250, 499, 499, 1, 375, 0]
+    for k, p in ((0, 1.0), (500, 1.0), (0, 0.9999)):
+        got = ops.sample_tokens(x.cuda(), u.cuda(), top_k=k, top_p=p)
+        assert got.ids.tolist() == want.tolist() and (got.logprob + math.log(500)).abs().max() < 2.0**-20, (k, p)
+
+
+@pytest.mark.parametrize("rows,V", SIZES)
+def test_numbers_that_are_none_and_min_p_above_one(rows, V):
+    at = _four(V)
+    x = torch.full((rows, V), -1.0)
+    x[:, at] = torch.tensor([0.0, 3.0, 1.0, 3.0])
+    nan, u = torch.full((rows,), NAN).cuda(), torch.full((rows,), 0.75).cuda()
+    for kw in (dict(top_k=1), dict(top_k=2), dict(top_p=0.001), dict(top_k=200, top_p=0.001), dict(min_p=0.9)):
+        assert (ops.sample_tokens(x.cuda(), nan, **kw).ids == at[1]).all(), kw
+    for kw in (dict(), dict(top_k=min(V - 1, 300)), dict(top_k=3), dict(top_p=0.9999)):
+        got = ops.sample_tokens(x.cuda(), u, min_p=torch.full((rows,), 1.5).cuda(), **kw)
+        assert (got.ids == at[3]).all() and (got.logprob + math.log(2)).abs().max() < 1e-6, kw
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("V,dtype", [(9, F32), (5003, F32), (5003, BF)])
+def test_a_token_named_several_times(V, dtype, tail):
+    """Entries of 0.1, 0.2 and 0.3 for one token against one of 0.6: the loss by
+    entries is less by the constant sum p_i log(P / p_i), the gradient the same."""
+    x = _randn(1, 4, V).to(dtype).cuda().requires_grad_(True)
+    losses, grads = [], []
+    for ids, p in (([5, 5, 5, 2], [0.1, 0.2, 0.3, 0.25]), ([5, 2], [0.6, 0.25])):
+        losses.append(ops.distill_loss(x, torch.tensor([ids] * 4).cuda(), torch.tensor([p] * 4).log().cuda(), tail=tail))
+        grads.append(torch.autograd.grad(losses[-1], [x])[0].double())
+    less = (1.0 if tail else 1 / 0.85) * sum(p * math.log(0.6 / p) for p in (0.1, 0.2, 0.3))
+    # fp32 values of order ten
+    assert abs(losses[1].item() - losses[0].item() - less) < 16 * 2.0**-22
+    # fp32 masses of order one, off by a few steps, over four rows; each rounded once
+    assert (grads[0] - grads[1]).abs().max() < 2.0**-22 + torch.finfo(dtype).eps * grads[1].abs().max()
