@@ -29,7 +29,11 @@
 // second load and store: 64 x 32000 with 2048 tokens, 16 token biases and a bit mask
 // 9 us, one row 5. The 4096 rows and their gradient took 502 when every vector of
 // 8192-column slices read 32-bit counts, 262 with 16 bits, larger slices and the list
-// in both, 235 where their pass reads 16-bit counts.
+// in both, 235 where their pass reads 16-bit counts. The 1024-thread forms need 64
+// (bf16) to 69 registers a thread; past 64 one workgroup is on a compute unit at a
+// time, in fp16 and in the gradients. In place 4096 x 32000 with 1024 tokens take 95, 380 to 480
+// with a bias or a mask, an element at a time (apart 131 to 158); 64 x 32000 8 and 13
+// to 14 (apart 9 to 10).
 
 #include <type_traits>
 

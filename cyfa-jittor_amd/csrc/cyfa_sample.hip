@@ -29,10 +29,14 @@
 // maximum, a second launch counts the parts' bins, and a third, a workgroup to a
 // row, goes on from there with the parts as runs.
 //
-// Bound by the VALU: an element's weight costs 17 operations in double, of 4.3 to 5
-// cycles of a SIMD each, and 6 others: 0.11 ns on 256 compute units, where its two
-// bytes take 0.04 from memory. Rows of a single compute unit each wait besides at
-// their dozen barriers.
+// An element's weight costs 17 operations in double, of 4.3 to 5 cycles of a SIMD
+// each, and 6 others, some 95 cycles a wave: 0.6 ps on 256 compute units, where two
+// bytes take 0.4 from memory and four 0.8. What bounds a call is that a row's steps
+// follow one another (its maximum from memory, its weights, and where it is cut a
+// 64-bit LDS atomic an element, the border's list and the draw) in few workgroups a
+// compute unit: 80 to 124 vector registers leave room for two or three of 512 threads.
+// Rows of a single compute unit each wait besides at their dozen barriers. us, bf16:
+// 1024 x 32000 whole 49, top_k 50 37, top_p 0.9 69; 1021 x 50001 fp32 80 to 84, 72, 140.
 #include <type_traits>
 
 #include "cyfa_internal.h"
@@ -982,9 +986,12 @@ __global__ __launch_bounds__(NT) void sample_kernel(SampleParams p) {
 // A workgroup takes rows in turn: while it forms a row's weights it finds the next
 // row's maximum, so that one row is on its way from memory while the exponentials
 // of the one before, which come from the caches a second time, keep the VALU busy.
+// (Past 1024 rows, 2048 of at most 8192 columns: up to there every row has a
+// workgroup of its own, and its maximum and its weights follow one another.)
 // A wave to each run of the row; the run that holds the token is formed again.
 // us on MI355X, by sample_kernel / by this one: 1021 x 50001 fp32 88 / 80 (2.6 TB/s
-// of one read; 58 with every row in the L2, for the VALU's 45), with min_p 0.05 76 /
+// of one read; 58 with every row in the L2, where the operations of the weights take
+// 31 to 35 and one read of the rows from memory 40), with min_p 0.05 76 /
 // 67; bf16, 4096 x 32000 156 / 149, with min_p 119 / 112; 256 x 32000 27 / 13; 1 x
 // 32000 16 / 12; 1024 x 4096 13 / 10.5; 16384 x 1000 81 / 79. Threads of a row, 256 /
 // 512 / 1024: 1021 x 50001 fp32 90 / 79 / 82, 4096 x 32000 154 / 148 / 170, 1024 x 4096
@@ -1202,7 +1209,9 @@ void launch_rows(SampleParams p, hipStream_t stream) {
     }
 }
 
-// Workgroups of a compute unit that the rows of sample_draw_kernel are shared out to.
+// Workgroups of a compute unit that the rows of sample_draw_kernel are shared out to,
+// of which (83 to 124 vector registers) two of 512 threads, or four or five of 256,
+// are resident.
 template <class E, int NT, bool KEEP>
 void launch_draw(const SampleParams& p, int per_unit, hipStream_t stream) {
     const long long slots = 256ll * per_unit, turns = (p.rows + slots - 1) / slots;

@@ -403,7 +403,8 @@ class GraphedDecodeStep:
 
     A step reads the token buffer, runs every layer's one-token path, writes
     the new recurrent states and conv histories, and stores the argmax token
-    (or that of a sampling.Sampler, which keeps it and counts its room) in the
+    (or that of a sampling.Sampler, which keeps it, counts its room and tells the
+    sequences that had no next token, ``stuck``) in the
     token buffer for the next replay. Two caches alternate: the step
     captured from cache 0 writes cache 1 and the other one back, so that no
     decode kernel updates a state in place (which lets it run several

@@ -111,7 +111,8 @@ def adjust_logits(logits, history=None, lengths=None, prompt_lengths=None, repet
     ``allowed``: bool [..., V], or int32 [..., ceil(V / 32)] with token j at bit
     j % 32 of word j // 32. Each of them may have any shape that broadcasts to the
     logits' leading one, and is read in place where it does.
-    ``out``: a tensor of the logits' shape and dtype, or the logits themselves.
+    ``out``: a tensor of the logits' shape and dtype, or the logits themselves
+    (with a bias or a mask an element at a time, up to three times as slow).
 
     Differentiable in the logits (not with ``out``): a row without allowed tokens is
     all -inf and gets a gradient of zeros, as every token that is not allowed."""
@@ -281,7 +282,8 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     first always), of those the ones with w >= ``min_p``. The token is the first
     kept one, by id, at which the running mass of the kept passes uniform times
     their mass, so that equal inputs give equal tokens: weights are held as
-    multiples of 2^-46 of the largest and added up exactly.
+    multiples of 2^-46 of the largest (past 2^16 columns of 2^(ceil(log2 V) - 62))
+    and added up exactly.
 
     Each option is a number or a tensor [...] (top_k int64 or int32, the others
     float, read in fp32). Temperature 0, or below in a tensor: the first largest
