@@ -127,7 +127,11 @@ class Sampler:
         if self._follows and generated is None:
             raise ValueError("the Sampling's mask follows the tokens: next needs the sequences' new ones")
         self.take()
-        return self._choose(logits, self.sampling.allowed(generated)) if self._follows else self.choose(logits)
+        try:
+            return self._choose(logits, self.sampling.allowed(generated)) if self._follows else self.choose(logits)
+        except Exception:  # (a choice that is refused has taken no room)
+            self.room += 1
+            raise
 
     @property
     def stuck(self):
@@ -138,7 +142,7 @@ class Sampler:
         """Tokens [B] that choose or next gave, on the host; ValueError where a
         sequence is stuck that has not ``ended`` (a truth value each), -1 where it has."""
         tokens = torch.where(self.stuck, -1, tokens).tolist()
-        self.check([t < 0 and not (ended and ended[n]) for n, t in enumerate(tokens)])
+        self.check([t < 0 and (ended is None or not ended[n]) for n, t in enumerate(tokens)])
         return tokens
 
     @staticmethod

@@ -147,3 +147,21 @@ def test_a_forced_token_goes_on():
         s = Sampling(temperature=temperature, token_bias={5: float("inf")})
         assert generate(_Model(), [1], 3, sampling=s) == [5, 5, 5]
         assert generate_batch(_Model(), [[1], [2, 3]], 2, sampling=s) == [[5, 5], [5, 5]]
+
+
+def test_a_refused_choice_takes_no_room():
+    sampler = _sampler(room=1, allowed=lambda rows: torch.ones(8, dtype=torch.bool) if rows[0] else None)
+    for logits, generated in ((torch.zeros(2, 9), [[], [], []]), (torch.zeros(3, 9), [[1], [1], [1]]), (torch.zeros(3, 9), None)):
+        with pytest.raises(ValueError):
+            sampler.next(logits, generated)
+        assert sampler.room == 1 and (sampler.lengths == 2).all()
+    sampler.next(torch.zeros(3, 9), [[], [], []])
+    with pytest.raises(ValueError, match="room"):
+        sampler.next(torch.zeros(3, 9), [[], [], []])
+    assert sampler.room == 0 and (sampler.lengths == 3).all()
+
+
+def test_generation_in_inference_mode():
+    with torch.inference_mode():
+        assert generate(_Model(), [1], 3, sampling=Sampling(top_k=1, frequency=0.5)) == [8, 8, 7]  # (8 - 2 x 0.5 is 7, and 7 the lower id)
+        assert generate_batch(_Model(), [[1], [2, 3]], 2, sampling=Sampling(top_k=1)) == [[8, 8], [8, 8]]
