@@ -88,9 +88,11 @@ def _plain(logits, ids, values, weights, temperature, tail):
     valid = (ids >= 0) & (ids < V) & (values != float("-inf"))
     count = valid.any(-1).float() if weights is None else valid.any(-1) * weights
     live = count != 0
-    x = torch.where(live[..., None], logits.float(), 0.0) / temperature
+    x = torch.where(live[..., None], logits.float(), 0.0)
     at = ids.clamp(0, V - 1)
-    x = x - x.detach().amax(-1, keepdim=True)
+    x = x - x.detach().amax(-1, keepdim=True)  # (before the temperature, which may take the lowest values past fp32)
+    x_at = x.gather(-1, at).double() / temperature
+    x = x / temperature
     lse = x.exp().sum(-1, keepdim=True).log()
     t = torch.where(valid, values.double(), 0.0)
     if tail:
@@ -102,7 +104,7 @@ def _plain(logits, ids, values, weights, temperature, tail):
     p = torch.where(valid & live[..., None], log_p.exp(), 0.0)
     given = p > 0
     log_p = torch.where(given, log_p, 0.0)
-    log_q = torch.where(given, x.gather(-1, at) - lse, 0.0)
+    log_q = torch.where(given, x_at - lse, 0.0)
     loss = (p * (log_p - log_q)).sum(-1)
     if tail:
         entry = torch.zeros(logits.shape, dtype=torch.int32, device=logits.device).scatter_add(-1, at, valid.int()) > 0

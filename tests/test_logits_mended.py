@@ -75,3 +75,28 @@ def test_equal_token_biases_are_added_up_before_the_logit():
     assert y.tolist() == [[1 + 2 * step, -0.0, 2.0, 0.5], [1.0, 1 + 2 * step, 1.0, -INF]] and y[0, 1].signbit()
     (dx,) = torch.autograd.grad(y, [x], torch.ones(2, 4))
     assert dx.tolist() == [[1.0] * 4] * 2
+
+
+@pytest.mark.parametrize("T", [0.25, 1.0, 4.0])
+def test_rows_of_the_lowest_value_at_any_temperature(T):
+    """They are rows of zeros: divided by a temperature below 1 first, they were of -inf."""
+    x, ids, values = torch.full((2, 6), torch.finfo(torch.float32).min), torch.tensor([[1, 3], [0, 2]]), torch.tensor([[-0.5, -1.0], [0.0, -2.0]])
+    results = []
+    for logits in (x, torch.zeros(2, 6)):
+        logits = logits.clone().requires_grad_(True)
+        loss = ops.distill_loss(logits, ids, values, temperature=T)
+        results.append((loss, torch.autograd.grad(loss, [logits])[0]))
+    assert results[0][0].isfinite() and torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    if T < 1:  # a quarter of the mass at a token that the mask took
+        x[0, 0] = 5.0
+        loss = ops.distill_loss(x[:1], torch.tensor([[0, 1]]), torch.tensor([[math.log(3.0), 0.0]]) * T, temperature=T)
+        assert loss == INF or abs(loss.item() / (0.25 / T * torch.finfo(torch.float32).max) - 1) < 2.0**-20
+
+
+def test_a_numbers_penalty_is_the_tensors():
+    """torch divides by a number by a product with its reciprocal on a GPU; either way the kernel divides."""
+    x = _randn(3, 4, 50)
+    history = torch.arange(50)[None]
+    y = ops.adjust_logits(x, history, repetition=1.3, presence=0.1, frequency=0.7)
+    per_row = {n: torch.full((4,), v) for n, v in (("repetition", 1.3), ("presence", 0.1), ("frequency", 0.7))}
+    assert torch.equal(y, ops.adjust_logits(x, history, **per_row))
