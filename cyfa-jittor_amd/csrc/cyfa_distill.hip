@@ -30,7 +30,8 @@ namespace cyfa {
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 0.6931471805599453;
 constexpr float kLowest = -3.402823466e38f;
 constexpr int DS_NV = 4;  // vectors of a thread in flight
 
@@ -236,9 +237,9 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillParams p) {
         double loss = 0.;
 #pragma unroll
         for (int q = 0; q < Q; q++)
-            if (id[q] >= 0 && p_[q] != 0.) {
-                const float lq = (e[q] - all.m) / p.temperature - kLn2 * ls;
-                loss += p_[q] * scale * ((((double)t[q] - top) / T - lognorm) - (double)lq);
+            if (id[q] >= 0 && p_[q] != 0.) {  // (in double: a mask's lowest value over T, or a row's sum, passes fp32)
+                const double lq = ((double)e[q] - (double)all.m) / T - kLn2 * (double)ls;
+                loss += p_[q] * scale * ((((double)t[q] - top) / T - lognorm) - lq);
             }
         loss = wave_sum(loss);
         DistillRow row;
@@ -253,14 +254,14 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(DistillParams p) {
         if (TAIL) {
             // the rest, where the student has any
             const double pr = a.s > 0.f ? fmax(0., 1. - mass) : 0.;
-            const double lqr = (double)(a.m - all.m) + (double)kLn2 * ((double)rls - (double)ls);
+            const double lqr = ((double)a.m - (double)all.m) + kLn2 * ((double)rls - (double)ls);
             if (pr > 0.) loss += pr * (log(pr) - lqr);
             row.entry = (float)(mass + pr);
             row.rest = (float)(exp(lqr) * (mass + pr) - pr);
         }
         row.loss = (float)loss;
         if (lane == 0) *keep = row;
-        part += (double)weight * (double)row.loss;
+        part += (double)weight * loss;
         parts += (double)weight;
     }
     if (lane == 0) {

@@ -94,3 +94,22 @@ def test_a_token_named_several_times(V, dtype, tail):
     assert abs(losses[1].item() - losses[0].item() - less) < 16 * 2.0**-22
     # fp32 masses of order one, off by a few steps, over four rows; each rounded once
     assert (grads[0] - grads[1]).abs().max() < 2.0**-22 + torch.finfo(dtype).eps * grads[1].abs().max()
+
+
+@pytest.mark.parametrize("V", [9, 5003])
+def test_large_divergences_whose_mean_fits(V):
+    """Tokens that a mask of the type's lowest value takes from the student: a row's
+    loss past fp32, or its logarithms over the temperature, beside a mean that is not."""
+    low = torch.finfo(F32).min
+    x = torch.full((3, V), low)
+    x[:, 0] = 5.0
+    x[1:, 4] = 5.0
+    # 0.5 e^1e-6 twice: with the tail row 0 costs 1.000001 times the largest value, the others log 2 and a little
+    ids, values = torch.tensor([[1, 2], [0, 4], [0, 4]]), torch.full((3, 2), math.log(0.5) + 1e-6)
+    loss = ops.distill_loss(x.cuda(), ids.cuda(), values.cuda(), tail=True)
+    assert abs(loss.item() / (-low / 3 * (1 + 1e-6)) - 1) < 2.0**-20
+    # a quarter of the mass at 2 x the lowest value below the largest
+    ids, values = torch.tensor([[0, 1]]), torch.tensor([[math.log(3.0), 0.0]]) * 0.5
+    loss = ops.distill_loss(x[:1].cuda(), ids.cuda(), values.cuda(), temperature=0.5)
+    assert abs(loss.item() / (0.25 * 2 * -low) - 1) < 2.0**-20
+    assert ops.distill_loss(x[:1].cuda(), ids.cuda() + 1, values.cuda(), temperature=0.5).item() == INF  # past fp32
