@@ -217,6 +217,8 @@ def _column(v):
 def _plain_adjust(logits, history, lengths, prompts, penalties, bias, tokens, allowed):
     """adjust_logits in torch operations."""
     repetition, presence, frequency = (_column(v) for v in penalties)
+    if not isinstance(repetition, torch.Tensor):  # (torch divides by a number by a product with its reciprocal)
+        repetition = torch.full((), repetition, dtype=torch.float32, device=logits.device)
     n, m, allowed = _tables(logits, history, lengths, prompts, allowed)
     y = logits.float()
     if n is not None:

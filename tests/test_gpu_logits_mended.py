@@ -113,3 +113,14 @@ def test_large_divergences_whose_mean_fits(V):
     loss = ops.distill_loss(x[:1].cuda(), ids.cuda(), values.cuda(), temperature=0.5)
     assert abs(loss.item() / (0.25 * 2 * -low) - 1) < 2.0**-20
     assert ops.distill_loss(x[:1].cuda(), ids.cuda() + 1, values.cuda(), temperature=0.5).item() == INF  # past fp32
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float16, F32])
+def test_a_numbers_penalty_in_torch_operations(dtype, monkeypatch):
+    """The torch form divides by a number as the kernel does, not by a product with its reciprocal."""
+    from cyclic_flow_attention.ops import sampling
+
+    x, history = (_randn(3, 4, 5003) * 3).to(dtype).cuda(), torch.arange(5003).cuda()[None]
+    y = ops.adjust_logits(x, history, repetition=1.3, presence=0.1, frequency=0.7)
+    monkeypatch.setattr(sampling, "kernel_ok", lambda *tensors: False)
+    assert torch.equal(y, ops.adjust_logits(x, history, repetition=1.3, presence=0.1, frequency=0.7))
